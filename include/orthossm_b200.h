@@ -47,7 +47,7 @@ enum ossm_status {
   OSSM_EWORKSPACE = 5 /* workspace missing or too small */
 };
 
-enum ossm_dtype { OSSM_F32 = 0, OSSM_BF16 = 1 };
+enum ossm_dtype { OSSM_F32 = 0, OSSM_BF16 = 1, OSSM_F16 = 2 /* attention and sampling only */ };
 
 /* Chebyshev evaluation mode (low 2 bits of flags). */
 #define OSSM_EVAL_CLENSHAW 0u      /* exact degree-K Clenshaw (sdpc_kernel.py:1147-1156) */
@@ -372,6 +372,79 @@ typedef struct {
 size_t ossm_ttt_run_workspace_bytes(const ossm_ttt_run_args* a);
 int ossm_ttt_wpred_run(const ossm_ttt_run_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Serving: attention over packed prompts or over a cache (inference only).
+ *
+ * Sequence b owns the queries q[cu_q[b] .. cu_q[b+1]) and Lk keys from
+ * k[cu_k[b]] on: Lk = cu_k[b+1] - cu_k[b], or kv_len[b] (clipped to that) if
+ * kv_len is not NULL, so that k and v can be a cache with room left in each
+ * sequence's slots.  Query i of Lq stands at position i + Lk - Lq and sees the
+ * keys j <= i + Lk - Lq, with window > 0 the last `window` of them only:
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j,  0 where no key is seen.
+ * Query head h reads key / value head h / (H / H_kv).  Hidden keys have no
+ * influence, whatever they hold (NaN and infinities included).  Softmax
+ * statistics and sums are fp32.  A value of cu_q / cu_k outside the tensors is
+ * clipped.  Rows of q outside every sequence are not written.
+ * No counterpart in the reference: its local attention is a masked SDPA over
+ * one dense batch (slr_module.py:83-243).
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  int32_t B, H, H_kv, head_dim;      /* head_dim a multiple of 8, at most 128; H a multiple of H_kv; B <= 16384 */
+  int64_t total_q, total_k;          /* rows of q / out and of k / v, below 2^31 */
+  int32_t max_seqlen_q;              /* the most queries a sequence has (chooses the kernels; never a bound) */
+  int32_t dtype;                     /* OSSM_BF16 or OSSM_F16: q, k, v, out */
+  const void *q, *k, *v;             /* [rows, heads, head_dim], 16-byte aligned, unit channel stride */
+  void* out;
+  int64_t q_stride_t, q_stride_h;    /* in elements, multiples of 8 */
+  int64_t k_stride_t, k_stride_h;
+  int64_t v_stride_t, v_stride_h;
+  int64_t out_stride_t, out_stride_h;
+  const int32_t* cu_q;               /* [B+1] on the device */
+  const int32_t* cu_k;               /* [B+1] on the device */
+  const int32_t* kv_len;             /* [B] on the device, or NULL */
+  int32_t window;                    /* 0: every earlier key */
+  float scale;                       /* positive, finite */
+} ossm_attn_args;
+
+/* Bytes of device workspace (zero-filled once when allocated, then reused by
+ * calls ordered on one stream; its first 256 bytes are a header that
+ * ossm_workspace_status reads); 0 for invalid arguments. */
+size_t ossm_attn_workspace_bytes(const ossm_attn_args* a);
+int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Serving: the next token of each row from given random numbers.
+ *
+ * Candidates are ordered by logit, at equal logits by index.  The first top_k
+ * stay (0: all); of these the shortest prefix whose probability under
+ * softmax(logits * inv_temperature) over the first top_k reaches top_p (1:
+ * all; at least one stays); of these the ones at least min_p times as likely
+ * as the first.  The token is the candidate that maximises
+ *   logit * inv_temperature - log(noise),
+ * ties to the lowest index; with noise from the standard exponential
+ * distribution it has the probability that the softmax over the candidates
+ * gives it.  noise == NULL, or a temperature that is not positive: the largest
+ * logit.  A NaN or -inf logit is never a candidate; a row with none gives -1.
+ * No counterpart in the reference, which stops at the logits (model.py:23-187).
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  int32_t B, V;
+  const void* logits;                /* [B, V], unit stride along V */
+  int32_t dtype;                     /* OSSM_F32, OSSM_BF16 or OSSM_F16 */
+  int64_t logits_stride;             /* row strides in elements */
+  const float* noise;                /* [B, V] or NULL */
+  int64_t noise_stride;
+  float inv_temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperature_row;      /* [B] on the device or NULL: per-row settings in the scalars' place */
+  const float* top_p_row;
+  const float* min_p_row;
+  const int32_t* top_k_row;
+  int64_t* out;                      /* [B] */
+} ossm_sample_args;
+
+int ossm_sample_tokens(const ossm_sample_args* a, ossm_stream_t stream);
+
 /* Library metadata. */
 const char* ossm_version(void);
 const char* ossm_status_string(int status);
@@ -381,6 +454,8 @@ size_t ossm_sizeof_lion_args(void);
 size_t ossm_sizeof_ttt_args(void);
 size_t ossm_sizeof_bwd_args(void);
 size_t ossm_sizeof_ttt_run_args(void);
+size_t ossm_sizeof_attn_args(void);
+size_t ossm_sizeof_sample_args(void);
 
 #ifdef __cplusplus
 }

@@ -12,6 +12,7 @@ from .sdpc_kernel import (  # noqa: F401
     init_chebyshev_coefficients, ttt_wpred_adam, workspace_status,
 )
 
+from .serving import packed_attention, sample_tokens  # noqa: F401
 from .state import ChebyStreamState, StreamingChebyRKV  # noqa: F401
 
 __version__ = "0.1.0"

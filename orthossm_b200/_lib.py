@@ -12,7 +12,7 @@ import threading
 from . import build as _build
 
 OSSM_OK, OSSM_EINVAL, OSSM_ELAUNCH, OSSM_ETIMEOUT, OSSM_ECOMM, OSSM_EWORKSPACE = range(6)
-OSSM_F32, OSSM_BF16 = 0, 1
+OSSM_F32, OSSM_BF16, OSSM_F16 = 0, 1, 2
 OSSM_EVAL_CLENSHAW, OSSM_EVAL_LUT, OSSM_EVAL_CLENSHAW_DEG4 = 0, 1, 2
 OSSM_F_FASTPATH = 1 << 2
 OSSM_F_PRECISE = 1 << 3
@@ -30,6 +30,8 @@ EXPORTED = (
     "ossm_sizeof_fwd_args", "ossm_sizeof_lion_args", "ossm_sizeof_ttt_args",
     "ossm_ttt_workspace_bytes", "ossm_ttt_wpred_step", "ossm_sizeof_bwd_args", "ossm_bwd_workspace_bytes",
     "ossm_cheby_ema_bwd", "ossm_ttt_run_workspace_bytes", "ossm_ttt_wpred_run", "ossm_sizeof_ttt_run_args",
+    "ossm_attn_workspace_bytes", "ossm_attention_fwd", "ossm_sizeof_attn_args",
+    "ossm_sample_tokens", "ossm_sizeof_sample_args",
 )
 
 _vp = C.c_void_p
@@ -96,6 +98,25 @@ class BwdArgs(C.Structure):
     ]
 
 
+class AttnArgs(C.Structure):
+    _fields_ = [
+        ("B", _i32), ("H", _i32), ("H_kv", _i32), ("head_dim", _i32), ("total_q", _i64), ("total_k", _i64),
+        ("max_seqlen_q", _i32), ("dtype", _i32), ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp),
+        ("q_stride_t", _i64), ("q_stride_h", _i64), ("k_stride_t", _i64), ("k_stride_h", _i64),
+        ("v_stride_t", _i64), ("v_stride_h", _i64), ("out_stride_t", _i64), ("out_stride_h", _i64),
+        ("cu_q", _vp), ("cu_k", _vp), ("kv_len", _vp), ("window", _i32), ("scale", _f32),
+    ]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("B", _i32), ("V", _i32), ("logits", _vp), ("dtype", _i32), ("logits_stride", _i64),
+        ("noise", _vp), ("noise_stride", _i64), ("inv_temperature", _f32), ("top_p", _f32), ("min_p", _f32),
+        ("top_k", _i32), ("temperature_row", _vp), ("top_p_row", _vp), ("min_p_row", _vp), ("top_k_row", _vp),
+        ("out", _vp),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -145,6 +166,16 @@ def _declare(lib):
     lib.ossm_ttt_wpred_run.restype = C.c_int
     lib.ossm_ttt_wpred_run.argtypes = [C.POINTER(TttRunArgs), _vp, C.c_size_t, _vp]
     lib.ossm_sizeof_ttt_run_args.restype = C.c_size_t
+    lib.ossm_attn_workspace_bytes.restype = C.c_size_t
+    lib.ossm_attn_workspace_bytes.argtypes = [C.POINTER(AttnArgs)]
+    lib.ossm_attention_fwd.restype = C.c_int
+    lib.ossm_attention_fwd.argtypes = [C.POINTER(AttnArgs), _vp, C.c_size_t, _vp]
+    lib.ossm_sample_tokens.restype = C.c_int
+    lib.ossm_sample_tokens.argtypes = [C.POINTER(SampleArgs), _vp]
+    lib.ossm_sizeof_attn_args.restype = C.c_size_t
+    lib.ossm_sizeof_sample_args.restype = C.c_size_t
+    if lib.ossm_sizeof_attn_args() != C.sizeof(AttnArgs) or lib.ossm_sizeof_sample_args() != C.sizeof(SampleArgs):
+        raise RuntimeError("orthossm_b200: ctypes struct layout does not match the C ABI")
     if lib.ossm_sizeof_ttt_run_args() != C.sizeof(TttRunArgs):
         raise RuntimeError("orthossm_b200: ctypes struct layout does not match the C ABI")
     if (lib.ossm_sizeof_fwd_args() != C.sizeof(FwdArgs) or lib.ossm_sizeof_lion_args() != C.sizeof(LionArgs)

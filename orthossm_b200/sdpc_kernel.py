@@ -107,12 +107,14 @@ def init_chebyshev_coefficients(batch, n_heads, degree, head_dim, device):
 
 _WS: dict = {}
 _WS_HOST: dict = {}  # host-buffer calls: staging buffers inside, never shared with the others
+_WS_ATTN: dict = {}  # packed_attention: partial sums inside, never shared with the others
 _WS_LOCK = threading.Lock()
 
 
-def _workspace(device, stream, nbytes, host=False):
+def _workspace(device, stream, nbytes, host=False, cache=None):
     key = (device, stream.cuda_stream)
-    cache = _WS_HOST if host else _WS
+    if cache is None:
+        cache = _WS_HOST if host else _WS
     with _WS_LOCK:
         ws = cache.get(key)
         if ws is None or ws.numel() < nbytes:
@@ -127,7 +129,7 @@ def workspace_status(device=None, clear=True):
     3 = a look-back wait timed out).  Synchronises each workspace's stream."""
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     worst = 0
-    for (d, sptr), ws in list(_WS.items()) + list(_WS_HOST.items()):
+    for (d, sptr), ws in list(_WS.items()) + list(_WS_HOST.items()) + list(_WS_ATTN.items()):
         if d != device:
             continue
         st = L._i32(0)

@@ -1,0 +1,256 @@
+"""packed_attention on the GPU against a float64 restatement that looks at the
+seen keys alone (tests/attention_ref.py), at the lengths, masks, layouts and
+values where it can go wrong; every bound is derived there."""
+import pytest
+import torch
+
+import orthossm_b200 as O
+from tests.attention_ref import bound, packed_attention_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def cum(v):
+    return torch.tensor([0] + list(v), device="cuda").cumsum(0).to(torch.int32)
+
+
+def check(out, q, k, v, cu_q, cu_k, **kw):
+    ref, mag, owned = packed_attention_ref(q, k, v, cu_q, cu_k, **kw)
+    got = out.double().cpu()
+    vmax = float(torch.nan_to_num(v, 0.0, 0.0, 0.0).abs().max()) if v.numel() else 0.0
+    lim = bound(ref, mag, q.dtype, k.shape[0], vmax)
+    bad = ((got - ref).abs() > lim) | ~torch.isfinite(got)
+    assert not bool(bad[owned].any()), f"{int(bad[owned].sum())} values off, worst " \
+        f"{float(((got - ref).abs() / lim)[owned].max())} of the bound"
+    return owned
+
+
+def packed(lens, H, Hkv, hd, dtype, seed=0):
+    """q, k, v of self-attending prompts as one projection leaves them."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    T = sum(lens)
+    qkv = torch.randn(T, H + 2 * Hkv, hd, device="cuda", generator=g).to(dtype)
+    return (*qkv.split([H, Hkv, Hkv], 1), cum(lens))
+
+
+HEADS = [(8, 8, 64), (4, 1, 64), (6, 2, 128), (2, 2, 32), (3, 3, 8), (4, 2, 80), (2, 1, 96), (1, 1, 120), (16, 2, 128)]
+
+
+@pytest.mark.parametrize("H,Hkv,hd", HEADS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_packed_prompts(H, Hkv, hd, dtype):
+    """Prompts of lengths around every tile edge, with empty ones between."""
+    lens = [1, 0, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 0, 255, 256, 257, 300, 390]
+    q, k, v, cu = packed(lens, H, Hkv, hd, dtype)
+    out = O.packed_attention(q, k, v, cu, max_seqlen_q=max(lens))
+    check(out, q, k, v, cu, cu)
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 100, 128, 129, 512, 5000])
+@pytest.mark.parametrize("H,Hkv,hd,dtype", [(2, 2, 64, torch.bfloat16), (4, 2, 128, torch.float16)])
+def test_windows(window, H, Hkv, hd, dtype):
+    lens = [1, 130, 700, 257, 1100]
+    q, k, v, cu = packed(lens, H, Hkv, hd, dtype, seed=window)
+    out = O.packed_attention(q, k, v, cu, max_seqlen_q=max(lens), window=window)
+    check(out, q, k, v, cu, cu, window=window)
+
+
+# (queries, keys) of each sequence: tokens and pieces against longer caches, no keys at all, more queries than keys
+# (the first queries then see nothing), no queries
+PAIRS = [
+    [(1, 1)], [(1, 0)], [(1, 1), (1, 17), (1, 0), (1, 1000), (1, 128)], [(1, 5000)],
+    [(2, 2), (3, 100), (5, 3), (0, 50), (4, 64), (2, 1500)], [(16, 16), (16, 1000), (7, 2), (17, 40)],
+    [(64, 3000), (1, 10), (33, 33)], [(200, 100), (130, 1), (5, 0)], [(300, 900), (128, 2000), (1, 1500)],
+    [(100, 4000)],
+]
+
+
+@pytest.mark.parametrize("pairs", PAIRS, ids=lambda p: "_".join(f"{a}x{b}" for a, b in p))
+@pytest.mark.parametrize("H,Hkv,hd,dtype", [(8, 8, 64, torch.bfloat16), (8, 1, 128, torch.bfloat16),
+                                            (6, 2, 64, torch.float16), (24, 1, 32, torch.float16),
+                                            (2, 2, 80, torch.bfloat16)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_against_a_cache(pairs, H, Hkv, hd, dtype, window):
+    """Queries against a cache with room left: NaN and infinities in the free
+    slots, in front of the first sequence and behind the last must not matter."""
+    g = torch.Generator(device="cuda").manual_seed(len(pairs))
+    slots = max(b for _, b in pairs) + 37
+    n = len(pairs)
+    q = torch.randn(sum(a for a, _ in pairs), H, hd, device="cuda", generator=g).to(dtype)
+    k, v = (torch.randn(n, slots, Hkv, hd, device="cuda", generator=g).to(dtype) for _ in range(2))
+    for b, (_, nk) in enumerate(pairs):
+        k[b, nk:] = float("nan")
+        v[b, nk:] = float("inf") if b % 2 else float("nan")
+    k, v = k.view(n * slots, Hkv, hd), v.view(n * slots, Hkv, hd)
+    cu_q, cu_k = cum(a for a, _ in pairs), cum([slots] * n)
+    kv = torch.tensor([b for _, b in pairs], device="cuda", dtype=torch.int32)
+    out = O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=max(a for a, _ in pairs), kv_lengths=kv, window=window)
+    check(out, q, k, v, cu_q, cu_k, kv_lengths=kv, window=window)
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq,nk", [(400, 400), (3, 300), (140, 700)])
+def test_hidden_values_do_not_matter(what, hd, nq, nk):
+    """Non-finite keys and values inside the sequence reach the queries that
+    see them and no others: ahead of the query, and behind its window."""
+    dtype, H, W = torch.bfloat16, 2, 150
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(nq, H, hd, device="cuda", generator=g).to(dtype)
+    k, v = (torch.randn(nk, H, hd, device="cuda", generator=g).to(dtype) for _ in range(2))
+    clean_k, clean_v = k.clone(), v.clone()
+    cu_q, cu_k = cum([nq]), cum([nk])
+    places = [nk - 1, nk - 2, max(0, nk - 170), 5]
+    for j in places:
+        v[j, 0, 3], v[j, 1, hd - 1] = what, what
+    k[nk - 1, 0, 0] = what
+    out = O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq, window=W)
+    ref, mag, _ = packed_attention_ref(q, clean_k, clean_v, cu_q, cu_k, window=W)
+    at = torch.arange(nq) + nk - nq
+    seen = torch.stack([(at >= j) & (at - j < W) for j in places]).any(0)
+    blind = ~seen
+    assert int(blind.sum()) > 0 or nq < 10
+    got, lim = out.double().cpu(), bound(ref, mag, dtype, nk, 6.0)
+    assert bool(((got - ref).abs() <= lim)[blind].all())
+    # the other channels of a query that sees a bad value are not touched by it
+    body = torch.ones(H, hd, dtype=torch.bool)
+    body[0], body[1, hd - 1] = False, False
+    assert bool(((got - ref).abs() <= lim)[:, body].all())
+    # a seen value arrives: channel hd - 1 of head 1 (finite weights)
+    if what == what:
+        assert bool((got[seen][:, 1, hd - 1] == what).all())
+    else:
+        assert bool(got[seen][:, 1, hd - 1].isnan().all())
+
+
+@pytest.mark.parametrize("nq,nk", [(1, 300), (200, 300)])
+def test_layouts(nq, nk):
+    """Head-major tensors, odd strides (copied), a shared head of stride zero, a given output with gaps."""
+    H, hd, dtype = 4, 64, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(9)
+    mk = lambda *s: torch.randn(*s, device="cuda", generator=g).to(dtype)  # noqa: E731
+    cu_q, cu_k = cum([nq]), cum([nk])
+    q = mk(H, nq, hd).transpose(0, 1)
+    k = mk(H, nk, hd).transpose(0, 1)
+    v = mk(nk, H, hd + 1)[..., 1:]          # rows not 16-byte aligned
+    out = torch.full((nq, H + 1, hd), 7.0, device="cuda", dtype=dtype)
+    got = O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq, out=out[:, :H])
+    assert got.data_ptr() == out.data_ptr()
+    check(got, q, k, v, cu_q, cu_k)
+    assert bool((out[:, H] == 7.0).all())
+    k1 = mk(nk, 1, hd).expand(nk, H, hd)
+    check(O.packed_attention(q, k1, v, cu_q, cu_k, max_seqlen_q=nq), q, k1, v, cu_q, cu_k)
+
+
+@pytest.mark.parametrize("nq", [1, 150])
+def test_rows_outside_the_sequences_are_left_alone(nq):
+    H, hd = 2, 64
+    q, k, v = (torch.randn(nq + 40, H, hd, device="cuda").to(torch.bfloat16) for _ in range(3))
+    cu = torch.tensor([20, 20 + nq], device="cuda", dtype=torch.int32)
+    out = torch.full_like(q, 3.0)
+    O.packed_attention(q, k, v, cu, max_seqlen_q=nq, out=out)
+    owned = check(out, q, k, v, cu, cu)
+    assert bool((out[~owned.cuda()] == 3.0).all())
+
+
+@pytest.mark.parametrize("nq", [1, 300])
+def test_large_scores_and_scale(nq):
+    """Scores of several hundred: the running maximum has to carry them; a
+    scale of its own."""
+    H, hd, nk, dtype = 2, 64, 700, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randn(nq, H, hd, device="cuda", generator=g)
+    k = torch.randn(nk, H, hd, device="cuda", generator=g)
+    k = k + q[-1] * torch.linspace(-1, 1, nk, device="cuda")[:, None, None]  # a maximum that rises along the keys
+    q, k = (q * 4).to(dtype), (k * 2).to(dtype)
+    v = torch.randn(nk, H, hd, device="cuda", generator=g).to(dtype)
+    cu_q, cu_k = cum([nq]), cum([nk])
+    out = O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq, scale=0.25)
+    check(out, q, k, v, cu_q, cu_k, scale=0.25)
+
+
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^32 bytes and 2^31 elements, read at its end."""
+    H, hd, slots, n = 4, 128, 1 << 20, 5
+    k, v = (torch.empty(n * slots, H, hd, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    L0, tail = 700, (n - 1) * slots
+    for t in (k, v):
+        t[tail:tail + L0] = torch.randn(L0, H, hd, device="cuda").to(torch.bfloat16)
+    kv = torch.tensor([0] * (n - 1) + [L0], device="cuda", dtype=torch.int32)
+    for nq in (1, 200):
+        q = torch.randn(nq, H, hd, device="cuda").to(torch.bfloat16)
+        cu_q, cu_k = cum([0] * (n - 1) + [nq]), cum([slots] * n)
+        out = O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq, kv_lengths=kv)
+        small = torch.tensor([0, L0], dtype=torch.int32)
+        check(out, q, k[tail:tail + L0], v[tail:tail + L0], cum([nq]), small)
+
+
+@pytest.mark.parametrize("n", [1, 1000])
+def test_many_sequences(n):
+    lens = [(i * 7) % 5 for i in range(n)]
+    q, k, v, cu = packed(lens, 2, 1, 64, torch.bfloat16)
+    if sum(lens) == 0:
+        assert O.packed_attention(q, k, v, cu, max_seqlen_q=1).shape == q.shape
+        return
+    check(O.packed_attention(q, k, v, cu, max_seqlen_q=max(lens)), q, k, v, cu, cu)
+    kv = torch.tensor([min(x, 2) for x in lens], device="cuda", dtype=torch.int32)
+    check(O.packed_attention(q, k, v, cu, max_seqlen_q=max(lens), kv_lengths=kv), q, k, v, cu, cu, kv_lengths=kv)
+
+
+@pytest.mark.parametrize("nq,nk", [(1, 3000), (260, 900)])
+def test_repeats_streams_and_graphs(nq, nk):
+    """Bitwise the same on repeated calls, on a side stream and replayed from a
+    graph on new inputs (nothing is kept from one call for the next)."""
+    H, hd = 4, 64
+    mk = lambda t: torch.randn(t, H, hd, device="cuda").to(torch.bfloat16)  # noqa: E731
+    cu_q, cu_k = cum([nq, nq]), cum([nk, nk // 2])
+    q, k, v = mk(2 * nq), mk(nk + nk // 2), mk(nk + nk // 2)
+    call = lambda o=None: O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq, out=o)  # noqa: E731
+    first = call()
+    assert all(torch.equal(first, call()) for _ in range(3))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = call()
+        out = torch.empty_like(first)
+        call(out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            call(out)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(first, other)
+    for t in (q, k, v):
+        t.copy_(torch.randn_like(t))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, call())
+    check(out, q, k, v, cu_q, cu_k)
+    assert O.workspace_status() == 0
+
+
+def test_refusals():
+    q = torch.zeros(4, 4, 64, device="cuda", dtype=torch.bfloat16)
+    k = torch.zeros(4, 2, 64, device="cuda", dtype=torch.bfloat16)
+    cu = cum([4])
+    ok = dict(max_seqlen_q=4)
+    f = O.packed_attention
+    for bad in [lambda: f(q.float(), k.float(), k.float(), cu, **ok), lambda: f(q, k.half(), k, cu, **ok),
+                lambda: f(q, k, k[:, :1], cu, **ok), lambda: f(q[:, :3], k, k, cu, **ok),
+                lambda: f(q[..., :60], k[..., :60], k[..., :60], cu, **ok),
+                lambda: f(q[0], k, k, cu, **ok), lambda: f(q, k, k, cu.long(), **ok),
+                lambda: f(q, k, k, cu, cu[:1], **ok), lambda: f(q, k, k, cu, window=0, **ok),
+                lambda: f(q, k, k, cu, scale=-1.0, **ok), lambda: f(q, k, k, cu, scale=float("inf"), **ok),
+                lambda: f(q, k, k, cu, kv_lengths=cu, **ok), lambda: f(q, k, k, cu, out=q[:2], **ok),
+                lambda: f(q, k, k, cu[:1], **ok),
+                lambda: f(torch.zeros(4, 4, 136, device="cuda", dtype=torch.bfloat16),
+                          torch.zeros(4, 4, 136, device="cuda", dtype=torch.bfloat16),
+                          torch.zeros(4, 4, 136, device="cuda", dtype=torch.bfloat16), cu, **ok)]:
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        f(q.cpu(), k, k, cu, **ok)
+    with pytest.raises(NotImplementedError):
+        f(q.requires_grad_(), k, k, cu, **ok)
+    with torch.no_grad():
+        f(q, k, k, cu, **ok)
