@@ -1,0 +1,79 @@
+// What the attention kernels share: arguments, a sequence's rows, types.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "orthossm_b200.h"
+#include "ossm_common.cuh"
+
+namespace ossm {
+namespace attn {
+
+constexpr int kMaxSeqs = 16384;
+constexpr int kMaxHD = 128;
+constexpr long long kMaxRows = 1LL << 30;  // positions and their differences stay within 32 bits
+
+struct Params {
+  int B, H, Hkv, hd;
+  int Tq, Tk;
+  const void *q, *k, *v;
+  void* out;
+  long long qst, qsh, kst, ksh, vst, vsh, ost, osh;
+  const int *cu_q, *cu_k, *kv_len;
+  int window;      // 0: none
+  float scale2;    // scale * log2(e): the softmax runs on base-2 exponents
+  WsHeader* hdr;
+  uint32_t* counts;  // per CTA: progress of the item that its last piece belongs to (0 between calls)
+  float* part;       // per CTA two partial results
+};
+
+// The rows of sequence b, clipped to the tensors.
+struct Seq {
+  int q0, nq, k0, nk;
+};
+OSSM_DEV Seq seq_of(const Params& p, int b) {
+  Seq s;
+  s.q0 = min(max(__ldg(p.cu_q + b), 0), p.Tq);
+  s.nq = min(max(__ldg(p.cu_q + b + 1), s.q0), p.Tq) - s.q0;
+  s.k0 = min(max(__ldg(p.cu_k + b), 0), p.Tk);
+  s.nk = min(max(__ldg(p.cu_k + b + 1), s.k0), p.Tk) - s.k0;
+  if (p.kv_len) s.nk = min(s.nk, max(__ldg(p.kv_len + b), 0));
+  return s;
+}
+
+template <typename T>
+OSSM_DEV float2 to_f2(uint32_t u);
+template <>
+OSSM_DEV float2 to_f2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <>
+OSSM_DEV float2 to_f2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<__half2*>(&u));
+}
+template <typename T>
+OSSM_DEV uint32_t pack2(float lo, float hi);
+template <>
+OSSM_DEV uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <>
+OSSM_DEV uint32_t pack2<__half>(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+// An infinity or NaN in either half of a packed pair.
+template <typename T>
+OSSM_DEV bool nonfinite2(uint32_t u) {
+  constexpr uint32_t e = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (u & e) == e || (u & (e << 16)) == (e << 16);
+}
+
+OSSM_DEV float ex2(float x) {  // 2^x, relative error 2^-22
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace attn
+}  // namespace ossm

@@ -1,0 +1,823 @@
+// Attention of many queries a sequence: prompts, pieces of prompts.
+//
+// Work item: two tiles of 128 query rows that share their keys: the same 128
+// queries of two neighbouring heads of a group (an even number of query heads
+// per key head), or 256 queries of one head.  An item walks its range of
+// 128-key tiles once with a running maximum and sum per row.
+//
+// One persistent CTA per SM, 11 warps:
+//   warps 0-3, 4-7  softmax of tile 0 / 1: a thread owns a row.  Scores from
+//                   tensor memory, mask, maximum, exponentials, weights back
+//                   to tensor memory over the scores; at the end the output
+//                   row out of the accumulator.
+//   warp 8          issues every tcgen05.mma: S_t = Q_t K^T (both operands in
+//                   shared memory) and O_t += P_t V (P_t in tensor memory, V
+//                   read MN-major, so it is never transposed).
+//   warp 9          walks the schedule, loads Q, K and V tiles by TMA.
+//   warp 10         looks through V tiles that some row does not see whole:
+//                   rows past the sequence are zeroed (a weight of 0 times
+//                   NaN would be NaN); if a seen row holds a non-finite value,
+//                   the softmax threads take that tile's product with the
+//                   seen rows alone instead of the tensor core.
+// Tensor memory: S_0 S_1 (128 columns each, P_t over S_t), O_0 O_1.  While
+// one tile's softmax runs, the tensor core works for the other.
+//
+// The maximum that the exponents are taken against follows the true one only
+// when a row has grown by more than 2^8 since: the weights then stay below
+// 2^8 and the accumulator is rescaled in a few tiles of a row instead of all.
+//
+// Schedule: the items of all sequences in one line, an item as long as its
+// number of key tiles plus kItemCost; the line is cut into equal parts, one a
+// CTA, so that causal masks and ragged lengths balance whatever they are.  A
+// cut near an item's edge moves to the edge; an item that stays cut leaves
+// partial sums in the workspace, and whichever CTA finishes it last joins
+// them, in the order of the cut.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "ossm_attn.cuh"
+#include "ossm_sm100.cuh"
+
+namespace ossm {
+namespace fast {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
+}
+namespace attn {
+
+using namespace sm100;
+
+constexpr int kT = 128;             // query rows and keys of a tile
+constexpr int kThreads = 352;
+constexpr int kGroups = 1024;       // entries of the schedule's prefix in shared memory
+constexpr int kItemCost = 2;        // an item's start and end, in key tiles
+constexpr int kMinPiece = 6;        // no cut closer to an item's edge
+constexpr int kBox = kT * 128;      // bytes of a [128 rows x 64 channels] box
+
+// ---------------------------------------------------------------- schedule
+typedef long long i64;
+
+OSSM_DEV int floor_div(int a, int b) { return a >= 0 ? a / b : -((b - 1 - a) / b); }
+OSSM_DEV int ceil_div(int a, int b) { return -floor_div(-a, b); }
+
+// sum over i < n of max(0, a + s i)
+OSSM_DEV i64 ramp(int n, int a, int s) {
+  const int i0 = a >= 0 ? 0 : (-a + s - 1) / s;
+  const i64 c = max(0, n - i0);
+  return c * a + (i64)s * (c * i0 + c * (c - 1) / 2);
+}
+
+// A sequence's blocks of s * 128 query rows: block i walks key tiles
+// [max(0, b + i s), min(max(0, a + (i + 1) s), t)).
+struct Shape {
+  int nblk, a, b, t, s;
+  OSSM_DEV int lo(int i) const { return max(0, b + i * s); }
+  OSSM_DEV int hi(int i) const { return min(max(0, a + (i + 1) * s), t); }
+  OSSM_DEV i64 before(int i) const {  // length of the blocks before i
+    return ramp(i, a + s, s) - ramp(i, a + s - t, s) - ramp(i, b, s) + (i64)i * kItemCost;
+  }
+};
+OSSM_DEV Shape shape_of(const Params& p, const Seq& q, int s) {
+  const int off = q.nk - q.nq;
+  Shape f;
+  f.s = s;
+  f.nblk = (q.nq + s * kT - 1) / (s * kT);
+  f.a = ceil_div(off, kT);
+  f.t = (q.nk + kT - 1) / kT;
+  // no window: the lower edge stays at 0 for every block
+  f.b = p.window ? floor_div(off - p.window + 1, kT) : -(f.nblk * s + 1);
+  return f;
+}
+
+struct Sched {
+  const Params& p;
+  const i64* pre;  // [ngroups + 1] length of the line before each group of sequences
+  int ngroups, gsz, s, units;
+  i64 total;
+  int ncta;
+
+  struct Item {
+    Seq q;
+    Shape f;
+    int unit, blk;
+    i64 start;  // on the line
+    OSSM_DEV int n() const { return f.hi(blk) - f.lo(blk); }
+    OSSM_DEV i64 end() const { return start + n() + kItemCost; }
+  };
+
+  // The item at a position of the line (0 <= pos < total).
+  OSSM_DEV Item at(i64 pos) const {
+    int lo = 0, hi = ngroups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= pos) lo = mid; else hi = mid;
+    }
+    i64 base = pre[lo];
+    Item it;
+    i64 one = 0;
+    for (int b = lo * gsz;; ++b) {
+      it.q = seq_of(p, b);
+      it.f = shape_of(p, it.q, s);
+      one = it.f.before(it.f.nblk);
+      if (pos < base + one * units || b + 1 >= min(p.B, (lo + 1) * gsz)) break;
+      base += one * units;
+    }
+    it.unit = (int)((pos - base) / one);
+    base += it.unit * one;
+    const i64 rel = pos - base;
+    lo = 0, hi = it.f.nblk;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (it.f.before(mid) <= rel) lo = mid; else hi = mid;
+    }
+    it.blk = lo;
+    it.start = base + it.f.before(lo);
+    return it;
+  }
+  // Where CTA c's part begins.
+  OSSM_DEV i64 cut(int c) const {
+    if (c <= 0) return 0;
+    if (c >= ncta) return total;
+    const i64 pos = total / ncta * c + total % ncta * c / ncta;
+    const Item it = at(pos);
+    const i64 near = max((i64)kMinPiece, total / ncta / 16);
+    if (pos - it.start <= near && pos - it.start <= it.end() - pos) return it.start;
+    if (it.end() - pos <= near + kItemCost) return it.end();
+    return pos - it.start <= near ? it.start : pos;
+  }
+};
+
+// A CTA's share of one item, as the roles read it.
+struct Piece {
+  int live;                // 0: no more pieces
+  int q0, nq, off, k0, nk; // the sequence
+  int head[2], row0[2];    // of the two tiles; row0: first row in the sequence
+  int j0, j1;              // the piece's key tiles
+  int lo[2], hi[2];        // each tile's share of them
+  int split;               // the item has other pieces
+  int slot, first, len;    // split: this piece's slot, the CTA with the item's first piece, the item's key tiles
+  i64 start;               // split: the item's start on the line
+};
+
+struct Bars {
+  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2];
+  uint64_t piece_full[2], piece_empty[2];
+  uint64_t kv_full[8], kv_empty[8], v_clean[8];
+};
+
+template <int HDP>
+struct Cfg {
+  static constexpr int kBoxes = HDP / 64;
+  static constexpr int kTile = kBoxes * kBox;
+  static constexpr int kSlots = HDP == 64 ? 8 : 4;
+  static constexpr size_t kSmem = (2 + kSlots) * (size_t)kTile + 1024;
+  static constexpr uint32_t kCols = 512;
+  static constexpr uint32_t kO = 256;  // first column of O_0
+  static constexpr size_t kPartFloats = 2 * kT * (size_t)(HDP + 2);
+};
+
+// Instruction descriptor: fp32 accumulator, 16-bit operands (format 0 = fp16,
+// 1 = bf16), bit 16 = B is MN-major, N/8 from bit 17, M/16 from bit 24.
+__host__ __device__ constexpr uint32_t idesc(int fmt, int n, int b_mn) {
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kT >> 4) << 24);
+}
+// Shared-memory descriptors, 128-byte swizzle.  K-major (Q, K): 8-row groups
+// 1024 bytes apart.  MN-major (V): 8-key groups 1024 bytes apart (stride
+// offset), the next 64 channels a box further (leading offset).
+OSSM_DEV uint64_t sdesc(uint32_t saddr, uint32_t lead) {
+  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+OSSM_DEV void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(ad), "l"(bd), "r"(id), "r"(acc)
+      : "memory");
+}
+OSSM_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t bd, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(bd), "r"(id), "r"(acc)
+      : "memory");
+}
+OSSM_DEV void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// 32 columns of this thread's lane, without the wait.
+OSSM_DEV void tmem_ld32_nowait(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+// Orders uses of v after the wait before it (the load's registers are not
+// valid until then, which the compiler cannot know).
+OSSM_DEV void pin32(float* v) {
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                    "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]));
+  asm volatile("" : "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+                    "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]));
+  asm volatile("" : "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
+}
+OSSM_DEV void tmem_st32(uint32_t taddr, const float* v) {
+  uint32_t u[16];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i]);
+    tmem_st16(taddr + 16 * h, u);
+  }
+}
+
+// Does some row of tile t miss a key of tile j?
+OSSM_DEV bool partly(const Params& p, const Piece& c, int t, int j) {
+  const int first = c.row0[t] + c.off, last = min(c.row0[t] + kT, c.nq) - 1 + c.off;
+  return j * kT + kT - 1 > first || (p.window && j * kT <= last - p.window);
+}
+
+struct Failed {
+  int* flag;
+  OSSM_DEV bool operator()(uint64_t* bar, uint32_t parity) const {  // true: give up
+    if (mbar_wait(bar, parity)) return false;
+    *flag = 1;
+    return true;
+  }
+};
+
+template <typename T, int HDP>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_prompt_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
+                       const __grid_constant__ CUtensorMap mV, const __grid_constant__ Params p, const int pair_heads) {
+  using C = Cfg<HDP>;
+  constexpr int NS = C::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* ring = smem + 2 * C::kTile;
+  __shared__ Bars bars;
+  __shared__ Piece pieces[2];
+  __shared__ i64 pre[kGroups + 1];
+  __shared__ int vflag[NS];
+  __shared__ uint32_t tslot;
+  __shared__ int failed, last_in;
+  __shared__ unsigned long long n_items;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+
+  // ------------------------------------------------------------ schedule
+  const int gsz = (p.B + kGroups - 1) / kGroups, ngroups = (p.B + gsz - 1) / gsz;
+  const int s = pair_heads ? 1 : 2, units = pair_heads ? p.H / 2 : p.H;
+  if (threadIdx.x == 0) {
+    n_items = 0;
+    failed = 0;
+  }
+  __syncthreads();
+  unsigned long long mine = 0;
+  for (int g = threadIdx.x; g < ngroups; g += kThreads) {
+    i64 len = 0;
+    for (int b = g * gsz; b < min(p.B, (g + 1) * gsz); ++b) {
+      const Shape f = shape_of(p, seq_of(p, b), s);
+      len += f.before(f.nblk) * units;
+      mine += (unsigned long long)f.nblk * units;
+    }
+    pre[g + 1] = len;
+  }
+  if (mine) atomicAdd(&n_items, mine);
+  __syncthreads();
+  if (warp == 0) {  // prefix sums, 32 groups at a time
+    i64 run = 0;
+    for (int g0 = 0; g0 < ngroups; g0 += 32) {
+      i64 v = g0 + lane < ngroups ? pre[g0 + lane + 1] : 0;
+#pragma unroll
+      for (int w = 1; w < 32; w *= 2) {
+        const i64 u = __shfl_up_sync(~0u, v, w);
+        if (lane >= w) v += u;
+      }
+      if (g0 + lane < ngroups) pre[g0 + lane + 1] = run + v;
+      run += __shfl_sync(~0u, v, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+  }
+  __syncthreads();
+  Sched sc{p, pre, ngroups, gsz, s, units, pre[ngroups], 0};
+  // as many CTAs as there are items or pieces of 8 key tiles
+  sc.ncta = (int)min((i64)gridDim.x, max((i64)n_items, sc.total / 8));
+  if (cta >= sc.ncta) return;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bars.q_full[t], 1);
+      mbar_init(&bars.q_empty[t], 1);
+      mbar_init(&bars.s_full[t], 1);
+      mbar_init(&bars.p_ready[t], 4);
+      mbar_init(&bars.o_full[t], 1);
+      mbar_init(&bars.piece_full[t], 1);
+      mbar_init(&bars.piece_empty[t], 10);
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&bars.kv_full[i], 1);
+      mbar_init(&bars.kv_empty[i], 1);
+      mbar_init(&bars.v_clean[i], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 8) tmem_alloc(&tslot, C::kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tslot;
+  const Failed gave_up{&failed};
+
+  if (warp == 9) {
+    // ---------------------------------------------------------- schedule and loads
+    if (lane == 0) {
+      prefetch_tmap(&mQ);
+      prefetch_tmap(&mK);
+      prefetch_tmap(&mV);
+      const i64 end = sc.cut(cta + 1);
+      i64 pos = sc.cut(cta);
+      int n = 0, nq[2] = {0, 0};
+      uint32_t it = 0;
+      bool ok = true;
+      for (;; ++n) {
+        Piece c;
+        c.live = 0;
+        while (pos < end) {  // the next piece with work
+          const Sched::Item x = sc.at(pos);
+          const int a = (int)min(pos - x.start, (i64)x.n()), b = (int)min(end - x.start, (i64)x.n());
+          const bool head = pos == x.start;
+          pos = min(end, x.end());
+          if (a >= b && !(head && x.n() == 0)) continue;
+          c.live = 1;
+          c.q0 = x.q.q0, c.nq = x.q.nq, c.k0 = x.q.k0, c.nk = x.q.nk, c.off = x.q.nk - x.q.nq;
+          const int base = x.f.lo(x.blk);
+          c.j0 = base + a, c.j1 = base + b;
+          for (int t = 0; t < 2; ++t) {
+            c.head[t] = pair_heads ? 2 * x.unit + t : x.unit;
+            c.row0[t] = pair_heads ? x.blk * kT : (2 * x.blk + t) * kT;
+            const int first = c.row0[t] + c.off, top = min(c.row0[t] + kT, c.nq) - 1 + c.off;
+            int lo = p.window ? max(0, first - p.window + 1) / kT : 0, hi = top < 0 ? 0 : top / kT + 1;
+            if (c.row0[t] >= c.nq) hi = lo = 0;
+            c.lo[t] = max(lo, c.j0);
+            c.hi[t] = max(c.lo[t], min(hi, c.j1));
+          }
+          c.split = b - a < x.n();
+          if (c.split) {
+            c.len = x.n();
+            c.start = x.start;
+            c.slot = head ? 2 * cta + 1 : 2 * cta;
+            int f = cta;
+            while (f > 0 && sc.cut(f) > x.start) --f;
+            c.first = f;
+          }
+          break;
+        }
+        const int sl = n & 1;
+        if (n >= 2 && gave_up(&bars.piece_empty[sl], ((n >> 1) & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        pieces[sl] = c;
+        mbar_arrive(&bars.piece_full[sl]);
+        if (!c.live) break;
+        for (int j = c.j0; j < c.j1 && ok; ++j) {
+          if (j == c.j0)
+            for (int t = 0; t < 2; ++t) {
+              if (c.lo[t] >= c.hi[t]) continue;
+              if (nq[t] && gave_up(&bars.q_empty[t], (nq[t] & 1) ^ 1)) {
+                ok = false;
+                break;
+              }
+              ++nq[t];
+              mbar_expect_tx(&bars.q_full[t], C::kTile);
+              for (int x = 0; x < C::kBoxes; ++x)
+                tma_load_3d(smem + t * C::kTile + x * kBox, &mQ, &bars.q_full[t], 64 * x, c.head[t], c.q0 + c.row0[t]);
+            }
+          for (int kv = 0; kv < 2 && ok; ++kv, ++it) {
+            const int r = it % NS;
+            if (it >= NS && gave_up(&bars.kv_empty[r], ((it / NS) & 1) ^ 1)) {
+              ok = false;
+              break;
+            }
+            mbar_expect_tx(&bars.kv_full[r], C::kTile);
+            for (int x = 0; x < C::kBoxes; ++x)
+              tma_load_3d(ring + r * C::kTile + x * kBox, kv ? &mV : &mK, &bars.kv_full[r], 64 * x,
+                          c.head[0] / (p.H / p.Hkv), c.k0 + j * kT);
+          }
+        }
+        if (!ok) break;
+      }
+      if (!ok) {  // no copy may still be landing when the CTA exits
+        for (int t = 0; t < 2; ++t)
+          if (nq[t]) gave_up(&bars.q_full[t], (nq[t] & 1) ^ 1);
+        for (uint32_t i = it > NS ? it - NS : 0; i < it; ++i) gave_up(&bars.kv_full[i % NS], (i / NS) & 1);
+      }
+    }
+  } else if (warp == 8) {
+    // ---------------------------------------------------------- products
+    constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
+    constexpr uint32_t id_s = idesc(fmt, kT, 0), id_o = idesc(fmt, HDP, 1);
+    if (lane == 0) {
+      uint32_t it = 0, nq[2] = {0, 0}, np[2] = {0, 0};
+      bool ok = true;
+      const int ksteps = (p.hd + 15) / 16;
+      for (int n = 0; ok; ++n) {
+        const int sl = n & 1;
+        if (gave_up(&bars.piece_full[sl], (n >> 1) & 1)) break;
+        const Piece& c = pieces[sl];
+        if (!c.live) break;
+        const int j0 = c.j0, j1 = c.j1;
+        int lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
+        mbar_arrive(&bars.piece_empty[sl]);
+        // S_t = Q_t K_j^T for the tiles that walk j, K_j in ring slot it + 2 (j - j0)
+        auto scores = [&](int t, int j) {
+          if (j < lo[t] || j >= hi[t]) return true;
+          if (j == lo[t] && gave_up(&bars.q_full[t], nq[t]++ & 1)) return false;
+          const uint32_t r = it + 2 * (j - j0);
+          if (gave_up(&bars.kv_full[r % NS], (r / NS) & 1)) return false;
+          tc_fence_after();
+          const uint32_t a = smem_u32(smem + t * C::kTile), b = smem_u32(ring + (r % NS) * C::kTile);
+          for (int kk = 0; kk < ksteps; ++kk) {
+            const uint32_t o = (kk >> 2) * kBox + (kk & 3) * 32;
+            mma_ss(tmem + t * kT, sdesc(a + o, 16), sdesc(b + o, 16), id_s, kk > 0);
+          }
+          mma_commit(&bars.s_full[t]);
+          if (j == hi[t] - 1) mma_commit(&bars.q_empty[t]);
+          return true;
+        };
+        if (j0 < j1) {
+          ok = scores(0, j0) && scores(1, j0);
+          mma_commit(&bars.kv_empty[it % NS]);
+        }
+        for (int j = j0; j < j1 && ok; ++j) {
+          const uint32_t rv = it + 2 * (j - j0) + 1;
+          if (gave_up(&bars.v_clean[rv % NS], (rv / NS) & 1)) {
+            ok = false;
+            break;
+          }
+          if (gave_up(&bars.kv_full[rv % NS], (rv / NS) & 1)) {  // passed already; orders the copy before the products
+            ok = false;
+            break;
+          }
+          const bool skip = *(volatile int*)&vflag[rv % NS];
+          const uint32_t vb = smem_u32(ring + (rv % NS) * C::kTile);
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (j >= lo[t] && j < hi[t]) {
+              if (gave_up(&bars.p_ready[t], np[t]++ & 1)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              if (!skip)
+                for (int kk = 0; kk < kT / 16; ++kk)
+                  mma_ts(tmem + C::kO + t * HDP, tmem + t * kT + kk * 8, sdesc(vb + kk * 2048, kBox), id_o,
+                         kk > 0 || j > lo[t]);
+              if (j == hi[t] - 1) mma_commit(&bars.o_full[t]);
+            }
+            if (j + 1 < j1) ok = scores(t, j + 1);
+          }
+          mma_commit(&bars.kv_empty[rv % NS]);
+          if (j + 1 < j1) mma_commit(&bars.kv_empty[(rv + 1) % NS]);
+        }
+        it += 2 * (j1 - j0);
+      }
+      if (!ok) failed = 1;
+    }
+  } else if (warp == 10) {
+    // ---------------------------------------------------------- V tiles that are not seen whole
+    uint32_t it = 0;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const int sl = n & 1;
+      if (__any_sync(~0u, gave_up(&bars.piece_full[sl], (n >> 1) & 1))) break;
+      const Piece& c = pieces[sl];
+      if (!c.live) break;
+      for (int j = c.j0; j < c.j1; ++j) {
+        const uint32_t r = it + 2 * (j - c.j0) + 1;
+        if (__any_sync(~0u, gave_up(&bars.kv_full[r % NS], (r / NS) & 1))) {
+          ok = false;
+          break;
+        }
+        bool bad = false;
+        if ((j >= c.lo[0] && j < c.hi[0] && partly(p, c, 0, j)) || (j >= c.lo[1] && j < c.hi[1] && partly(p, c, 1, j))) {
+          const int rows = min(kT, c.nk - j * kT);
+          uint4* v = reinterpret_cast<uint4*>(ring + (r % NS) * C::kTile);
+          for (int x = 0; x < C::kBoxes; ++x) {
+#pragma unroll 8
+            for (int i = lane; i < kT * 8; i += 32) {
+              if ((i >> 3) < rows) {
+                const uint4 u = v[x * (kBox / 16) + i];
+                bad |= nonfinite2<T>(u.x) || nonfinite2<T>(u.y) || nonfinite2<T>(u.z) || nonfinite2<T>(u.w);
+              } else {
+                v[x * (kBox / 16) + i] = make_uint4(0, 0, 0, 0);
+              }
+            }
+          }
+          fence_proxy_async_smem();  // the zeros, before the tensor core reads them
+          bad = __any_sync(~0u, bad);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          vflag[r % NS] = bad;
+          mbar_arrive(&bars.v_clean[r % NS]);
+        }
+      }
+      it += 2 * (c.j1 - c.j0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
+    }
+  } else {
+    // ---------------------------------------------------------- softmax and output
+    const int t = warp >> 2, row = threadIdx.x & (kT - 1);
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), tS = tl + t * kT, tO = tl + C::kO + t * HDP;
+    uint32_t ns = 0, no = 0, it = 0;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const int sl = n & 1;
+      if (__any_sync(~0u, gave_up(&bars.piece_full[sl], (n >> 1) & 1))) break;
+      const Piece c = pieces[sl];
+      if (!c.live) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
+      const int lo = c.lo[t], hi = c.hi[t];
+      const int at = c.row0[t] + row + c.off;  // the row's position
+      float m = -INFINITY, l = 0.f;
+      for (int j = lo; j < hi; ++j) {
+        if (__any_sync(~0u, gave_up(&bars.s_full[t], ns & 1))) {
+          ok = false;
+          break;
+        }
+        ++ns;
+        tc_fence_after();
+        float x[kT];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld32_nowait(tS + 32 * i, x + 32 * i);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pin32(x + 32 * i);
+        const bool part = partly(p, c, t, j);
+        const int k_hi = at - j * kT, k_lo = p.window ? k_hi - p.window + 1 : -1;  // seen: k_lo <= key <= k_hi
+        if (part) {
+#pragma unroll
+          for (int i = 0; i < kT; ++i)
+            if (i > k_hi || i < k_lo) x[i] = -INFINITY;
+        }
+        float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int i = 4; i < kT; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
+        const bool grow = top > m + 8.f;
+        if (__any_sync(~0u, grow)) {
+          const float mn = grow ? top : m;
+          const float f = grow ? ex2(m - mn) : 1.f;
+          m = mn;
+          l *= f;
+          if (j > lo) {
+#pragma unroll 1
+            for (int i = 0; i < HDP / 32; ++i) {
+              float o[32];
+              tmem_ld32_nowait(tO + 32 * i, o);
+              tmem_wait_ld();
+              pin32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= f;
+              tmem_st32(tO + 32 * i, o);
+            }
+          }
+        }
+        const float ms = m == -INFINITY ? 0.f : m;  // a row that has seen no key yet
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kT; ++i) {
+          x[i] = ex2(fmaf(x[i], p.scale2, -ms));
+          sum[i & 3] += x[i];
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        bool scalar = false;
+        if (part) {
+          const uint32_t r = it + 2 * (j - c.j0) + 1;
+          if (__any_sync(~0u, gave_up(&bars.v_clean[r % NS], (r / NS) & 1))) {
+            ok = false;
+            break;
+          }
+          scalar = *(volatile int*)&vflag[r % NS];
+          if (scalar) {  // O += P V over the seen keys alone
+            float w[kT];
+#pragma unroll
+            for (int i = 0; i < kT; ++i) w[i] = x[i];
+            const uint8_t* vt = ring + (r % NS) * C::kTile;
+#pragma unroll 1
+            for (int i = 0; i < HDP / 32; ++i) {
+              float o[32];
+              if (j > lo) {
+                tmem_ld32_nowait(tO + 32 * i, o);
+                tmem_wait_ld();
+                pin32(o);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0.f;
+              }
+              const uint8_t* vb = vt + (i >> 1) * kBox;
+#pragma unroll 1
+              for (int k = max(k_lo, 0); k <= min(k_hi, kT - 1); ++k) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const float2 v2 = to_f2<T>(*reinterpret_cast<const uint32_t*>(
+                      vb + k * 128 + ((((i & 1) * 64 + e * 4)) ^ ((k & 7) << 4))));
+                  o[2 * e] = fmaf(w[k], v2.x, o[2 * e]);
+                  o[2 * e + 1] = fmaf(w[k], v2.y, o[2 * e + 1]);
+                }
+              }
+              __syncwarp();
+              tmem_st32(tO + 32 * i, o);
+            }
+          }
+        }
+        if (!scalar) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t u[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = pack2<T>(x[32 * i + 2 * e], x[32 * i + 2 * e + 1]);
+            tmem_st16(tS + 16 * i, u);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_ready[t]);
+      }
+      it += 2 * (c.j1 - c.j0);
+      if (!ok) break;
+      if (hi > lo) {
+        if (__any_sync(~0u, gave_up(&bars.o_full[t], no & 1))) {
+          ok = false;
+          break;
+        }
+        ++no;
+        tc_fence_after();
+      }
+      const bool mine_row = c.row0[t] + row < c.nq;
+      T* out = static_cast<T*>(p.out) + (i64)(c.q0 + c.row0[t] + row) * p.ost + (i64)c.head[t] * p.osh;
+      if (!c.split) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int i = 0; i < HDP / 32; ++i) {
+          float o[32];
+          if (hi > lo) {
+            tmem_ld32_nowait(tO + 32 * i, o);
+            tmem_wait_ld();
+            pin32(o);
+          }
+          if (mine_row) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (32 * i + 8 * e >= p.hd) break;
+              uint4 u = make_uint4(0, 0, 0, 0);
+              if (hi > lo && l != 0.f) {
+                u.x = pack2<T>(o[8 * e] * inv, o[8 * e + 1] * inv);
+                u.y = pack2<T>(o[8 * e + 2] * inv, o[8 * e + 3] * inv);
+                u.z = pack2<T>(o[8 * e + 4] * inv, o[8 * e + 5] * inv);
+                u.w = pack2<T>(o[8 * e + 6] * inv, o[8 * e + 7] * inv);
+              }
+              *reinterpret_cast<uint4*>(out + 32 * i + 8 * e) = u;
+            }
+          }
+          __syncwarp();
+        }
+        tc_fence_before();
+        continue;
+      }
+      // a piece of an item: (m, l, O) to the workspace; float4 e of every row side by side
+      float* mine_part = p.part + (size_t)c.slot * C::kPartFloats;
+      const int r2 = t * kT + row;
+      const bool any = hi > lo;
+      mine_part[r2] = m;
+      mine_part[2 * kT + r2] = l;
+      float4* po = reinterpret_cast<float4*>(mine_part + 4 * kT);
+#pragma unroll 1
+      for (int i = 0; i < HDP / 32; ++i) {
+        float o[32];
+        if (any) {
+          tmem_ld32_nowait(tO + 32 * i, o);
+          tmem_wait_ld();
+          pin32(o);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          po[(8 * i + e) * 2 * kT + r2] =
+              any ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      tc_fence_before();
+      __threadfence();
+      named_sync(1, 2 * kT);
+      if (threadIdx.x == 0) {
+        const uint32_t done = atomicAdd(p.counts + c.first, (uint32_t)(c.j1 - c.j0)) + (c.j1 - c.j0);
+        last_in = done == (uint32_t)c.len;
+        if (last_in) p.counts[c.first] = 0;  // for the next call
+      }
+      named_sync(1, 2 * kT);
+      if (!last_in) continue;
+      __threadfence();
+      // the last one in joins the pieces in the order of the cut
+      const i64 stop = c.start + c.len;
+      float M = -INFINITY, Ls = 0.f;
+      int npieces = 1;
+      while (c.first + npieces < sc.ncta && sc.cut(c.first + npieces) < stop) ++npieces;
+      for (int k = 0; k < npieces; ++k) {
+        const float* q = p.part + (size_t)(k ? 2 * (c.first + k) : 2 * c.first + 1) * C::kPartFloats;
+        M = fmaxf(M, __ldcg(q + r2));
+      }
+      const float Ms = M == -INFINITY ? 0.f : M;
+      for (int k = 0; k < npieces; ++k) {
+        const float* q = p.part + (size_t)(k ? 2 * (c.first + k) : 2 * c.first + 1) * C::kPartFloats;
+        Ls += __ldcg(q + 2 * kT + r2) * ex2(__ldcg(q + r2) - Ms);
+      }
+      const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+      if (mine_row) {
+#pragma unroll 1
+        for (int e = 0; e < p.hd / 4; e += 2) {
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+          for (int k = 0; k < npieces; ++k) {
+            const float* q = p.part + (size_t)(k ? 2 * (c.first + k) : 2 * c.first + 1) * C::kPartFloats;
+            const float w = ex2(__ldcg(q + r2) - Ms);
+            if (!(w != 0.f)) continue;  // a piece without a seen key
+            const float4* qo = reinterpret_cast<const float4*>(q + 4 * kT);
+            const float4 u = __ldcg(qo + e * 2 * kT + r2), v = __ldcg(qo + (e + 1) * 2 * kT + r2);
+            a = make_float4(fmaf(w, u.x, a.x), fmaf(w, u.y, a.y), fmaf(w, u.z, a.z), fmaf(w, u.w, a.w));
+            b = make_float4(fmaf(w, v.x, b.x), fmaf(w, v.y, b.y), fmaf(w, v.z, b.z), fmaf(w, v.w, b.w));
+          }
+          uint4 u = make_uint4(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv),
+                               pack2<T>(b.x * inv, b.y * inv), pack2<T>(b.z * inv, b.w * inv));
+          if (Ls == 0.f) u = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(out + 4 * e) = u;
+        }
+      }
+      named_sync(1, 2 * kT);  // last_in is read by all before the next piece writes it
+    }
+    if (!ok) failed = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+  if (threadIdx.x == 0 && failed) atomicExch(&p.hdr->status, (uint32_t)OSSM_ETIMEOUT);
+}
+
+// [rows, heads, hd] as (channel, head, row); box: 128 rows of 64 channels of
+// one head; channels past hd and rows past the end read as zero.
+bool encode(CUtensorMap* map, int dtype, const void* base, int hd, int heads, i64 rows, i64 st, i64 sh) {
+  // a single row or head has no stride of its own to respect
+  if (heads == 1) sh = hd;
+  if (rows == 1) st = std::max(st, (i64)heads * std::max(sh, (i64)hd));
+  cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
+  cuuint32_t box[3] = {64, 1, kT};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fast::encode_fn()(map, dtype == OSSM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HDP>
+cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid,
+                   cudaStream_t st) {
+  auto kern = attn_prompt_kernel<T, HDP>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HDP>::kSmem);
+  if (e != cudaSuccess) return e;
+  kern<<<grid, kThreads, Cfg<HDP>::kSmem, st>>>(q, k, v, p, (p.H / p.Hkv) % 2 == 0);
+  return cudaGetLastError();
+}
+
+size_t prompt_part_floats(int hd) { return 2 * (hd <= 64 ? Cfg<64>::kPartFloats : Cfg<128>::kPartFloats); }
+
+int prompt_forward(const ossm_attn_args* a, const Params& p, int grid, cudaStream_t st) {
+  if (!fast::encode_fn()) return OSSM_ELAUNCH;
+  CUtensorMap q, k, v;
+  if (!encode(&q, a->dtype, p.q, p.hd, p.H, p.Tq, p.qst, p.qsh) ||
+      !encode(&k, a->dtype, p.k, p.hd, p.Hkv, p.Tk, p.kst, p.ksh) ||
+      !encode(&v, a->dtype, p.v, p.hd, p.Hkv, p.Tk, p.vst, p.vsh))
+    return OSSM_EINVAL;
+  const bool bf = a->dtype == OSSM_BF16;
+  cudaError_t e;
+  if (p.hd <= 64)
+    e = bf ? launch<__nv_bfloat16, 64>(q, k, v, p, grid, st) : launch<__half, 64>(q, k, v, p, grid, st);
+  else
+    e = bf ? launch<__nv_bfloat16, 128>(q, k, v, p, grid, st) : launch<__half, 128>(q, k, v, p, grid, st);
+  return e == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
+}
+
+}  // namespace attn
+}  // namespace ossm
