@@ -5,7 +5,7 @@
 // per key head), or 256 queries of one head.  An item walks its range of
 // 128-key tiles once with a running maximum and sum per row.
 //
-// One persistent CTA per SM, 11 warps:
+// One persistent CTA per SM, three warpgroups:
 //   warps 0-3, 4-7  softmax of tile 0 / 1: a thread owns a row.  Scores from
 //                   tensor memory, mask, maximum, exponentials, weights back
 //                   to tensor memory over the scores; at the end the output
@@ -50,7 +50,7 @@ namespace attn {
 using namespace sm100;
 
 constexpr int kT = 128;             // query rows and keys of a tile
-constexpr int kThreads = 352;
+constexpr int kThreads = 384;       // three warpgroups of 168 registers a thread at launch
 constexpr int kGroups = 1024;       // entries of the schedule's prefix in shared memory
 constexpr int kItemCost = 2;        // an item's start and end, in key tiles
 constexpr int kMinPiece = 6;        // no cut closer to an item's edge
@@ -191,6 +191,12 @@ OSSM_DEV uint64_t sdesc(uint32_t saddr, uint32_t lead) {
   return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// One lane of a converged warp.
+OSSM_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
 OSSM_DEV void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t id, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -228,6 +234,27 @@ OSSM_DEV void pin32(float* v) {
                     "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]));
   asm volatile("" : "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
 }
+// One column of this thread's lane.
+OSSM_DEV float tmem_ld1(uint32_t taddr) {
+  uint32_t u;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(u)
+               : "r"(taddr)
+               : "memory");
+  return __uint_as_float(u);
+}
+// 16 columns of this thread's lane times f, in place.
+OSSM_DEV void tmem_scale16(uint32_t taddr, float f) {
+  uint32_t u[16];
+  tmem_ld16_nowait(taddr, u);
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    asm volatile("" : "+r"(u[i]));
+    u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
+  }
+  tmem_st16(taddr, u);
+}
 OSSM_DEV void tmem_st32(uint32_t taddr, const float* v) {
   uint32_t u[16];
 #pragma unroll
@@ -238,10 +265,13 @@ OSSM_DEV void tmem_st32(uint32_t taddr, const float* v) {
   }
 }
 
-// Does some row of tile t miss a key of tile j?
+// Does some row of a tile, at positions first to last, miss a key of key tile j?
+OSSM_DEV bool partly(int window, int first, int last, int j) {
+  return j * kT + kT - 1 > first || (window && j * kT <= last - window);
+}
 OSSM_DEV bool partly(const Params& p, const Piece& c, int t, int j) {
-  const int first = c.row0[t] + c.off, last = min(c.row0[t] + kT, c.nq) - 1 + c.off;
-  return j * kT + kT - 1 > first || (p.window && j * kT <= last - p.window);
+  return j >= c.lo[t] && j < c.hi[t] &&
+         partly(p.window, c.row0[t] + c.off, min(c.row0[t] + kT, c.nq) - 1 + c.off, j);
 }
 
 struct Failed {
@@ -270,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int failed, last_in;
   __shared__ unsigned long long n_items;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, cta = blockIdx.x;
 
   // ------------------------------------------------------------ schedule
   const int gsz = (p.B + kGroups - 1) / kGroups, ngroups = (p.B + gsz - 1) / gsz;
@@ -336,6 +366,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tslot;
   const Failed gave_up{&failed};
 
+  // 256 x 200 + 128 x 104 = 384 x 168 registers
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 9) {
     // ---------------------------------------------------------- schedule and loads
     if (lane == 0) {
@@ -423,74 +456,88 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 8) {
     // ---------------------------------------------------------- products
+    // The whole warp walks the loop, so that operands stay uniform; one lane issues.
     constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
     constexpr uint32_t id_s = idesc(fmt, kT, 0), id_o = idesc(fmt, HDP, 1);
-    if (lane == 0) {
-      uint32_t it = 0, nq[2] = {0, 0}, np[2] = {0, 0};
-      bool ok = true;
-      const int ksteps = (p.hd + 15) / 16;
-      for (int n = 0; ok; ++n) {
-        const int sl = n & 1;
-        if (gave_up(&bars.piece_full[sl], (n >> 1) & 1)) break;
-        const Piece& c = pieces[sl];
-        if (!c.live) break;
-        const int j0 = c.j0, j1 = c.j1;
-        int lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
-        mbar_arrive(&bars.piece_empty[sl]);
-        // S_t = Q_t K_j^T for the tiles that walk j, K_j in ring slot it + 2 (j - j0)
-        auto scores = [&](int t, int j) {
-          if (j < lo[t] || j >= hi[t]) return true;
-          if (j == lo[t] && gave_up(&bars.q_full[t], nq[t]++ & 1)) return false;
-          const uint32_t r = it + 2 * (j - j0);
-          if (gave_up(&bars.kv_full[r % NS], (r / NS) & 1)) return false;
-          tc_fence_after();
-          const uint32_t a = smem_u32(smem + t * C::kTile), b = smem_u32(ring + (r % NS) * C::kTile);
-          for (int kk = 0; kk < ksteps; ++kk) {
-            const uint32_t o = (kk >> 2) * kBox + (kk & 3) * 32;
-            mma_ss(tmem + t * kT, sdesc(a + o, 16), sdesc(b + o, 16), id_s, kk > 0);
+    const bool leader = elect_one();
+    const uint32_t qb = smem_u32(smem), rb = smem_u32(ring);
+    uint32_t it = 0, nq[2] = {0, 0}, np[2] = {0, 0};
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const int sl = n & 1;
+      if (gave_up(&bars.piece_full[sl], (n >> 1) & 1)) break;
+      const Piece& c = pieces[sl];
+      if (!c.live) break;
+      const int j0 = c.j0, j1 = c.j1;
+      const int lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
+      __syncwarp();
+      if (leader) mbar_arrive(&bars.piece_empty[sl]);
+      // S_t = Q_t K_j^T for the tiles that walk j, K_j in ring slot it + 2 (j - j0)
+      auto scores = [&](int t, int j) {
+        if (j < lo[t] || j >= hi[t]) return true;
+        if (j == lo[t] && gave_up(&bars.q_full[t], nq[t]++ & 1)) return false;
+        const uint32_t r = it + 2 * (j - j0);
+        if (gave_up(&bars.kv_full[r % NS], (r / NS) & 1)) return false;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t a = sdesc(qb + t * C::kTile, 16), b = sdesc(rb + (r % NS) * C::kTile, 16);
+#pragma unroll
+          for (int kk = 0; kk < HDP / 16; ++kk) {
+            const uint32_t o = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+            mma_ss(tmem + t * kT, a + o, b + o, id_s, kk > 0);
           }
           mma_commit(&bars.s_full[t]);
           if (j == hi[t] - 1) mma_commit(&bars.q_empty[t]);
-          return true;
-        };
-        if (j0 < j1) {
-          ok = scores(0, j0) && scores(1, j0);
-          mma_commit(&bars.kv_empty[it % NS]);
         }
-        for (int j = j0; j < j1 && ok; ++j) {
-          const uint32_t rv = it + 2 * (j - j0) + 1;
-          if (gave_up(&bars.v_clean[rv % NS], (rv / NS) & 1)) {
-            ok = false;
-            break;
-          }
-          if (gave_up(&bars.kv_full[rv % NS], (rv / NS) & 1)) {  // passed already; orders the copy before the products
-            ok = false;
-            break;
-          }
-          const bool skip = *(volatile int*)&vflag[rv % NS];
-          const uint32_t vb = smem_u32(ring + (rv % NS) * C::kTile);
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (j >= lo[t] && j < hi[t]) {
-              if (gave_up(&bars.p_ready[t], np[t]++ & 1)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              if (!skip)
+        __syncwarp();
+        return true;
+      };
+      if (j0 < j1) {
+        ok = scores(0, j0) && scores(1, j0);
+        if (leader) mma_commit(&bars.kv_empty[it % NS]);
+      }
+      for (int j = j0; j < j1 && ok; ++j) {
+        const uint32_t rv = it + 2 * (j - j0) + 1;
+        // the second wait has passed by then; it orders the copy before the products
+        if (gave_up(&bars.v_clean[rv % NS], (rv / NS) & 1) || gave_up(&bars.kv_full[rv % NS], (rv / NS) & 1)) {
+          ok = false;
+          break;
+        }
+        const bool skip = *(volatile int*)&vflag[rv % NS];
+        const uint64_t vb = sdesc(rb + (rv % NS) * C::kTile, kBox);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (j >= lo[t] && j < hi[t]) {
+            if (gave_up(&bars.p_ready[t], np[t]++ & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (leader) {
+              if (!skip) {
+#pragma unroll
                 for (int kk = 0; kk < kT / 16; ++kk)
-                  mma_ts(tmem + C::kO + t * HDP, tmem + t * kT + kk * 8, sdesc(vb + kk * 2048, kBox), id_o,
+                  mma_ts(tmem + C::kO + t * HDP, tmem + t * kT + kk * 8, vb + kk * (2048 >> 4), id_o,
                          kk > 0 || j > lo[t]);
+              }
               if (j == hi[t] - 1) mma_commit(&bars.o_full[t]);
             }
-            if (j + 1 < j1) ok = scores(t, j + 1);
+            __syncwarp();
           }
+          if (j + 1 < j1 && !scores(t, j + 1)) {
+            ok = false;
+            break;
+          }
+        }
+        if (leader) {
           mma_commit(&bars.kv_empty[rv % NS]);
           if (j + 1 < j1) mma_commit(&bars.kv_empty[(rv + 1) % NS]);
         }
-        it += 2 * (j1 - j0);
+        __syncwarp();
       }
-      if (!ok) failed = 1;
+      it += 2 * (j1 - j0);
     }
+    if (!ok) failed = 1;
   } else if (warp == 10) {
     // ---------------------------------------------------------- V tiles that are not seen whole
     uint32_t it = 0;
@@ -507,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         bool bad = false;
-        if ((j >= c.lo[0] && j < c.hi[0] && partly(p, c, 0, j)) || (j >= c.lo[1] && j < c.hi[1] && partly(p, c, 1, j))) {
+        if (partly(p, c, 0, j) || partly(p, c, 1, j)) {
           const int rows = min(kT, c.nk - j * kT);
           uint4* v = reinterpret_cast<uint4*>(ring + (r % NS) * C::kTile);
           for (int x = 0; x < C::kBoxes; ++x) {
@@ -534,7 +581,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------------------------------------------------- softmax and output
     const int t = warp >> 2, row = threadIdx.x & (kT - 1);
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), tS = tl + t * kT, tO = tl + C::kO + t * HDP;
@@ -543,12 +592,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int n = 0; ok; ++n) {
       const int sl = n & 1;
       if (__any_sync(~0u, gave_up(&bars.piece_full[sl], (n >> 1) & 1))) break;
-      const Piece c = pieces[sl];
+      const Piece& c = pieces[sl];  // given back at the piece's end
       if (!c.live) break;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
-      const int lo = c.lo[t], hi = c.hi[t];
-      const int at = c.row0[t] + row + c.off;  // the row's position
+      const int lo = c.lo[t], hi = c.hi[t], j0 = c.j0;
+      const int first = c.row0[t] + c.off, at = first + row;  // the position of the tile's first row, and of this one
+      const int last = min(c.row0[t] + kT, c.nq) - 1 + c.off;
       float m = -INFINITY, l = 0.f;
       for (int j = lo; j < hi; ++j) {
         if (__any_sync(~0u, gave_up(&bars.s_full[t], ns & 1))) {
@@ -563,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 4; ++i) pin32(x + 32 * i);
-        const bool part = partly(p, c, t, j);
+        const bool part = partly(p.window, first, last, j);
         const int k_hi = at - j * kT, k_lo = p.window ? k_hi - p.window + 1 : -1;  // seen: k_lo <= key <= k_hi
         if (part) {
 #pragma unroll
@@ -582,15 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= f;
           if (j > lo) {
 #pragma unroll 1
-            for (int i = 0; i < HDP / 32; ++i) {
-              float o[32];
-              tmem_ld32_nowait(tO + 32 * i, o);
-              tmem_wait_ld();
-              pin32(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= f;
-              tmem_st32(tO + 32 * i, o);
-            }
+            for (int i = 0; i < HDP / 16; ++i) tmem_scale16(tO + 16 * i, f);
           }
         }
         const float ms = m == -INFINITY ? 0.f : m;  // a row that has seen no key yet
@@ -603,16 +643,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         bool scalar = false;
         if (part) {
-          const uint32_t r = it + 2 * (j - c.j0) + 1;
+          const uint32_t r = it + 2 * (j - j0) + 1;
           if (__any_sync(~0u, gave_up(&bars.v_clean[r % NS], (r / NS) & 1))) {
             ok = false;
             break;
           }
           scalar = *(volatile int*)&vflag[r % NS];
           if (scalar) {  // O += P V over the seen keys alone
-            float w[kT];
 #pragma unroll
-            for (int i = 0; i < kT; ++i) w[i] = x[i];
+            for (int i = 0; i < 4; ++i) tmem_st32(tS + 32 * i, x + 32 * i);
+            tmem_wait_st();
             const uint8_t* vt = ring + (r % NS) * C::kTile;
 #pragma unroll 1
             for (int i = 0; i < HDP / 32; ++i) {
@@ -627,16 +667,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               const uint8_t* vb = vt + (i >> 1) * kBox;
 #pragma unroll 1
-              for (int k = max(k_lo, 0); k <= min(k_hi, kT - 1); ++k) {
+              for (int k = 0; k < kT; ++k) {
+                const float w = tmem_ld1(tS + k);
+                if (k >= k_lo && k <= k_hi) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const float2 v2 = to_f2<T>(*reinterpret_cast<const uint32_t*>(
-                      vb + k * 128 + ((((i & 1) * 64 + e * 4)) ^ ((k & 7) << 4))));
-                  o[2 * e] = fmaf(w[k], v2.x, o[2 * e]);
-                  o[2 * e + 1] = fmaf(w[k], v2.y, o[2 * e + 1]);
+                  for (int e = 0; e < 16; ++e) {
+                    const float2 v2 = to_f2<T>(*reinterpret_cast<const uint32_t*>(
+                        vb + k * 128 + ((((i & 1) * 64 + e * 4)) ^ ((k & 7) << 4))));
+                    o[2 * e] = fmaf(w, v2.x, o[2 * e]);
+                    o[2 * e + 1] = fmaf(w, v2.y, o[2 * e + 1]);
+                  }
                 }
+                __syncwarp();
               }
-              __syncwarp();
               tmem_st32(tO + 32 * i, o);
             }
           }
@@ -655,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.p_ready[t]);
       }
-      it += 2 * (c.j1 - c.j0);
+      it += 2 * (c.j1 - j0);
       if (!ok) break;
       if (hi > lo) {
         if (__any_sync(~0u, gave_up(&bars.o_full[t], no & 1))) {
@@ -694,6 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         tc_fence_before();
+        if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
         continue;
       }
       // a piece of an item: (m, l, O) to the workspace; float4 e of every row side by side
@@ -725,7 +769,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (last_in) p.counts[c.first] = 0;  // for the next call
       }
       named_sync(1, 2 * kT);
-      if (!last_in) continue;
+      if (!last_in) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
+        continue;
+      }
       __threadfence();
       // the last one in joins the pieces in the order of the cut
       const i64 stop = c.start + c.len;
@@ -762,6 +810,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       named_sync(1, 2 * kT);  // last_in is read by all before the next piece writes it
+      if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
     }
     if (!ok) failed = 1;
   }
