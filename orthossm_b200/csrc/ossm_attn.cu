@@ -95,7 +95,7 @@ using namespace ossm;
 
 namespace {
 
-// Workspace: header, one progress counter a CTA, two partial results a CTA.
+// Workspace: header, two progress counters a CTA, two partial results a CTA.
 constexpr int kMaxCtas = 1024;
 
 int sm_count() {
@@ -107,7 +107,7 @@ int sm_count() {
 }
 
 size_t ws_bytes(const ossm_attn_args* a) {
-  return sizeof(WsHeader) + kMaxCtas * sizeof(uint32_t) + (size_t)sm_count() * attn::prompt_part_floats(a->head_dim) * 4;
+  return sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t) + (size_t)sm_count() * attn::prompt_part_floats(a->head_dim) * 4;
 }
 
 }  // namespace
@@ -126,7 +126,7 @@ extern "C" int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size
                        a->window >= a->total_k ? 0 : a->window,  // as wide as all keys: none
                        a->scale * 1.4426950408889634f, reinterpret_cast<WsHeader*>(w),
                        reinterpret_cast<uint32_t*>(w + sizeof(WsHeader)),
-                       reinterpret_cast<float*>(w + sizeof(WsHeader) + kMaxCtas * sizeof(uint32_t))};
+                       reinterpret_cast<float*>(w + sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t))};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a->max_seqlen_q > 16 && a->total_k > 0) return attn::prompt_forward(a, p, sm_count(), st);
   const dim3 grid((unsigned)((a->total_q + 3) / 4), a->H);

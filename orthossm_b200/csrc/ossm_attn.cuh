@@ -25,7 +25,7 @@ struct Params {
   int window;      // 0: none
   float scale2;    // scale * log2(e): the softmax runs on base-2 exponents
   WsHeader* hdr;
-  uint32_t* counts;  // per CTA: progress of the item that its last piece belongs to (0 between calls)
+  uint32_t* counts;  // per CTA and tile: progress of the item that its last piece belongs to (0 between calls)
   float* part;       // per CTA two partial results
 };
 
@@ -69,6 +69,15 @@ OSSM_DEV bool nonfinite2(uint32_t u) {
   return (u & e) == e || (u & (e << 16)) == (e << 16);
 }
 
+OSSM_DEV float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 OSSM_DEV float ex2(float x) {  // 2^x, relative error 2^-22
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

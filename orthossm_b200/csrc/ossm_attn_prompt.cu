@@ -10,17 +10,16 @@
 //                   tensor memory, mask, maximum, exponentials, weights back
 //                   to tensor memory over the scores; at the end the output
 //                   row out of the accumulator.
-//   warp 8          issues every tcgen05.mma: S_t = Q_t K^T (both operands in
-//                   shared memory) and O_t += P_t V (P_t in tensor memory, V
-//                   read MN-major, so it is never transposed).
+//   warp 8          issues the products S_t = Q_t K^T (tcgen05.mma, both operands
+//                   in shared memory).
+//   warp 10         issues O_t += P_t V (P_t in tensor memory, V read MN-major, so
+//                   it is never transposed).
 //   warp 9          walks the schedule, loads Q, K and V tiles by TMA.
-//   warp 10         looks through V tiles that some row does not see whole:
-//                   rows past the sequence are zeroed (a weight of 0 times
-//                   NaN would be NaN); if a seen row holds a non-finite value,
-//                   the softmax threads take that tile's product with the
-//                   seen rows alone instead of the tensor core.
-// Tensor memory: S_0 S_1 (128 columns each, P_t over S_t), O_0 O_1.  While
-// one tile's softmax runs, the tensor core works for the other.
+// Tensor memory (512 columns): scores, weights P_0 P_1, accumulators O_0 O_1.
+// Up to 64 channels each tile has a score buffer of its own; above that there
+// is room for one, which the tiles use in turn: a softmax takes its scores
+// into registers at once and frees the buffer, and the next ones are formed
+// while it computes.
 //
 // The maximum that the exponents are taken against follows the true one only
 // when a row has grown by more than 2^8 since: the weights then stay below
@@ -161,20 +160,25 @@ struct Piece {
   i64 start;               // split: the item's start on the line
 };
 
+constexpr int kPieces = 4;  // ring of pieces
 struct Bars {
-  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2];
-  uint64_t piece_full[2], piece_empty[2];
-  uint64_t kv_full[8], kv_empty[8], v_clean[8];
+  uint64_t q_full[2], q_empty[2], s_full[2], s_free[2], p_ready[2], pv_done[2];
+  uint64_t piece_full[kPieces], piece_empty[kPieces];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
 };
 
 template <int HDP>
 struct Cfg {
   static constexpr int kBoxes = HDP / 64;
   static constexpr int kTile = kBoxes * kBox;
-  static constexpr int kSlots = HDP == 64 ? 8 : 4;
-  static constexpr size_t kSmem = (2 + kSlots) * (size_t)kTile + 1024;
-  static constexpr uint32_t kCols = 512;
-  static constexpr uint32_t kO = 256;  // first column of O_0
+  static constexpr int kSlots = HDP == 64 ? 4 : 2;  // ring slots of K, and of V
+  static constexpr size_t kSmem = (2 + 2 * kSlots) * (size_t)kTile + 1024;
+  // columns: scores of 128 keys (one buffer a tile, or one for both), weights
+  // as pairs of 16 bits, accumulators
+  static constexpr int kS = HDP == 64 ? 2 : 1;
+  static constexpr uint32_t kCols = 512, kP = kS * kT, kO = kP + 2 * (kT / 2);
+  static constexpr int kPoly = HDP == 64 ? 3 : 2;
+  static_assert(kO + 2 * HDP <= kCols, "tensor memory");
   static constexpr size_t kPartFloats = 2 * kT * (size_t)(HDP + 2);
 };
 
@@ -235,13 +239,13 @@ OSSM_DEV void pin32(float* v) {
   asm volatile("" : "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
 }
 // One column of this thread's lane.
-OSSM_DEV float tmem_ld1(uint32_t taddr) {
+OSSM_DEV uint32_t tmem_ld1(uint32_t taddr) {
   uint32_t u;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
                : "=r"(u)
                : "r"(taddr)
                : "memory");
-  return __uint_as_float(u);
+  return u;
 }
 // 16 columns of this thread's lane times f, in place.
 OSSM_DEV void tmem_scale16(uint32_t taddr, float f) {
@@ -265,21 +269,127 @@ OSSM_DEV void tmem_st32(uint32_t taddr, const float* v) {
   }
 }
 
+// The largest of three, NaN if one is.
+OSSM_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// w = 2^(c x - ms) for a row's 128 scores, packed to the type; returns their
+// fp32 sum.  Of each 8 pairs, POLY are taken on the FMA pipe: the special
+// function unit alone (16 a clock and SM) would take longer than the tile's
+// two products.  There y is clamped to -125 (so never 0: not for masked keys),
+// 2^round(y) goes through the exponent bits and 2^f on [-1/2, 1/2] is the
+// polynomial of least relative error, of degree 3 (7.5e-5, a fraction of
+// bf16's rounding) or 4 (2.7e-6, fp16).  Step by step over the pairs, so that
+// the chains overlap.
+template <typename T, int POLY>
+OSSM_DEV float weights(const float (&x)[kT], float c, float ms, uint32_t (&w)[kT / 2]) {
+  const float2 c2 = make_float2(c, c), m2 = make_float2(-ms, -ms);
+  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: adding it rounds to an integer
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  auto both = [](float v) { return make_float2(v, v); };
+  float2 sum[2] = {both(0.f), both(0.f)};
+#pragma unroll
+  for (int g = 0; g < kT / 16; ++g) {
+    float2 y[8], t[8], f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = fma2(make_float2(x[16 * g + 2 * i], x[16 * g + 2 * i + 1]), c2, m2);
+#pragma unroll
+    for (int i = POLY; i < 8; ++i) y[i].x = ex2(y[i].x), y[i].y = ex2(y[i].y);
+#pragma unroll
+    for (int i = 0; i < POLY; ++i) y[i] = make_float2(fmaxf(y[i].x, -125.f), fmaxf(y[i].y, -125.f));
+#pragma unroll
+    for (int i = 0; i < POLY; ++i) t[i] = add2(y[i], magic);
+#pragma unroll
+    for (int i = 0; i < POLY; ++i) f[i] = sub2(t[i], magic);
+#pragma unroll
+    for (int i = 0; i < POLY; ++i) f[i] = sub2(y[i], f[i]);
+#pragma unroll
+    for (int i = 0; i < POLY; ++i)
+      y[i] = kHalf ? fma2(both(0.009570102207f), f[i], both(0.05591785908f))
+                   : fma2(both(0.05517166853f), f[i], both(0.2426111251f));
+#pragma unroll
+    for (int i = 0; i < POLY; ++i) y[i] = fma2(y[i], f[i], both(kHalf ? 0.2402474433f : 0.6932609677f));
+#pragma unroll
+    for (int i = 0; i < POLY; ++i) y[i] = fma2(y[i], f[i], both(kHalf ? 0.6931217909f : 0.9999280572f));
+    if (kHalf) {
+#pragma unroll
+      for (int i = 0; i < POLY; ++i) y[i] = fma2(y[i], f[i], both(0.9999992847f));
+    }
+#pragma unroll
+    for (int i = 0; i < POLY; ++i)
+      y[i] = make_float2(__int_as_float(__float_as_int(y[i].x) + (__float_as_int(t[i].x) << 23)),
+                         __int_as_float(__float_as_int(y[i].y) + (__float_as_int(t[i].y) << 23)));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sum[i & 1] = add2(sum[i & 1], y[i]);
+      w[8 * g + i] = pack2<T>(y[i].x, y[i].y);
+    }
+  }
+  sum[0] = add2(sum[0], sum[1]);
+  return sum[0].x + sum[0].y;
+}
+
+// Does the predicate hold in any of the n threads that meet at barrier id?
+OSSM_DEV bool meet_any(uint32_t id, uint32_t n, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbarrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(n), "r"((uint32_t)pred)
+      : "memory");
+  return r != 0;
+}
+
 // Does some row of a tile, at positions first to last, miss a key of key tile j?
 OSSM_DEV bool partly(int window, int first, int last, int j) {
   return j * kT + kT - 1 > first || (window && j * kT <= last - window);
 }
-OSSM_DEV bool partly(const Params& p, const Piece& c, int t, int j) {
-  return j >= c.lo[t] && j < c.hi[t] &&
-         partly(p.window, c.row0[t] + c.off, min(c.row0[t] + kT, c.nq) - 1 + c.off, j);
-}
 
+OSSM_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {  // has the phase passed? (may doze off for a moment)
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+constexpr long long kWaitCycles = 1LL << 31;  // about a second
+// A wait that ran out ends the role; the others run out in turn.
 struct Failed {
   int* flag;
-  OSSM_DEV bool operator()(uint64_t* bar, uint32_t parity) const {  // true: give up
-    if (mbar_wait(bar, parity)) return false;
-    *flag = 1;
-    return true;
+  OSSM_DEV bool one(uint64_t* bar, uint32_t parity) const {  // one thread; true: give up
+    const long long t0 = clock64();
+    while (!mbar_test(bar, parity))
+      if (clock64() - t0 > kWaitCycles) {
+        *flag = 1;
+        return true;
+      }
+    return false;
+  }
+  OSSM_DEV bool operator()(uint64_t* bar, uint32_t parity) const {  // a whole warp, of one mind
+    if (__all_sync(~0u, mbar_test(bar, parity))) return false;
+    const long long t0 = clock64();
+    while (!__all_sync(~0u, mbar_test(bar, parity)))
+      if (__any_sync(~0u, clock64() - t0 > kWaitCycles)) {
+        *flag = 1;
+        return true;
+      }
+    return false;
+  }
+};
+
+// The waits of warps that also meet at named barriers: one that ran out is
+// remembered (dead) and the warp goes on without waiting, so that the others
+// are not left at a barrier; they agree to stop at the next piece.
+struct Waits {
+  const Failed& f;
+  bool dead;
+  OSSM_DEV void operator()(uint64_t* bar, uint32_t parity) {
+    if (!dead) dead = f(bar, parity);
   }
 };
 
@@ -291,13 +401,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int NS = C::kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* ring = smem + 2 * C::kTile;
+  uint8_t *kring = smem + 2 * C::kTile, *vring = kring + NS * C::kTile;
   __shared__ Bars bars;
-  __shared__ Piece pieces[2];
+  __shared__ Piece pieces[kPieces];
   __shared__ i64 pre[kGroups + 1];
-  __shared__ int vflag[NS];
+  __shared__ int scalar[2];  // a tile's softmax has added its output itself
   __shared__ uint32_t tslot;
-  __shared__ int failed, last_in;
+  __shared__ int failed, last_in[2];
   __shared__ unsigned long long n_items;
 
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, cta = blockIdx.x;
@@ -347,15 +457,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars.q_full[t], 1);
       mbar_init(&bars.q_empty[t], 1);
       mbar_init(&bars.s_full[t], 1);
+      mbar_init(&bars.s_free[t], 4);
       mbar_init(&bars.p_ready[t], 4);
-      mbar_init(&bars.o_full[t], 1);
-      mbar_init(&bars.piece_full[t], 1);
-      mbar_init(&bars.piece_empty[t], 10);
+      mbar_init(&bars.pv_done[t], 1);
+    }
+    for (int i = 0; i < kPieces; ++i) {
+      mbar_init(&bars.piece_full[i], 1);
+      mbar_init(&bars.piece_empty[i], 10);
     }
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&bars.kv_full[i], 1);
-      mbar_init(&bars.kv_empty[i], 1);
-      mbar_init(&bars.v_clean[i], 1);
+      mbar_init(&bars.k_full[i], 1);
+      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.v_full[i], 1);
+      mbar_init(&bars.v_empty[i], 1);
     }
     fence_mbar_init();
   }
@@ -378,8 +492,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       const i64 end = sc.cut(cta + 1);
       i64 pos = sc.cut(cta);
       int n = 0, nq[2] = {0, 0};
-      uint32_t it = 0;
+      uint32_t ki = 0, vi = 0;  // K and V tiles loaded; V runs one behind
       bool ok = true;
+      auto load = [&](bool v, int head, int row) {
+        const uint32_t i = v ? vi++ : ki++, r = i % NS;
+        uint64_t* full = v ? &bars.v_full[r] : &bars.k_full[r];
+        if (i >= NS && gave_up.one(v ? &bars.v_empty[r] : &bars.k_empty[r], ((i / NS) & 1) ^ 1)) {
+          --(v ? vi : ki);
+          return false;
+        }
+        mbar_expect_tx(full, C::kTile);
+        for (int x = 0; x < C::kBoxes; ++x)
+          tma_load_3d((v ? vring : kring) + r * C::kTile + x * kBox, v ? &mV : &mK, full, 64 * x, head, row);
+        return true;
+      };
       for (;; ++n) {
         Piece c;
         c.live = 0;
@@ -413,19 +539,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           break;
         }
-        const int sl = n & 1;
-        if (n >= 2 && gave_up(&bars.piece_empty[sl], ((n >> 1) & 1) ^ 1)) {
+        const int sl = n % kPieces;
+        if (n >= kPieces && gave_up.one(&bars.piece_empty[sl], ((n / kPieces) & 1) ^ 1)) {
           ok = false;
           break;
         }
         pieces[sl] = c;
         mbar_arrive(&bars.piece_full[sl]);
         if (!c.live) break;
+        const int kvh = c.head[0] / (p.H / p.Hkv);
         for (int j = c.j0; j < c.j1 && ok; ++j) {
           if (j == c.j0)
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < 2 && ok; ++t) {
               if (c.lo[t] >= c.hi[t]) continue;
-              if (nq[t] && gave_up(&bars.q_empty[t], (nq[t] & 1) ^ 1)) {
+              if (nq[t] && gave_up.one(&bars.q_empty[t], (nq[t] & 1) ^ 1)) {
                 ok = false;
                 break;
               }
@@ -434,164 +561,140 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int x = 0; x < C::kBoxes; ++x)
                 tma_load_3d(smem + t * C::kTile + x * kBox, &mQ, &bars.q_full[t], 64 * x, c.head[t], c.q0 + c.row0[t]);
             }
-          for (int kv = 0; kv < 2 && ok; ++kv, ++it) {
-            const int r = it % NS;
-            if (it >= NS && gave_up(&bars.kv_empty[r], ((it / NS) & 1) ^ 1)) {
-              ok = false;
-              break;
-            }
-            mbar_expect_tx(&bars.kv_full[r], C::kTile);
-            for (int x = 0; x < C::kBoxes; ++x)
-              tma_load_3d(ring + r * C::kTile + x * kBox, kv ? &mV : &mK, &bars.kv_full[r], 64 * x,
-                          c.head[0] / (p.H / p.Hkv), c.k0 + j * kT);
-          }
+          ok = ok && load(false, kvh, c.k0 + j * kT) && (j == c.j0 || load(true, kvh, c.k0 + (j - 1) * kT));
         }
+        if (c.j0 < c.j1) ok = ok && load(true, kvh, c.k0 + (c.j1 - 1) * kT);
         if (!ok) break;
       }
       if (!ok) {  // no copy may still be landing when the CTA exits
         for (int t = 0; t < 2; ++t)
-          if (nq[t]) gave_up(&bars.q_full[t], (nq[t] & 1) ^ 1);
-        for (uint32_t i = it > NS ? it - NS : 0; i < it; ++i) gave_up(&bars.kv_full[i % NS], (i / NS) & 1);
+          if (nq[t]) gave_up.one(&bars.q_full[t], (nq[t] & 1) ^ 1);
+        for (uint32_t i = ki > NS ? ki - NS : 0; i < ki; ++i) gave_up.one(&bars.k_full[i % NS], (i / NS) & 1);
+        for (uint32_t i = vi > NS ? vi - NS : 0; i < vi; ++i) gave_up.one(&bars.v_full[i % NS], (i / NS) & 1);
       }
     }
   } else if (warp == 8) {
-    // ---------------------------------------------------------- products
-    // The whole warp walks the loop, so that operands stay uniform; one lane issues.
-    constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
-    constexpr uint32_t id_s = idesc(fmt, kT, 0), id_o = idesc(fmt, HDP, 1);
+    // ---------------------------------------------------------- S_t = Q_t K^T
+    // Scores and outputs are issued by a warp each: one for both was busy with
+    // its waits and left the tensor core idle.  The whole warp walks the loop,
+    // so that operands stay uniform; one lane issues.
+    constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, kT, 0);
     const bool leader = elect_one();
-    const uint32_t qb = smem_u32(smem), rb = smem_u32(ring);
-    uint32_t it = 0, nq[2] = {0, 0}, np[2] = {0, 0};
+    const uint32_t qb = smem_u32(smem), kb = smem_u32(kring);
+    uint32_t nq[2] = {0, 0}, ns[2] = {0, 0}, g = 0;
     bool ok = true;
     for (int n = 0; ok; ++n) {
-      const int sl = n & 1;
-      if (gave_up(&bars.piece_full[sl], (n >> 1) & 1)) break;
+      const int sl = n % kPieces;
+      if (gave_up(&bars.piece_full[sl], (n / kPieces) & 1)) break;
       const Piece& c = pieces[sl];
       if (!c.live) break;
-      const int j0 = c.j0, j1 = c.j1;
-      const int lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
+      const int j1 = c.j1, lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
+      int j = c.j0;
       __syncwarp();
       if (leader) mbar_arrive(&bars.piece_empty[sl]);
-      // S_t = Q_t K_j^T for the tiles that walk j, K_j in ring slot it + 2 (j - j0)
-      auto scores = [&](int t, int j) {
-        if (j < lo[t] || j >= hi[t]) return true;
-        if (j == lo[t] && gave_up(&bars.q_full[t], nq[t]++ & 1)) return false;
-        const uint32_t r = it + 2 * (j - j0);
-        if (gave_up(&bars.kv_full[r % NS], (r / NS) & 1)) return false;
-        tc_fence_after();
-        if (leader) {
-          const uint64_t a = sdesc(qb + t * C::kTile, 16), b = sdesc(rb + (r % NS) * C::kTile, 16);
-#pragma unroll
-          for (int kk = 0; kk < HDP / 16; ++kk) {
-            const uint32_t o = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
-            mma_ss(tmem + t * kT, a + o, b + o, id_s, kk > 0);
-          }
-          mma_commit(&bars.s_full[t]);
-          if (j == hi[t] - 1) mma_commit(&bars.q_empty[t]);
-        }
-        __syncwarp();
-        return true;
-      };
-      if (j0 < j1) {
-        ok = scores(0, j0) && scores(1, j0);
-        if (leader) mma_commit(&bars.kv_empty[it % NS]);
-      }
-      for (int j = j0; j < j1 && ok; ++j) {
-        const uint32_t rv = it + 2 * (j - j0) + 1;
-        // the second wait has passed by then; it orders the copy before the products
-        if (gave_up(&bars.v_clean[rv % NS], (rv / NS) & 1) || gave_up(&bars.kv_full[rv % NS], (rv / NS) & 1)) {
+      for (; j < j1 && ok; ++j, ++g) {
+        const uint32_t r = g % NS;
+        if (gave_up(&bars.k_full[r], (g / NS) & 1)) {
           ok = false;
           break;
         }
-        const bool skip = *(volatile int*)&vflag[rv % NS];
-        const uint64_t vb = sdesc(rb + (rv % NS) * C::kTile, kBox);
+        const uint64_t kd = sdesc(kb + r * C::kTile, 16);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (j >= lo[t] && j < hi[t]) {
-            if (gave_up(&bars.p_ready[t], np[t]++ & 1)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            if (leader) {
-              if (!skip) {
-#pragma unroll
-                for (int kk = 0; kk < kT / 16; ++kk)
-                  mma_ts(tmem + C::kO + t * HDP, tmem + t * kT + kk * 8, vb + kk * (2048 >> 4), id_o,
-                         kk > 0 || j > lo[t]);
-              }
-              if (j == hi[t] - 1) mma_commit(&bars.o_full[t]);
-            }
-            __syncwarp();
-          }
-          if (j + 1 < j1 && !scores(t, j + 1)) {
+          if (j < lo[t] || j >= hi[t]) continue;
+          constexpr int kS = C::kS;
+          const int b = t % kS;
+          if ((j == lo[t] && gave_up(&bars.q_full[t], nq[t]++ & 1)) ||
+              (ns[b] && gave_up(&bars.s_free[b], (ns[b] & 1) ^ 1))) {
             ok = false;
             break;
           }
+          ++ns[b];
+          tc_fence_after();
+          if (leader) {
+            const uint64_t qd = sdesc(qb + t * C::kTile, 16);
+#pragma unroll
+            for (int kk = 0; kk < HDP / 16; ++kk) {
+              const uint32_t o = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+              mma_ss(tmem + b * kT, qd + o, kd + o, id, kk > 0);
+            }
+            mma_commit(&bars.s_full[t]);
+            if (j == hi[t] - 1) mma_commit(&bars.q_empty[t]);
+          }
         }
-        if (leader) {
-          mma_commit(&bars.kv_empty[rv % NS]);
-          if (j + 1 < j1) mma_commit(&bars.kv_empty[(rv + 1) % NS]);
-        }
-        __syncwarp();
+        if (leader) mma_commit(&bars.k_empty[r]);
       }
-      it += 2 * (j1 - j0);
     }
     if (!ok) failed = 1;
   } else if (warp == 10) {
-    // ---------------------------------------------------------- V tiles that are not seen whole
-    uint32_t it = 0;
+    // ---------------------------------------------------------- O_t += P_t V
+    constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, HDP, 1);
+    const bool leader = elect_one();
+    const uint32_t vb = smem_u32(vring);
+    uint32_t np[2] = {0, 0}, g = 0;
     bool ok = true;
     for (int n = 0; ok; ++n) {
-      const int sl = n & 1;
-      if (__any_sync(~0u, gave_up(&bars.piece_full[sl], (n >> 1) & 1))) break;
+      const int sl = n % kPieces;
+      if (gave_up(&bars.piece_full[sl], (n / kPieces) & 1)) break;
       const Piece& c = pieces[sl];
       if (!c.live) break;
-      for (int j = c.j0; j < c.j1; ++j) {
-        const uint32_t r = it + 2 * (j - c.j0) + 1;
-        if (__any_sync(~0u, gave_up(&bars.kv_full[r % NS], (r / NS) & 1))) {
+      const int j1 = c.j1, lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
+      int j = c.j0;
+      __syncwarp();
+      if (leader) mbar_arrive(&bars.piece_empty[sl]);
+      for (; j < j1 && ok; ++j, ++g) {
+        const uint32_t r = g % NS;
+        if (gave_up(&bars.v_full[r], (g / NS) & 1)) {
           ok = false;
           break;
         }
-        bool bad = false;
-        if (partly(p, c, 0, j) || partly(p, c, 1, j)) {
-          const int rows = min(kT, c.nk - j * kT);
-          uint4* v = reinterpret_cast<uint4*>(ring + (r % NS) * C::kTile);
-          for (int x = 0; x < C::kBoxes; ++x) {
-#pragma unroll 8
-            for (int i = lane; i < kT * 8; i += 32) {
-              if ((i >> 3) < rows) {
-                const uint4 u = v[x * (kBox / 16) + i];
-                bad |= nonfinite2<T>(u.x) || nonfinite2<T>(u.y) || nonfinite2<T>(u.z) || nonfinite2<T>(u.w);
-              } else {
-                v[x * (kBox / 16) + i] = make_uint4(0, 0, 0, 0);
-              }
-            }
+        const uint64_t vd = sdesc(vb + r * C::kTile, kBox);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (j < lo[t] || j >= hi[t]) continue;
+          if (gave_up(&bars.p_ready[t], np[t]++ & 1)) {
+            ok = false;
+            break;
           }
-          fence_proxy_async_smem();  // the zeros, before the tensor core reads them
-          bad = __any_sync(~0u, bad);
+          tc_fence_after();
+          if (leader) {
+            if (!*(volatile int*)&scalar[t]) {
+#pragma unroll
+              for (int kk = 0; kk < kT / 16; ++kk)
+                mma_ts(tmem + C::kO + t * HDP, tmem + C::kP + t * (kT / 2) + kk * 8, vd + kk * (2048 >> 4), id,
+                       kk > 0 || j > lo[t]);
+            }
+            mma_commit(&bars.pv_done[t]);
+          }
         }
-        __syncwarp();
-        if (lane == 0) {
-          vflag[r % NS] = bad;
-          mbar_arrive(&bars.v_clean[r % NS]);
-        }
+        if (leader) mma_commit(&bars.v_empty[r]);
       }
-      it += 2 * (c.j1 - c.j0);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
     }
+    if (!ok) failed = 1;
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------------------------------------------------- softmax and output
     const int t = warp >> 2, row = threadIdx.x & (kT - 1);
-    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), tS = tl + t * kT, tO = tl + C::kO + t * HDP;
-    uint32_t ns = 0, no = 0, it = 0;
-    bool ok = true;
-    for (int n = 0; ok; ++n) {
-      const int sl = n & 1;
-      if (__any_sync(~0u, gave_up(&bars.piece_full[sl], (n >> 1) & 1))) break;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), tS = tl + (t % C::kS) * kT,
+                   tP = tl + C::kP + t * (kT / 2), tO = tl + C::kO + t * HDP;
+    uint32_t ns = 0, npv = 0, it = 0;  // score tiles seen, outputs waited for, steps before the piece
+    Waits wait{gave_up, false};
+    auto settled = [&](uint32_t upto) {  // the outputs of all score tiles before this one are in
+      if (npv == upto) return;
+      wait(&bars.pv_done[t], npv & 1);
+      ++npv;
+      tc_fence_after();
+    };
+    auto free_scores = [&]() {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.s_free[t % C::kS]);
+    };
+    for (int n = 0;; ++n) {
+      const int sl = n % kPieces;
+      wait(&bars.piece_full[sl], (n / kPieces) & 1);
+      if (meet_any(1 + t, kT, wait.dead)) break;
       const Piece& c = pieces[sl];  // given back at the piece's end
       if (!c.live) break;
       const int lo = c.lo[t], hi = c.hi[t], j0 = c.j0;
@@ -599,10 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int last = min(c.row0[t] + kT, c.nq) - 1 + c.off;
       float m = -INFINITY, l = 0.f;
       for (int j = lo; j < hi; ++j) {
-        if (__any_sync(~0u, gave_up(&bars.s_full[t], ns & 1))) {
-          ok = false;
-          break;
-        }
+        wait(&bars.s_full[t], ns & 1);
         ++ns;
         tc_fence_after();
         float x[kT];
@@ -611,17 +711,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 4; ++i) pin32(x + 32 * i);
+        free_scores();
         const bool part = partly(p.window, first, last, j);
         const int k_hi = at - j * kT, k_lo = p.window ? k_hi - p.window + 1 : -1;  // seen: k_lo <= key <= k_hi
         if (part) {
 #pragma unroll
-          for (int i = 0; i < kT; ++i)
-            if (i > k_hi || i < k_lo) x[i] = -INFINITY;
-        }
-        float mx[4] = {x[0], x[1], x[2], x[3]};
+          for (int i = 0; i < 4; ++i) {  // bit e: key 32 i + e is seen
+            const int a = k_lo - 32 * i, b = k_hi - 32 * i;
+            const uint32_t up = b >= 31 ? ~0u : b < 0 ? 0u : (2u << b) - 1u, low = a <= 0 ? ~0u : a > 31 ? 0u : ~0u << a;
+            const uint32_t seen = up & low;
 #pragma unroll
-        for (int i = 4; i < kT; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
+            for (int e = 0; e < 32; ++e) x[32 * i + e] = (seen >> e & 1u) ? x[32 * i + e] : -INFINITY;
+          }
+        }
+        float mx[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          mx[i] = x[32 * i];
+#pragma unroll
+          for (int e = 1; e < 31; e += 2) mx[i] = max3(mx[i], x[32 * i + e], x[32 * i + e + 1]);
+        }
+        mx[0] = max3(mx[0], mx[1], x[31]);
+        mx[1] = max3(mx[2], mx[3], x[63]);
+        mx[0] = max3(mx[0], mx[1], x[95]);
+        const float top = max3(mx[0], x[127], x[127]) * p.scale2;
+        if (!(top < INFINITY)) m = NAN;  // a seen score is NaN or infinite: so is the softmax's sum
         const bool grow = top > m + 8.f;
         if (__any_sync(~0u, grow)) {
           const float mn = grow ? top : m;
@@ -629,31 +743,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = mn;
           l *= f;
           if (j > lo) {
+            settled(ns - 1);
 #pragma unroll 1
             for (int i = 0; i < HDP / 16; ++i) tmem_scale16(tO + 16 * i, f);
           }
         }
         const float ms = m == -INFINITY ? 0.f : m;  // a row that has seen no key yet
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t w[kT / 2];
+        l += part ? weights<T, 0>(x, p.scale2, ms, w) : weights<T, C::kPoly>(x, p.scale2, ms, w);
+        settled(ns - 1);
 #pragma unroll
-        for (int i = 0; i < kT; ++i) {
-          x[i] = ex2(fmaf(x[i], p.scale2, -ms));
-          sum[i & 3] += x[i];
+        for (int i = 0; i < 4; ++i) {
+          uint32_t u[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) u[e] = w[16 * i + e];
+          tmem_st16(tP + 16 * i, u);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        bool scalar = false;
         if (part) {
-          const uint32_t r = it + 2 * (j - j0) + 1;
-          if (__any_sync(~0u, gave_up(&bars.v_clean[r % NS], (r / NS) & 1))) {
-            ok = false;
-            break;
-          }
-          scalar = *(volatile int*)&vflag[r % NS];
-          if (scalar) {  // O += P V over the seen keys alone
+          const uint32_t g = it + (j - j0);
+          wait(&bars.v_full[g % NS], (g / NS) & 1);
+          // A weight of 0 times NaN is NaN: V rows past the sequence become
+          // zeros, and if another one holds a non-finite value, the product
+          // is taken here over the seen keys alone.
+          uint4* vr = reinterpret_cast<uint4*>(vring + (g % NS) * C::kTile + row * 128);
+          bool bad = false;
+          if (j * kT + row < c.nk) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_st32(tS + 32 * i, x + 32 * i);
+            for (int i = 0; i < 8 * C::kBoxes; ++i) {  // in an order that spreads the rows over the banks
+              const uint4 u = vr[(i >> 3) * (kBox / 16) + ((i ^ row) & 7)];
+              bad |= nonfinite2<T>(u.x) || nonfinite2<T>(u.y) || nonfinite2<T>(u.z) || nonfinite2<T>(u.w);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8 * C::kBoxes; ++i)
+              vr[(i >> 3) * (kBox / 16) + ((i ^ row) & 7)] = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();  // before the tensor core reads them
+          }
+          const bool own = meet_any(1 + t, kT, bad);
+          if (row == 0) scalar[t] = own;
+          if (own) {
             tmem_wait_st();
-            const uint8_t* vt = ring + (r % NS) * C::kTile;
+            const uint8_t* vt = vring + (g % NS) * C::kTile;
 #pragma unroll 1
             for (int i = 0; i < HDP / 32; ++i) {
               float o[32];
@@ -668,7 +798,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint8_t* vb = vt + (i >> 1) * kBox;
 #pragma unroll 1
               for (int k = 0; k < kT; ++k) {
-                const float w = tmem_ld1(tS + k);
+                const float2 w2 = to_f2<T>(tmem_ld1(tP + (k >> 1)));
+                const float w = (k & 1) ? w2.y : w2.x;
                 if (k >= k_lo && k <= k_hi) {
 #pragma unroll
                   for (int e = 0; e < 16; ++e) {
@@ -684,30 +815,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (!scalar) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t u[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) u[e] = pack2<T>(x[32 * i + 2 * e], x[32 * i + 2 * e + 1]);
-            tmem_st16(tS + 16 * i, u);
-          }
-        }
+        if (!part && row == 0) scalar[t] = 0;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.p_ready[t]);
       }
-      it += 2 * (c.j1 - j0);
-      if (!ok) break;
-      if (hi > lo) {
-        if (__any_sync(~0u, gave_up(&bars.o_full[t], no & 1))) {
-          ok = false;
-          break;
-        }
-        ++no;
-        tc_fence_after();
-      }
+      it += c.j1 - j0;
+      settled(ns);
       const bool mine_row = c.row0[t] + row < c.nq;
       T* out = static_cast<T*>(p.out) + (i64)(c.q0 + c.row0[t] + row) * p.ost + (i64)c.head[t] * p.osh;
       if (!c.split) {
@@ -762,14 +877,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __threadfence();
-      named_sync(1, 2 * kT);
-      if (threadIdx.x == 0) {
-        const uint32_t done = atomicAdd(p.counts + c.first, (uint32_t)(c.j1 - c.j0)) + (c.j1 - c.j0);
-        last_in = done == (uint32_t)c.len;
-        if (last_in) p.counts[c.first] = 0;  // for the next call
+      // the tiles join apart: neither softmax may wait for the other here, whose
+      // products can be queued behind this one's next scores
+      named_sync(1 + t, kT);
+      if (row == 0) {
+        uint32_t* count = p.counts + 2 * c.first + t;
+        const uint32_t done = atomicAdd(count, (uint32_t)(c.j1 - c.j0)) + (c.j1 - c.j0);
+        last_in[t] = done == (uint32_t)c.len;
+        if (last_in[t]) *count = 0;  // for the next call
       }
-      named_sync(1, 2 * kT);
-      if (!last_in) {
+      named_sync(1 + t, kT);
+      if (!last_in[t]) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
         continue;
@@ -809,10 +927,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint4*>(out + 4 * e) = u;
         }
       }
-      named_sync(1, 2 * kT);  // last_in is read by all before the next piece writes it
+      __syncwarp();
       if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
     }
-    if (!ok) failed = 1;
   }
   tc_fence_before();
   __syncthreads();
