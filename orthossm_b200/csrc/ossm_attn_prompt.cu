@@ -12,7 +12,7 @@
 //                   row out of the accumulator.
 //   warp 8          issues the products S_t = Q_t K^T (tcgen05.mma, both operands
 //                   in shared memory).
-//   warp 10         issues O_t += P_t V (P_t in tensor memory, V read MN-major, so
+//   warps 10, 11    issue O_t += P_t V for tile 0 / 1 (P_t in tensor memory, V read MN-major, so
 //                   it is never transposed).
 //   warp 9          walks the schedule, loads Q, K and V tiles by TMA.
 // Tensor memory (512 columns): scores, weights P_0 P_1, accumulators O_0 O_1.
@@ -177,7 +177,6 @@ struct Cfg {
   // as pairs of 16 bits, accumulators
   static constexpr int kS = HDP == 64 ? 2 : 1;
   static constexpr uint32_t kCols = 512, kP = kS * kT, kO = kP + 2 * (kT / 2);
-  static constexpr int kPoly = HDP == 64 ? 3 : 2;
   static_assert(kO + 2 * HDP <= kCols, "tensor memory");
   static constexpr size_t kPartFloats = 2 * kT * (size_t)(HDP + 2);
 };
@@ -276,59 +275,23 @@ OSSM_DEV float max3(float a, float b, float c) {
   return d;
 }
 // w = 2^(c x - ms) for a row's 128 scores, packed to the type; returns their
-// fp32 sum.  Of each 8 pairs, POLY are taken on the FMA pipe: the special
-// function unit alone (16 a clock and SM) would take longer than the tile's
-// two products.  There y is clamped to -125 (so never 0: not for masked keys),
-// 2^round(y) goes through the exponent bits and 2^f on [-1/2, 1/2] is the
-// polynomial of least relative error, of degree 3 (7.5e-5, a fraction of
-// bf16's rounding) or 4 (2.7e-6, fp16).  Step by step over the pairs, so that
-// the chains overlap.
-template <typename T, int POLY>
+// fp32 sum.
+template <typename T>
 OSSM_DEV float weights(const float (&x)[kT], float c, float ms, uint32_t (&w)[kT / 2]) {
   const float2 c2 = make_float2(c, c), m2 = make_float2(-ms, -ms);
-  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: adding it rounds to an integer
-  constexpr bool kHalf = std::is_same<T, __half>::value;
-  auto both = [](float v) { return make_float2(v, v); };
-  float2 sum[2] = {both(0.f), both(0.f)};
+  float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
-  for (int g = 0; g < kT / 16; ++g) {
-    float2 y[8], t[8], f[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = fma2(make_float2(x[16 * g + 2 * i], x[16 * g + 2 * i + 1]), c2, m2);
-#pragma unroll
-    for (int i = POLY; i < 8; ++i) y[i].x = ex2(y[i].x), y[i].y = ex2(y[i].y);
-#pragma unroll
-    for (int i = 0; i < POLY; ++i) y[i] = make_float2(fmaxf(y[i].x, -125.f), fmaxf(y[i].y, -125.f));
-#pragma unroll
-    for (int i = 0; i < POLY; ++i) t[i] = add2(y[i], magic);
-#pragma unroll
-    for (int i = 0; i < POLY; ++i) f[i] = sub2(t[i], magic);
-#pragma unroll
-    for (int i = 0; i < POLY; ++i) f[i] = sub2(y[i], f[i]);
-#pragma unroll
-    for (int i = 0; i < POLY; ++i)
-      y[i] = kHalf ? fma2(both(0.009570102207f), f[i], both(0.05591785908f))
-                   : fma2(both(0.05517166853f), f[i], both(0.2426111251f));
-#pragma unroll
-    for (int i = 0; i < POLY; ++i) y[i] = fma2(y[i], f[i], both(kHalf ? 0.2402474433f : 0.6932609677f));
-#pragma unroll
-    for (int i = 0; i < POLY; ++i) y[i] = fma2(y[i], f[i], both(kHalf ? 0.6931217909f : 0.9999280572f));
-    if (kHalf) {
-#pragma unroll
-      for (int i = 0; i < POLY; ++i) y[i] = fma2(y[i], f[i], both(0.9999992847f));
-    }
-#pragma unroll
-    for (int i = 0; i < POLY; ++i)
-      y[i] = make_float2(__int_as_float(__float_as_int(y[i].x) + (__float_as_int(t[i].x) << 23)),
-                         __int_as_float(__float_as_int(y[i].y) + (__float_as_int(t[i].y) << 23)));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum[i & 1] = add2(sum[i & 1], y[i]);
-      w[8 * g + i] = pack2<T>(y[i].x, y[i].y);
-    }
+  for (int i = 0; i < kT / 2; ++i) {
+    float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), c2, m2);
+    y = make_float2(ex2(y.x), ex2(y.y));
+    if (i & 1)
+      s1 = add2(s1, y);
+    else
+      s0 = add2(s0, y);
+    w[i] = pack2<T>(y.x, y.y);
   }
-  sum[0] = add2(sum[0], sum[1]);
-  return sum[0].x + sum[0].y;
+  s0 = add2(s0, s1);
+  return s0.x + s0.y;
 }
 
 // Does the predicate hold in any of the n threads that meet at barrier id?
@@ -463,13 +426,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kPieces; ++i) {
       mbar_init(&bars.piece_full[i], 1);
-      mbar_init(&bars.piece_empty[i], 10);
+      mbar_init(&bars.piece_empty[i], 11);
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&bars.k_full[i], 1);
       mbar_init(&bars.k_empty[i], 1);
       mbar_init(&bars.v_full[i], 1);
-      mbar_init(&bars.v_empty[i], 1);
+      mbar_init(&bars.v_empty[i], 2);
     }
     fence_mbar_init();
   }
@@ -626,48 +589,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok) failed = 1;
-  } else if (warp == 10) {
+  } else {
     // ---------------------------------------------------------- O_t += P_t V
     constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, HDP, 1);
     const bool leader = elect_one();
     const uint32_t vb = smem_u32(vring);
-    uint32_t np[2] = {0, 0}, g = 0;
+    const int t = warp - 10;
+    uint32_t np = 0, g = 0;
     bool ok = true;
     for (int n = 0; ok; ++n) {
       const int sl = n % kPieces;
       if (gave_up(&bars.piece_full[sl], (n / kPieces) & 1)) break;
       const Piece& c = pieces[sl];
       if (!c.live) break;
-      const int j1 = c.j1, lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
+      const int j1 = c.j1, lo = c.lo[t], hi = c.hi[t];
       int j = c.j0;
       __syncwarp();
       if (leader) mbar_arrive(&bars.piece_empty[sl]);
-      for (; j < j1 && ok; ++j, ++g) {
+      for (; j < j1; ++j, ++g) {
         const uint32_t r = g % NS;
-        if (gave_up(&bars.v_full[r], (g / NS) & 1)) {
+        const bool act = j >= lo && j < hi;
+        if (gave_up(&bars.v_full[r], (g / NS) & 1) || (act && gave_up(&bars.p_ready[t], np++ & 1))) {
           ok = false;
           break;
         }
-        const uint64_t vd = sdesc(vb + r * C::kTile, kBox);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j < lo[t] || j >= hi[t]) continue;
-          if (gave_up(&bars.p_ready[t], np[t]++ & 1)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (leader) {
+        tc_fence_after();
+        if (leader) {
+          if (act) {
             if (!*(volatile int*)&scalar[t]) {
+              const uint64_t vd = sdesc(vb + r * C::kTile, kBox);
 #pragma unroll
               for (int kk = 0; kk < kT / 16; ++kk)
                 mma_ts(tmem + C::kO + t * HDP, tmem + C::kP + t * (kT / 2) + kk * 8, vd + kk * (2048 >> 4), id,
-                       kk > 0 || j > lo[t]);
+                       kk > 0 || j > lo);
             }
             mma_commit(&bars.pv_done[t]);
           }
+          mma_commit(&bars.v_empty[r]);
         }
-        if (leader) mma_commit(&bars.v_empty[r]);
+        __syncwarp();
       }
     }
     if (!ok) failed = 1;
@@ -750,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float ms = m == -INFINITY ? 0.f : m;  // a row that has seen no key yet
         uint32_t w[kT / 2];
-        l += part ? weights<T, 0>(x, p.scale2, ms, w) : weights<T, C::kPoly>(x, p.scale2, ms, w);
+        l += weights<T>(x, p.scale2, ms, w);
         settled(ns - 1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -142,6 +142,27 @@ def test_layouts(nq, nk):
     check(O.packed_attention(q, k1, v, cu_q, cu_k, max_seqlen_q=nq), q, k1, v, cu_q, cu_k)
 
 
+@pytest.mark.parametrize("H,Hkv,hd", [(3, 3, 128), (8, 2, 64), (6, 1, 96)])
+@pytest.mark.parametrize("nq,nk,window", [(9000, 9000, None), (7000, 7000, 300), (900, 20000, None), (260, 40000, None)])
+def test_long_sequences(H, Hkv, hd, nq, nk, window):
+    """Many items a CTA, and items cut between CTAs: rows spread over the
+    sequence against the reference."""
+    dtype = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(nq)
+    mk = lambda n, h: torch.randn(n, h, hd, device="cuda", generator=g).to(dtype)  # noqa: E731
+    q, k, v = mk(nq + 5, H), mk(nk + 7, Hkv), mk(nk + 7, Hkv)
+    cu_q, cu_k = cum([5, nq]), cum([7, nk])
+    out = O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq, window=window)
+    assert bool(torch.isfinite(out).all())
+    for i in [0, 1, 127, 128, nq // 3, nq // 2, nq - 200, nq - 130, nq - 2, nq - 1]:
+        end = i + nk - nq + 1  # the row as a sequence of one query and the keys before it
+        one = torch.tensor([0, 1]), torch.tensor([0, end])
+        ref, mag, _ = packed_attention_ref(q[5 + i:6 + i], k[7:7 + end], v[7:7 + end], *one, window=window)
+        lim = bound(ref, mag, dtype, end, 6.0)
+        assert bool(((out[5 + i].double().cpu() - ref[0]).abs() <= lim[0]).all()), i
+    assert O.workspace_status() == 0
+
+
 @pytest.mark.parametrize("nq", [1, 150])
 def test_rows_outside_the_sequences_are_left_alone(nq):
     H, hd = 2, 64
