@@ -390,7 +390,7 @@ int ossm_ttt_wpred_run(const ossm_ttt_run_args* a, void* workspace, size_t works
  * ------------------------------------------------------------------------ */
 typedef struct {
   int32_t B, H, H_kv, head_dim;      /* head_dim a multiple of 8, at most 128; H a multiple of H_kv; B <= 16384 */
-  int64_t total_q, total_k;          /* rows of q / out and of k / v, at most 2^30 */
+  int64_t total_q, total_k;          /* rows of q / out and of k / v: at most 2^30, total_q * H below 2^31 */
   int32_t max_seqlen_q;              /* the most queries a sequence has (chooses the kernels; never a bound) */
   int32_t dtype;                     /* OSSM_BF16 or OSSM_F16: q, k, v, out */
   const void *q, *k, *v;             /* [rows, heads, head_dim], 16-byte aligned, unit channel stride */
