@@ -2,13 +2,26 @@
 //
 // Every filter keeps a prefix of the candidates ordered by (logit descending,
 // index ascending), so what stays is described by one 64-bit key: the logit's
-// order-preserving bits above the inverted index.  One CTA per row finds the
-// top-k key and then the top-p key by a radix search of 8 bits a pass (counts,
-// or probability masses summed as 64-bit fixed point, whose sum does not
-// depend on the order of the additions), and a last pass takes the largest
-// score among the candidates at or above it.
+// order-preserving bits above the inverted index.
+//
+// A row is shared by a cluster of up to 8 CTAs.  One pass over the logits finds
+// the largest and the sum of the weights, from which follows a logit that the
+// prefix cannot reach below (Bound); a second pass, out of L2, collects the
+// candidates above it into the first CTA's shared memory, where they are
+// ordered and the prefix and its best score are found.  The noise is read for
+// the prefix alone.  Where too many candidates are collected (nearly flat rows)
+// the first CTA finds the prefix by radix passes over the whole row instead.
+// Masses that are compared are 64-bit fixed-point sums, which do not depend on
+// the order of the additions.
+//
+// Without filters the score of every candidate is needed: one pass over logits
+// and noise.  The logarithm is first taken in its fast form, and exactly only
+// where that comes within its error of the best score so far.
 #include <cuda_fp16.h>
 
+#include <cooperative_groups.h>
+
+#include <algorithm>
 #include <cmath>
 
 #include "orthossm_b200.h"
@@ -17,8 +30,13 @@
 namespace ossm {
 namespace smp {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 1024;
+constexpr int kList = 4096;    // candidates that are ordered in shared memory
+constexpr int kRank = 512;     // up to here by counting the larger ones, above by a bitonic sort
 typedef unsigned long long u64;
+typedef long long i64;
 
 struct Params {
   int V;
@@ -78,112 +96,457 @@ OSSM_DEV void better(Best& a, float s, int i) {
   }
 }
 
-OSSM_DEV u64 block_max(u64 v, u64* red) {
-  for (int w = 16; w; w >>= 1) v = max(v, __shfl_xor_sync(~0u, v, w));
+template <typename T>
+struct Vec {
+  static constexpr int n = 16 / sizeof(T);
+};
+OSSM_DEV void unpack(const uint4& u, float (&l)[4], float) {
+  l[0] = __uint_as_float(u.x), l[1] = __uint_as_float(u.y), l[2] = __uint_as_float(u.z), l[3] = __uint_as_float(u.w);
+}
+OSSM_DEV void unpack(const uint4& u, float (&l)[8], __nv_bfloat16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) l[2 * i] = __uint_as_float(w[i] << 16), l[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+OSSM_DEV void unpack(const uint4& u, float (&l)[8], __half) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    l[2 * i] = f.x, l[2 * i + 1] = f.y;
+  }
+}
+
+// This CTA's share of a row: f(l, i, n) for the n logits from index i on, 16
+// aligned bytes at a time; the row's unaligned ends go to the first CTA, one by
+// one.  What is not a candidate (NaN) arrives as -inf.
+template <typename T, typename F>
+OSSM_DEV void scan(const T* row, int V, int rank, int nrank, F f) {
+  constexpr int N = Vec<T>::n;
+  const int head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
+  const int nv = (V - head) / N, v0 = (int)((i64)nv * rank / nrank), v1 = (int)((i64)nv * (rank + 1) / nrank);
+  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  for (int v = v0 + threadIdx.x; v < v1; v += 4 * kThreads) {
+    uint4 u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (v + k * kThreads < v1) u[k] = __ldg(body + v + k * kThreads);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (v + k * kThreads >= v1) break;
+      float l[N];
+      unpack(u[k], l, T());
+#pragma unroll
+      for (int e = 0; e < N; ++e) l[e] = fmaxf(l[e], -INFINITY);  // a NaN operand loses
+      f(l, head + (v + k * kThreads) * N, N);
+    }
+  }
+  if (rank == 0) {
+    const int tail = V - head - nv * N, e = threadIdx.x;
+    if (e < head + tail) {
+      const int i = e < head ? e : V - tail + (e - head);
+      float l[N];
+      l[0] = fmaxf(to_f(row[i]), -INFINITY);
+      f(l, i, 1);
+    }
+  }
+}
+
+template <typename V, typename Op>
+OSSM_DEV V block_reduce(V v, V* red, Op op) {  // the result in every thread
+#pragma unroll
+  for (int w = 16; w; w >>= 1) v = op(v, __shfl_xor_sync(~0u, v, w));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = red[threadIdx.x & 31];
-  for (int w = 16; w; w >>= 1) v = max(v, __shfl_xor_sync(~0u, v, w));
+#pragma unroll
+  for (int w = 16; w; w >>= 1) v = op(v, __shfl_xor_sync(~0u, v, w));
   return v;
 }
 
+OSSM_DEV Best block_best(Best b, Best* bests) {  // the result in warp 0
+  for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) bests[threadIdx.x >> 5] = b;
+  __syncthreads();
+  b = bests[threadIdx.x & 31];
+  for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
+  return b;
+}
+
+// A row's settings, in force together.
+struct Row {
+  float inv_t, top_p, min_p;
+  int top_k;     // 0: off
+  bool greedy;
+  OSSM_DEV bool open() const { return !greedy && top_k == 0 && top_p >= 1.f && !(min_p > 0.f); }
+};
+OSSM_DEV Row row_of(const Params& p, int row) {
+  Row r;
+  r.inv_t = p.t_row ? 1.0f / p.t_row[row] : p.inv_t;
+  r.top_k = p.k_row ? p.k_row[row] : p.top_k;
+  r.top_p = p.p_row ? p.p_row[row] : p.top_p;
+  r.min_p = p.m_row ? p.m_row[row] : p.min_p;
+  if (r.top_k <= 0 || r.top_k >= p.V) r.top_k = 0;
+  if (!(r.top_p >= 0.f)) r.top_p = 0.f;
+  r.greedy = !p.noise || !(r.inv_t > 0.f) || r.inv_t == INFINITY;
+  return r;
+}
+
+// The prefix by radix passes over the whole row, 8 bits of the key at a time:
+// its smallest key.  One CTA; the row's first candidate has logit m.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
-  __shared__ u64 hist[256];
-  __shared__ u64 red[32];
-  __shared__ u64 sh_prefix, sh_left;
-  __shared__ Best bests[32];
-  const int row = blockIdx.x, tid = threadIdx.x;
-  const T* lg = static_cast<const T*>(p.logits) + row * p.lst;
-  const float* nz = p.noise ? p.noise + row * p.nst : nullptr;
-  float inv_t = p.inv_t;
-  if (p.t_row) inv_t = 1.0f / p.t_row[row];
-  const bool greedy = !nz || !(inv_t > 0.f) || inv_t == INFINITY;
-  const int top_k = p.k_row ? p.k_row[row] : p.top_k;
-  const float top_p = p.p_row ? p.p_row[row] : p.top_p, min_p = p.m_row ? p.m_row[row] : p.min_p;
-
-  u64 best = 0;
-  for (int i = tid; i < p.V; i += kThreads) {
-    const float l = to_f(lg[i]);
-    if (live(l)) best = max(best, key_of(l, i));
-  }
-  best = block_max(best, red);
-  if (best == 0 || greedy) {
-    if (tid == 0) p.out[row] = best == 0 ? -1 : (int64_t)(0xffffffffu - (uint32_t)best);
-    return;
-  }
-  const float m = logit_of(best);
-
-  // keep = the smallest key that stays
+OSSM_DEV u64 radix_prefix(const Row& r, const T* lg, int V, float m, u64* hist, u64* red, u64* sh) {
   u64 keep = 0;
   for (int what = 0; what < 2; ++what) {  // 0: by count, 1: by mass
     u64 target;
     if (what == 0) {
-      if (top_k <= 0 || top_k >= p.V) continue;
-      target = top_k;
+      if (r.top_k == 0) continue;
+      target = r.top_k;
     } else {
-      if (top_p >= 1.f) continue;
+      if (r.top_p >= 1.f) continue;
       u64 z = 0;
-      for (int i = tid; i < p.V; i += kThreads) {
-        const float l = to_f(lg[i]);
-        if (live(l) && key_of(l, i) >= keep) z += mass_of(weight(l, m, inv_t));
-      }
-      for (int w = 16; w; w >>= 1) z += __shfl_xor_sync(~0u, z, w);
-      __syncthreads();
-      if ((tid & 31) == 0) red[tid >> 5] = z;
-      __syncthreads();
-      z = red[tid & 31];
-      for (int w = 16; w; w >>= 1) z += __shfl_xor_sync(~0u, z, w);
-      target = max((u64)1, (u64)__double2ull_ru((double)fmaxf(top_p, 0.f) * (double)z));
+      scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
+        for (int e = 0; e < n; ++e)
+          if (live(l[e]) && key_of(l[e], i + e) >= keep) z += mass_of(weight(l[e], m, r.inv_t));
+      });
+      z = block_reduce(z, red, [](u64 a, u64 b) { return a + b; });
+      target = max((u64)1, (u64)__double2ull_ru((double)r.top_p * (double)z));
     }
     u64 prefix = 0;
     bool found = true;
-    for (int shift = 56; shift >= 0; shift -= 8) {
+    for (int shift = 56; shift >= 0 && found; shift -= 8) {
       __syncthreads();
-      if (tid < 256) hist[tid] = 0;
+      if (threadIdx.x < 256) hist[threadIdx.x] = 0;
       __syncthreads();
-      for (int i = tid; i < p.V; i += kThreads) {
-        const float l = to_f(lg[i]);
-        if (!live(l)) continue;
-        const u64 key = key_of(l, i);
-        if (key < keep || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
-        atomicAdd(&hist[(key >> shift) & 255], what ? mass_of(weight(l, m, inv_t)) : (u64)1);
-      }
+      scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
+        for (int e = 0; e < n; ++e) {
+          if (!live(l[e])) continue;
+          const u64 key = key_of(l[e], i + e);
+          if (key < keep || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
+          atomicAdd(&hist[(key >> shift) & 255], what ? mass_of(weight(l[e], m, r.inv_t)) : (u64)1);
+        }
+      });
       __syncthreads();
-      if (tid == 0) {
+      if (threadIdx.x == 0) {
         u64 left = target;
         int d = 255;
         for (; d > 0 && hist[d] < left; --d) left -= hist[d];
-        sh_left = hist[d] < left ? 0 : left;  // 0: fewer than asked for are there
-        sh_prefix = (prefix << 8) | d;
+        sh[0] = hist[d] < left ? 0 : left;  // 0: fewer than asked for are there
+        sh[1] = (prefix << 8) | d;
       }
       __syncthreads();
-      target = sh_left;
-      prefix = sh_prefix;
-      if (target == 0) {
-        found = false;
-        break;
-      }
+      target = sh[0];
+      prefix = sh[1];
+      found = target != 0;
     }
     if (found) keep = prefix;
   }
+  return keep;
+}
 
+// What the CTAs of a cluster tell each other.
+struct Told {
+  float m, z;      // largest logit; sum of the weights relative to it
+  uint32_t tk;     // order bits that at least top_k candidates reach
+  int count;       // candidates collected (the first CTA's)
+  Best best;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
+  __shared__ u64 list[kList];
+  __shared__ u64 hist[256];
+  __shared__ u64 red[32], sh[2];
+  __shared__ float redf[32];
+  __shared__ Best bests[32];
+  __shared__ Told told;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int nrank = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int row = blockIdx.x / nrank, tid = threadIdx.x;
+  const T* lg = static_cast<const T*>(p.logits) + row * p.lst;
+  const float* nz = p.noise ? p.noise + row * p.nst : nullptr;
+  const Row r = row_of(p, row);
+  if (tid == 0) told.count = 0;
+
+  if (r.open()) {
+    Best b{0.f, -1};
+    const bool aligned = Vec<T>::n >= 4 && [&] {
+      const int head = (int)((16 - ((uintptr_t)lg & 15)) & 15) / (int)sizeof(T);
+      return ((uintptr_t)(nz + head) & 15) == 0;
+    }();
+    scan(lg, p.V, rank, nrank, [&](const float* l, int i, int n) {
+      float e[Vec<T>::n];
+      if (n > 1 && aligned) {
+#pragma unroll
+        for (int k = 0; k < Vec<T>::n; k += 4) {
+          const float4 f = __ldcs(reinterpret_cast<const float4*>(nz + i + k));
+          e[k] = f.x, e[k + 1] = f.y, e[k + 2] = f.z, e[k + 3] = f.w;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < Vec<T>::n; ++k)
+          if (k < n) e[k] = nz[i + k];
+      }
+#pragma unroll
+      for (int k = 0; k < Vec<T>::n; ++k) {
+        if (k >= n || !live(l[k])) continue;
+        // log2.approx is within 2^-22 (of 1, or of its value): far below this slack
+        const float x = l[k] * r.inv_t, s = fmaf(-0.693147181f, __log2f(e[k]), x);
+        if (!(s < b.s - (1e-4f + 1e-6f * fabsf(x))) || b.i < 0) better(b, score_of(l[k], r.inv_t, e[k]), i + k);
+      }
+    });
+    b = block_best(b, bests);
+    if (nrank > 1) {
+      if (tid == 0) told.best = b;
+      cluster.sync();
+      if (rank == 0 && tid < 32) {
+        b = Best{0.f, -1};
+        if (tid < nrank) b = cluster.map_shared_rank(&told, tid)->best;
+        for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
+      }
+      cluster.sync();  // the others' memory is read before they leave
+    }
+    if (rank == 0 && tid == 0) p.out[row] = b.i;
+    return;
+  }
+
+  // ---------------------------------------------------------------- the largest logit, the weights' sum
+  const int top_k = r.greedy ? 1 : r.top_k;
+  const bool by_mass = !r.greedy && r.top_p < 1.f;
+  const bool need_z = by_mass && top_k == 0;
+  const float c = r.inv_t * 1.44269504f;
+  float m = -INFINITY, z = 0.f;
+  scan(lg, p.V, rank, nrank, [&](const float* l, int, int n) {
+    float top = l[0];
+#pragma unroll
+    for (int e = 1; e < Vec<T>::n; ++e)
+      if (e < n) top = fmaxf(top, l[e]);
+    if (top > m) {
+      z = m == -INFINITY ? 0.f : z * exp2f((m - top) * c);
+      m = top;
+    }
+    if (need_z && live(m)) {
+#pragma unroll
+      for (int e = 0; e < Vec<T>::n; ++e)
+        if (e < n) z += l[e] == m ? 1.f : exp2f((l[e] - m) * c);
+    }
+  });
+  const float cta_m = block_reduce(m, redf, [](float a, float b) { return fmaxf(a, b); });
+  if (need_z)
+    z = block_reduce(live(m) ? z * (m == cta_m ? 1.f : exp2f((m - cta_m) * c)) : 0.f, redf,
+                     [](float a, float b) { return a + b; });
+  // order bits that at least top_k of this CTA's threads' largest logits reach,
+  // so at least top_k candidates: the 16 high bits by bisection
+  uint32_t tk = 0;
+  if (top_k && top_k <= kThreads) {
+    const uint32_t mine = live(m) ? ord(m) : 0u;
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t t = tk | (1u << bit);
+      if (__syncthreads_count(mine >= t) >= top_k) tk = t;
+    }
+  }
+  if (nrank > 1) {
+    if (tid == 0) {
+      told.m = cta_m;
+      told.z = z;
+      told.tk = tk;
+    }
+    cluster.sync();
+    m = -INFINITY;
+    for (int k = 0; k < nrank; ++k) {
+      const Told* o = cluster.map_shared_rank(&told, k);
+      m = fmaxf(m, o->m);
+      tk = max(tk, o->tk);
+    }
+    z = 0.f;
+    for (int k = 0; need_z && k < nrank; ++k) {
+      const Told* o = cluster.map_shared_rank(&told, k);
+      if (live(o->m)) z += o->z * (o->m == m ? 1.f : exp2f((o->m - m) * c));
+    }
+  } else {
+    m = cta_m;
+    __syncthreads();  // told.count is 0
+  }
+  if (!live(m)) {
+    if (nrank > 1) cluster.sync();
+    if (rank == 0 && tid == 0) p.out[row] = -1;
+    return;
+  }
+
+  // ---------------------------------------------------------------- Bound, and the candidates above it
+  // With top_k: its own bound alone, as its mass counts for top_p.  Without:
+  // the candidates below (1 - top_p) z / V weigh less than (1 - top_p) z
+  // together, so the prefix ends above them.  min_p only ever shortens.  The
+  // logarithms' and the products' roundings are covered by the slack.
+  uint32_t bound = tk;
+  if (!(top_k && by_mass)) {
+    float y = -INFINITY;
+    if (need_z) y = logf((1.f - r.top_p) * z / (float)p.V);
+    if (!r.greedy && r.min_p > 0.f) y = fmaxf(y, logf(fminf(r.min_p, 1.f)));
+    if (y > -INFINITY && m < INFINITY) {
+      const float lb = m + (y - 1e-3f - 1e-5f * fabsf(y)) / r.inv_t;
+      bound = max(bound, ord(fminf(lb - 1e-5f * (fabsf(m) + fabsf(lb)), m)));
+    }
+  }
+  Told* first = nrank > 1 ? cluster.map_shared_rank(&told, 0) : &told;
+  u64* first_list = nrank > 1 ? cluster.map_shared_rank(list, 0) : list;
+  scan(lg, p.V, rank, nrank, [&](const float* l, int i, int n) {
+    uint32_t in = 0;
+#pragma unroll
+    for (int e = 0; e < Vec<T>::n; ++e)
+      if (e < n && live(l[e]) && ord(l[e]) >= bound) in |= 1u << e;
+    if (in) {
+      int at = atomicAdd(&first->count, __popc(in));
+#pragma unroll
+      for (int e = 0; e < Vec<T>::n; ++e)
+        if (in >> e & 1u) {
+          if (at < kList) first_list[at] = key_of(l[e], i + e);
+          ++at;
+        }
+    }
+  });
+  if (nrank > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  if (rank != 0) return;
+
+  // ---------------------------------------------------------------- the prefix and its best score
+  const int N = told.count;
   Best b{0.f, -1};
-  for (int i = tid; i < p.V; i += kThreads) {
-    const float l = to_f(lg[i]);
-    if (!live(l) || key_of(l, i) < keep) continue;
-    if (min_p > 0.f && i != (int)(0xffffffffu - (uint32_t)best) && weight(l, m, inv_t) < min_p) continue;
-    better(b, score_of(l, inv_t, nz[i]), i);
+  auto consider = [&](u64 key) {
+    const int i = (int)(0xffffffffu - (uint32_t)key);
+    better(b, r.greedy ? 0.f : score_of(logit_of(key), r.inv_t, nz[i]), i);
+  };
+  if (N > kList) {
+    u64 top = 0;
+    if (r.greedy || r.min_p > 0.f) {  // the first candidate stays whatever min_p is
+      scan(lg, p.V, 0, 1, [&](const float* l, int i, int n) {
+        for (int e = 0; e < n; ++e)
+          if (live(l[e])) top = max(top, key_of(l[e], i + e));
+      });
+      top = block_reduce(top, red, [](u64 a, u64 b) { return max(a, b); });
+    }
+    if (r.greedy) {
+      if (tid == 0) consider(top);
+    } else {
+      const u64 keep = radix_prefix(r, lg, p.V, m, hist, red, sh);
+      scan(lg, p.V, 0, 1, [&](const float* l, int i, int n) {
+        for (int e = 0; e < n; ++e) {
+          const u64 key = key_of(l[e], i + e);
+          if (live(l[e]) && key >= keep && (!(r.min_p > 0.f) || key == top || weight(l[e], m, r.inv_t) >= r.min_p))
+            consider(key);
+        }
+      });
+    }
+  } else {
+    // in order, into registers: sorted position tid + k kThreads
+    constexpr int kPer = kList / kThreads;
+    u64 mine[kPer] = {};
+    if (N <= kRank) {
+      // a key's position is the number of larger ones; parts of the count by neighbouring threads
+      int parts = 1;
+      while (parts < 32 && N * parts * 2 <= kThreads) parts *= 2;
+      const int e = tid / parts, q = tid % parts;
+      u64 key = 0;
+      int larger = 0;
+      if (e < N) {
+        key = list[e];
+        for (int k = q; k < N; k += parts) larger += list[k] > key;
+      }
+      for (int w = 1; w < parts; w *= 2) larger += __shfl_xor_sync(~0u, larger, w);
+      __syncthreads();
+      if (e < N && q == 0) list[larger] = key;
+      __syncthreads();
+    } else {
+      int size = 1024;
+      while (size < N) size *= 2;
+      for (int k = N + tid; k < size; k += kThreads) list[k] = 0;
+      for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j; j /= 2) {
+          __syncthreads();
+          for (int e = tid; e < size / 2; e += kThreads) {
+            const int a = 2 * j * (e / j) + e % j, o = a + j;
+            const u64 x = list[a], y = list[o];
+            if ((x < y) == ((a & k) == 0)) list[a] = y, list[o] = x;  // descending
+          }
+        }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int e = tid + k * kThreads;
+      if (e < N) mine[k] = list[e];
+    }
+    int n = top_k ? min(top_k, N) : N;
+    if (by_mass) {
+      // mass up to and including each position, kThreads at a time
+      u64 upto[kPer], base = 0;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        upto[k] = 0;
+        if (k * kThreads >= N) continue;
+        u64 v = tid + k * kThreads < n ? mass_of(weight(logit_of(mine[k]), m, r.inv_t)) : 0;
+#pragma unroll
+        for (int w = 1; w < 32; w *= 2) {
+          const u64 u = __shfl_up_sync(~0u, v, w);
+          if ((tid & 31) >= w) v += u;
+        }
+        __syncthreads();
+        if ((tid & 31) == 31) red[tid >> 5] = v;
+        __syncthreads();
+        u64 before = (tid & 31) < (tid >> 5) ? red[tid & 31] : 0, all = red[tid & 31];
+#pragma unroll
+        for (int w = 16; w; w >>= 1) {
+          before += __shfl_xor_sync(~0u, before, w);
+          all += __shfl_xor_sync(~0u, all, w);
+        }
+        upto[k] = base + before + v;
+        base += all;
+      }
+      const double whole = top_k ? (double)base : (double)z * 0x1p40;
+      const double target = (double)r.top_p * whole;
+      int stay = 0;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        if (k * kThreads >= N) continue;
+        const int e = tid + k * kThreads;
+        const u64 own = e < n ? mass_of(weight(logit_of(mine[k]), m, r.inv_t)) : 0;
+        stay += __syncthreads_count(e < n && (double)(upto[k] - own) < target);
+      }
+      n = max(1, stay);
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int e = tid + k * kThreads;
+      if (e < n && (e == 0 || r.greedy || !(r.min_p > 0.f) || weight(logit_of(mine[k]), m, r.inv_t) >= r.min_p))
+        consider(mine[k]);
+    }
   }
-  for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
-  if ((tid & 31) == 0) bests[tid >> 5] = b;
-  __syncthreads();
-  if (tid < 32) {
-    b = bests[tid];
-    for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
-    if (tid == 0) p.out[row] = b.i;
-  }
+  b = block_best(b, bests);
+  if (tid == 0) p.out[row] = b.i;
+}
+
+// CTAs a row: as many as fill the GPU about once, with 2048 logits each at least.
+template <typename T>
+cudaError_t launch(const Params& p, int B, cudaStream_t st) {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  int c = 1;
+  while (c < 8 && (i64)B * c * 2 <= sms && p.V / (2 * c) >= 2048) c *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)B * c);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = c, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
 }
 
 }  // namespace smp
@@ -192,7 +555,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
 using namespace ossm;
 
 extern "C" int ossm_sample_tokens(const ossm_sample_args* a, ossm_stream_t stream) {
-  if (!a || a->B < 0 || a->V < 1 || a->V >= (1 << 23) || !a->logits || !a->out) return OSSM_EINVAL;
+  if (!a || a->B < 0 || a->B > (1 << 27) || a->V < 1 || a->V >= (1 << 23) || !a->logits || !a->out) return OSSM_EINVAL;
   const int el = a->dtype == OSSM_F32 ? 4 : 2;
   if ((a->dtype != OSSM_F32 && a->dtype != OSSM_BF16 && a->dtype != OSSM_F16) || (uintptr_t)a->logits % el ||
       (uintptr_t)a->noise % 4 || (uintptr_t)a->out % 8)
@@ -202,11 +565,12 @@ extern "C" int ossm_sample_tokens(const ossm_sample_args* a, ossm_stream_t strea
   const smp::Params p{a->V, a->logits, a->logits_stride, a->noise, a->noise_stride, a->inv_temperature, a->top_p,
                       a->min_p, a->top_k, a->temperature_row, a->top_p_row, a->min_p_row, a->top_k_row, a->out};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
   if (a->dtype == OSSM_F32)
-    smp::sample_kernel<float><<<a->B, smp::kThreads, 0, st>>>(p);
+    e = smp::launch<float>(p, a->B, st);
   else if (a->dtype == OSSM_BF16)
-    smp::sample_kernel<__nv_bfloat16><<<a->B, smp::kThreads, 0, st>>>(p);
+    e = smp::launch<__nv_bfloat16>(p, a->B, st);
   else
-    smp::sample_kernel<__half><<<a->B, smp::kThreads, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
+    e = smp::launch<__half>(p, a->B, st);
+  return e == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
 }
