@@ -9,8 +9,9 @@
 // prefix cannot reach below (Bound); a second pass, out of L2, collects the
 // candidates above it into the first CTA's shared memory, where they are
 // ordered and the prefix and its best score are found.  The noise is read for
-// the prefix alone.  Where too many candidates are collected (nearly flat rows)
-// the first CTA finds the prefix by radix passes over the whole row instead.
+// the prefix alone.  Where too many candidates are collected (wide or nearly
+// flat rows) the first CTA finds the prefix's end in a histogram of the logits
+// instead, and orders the candidates of one bin.
 // Masses that are compared are 64-bit fixed-point sums, which do not depend on
 // the order of the additions.
 //
@@ -73,6 +74,11 @@ OSSM_DEV float logit_of(u64 key) {
 // where both are +inf.
 OSSM_DEV float weight(float l, float m, float inv_t) {
   return l == m ? 1.f : expf(__fmul_rn(__fsub_rn(l, m), inv_t));
+}
+OSSM_DEV float ex2(float x) {  // 2^x, relative error 2^-22
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // 2^-40 steps: a row's sum stays below 2^63 for V < 2^23 equal candidates.
 OSSM_DEV u64 mass_of(float w) { return (u64)__float2ull_rn(w * 0x1p40f); }
@@ -194,56 +200,242 @@ OSSM_DEV Row row_of(const Params& p, int row) {
   return r;
 }
 
-// The prefix by radix passes over the whole row, 8 bits of the key at a time:
-// its smallest key.  One CTA; the row's first candidate has logit m.
-template <typename T>
-OSSM_DEV u64 radix_prefix(const Row& r, const T* lg, int V, float m, u64* hist, u64* red, u64* sh) {
-  u64 keep = 0;
-  for (int what = 0; what < 2; ++what) {  // 0: by count, 1: by mass
-    u64 target;
-    if (what == 0) {
-      if (r.top_k == 0) continue;
-      target = r.top_k;
-    } else {
-      if (r.top_p >= 1.f) continue;
-      u64 z = 0;
-      scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
-        for (int e = 0; e < n; ++e)
-          if (live(l[e]) && key_of(l[e], i + e) >= keep) z += mass_of(weight(l[e], m, r.inv_t));
-      });
-      z = block_reduce(z, red, [](u64 a, u64 b) { return a + b; });
-      target = max((u64)1, (u64)__double2ull_ru((double)r.top_p * (double)z));
+// Shared memory of the work on one row.
+struct Room {
+  u64 list[kList];
+  u64 red[32];
+  u64 sh[4];
+};
+constexpr int kPer = kList / kThreads;
+constexpr int kBins = 1024;
+
+// The N keys of the list in descending order.
+OSSM_DEV void order(u64* list, int N) {
+  const int tid = threadIdx.x;
+  if (N <= kRank) {
+    // a key's position is the number of larger ones; parts of the count by neighbouring threads
+    int parts = 1;
+    while (parts < 32 && N * parts * 2 <= kThreads) parts *= 2;
+    const int e = tid / parts, q = tid % parts;
+    u64 key = 0;
+    int larger = 0;
+    if (e < N) {
+      key = list[e];
+      for (int k = q; k < N; k += parts) larger += list[k] > key;
     }
-    u64 prefix = 0;
-    bool found = true;
-    for (int shift = 56; shift >= 0 && found; shift -= 8) {
-      __syncthreads();
-      if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-      __syncthreads();
-      scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
-        for (int e = 0; e < n; ++e) {
-          if (!live(l[e])) continue;
-          const u64 key = key_of(l[e], i + e);
-          if (key < keep || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
-          atomicAdd(&hist[(key >> shift) & 255], what ? mass_of(weight(l[e], m, r.inv_t)) : (u64)1);
+    for (int w = 1; w < parts; w *= 2) larger += __shfl_xor_sync(~0u, larger, w);
+    __syncthreads();
+    if (e < N && q == 0) list[larger] = key;
+  } else {
+    int size = 1024;
+    while (size < N) size *= 2;
+    for (int k = N + tid; k < size; k += kThreads) list[k] = 0;
+    for (int k = 2; k <= size; k *= 2)
+      for (int j = k / 2; j; j /= 2) {
+        __syncthreads();
+        for (int e = tid; e < size / 2; e += kThreads) {
+          const int a = 2 * j * (e / j) + e % j, o = a + j;
+          const u64 x = list[a], y = list[o];
+          if ((x < y) == ((a & k) == 0)) list[a] = y, list[o] = x;
         }
-      });
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        u64 left = target;
-        int d = 255;
-        for (; d > 0 && hist[d] < left; --d) left -= hist[d];
-        sh[0] = hist[d] < left ? 0 : left;  // 0: fewer than asked for are there
-        sh[1] = (prefix << 8) | d;
       }
-      __syncthreads();
-      target = sh[0];
-      prefix = sh[1];
-      found = target != 0;
-    }
-    if (found) keep = prefix;
   }
-  return keep;
+  __syncthreads();
+}
+
+// Sum of v over the threads up to and including this one; all: over every thread.
+OSSM_DEV u64 block_scan(u64 v, u64* red, u64& all) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int w = 1; w < 32; w *= 2) {
+    const u64 u = __shfl_up_sync(~0u, v, w);
+    if ((tid & 31) >= w) v += u;
+  }
+  __syncthreads();
+  if ((tid & 31) == 31) red[tid >> 5] = v;
+  __syncthreads();
+  u64 before = (tid & 31) < (tid >> 5) ? red[tid & 31] : 0;
+  all = red[tid & 31];
+#pragma unroll
+  for (int w = 16; w; w >>= 1) {
+    before += __shfl_xor_sync(~0u, before, w);
+    all += __shfl_xor_sync(~0u, all, w);
+  }
+  return before + v;
+}
+
+// Mass of the ordered list's first n keys up to and including this thread's
+// positions tid + k kThreads; the sum over all.
+OSSM_DEV u64 masses(Room& s, int n, float m, float inv_t, u64 (&own)[kPer], u64 (&upto)[kPer]) {
+  u64 base = 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int e = threadIdx.x + k * kThreads;
+    own[k] = upto[k] = 0;
+    if (k * kThreads >= n) continue;
+    if (e < n) own[k] = mass_of(weight(logit_of(s.list[e]), m, inv_t));
+    u64 all;
+    upto[k] = base + block_scan(own[k], s.red, all);
+    base += all;
+  }
+  return base;
+}
+// How many of them the prefix holds that reaches `target` (at least one).
+OSSM_DEV int reaching(int n, const u64 (&own)[kPer], const u64 (&upto)[kPer], u64 target) {
+  int stay = 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k)
+    if (k * kThreads < n)
+      stay += __syncthreads_count((int)threadIdx.x + k * kThreads < n && upto[k] - own[k] < target);
+  return max(1, stay);
+}
+OSSM_DEV u64 share(float top_p, u64 whole) {  // the mass that a prefix has to reach
+  return max((u64)1, (u64)__double2ull_ru((double)top_p * (double)whole));
+}
+
+// The smallest key of the prefix of the candidates at or above `floor` that
+// holds `count` of them, or (count == 0) the share top_p of their mass; `whole`:
+// that mass where it is known, else 0.  Candidates below logit lb are known to
+// lie behind the prefix.  One CTA: a histogram of the logits between lb and the
+// largest, m; the keys of the bin where the prefix ends, in order; if they are
+// too many, radix passes of 8 bits over them.
+template <typename T>
+OSSM_DEV u64 select(const Row& r, const T* lg, int V, float m, float lb, u64 floor, u64 count, u64 whole, Room& s) {
+  const int tid = threadIdx.x;
+  const float scale = m > lb && m - lb < INFINITY ? (kBins - 1) / (m - lb) : 0.f;
+  const float c = r.inv_t * 1.44269504f;
+  auto rough = [&](float l) { return l == m ? 1.f : ex2((l - m) * c); };  // weight, to a few 2^-22
+  auto bin_of = [&](float l) { return m == l ? 0 : min(kBins - 1, (int)fminf((m - l) * scale, (float)kBins)); };
+  // Masses in steps of 2^-28 (the sums are compared with a share of the whole,
+  // which is at least 1), in two parts that 2^17 candidates cannot overflow;
+  // longer rows take one 64-bit sum, which costs a loop of exchanges.
+  const bool two = V <= (1 << 17);
+  uint32_t* part = reinterpret_cast<uint32_t*>(s.list);  // low 14 bits, high 15 bits; or the count
+  u64* wide = s.list;
+  __syncthreads();
+  for (int i = tid; i < kBins; i += kThreads) wide[i] = 0;
+  __syncthreads();
+  const float first = logit_of(floor);  // floor's logit: only there the index decides
+  scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
+#pragma unroll
+    for (int e = 0; e < Vec<T>::n; ++e) {
+      const bool in = e < n && live(l[e]) && l[e] >= lb && (floor == 0 || l[e] > first || key_of(l[e], i + e) >= floor);
+      if (!__any_sync(__activemask(), in)) continue;
+      const int b = bin_of(l[e]);
+      const uint32_t q = __float2uint_rn(rough(l[e]) * 0x1p28f);
+      if (!in) continue;
+      if (count) {
+        atomicAdd(part + 2 * b, 1u);
+      } else if (two) {
+        atomicAdd(part + 2 * b, q & 0x3fffu);
+        atomicAdd(part + 2 * b + 1, q >> 14);
+      } else {
+        atomicAdd(wide + b, (u64)q);
+      }
+    }
+  });
+  __syncthreads();
+  static_assert(kBins == kThreads, "a bin a thread");
+  const u64 own = count ? part[2 * tid] : two ? part[2 * tid] + ((u64)part[2 * tid + 1] << 14) : wide[tid];
+  u64 all;
+  const u64 upto = block_scan(own, s.red, all);
+  const u64 target = count ? count : share(r.top_p, whole ? whole >> 12 : all);
+  if (tid == 0) s.sh[0] = ~(u64)0;
+  __syncthreads();
+  if (upto - own < target && target <= upto) {
+    s.sh[0] = tid;
+    s.sh[1] = upto - own;
+  }
+  __syncthreads();
+  if (s.sh[0] == ~(u64)0) return floor;  // all of them stay
+  const int cut = (int)s.sh[0];
+  u64 left = target - s.sh[1];  // from the bin itself
+  __syncthreads();
+  auto each = [&](auto f) {  // the keys of the bin
+    scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
+#pragma unroll
+      for (int e = 0; e < Vec<T>::n; ++e)
+        if (e < n && live(l[e]) && l[e] >= lb && bin_of(l[e]) == cut) {
+          const u64 key = key_of(l[e], i + e);
+          if (key >= floor) f(key);
+        }
+    });
+    __syncthreads();
+  };
+  if (!count) left <<= 12;  // as masses of single candidates are: 2^-40
+  int* fill = reinterpret_cast<int*>(&s.sh[3]);
+  if (tid == 0) *fill = 0;
+  __syncthreads();
+  each([&](u64 key) {
+    const int at = atomicAdd(fill, 1);
+    if (at < kList) s.list[at] = key;
+  });
+  const int size = *fill;
+  if (size <= kList) {
+    order(s.list, size);
+    int at = (int)left;
+    if (!count) {
+      u64 o[kPer], u[kPer];
+      masses(s, size, m, r.inv_t, o, u);
+      at = reaching(size, o, u, left);
+    }
+    const u64 key = s.list[at - 1];
+    __syncthreads();
+    return key;
+  }
+  u64 prefix = 0;
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    __syncthreads();
+    if (tid < 256) s.list[tid] = 0;
+    __syncthreads();
+    each([&](u64 key) {
+      if (shift == 56 || (key >> (shift + 8)) == prefix)
+        atomicAdd(s.list + ((key >> shift) & 255), count ? (u64)1 : mass_of(weight(logit_of(key), m, r.inv_t)));
+    });
+    if (tid == 0) {
+      int d = 255;
+      for (; d > 0 && s.list[d] < left; --d) left -= s.list[d];
+      s.sh[0] = left;
+      s.sh[1] = (prefix << 8) | d;
+    }
+    __syncthreads();
+    left = s.sh[0];
+    prefix = s.sh[1];
+    __syncthreads();
+  }
+  return prefix;
+}
+
+// May the noise of a vector of logits be loaded 16 bytes at a time?
+template <typename T>
+OSSM_DEV bool noise_aligned(const T* lg, const float* nz) {
+  const int head = (int)((16 - ((uintptr_t)lg & 15)) & 15) / (int)sizeof(T);
+  return ((uintptr_t)(nz + head) & 15) == 0;
+}
+// The scores of the candidates `in` of a vector against the best so far.  The
+// logarithm in its fast form is within 2^-22 (of 1, or of its value), far below
+// the slack; the exact score is only taken of those that come that near.
+template <typename T>
+OSSM_DEV void race(const float* l, int i, int n, uint32_t in, const float* nz, bool aligned, float inv_t, Best& b) {
+  float e[Vec<T>::n];
+#pragma unroll
+  for (int k = 0; k < Vec<T>::n; k += 4) {
+    if (!(in >> k & 15u)) continue;
+    if (n > 1 && aligned) {
+      const float4 f = __ldcs(reinterpret_cast<const float4*>(nz + i + k));
+      e[k] = f.x, e[k + 1] = f.y, e[k + 2] = f.z, e[k + 3] = f.w;
+    } else {
+#pragma unroll
+      for (int h = k; h < k + 4; ++h)
+        if (in >> h & 1u) e[h] = nz[i + h];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < Vec<T>::n; ++k) {
+    const float x = l[k] * inv_t, s = fmaf(-0.693147181f, __log2f(e[k]), x);
+    if ((in >> k & 1u) && (!(s < b.s - (1e-4f + 1e-6f * fabsf(x))) || b.i < 0))
+      better(b, score_of(l[k], inv_t, e[k]), i + k);
+  }
 }
 
 // What the CTAs of a cluster tell each other.
@@ -256,9 +448,7 @@ struct Told {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
-  __shared__ u64 list[kList];
-  __shared__ u64 hist[256];
-  __shared__ u64 red[32], sh[2];
+  __shared__ Room room;
   __shared__ float redf[32];
   __shared__ Best bests[32];
   __shared__ Told told;
@@ -272,30 +462,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
 
   if (r.open()) {
     Best b{0.f, -1};
-    const bool aligned = Vec<T>::n >= 4 && [&] {
-      const int head = (int)((16 - ((uintptr_t)lg & 15)) & 15) / (int)sizeof(T);
-      return ((uintptr_t)(nz + head) & 15) == 0;
-    }();
+    const bool aligned = noise_aligned(lg, nz);
     scan(lg, p.V, rank, nrank, [&](const float* l, int i, int n) {
-      float e[Vec<T>::n];
-      if (n > 1 && aligned) {
+      uint32_t in = 0;
 #pragma unroll
-        for (int k = 0; k < Vec<T>::n; k += 4) {
-          const float4 f = __ldcs(reinterpret_cast<const float4*>(nz + i + k));
-          e[k] = f.x, e[k + 1] = f.y, e[k + 2] = f.z, e[k + 3] = f.w;
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < Vec<T>::n; ++k)
-          if (k < n) e[k] = nz[i + k];
-      }
-#pragma unroll
-      for (int k = 0; k < Vec<T>::n; ++k) {
-        if (k >= n || !live(l[k])) continue;
-        // log2.approx is within 2^-22 (of 1, or of its value): far below this slack
-        const float x = l[k] * r.inv_t, s = fmaf(-0.693147181f, __log2f(e[k]), x);
-        if (!(s < b.s - (1e-4f + 1e-6f * fabsf(x))) || b.i < 0) better(b, score_of(l[k], r.inv_t, e[k]), i + k);
-      }
+      for (int k = 0; k < Vec<T>::n; ++k) in |= k < n && live(l[k]) ? 1u << k : 0u;
+      race<T>(l, i, n, in, nz, aligned, r.inv_t, b);
     });
     b = block_best(b, bests);
     if (nrank > 1) {
@@ -324,18 +496,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     for (int e = 1; e < Vec<T>::n; ++e)
       if (e < n) top = fmaxf(top, l[e]);
     if (top > m) {
-      z = m == -INFINITY ? 0.f : z * exp2f((m - top) * c);
+      z = m == -INFINITY ? 0.f : z * ex2((m - top) * c);
       m = top;
     }
     if (need_z && live(m)) {
 #pragma unroll
       for (int e = 0; e < Vec<T>::n; ++e)
-        if (e < n) z += l[e] == m ? 1.f : exp2f((l[e] - m) * c);
+        if (e < n) z += ex2((l[e] - m) * c);
     }
   });
   const float cta_m = block_reduce(m, redf, [](float a, float b) { return fmaxf(a, b); });
   if (need_z)
-    z = block_reduce(live(m) ? z * (m == cta_m ? 1.f : exp2f((m - cta_m) * c)) : 0.f, redf,
+    z = block_reduce(live(m) ? z * (m == cta_m ? 1.f : ex2((m - cta_m) * c)) : 0.f, redf,
                      [](float a, float b) { return a + b; });
   // order bits that at least top_k of this CTA's threads' largest logits reach,
   // so at least top_k candidates: the 16 high bits by bisection
@@ -363,7 +535,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     z = 0.f;
     for (int k = 0; need_z && k < nrank; ++k) {
       const Told* o = cluster.map_shared_rank(&told, k);
-      if (live(o->m)) z += o->z * (o->m == m ? 1.f : exp2f((o->m - m) * c));
+      if (live(o->m)) z += o->z * (o->m == m ? 1.f : ex2((o->m - m) * c));
     }
   } else {
     m = cta_m;
@@ -374,6 +546,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     if (rank == 0 && tid == 0) p.out[row] = -1;
     return;
   }
+  // next to an infinite logit nothing else has weight; the sum is taken over the candidates then
+  const u64 whole = need_z && m < INFINITY ? (u64)((double)z * 0x1p40) : 0;
 
   // ---------------------------------------------------------------- Bound, and the candidates above it
   // With top_k: its own bound alone, as its mass counts for top_p.  Without:
@@ -381,24 +555,28 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   // together, so the prefix ends above them.  min_p only ever shortens.  The
   // logarithms' and the products' roundings are covered by the slack.
   uint32_t bound = tk;
+  float lb = -INFINITY;  // the same as a logit, of the bounds by mass
   if (!(top_k && by_mass)) {
     float y = -INFINITY;
     if (need_z) y = logf((1.f - r.top_p) * z / (float)p.V);
     if (!r.greedy && r.min_p > 0.f) y = fmaxf(y, logf(fminf(r.min_p, 1.f)));
     if (y > -INFINITY && m < INFINITY) {
-      const float lb = m + (y - 1e-3f - 1e-5f * fabsf(y)) / r.inv_t;
-      bound = max(bound, ord(fminf(lb - 1e-5f * (fabsf(m) + fabsf(lb)), m)));
+      lb = m + (y - 1e-3f - 1e-5f * fabsf(y)) / r.inv_t;
+      lb = fminf(lb - 1e-5f * (fabsf(m) + fabsf(lb)), m);
+      bound = max(bound, ord(lb));
     }
   }
   Told* first = nrank > 1 ? cluster.map_shared_rank(&told, 0) : &told;
-  u64* first_list = nrank > 1 ? cluster.map_shared_rank(list, 0) : list;
+  u64* first_list = nrank > 1 ? cluster.map_shared_rank(room.list, 0) : room.list;
+  const float low = bound ? fmaxf(logit_of((u64)bound << 32), -3.402823466e38f) : -3.402823466e38f;
+  bool over = false;  // the list is full: its end is found in another way
   scan(lg, p.V, rank, nrank, [&](const float* l, int i, int n) {
     uint32_t in = 0;
 #pragma unroll
-    for (int e = 0; e < Vec<T>::n; ++e)
-      if (e < n && live(l[e]) && ord(l[e]) >= bound) in |= 1u << e;
-    if (in) {
+    for (int e = 0; e < Vec<T>::n; ++e) in |= e < n && l[e] >= low ? 1u << e : 0u;
+    if (in && !over) {
       int at = atomicAdd(&first->count, __popc(in));
+      over = at >= kList;
 #pragma unroll
       for (int e = 0; e < Vec<T>::n; ++e)
         if (in >> e & 1u) {
@@ -421,108 +599,56 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     better(b, r.greedy ? 0.f : score_of(logit_of(key), r.inv_t, nz[i]), i);
   };
   if (N > kList) {
-    u64 top = 0;
-    if (r.greedy || r.min_p > 0.f) {  // the first candidate stays whatever min_p is
+    u64 top = 0, keep = 0;  // the first candidate (which stays whatever min_p is), the last one's key
+    float least = INFINITY;
+    if (r.greedy || r.min_p > 0.f || top_k || !live(lb)) {
       scan(lg, p.V, 0, 1, [&](const float* l, int i, int n) {
-        for (int e = 0; e < n; ++e)
-          if (live(l[e])) top = max(top, key_of(l[e], i + e));
+#pragma unroll
+        for (int e = 0; e < Vec<T>::n; ++e)
+          if (e < n && live(l[e])) top = max(top, key_of(l[e], i + e)), least = fminf(least, l[e]);
       });
-      top = block_reduce(top, red, [](u64 a, u64 b) { return max(a, b); });
+      top = block_reduce(top, room.red, [](u64 a, u64 b) { return max(a, b); });
+      least = block_reduce(least, redf, [](float a, float b) { return fminf(a, b); });
     }
     if (r.greedy) {
-      if (tid == 0) consider(top);
+      keep = top;
     } else {
-      const u64 keep = radix_prefix(r, lg, p.V, m, hist, red, sh);
-      scan(lg, p.V, 0, 1, [&](const float* l, int i, int n) {
-        for (int e = 0; e < n; ++e) {
-          const u64 key = key_of(l[e], i + e);
-          if (live(l[e]) && key >= keep && (!(r.min_p > 0.f) || key == top || weight(l[e], m, r.inv_t) >= r.min_p))
-            consider(key);
-        }
-      });
+      if (top_k) keep = select(r, lg, p.V, m, least, 0, (u64)top_k, 0, room);
+      if (by_mass)
+        keep = select(r, lg, p.V, m, live(lb) ? lb : top_k ? logit_of(keep) : least, keep, 0,
+                      whole, room);
     }
-  } else {
-    // in order, into registers: sorted position tid + k kThreads
-    constexpr int kPer = kList / kThreads;
-    u64 mine[kPer] = {};
-    if (N <= kRank) {
-      // a key's position is the number of larger ones; parts of the count by neighbouring threads
-      int parts = 1;
-      while (parts < 32 && N * parts * 2 <= kThreads) parts *= 2;
-      const int e = tid / parts, q = tid % parts;
-      u64 key = 0;
-      int larger = 0;
-      if (e < N) {
-        key = list[e];
-        for (int k = q; k < N; k += parts) larger += list[k] > key;
-      }
-      for (int w = 1; w < parts; w *= 2) larger += __shfl_xor_sync(~0u, larger, w);
-      __syncthreads();
-      if (e < N && q == 0) list[larger] = key;
-      __syncthreads();
-    } else {
-      int size = 1024;
-      while (size < N) size *= 2;
-      for (int k = N + tid; k < size; k += kThreads) list[k] = 0;
-      for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j; j /= 2) {
-          __syncthreads();
-          for (int e = tid; e < size / 2; e += kThreads) {
-            const int a = 2 * j * (e / j) + e % j, o = a + j;
-            const u64 x = list[a], y = list[o];
-            if ((x < y) == ((a & k) == 0)) list[a] = y, list[o] = x;  // descending
-          }
-        }
-      __syncthreads();
-    }
+    const float end = keep ? logit_of(keep) : -INFINITY;  // the last one's logit: only there the index decides
+    const bool aligned = noise_aligned(lg, nz);
+    scan(lg, p.V, 0, 1, [&](const float* l, int i, int n) {
+      uint32_t in = 0;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int e = tid + k * kThreads;
-      if (e < N) mine[k] = list[e];
-    }
+      for (int e = 0; e < Vec<T>::n; ++e)
+        in |= e < n && live(l[e]) && l[e] >= lb && (l[e] > end || (l[e] == end && key_of(l[e], i + e) >= keep))
+                  ? 1u << e : 0u;
+      if (r.min_p > 0.f) {
+#pragma unroll
+        for (int e = 0; e < Vec<T>::n; ++e)
+          if ((in >> e & 1u) && key_of(l[e], i + e) != top && weight(l[e], m, r.inv_t) < r.min_p) in &= ~(1u << e);
+      }
+      if (!in) return;
+      if (r.greedy) {
+        consider(keep);
+        return;
+      }
+      race<T>(l, i, n, in, nz, aligned, r.inv_t, b);
+    });
+  } else {
+    order(room.list, N);
     int n = top_k ? min(top_k, N) : N;
     if (by_mass) {
-      // mass up to and including each position, kThreads at a time
-      u64 upto[kPer], base = 0;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        upto[k] = 0;
-        if (k * kThreads >= N) continue;
-        u64 v = tid + k * kThreads < n ? mass_of(weight(logit_of(mine[k]), m, r.inv_t)) : 0;
-#pragma unroll
-        for (int w = 1; w < 32; w *= 2) {
-          const u64 u = __shfl_up_sync(~0u, v, w);
-          if ((tid & 31) >= w) v += u;
-        }
-        __syncthreads();
-        if ((tid & 31) == 31) red[tid >> 5] = v;
-        __syncthreads();
-        u64 before = (tid & 31) < (tid >> 5) ? red[tid & 31] : 0, all = red[tid & 31];
-#pragma unroll
-        for (int w = 16; w; w >>= 1) {
-          before += __shfl_xor_sync(~0u, before, w);
-          all += __shfl_xor_sync(~0u, all, w);
-        }
-        upto[k] = base + before + v;
-        base += all;
-      }
-      const double whole = top_k ? (double)base : (double)z * 0x1p40;
-      const double target = (double)r.top_p * whole;
-      int stay = 0;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        if (k * kThreads >= N) continue;
-        const int e = tid + k * kThreads;
-        const u64 own = e < n ? mass_of(weight(logit_of(mine[k]), m, r.inv_t)) : 0;
-        stay += __syncthreads_count(e < n && (double)(upto[k] - own) < target);
-      }
-      n = max(1, stay);
+      u64 own[kPer], upto[kPer];
+      const u64 all = masses(room, n, m, r.inv_t, own, upto);
+      n = reaching(n, own, upto, share(r.top_p, whole ? whole : all));
     }
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int e = tid + k * kThreads;
-      if (e < n && (e == 0 || r.greedy || !(r.min_p > 0.f) || weight(logit_of(mine[k]), m, r.inv_t) >= r.min_p))
-        consider(mine[k]);
+    for (int e = tid; e < n; e += kThreads) {
+      const u64 key = room.list[e];
+      if (e == 0 || r.greedy || !(r.min_p > 0.f) || weight(logit_of(key), m, r.inv_t) >= r.min_p) consider(key);
     }
   }
   b = block_best(b, bests);
