@@ -3,6 +3,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include <type_traits>
 
 #include "orthossm_b200.h"
@@ -14,6 +16,19 @@ namespace attn {
 constexpr int kMaxSeqs = 16384;
 constexpr int kMaxHD = 128;
 constexpr long long kMaxRows = 1LL << 30;  // positions and their differences stay within 32 bits
+
+// Lets a kernel have `bytes` of dynamic shared memory, once a device.
+template <typename K>
+cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 struct Params {
   int B, H, Hkv, hd;

@@ -921,7 +921,8 @@ template <typename T, int HDP>
 cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid,
                    cudaStream_t st) {
   auto kern = attn_prompt_kernel<T, HDP>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HDP>::kSmem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(kern, (int)Cfg<HDP>::kSmem, done);
   if (e != cudaSuccess) return e;
   kern<<<grid, kThreads, Cfg<HDP>::kSmem, st>>>(q, k, v, p, (p.H / p.Hkv) % 2 == 0);
   return cudaGetLastError();

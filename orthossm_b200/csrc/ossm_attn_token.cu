@@ -493,7 +493,8 @@ template <typename T, int HDP>
 cudaError_t launch(const Params& p, int sms, cudaStream_t st) {
   using C = Cfg<HDP>;
   auto kern = attn_token_kernel<T, HDP>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(kern, C::kSmem, done);
   if (e != cudaSuccess) return e;
   kern<<<sms * C::kCtas, kThreads, C::kSmem, st>>>(p);
   return cudaGetLastError();

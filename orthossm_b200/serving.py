@@ -22,19 +22,54 @@ _DT_ATTN = {torch.bfloat16: L.OSSM_BF16, torch.float16: L.OSSM_F16}
 _DT_SAMPLE = {torch.float32: L.OSSM_F32, torch.bfloat16: L.OSSM_BF16, torch.float16: L.OSSM_F16}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a Stream object (2 us)
+_ATTN_WS: dict = {}  # (device index, stream) -> (workspace address, bytes), of the tensors in _WS_ATTN
+
+
+def _rows_ok(st, sh, sd, n, heads, ptr):
+    """Strides and base of a [n, heads, head_dim] tensor that suit 16-byte accesses."""
+    return sd == 1 and not (st % 8 or sh % 8 or ptr % 16) and (st > 0 or n <= 1) and (sh > 0 or heads <= 1)
+
+
 def _tma_rows(t):
-    """t [rows, heads, head_dim] itself where its strides and base suit 16-byte
-    accesses, else a contiguous copy."""
-    st, sh, sd = t.stride()
-    ok = (sd == 1 and st % 8 == 0 and sh % 8 == 0 and (st > 0 or t.shape[0] <= 1) and (sh > 0 or t.shape[1] <= 1)
-          and t.data_ptr() % 16 == 0)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    """t [rows, heads, head_dim] itself where it can be read as it is, else a contiguous copy."""
+    return t if _rows_ok(*t.stride(), t.shape[0], t.shape[1], t.data_ptr()) else \
+        t.clone(memory_format=torch.contiguous_format)
 
 
-def _index(t, n, what, dev):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != dev:
-        raise ValueError(f"packed_attention: {what} must be an int32 vector of {n} on {dev}")
-    return t if t.is_contiguous() else t.contiguous()
+def _vector(t, n, dev):
+    return t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.get_device() == dev
+
+
+def _refuse_attention(q, k, v, cu_q, cu_k, kv_lengths, window, scale, out):
+    """Raises for the first argument of packed_attention that does not fit."""
+    _need_cuda(q, k, v, cu_q, cu_k, kv_lengths, out)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+        raise ValueError(f"packed_attention: q [Tq,H,hd] and k, v [Tk,Hkv,hd] expected, got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in _DT_ATTN or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"packed_attention: q, k, v must share bf16 or fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    dev = q.get_device()
+    if k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("packed_attention: q, k, v must be on one device")
+    B = cu_q.shape[0] - 1 if cu_q.dim() == 1 else 0
+    if not 1 <= B <= 16384:
+        raise ValueError(f"packed_attention: 1 to 16384 sequences, got {B}")
+    for t, n, what in ((cu_q, B + 1, "cu_seqlens_q"), (cu_k, B + 1, "cu_seqlens_k"), (kv_lengths, B, "kv_lengths")):
+        if t is not None and not _vector(t, n, dev):
+            raise ValueError(f"packed_attention: {what} must be an int32 vector of {n} on {q.device}")
+    if window is not None and window < 1:
+        raise ValueError(f"packed_attention: window must be at least 1, got {window}")
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
+    if out is not None:
+        if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev:
+            raise ValueError("packed_attention: out must have q's shape, dtype and device")
+        if _tma_rows(out) is not out:
+            raise ValueError("packed_attention: out needs a unit channel stride and 16-byte aligned rows")
+    hd, H, Hkv = q.shape[2], q.shape[1], k.shape[1]
+    raise ValueError(f"packed_attention: head_dim {hd} and {k.shape[2]} (equal, a multiple of 8, at most 128) or heads "
+                     f"{H} / {Hkv} (a multiple) not supported")
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -62,75 +97,85 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     and values that a query does not see do not reach its output, whatever
     they hold.  scale: default 1 / sqrt(hd).  Rows of q outside every sequence
     are not written.  Returns [Tq, H, hd] in q's dtype (``out`` if given)."""
-    _need_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, kv_lengths, out)
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
-        raise ValueError(f"packed_attention: q [Tq,H,hd] and k, v [Tk,Hkv,hd] expected, got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    dev = q.get_device()
     dt = _DT_ATTN.get(q.dtype)
-    if dt is None or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"packed_attention: q, k, v must share bf16 or fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
-    Tq, H, hd = q.shape
-    Tk, Hkv, _ = k.shape
-    if k.shape[2] != hd or hd % 8 or not 8 <= hd <= 128 or Hkv < 1 or H < 1 or H % Hkv:
-        raise ValueError(f"packed_attention: head_dim {hd} (a multiple of 8 up to 128, the same in k) or heads "
-                         f"{H} / {Hkv} (a multiple) not supported")
-    dev = q.device
-    if k.device != dev or v.device != dev:
-        raise ValueError("packed_attention: q, k, v must be on one device")
-    B = cu_seqlens_q.shape[0] - 1
-    if not 1 <= B <= 16384:
-        raise ValueError(f"packed_attention: 1 to 16384 sequences, got {B}")
-    cu_q = _index(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
-    cu_k = cu_q if cu_seqlens_k is None else _index(cu_seqlens_k, B + 1, "cu_seqlens_k", dev)
-    if kv_lengths is not None:
-        kv_lengths = _index(kv_lengths, B, "kv_lengths", dev)
-    if window is not None and window < 1:
-        raise ValueError(f"packed_attention: window must be at least 1, got {window}")
-    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"packed_attention: scale must be positive and finite, got {scale}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    scale_ = scale
+    ok = dev >= 0 and dt is not None and q.dim() == 3 and k.dim() == 3 and cu_seqlens_q.dim() == 1
+    if ok:
+        Tq, H, hd = q.shape
+        Tk, Hkv, hdk = k.shape
+        B = cu_seqlens_q.shape[0] - 1
+        cu_k = cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k
+        scale_ = hd ** -0.5 if scale is None and hd else scale
+        ok = (v.shape == k.shape and k.dtype == q.dtype and v.dtype == q.dtype and k.get_device() == dev
+              and v.get_device() == dev and hdk == hd and hd % 8 == 0 and 8 <= hd <= 128 and Hkv > 0 and H > 0
+              and H % Hkv == 0 and 1 <= B <= 16384 and _vector(cu_seqlens_q, B + 1, dev)
+              and (cu_k is cu_seqlens_q or _vector(cu_k, B + 1, dev))
+              and (kv_lengths is None or _vector(kv_lengths, B, dev)) and (window is None or window >= 1)
+              and 0.0 < scale_ < math.inf
+              and (out is None or (out.shape == q.shape and out.dtype == q.dtype and out.get_device() == dev)))
+    if not ok:
+        _refuse_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, kv_lengths, window, 1.0 if scale_ is None else scale_,
+                          out)
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError("packed_attention has no backward pass: call it under torch.no_grad()")
     if out is None:
-        out = torch.empty(Tq, H, hd, dtype=q.dtype, device=dev)
-    else:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
-            raise ValueError("packed_attention: out must have q's shape, dtype and device")
-        if _tma_rows(out) is not out:
-            raise ValueError("packed_attention: out needs a unit channel stride and 16-byte aligned rows")
+        out = torch.empty((Tq, H, hd), dtype=q.dtype, device=q.device)
     if Tq == 0:
         return out
-    q, k, v = _tma_rows(q), _tma_rows(k), _tma_rows(v)
-    a = L.AttnArgs(B, H, Hkv, hd, Tq, Tk, int(max_seqlen_q), dt, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                   out.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                   out.stride(0), out.stride(1), cu_q.data_ptr(), cu_k.data_ptr(), _ptr(kv_lengths),
-                   min(int(window), 0x7fffffff) if window is not None else 0, scale)
-    lib = L.lib()
-    ref = L.C.byref(a)
-    if dev.index != torch.cuda.current_device():
+    layout = []
+    for t, n, heads in ((q, Tq, H), (k, Tk, Hkv), (v, Tk, Hkv), (out, Tq, H)):
+        st, sh, sd = t.stride()
+        ptr = t.data_ptr()
+        if not _rows_ok(st, sh, sd, n, heads, ptr):
+            if t is out:
+                _refuse_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, kv_lengths, window, scale_, out)
+            t = t.clone(memory_format=torch.contiguous_format)
+            st, sh, _ = t.stride()
+            ptr = t.data_ptr()
+        layout.append((t, ptr, st, sh))  # t: kept until the launch
+    (_, qp, qt, qh), (_, kp, kt, kh), (_, vp, vt, vh), (_, op, ot, oh) = layout
+    if not cu_seqlens_q.is_contiguous():
+        cu_seqlens_q, cu_k = cu_seqlens_q.contiguous(), cu_k.contiguous()
+    elif not cu_k.is_contiguous():
+        cu_k = cu_k.contiguous()
+    if kv_lengths is not None and not kv_lengths.is_contiguous():
+        kv_lengths = kv_lengths.contiguous()
+    a = L.AttnArgs(B, H, Hkv, hd, Tq, Tk, min(int(max_seqlen_q), 0x7fffffff), dt, qp, kp, vp, op, qt, qh, kt, kh, vt,
+                   vh, ot, oh, cu_seqlens_q.data_ptr(), cu_k.data_ptr(),
+                   None if kv_lengths is None else kv_lengths.data_ptr(),
+                   0 if window is None else min(int(window), 0x7fffffff), scale_)
+    if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _attention(lib, ref, dev, out)
-    return _attention(lib, ref, dev, out)
-
-
-def _attention(lib, ref, dev, out):
-    nbytes = lib.ossm_attn_workspace_bytes(ref)
-    if nbytes == 0:
-        L.check(L.OSSM_EINVAL, "packed_attention (argument check)")
-    stream = torch.cuda.current_stream(dev)
-    ws = _workspace(dev, stream, nbytes, cache=_WS_ATTN)
-    L.check(lib.ossm_attention_fwd(ref, ws.data_ptr(), ws.numel(), stream.cuda_stream), "packed_attention")
+            _attention(a, dev)
+    else:
+        _attention(a, dev)
     return out
 
 
+def _attention(a, dev):
+    lib = L.lib()
+    stream = _raw_stream(dev)
+    ref = L.C.byref(a)
+    ws = _ATTN_WS.get((dev, stream))
+    status = L.OSSM_EWORKSPACE if ws is None else lib.ossm_attention_fwd(ref, ws[0], ws[1], stream)
+    if status == L.OSSM_EWORKSPACE:  # the first call on this stream, or one that needs more
+        nbytes = lib.ossm_attn_workspace_bytes(ref)
+        if nbytes == 0:
+            L.check(L.OSSM_EINVAL, "packed_attention (argument check)")
+        device = torch.device("cuda", dev)
+        t = _workspace(device, torch.cuda.current_stream(device), nbytes, cache=_WS_ATTN)
+        _ATTN_WS[dev, stream] = (t.data_ptr(), t.numel())
+        status = lib.ossm_attention_fwd(ref, t.data_ptr(), t.numel(), stream)
+    if status != L.OSSM_OK:
+        L.check(status, "packed_attention")
+
+
 def _setting(x, dtype, B, what, dev):
-    """(scalar, pointer, tensor to keep) of a setting given as a number or as a tensor [B]."""
-    if isinstance(x, torch.Tensor):
-        if x.dim() != 1 or x.shape[0] != B or x.device != dev:
-            raise ValueError(f"sample_tokens: {what} must be a number or a vector of {B} on {dev}")
-        x = x.to(dtype).contiguous()
-        return 0, x.data_ptr(), x
-    return x, None, None
+    """A setting given as a tensor [B], in the kernel's type."""
+    if x.dim() != 1 or x.shape[0] != B or x.get_device() != dev:
+        raise ValueError(f"sample_tokens: {what} must be a number or a vector of {B} on the logits' device")
+    return x if x.dtype == dtype and x.is_contiguous() else x.to(dtype).contiguous()
 
 
 def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
@@ -155,42 +200,52 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
     and -inf logits are never drawn; a row that has nothing else gives -1.
     Returns int64 [B] (``out`` if given)."""
     _need_cuda(logits, noise, out)
-    if logits.dim() != 2 or logits.dtype not in _DT_SAMPLE:
+    dt = _DT_SAMPLE.get(logits.dtype)
+    if logits.dim() != 2 or dt is None:
         raise ValueError(f"sample_tokens: logits [B,V] in fp32, bf16 or fp16 expected, got {tuple(logits.shape)} "
                          f"{logits.dtype}")
     B, V = logits.shape
-    dev = logits.device
+    dev = logits.get_device()
     if V < 1:
         raise ValueError("sample_tokens: no candidates")
-    if noise is not None:
-        if noise.shape != logits.shape or noise.dtype != torch.float32 or noise.device != dev:
-            raise ValueError("sample_tokens: noise must be fp32 with the logits' shape and device")
-        if noise.stride(1) != 1:
-            noise = noise.contiguous()
-    if logits.stride(1) != 1:
+    lst, unit = logits.stride()
+    if unit != 1:
         logits = logits.contiguous()
+        lst = logits.stride(0)
+    nst = 0
+    if noise is not None:
+        if noise.shape != logits.shape or noise.dtype != torch.float32 or noise.get_device() != dev:
+            raise ValueError("sample_tokens: noise must be fp32 with the logits' shape and device")
+        nst, unit = noise.stride()
+        if unit != 1:
+            noise = noise.contiguous()
+            nst = noise.stride(0)
     if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=dev)
-    elif out.shape != (B,) or out.dtype != torch.int64 or out.device != dev or not out.is_contiguous():
+        out = torch.empty(B, dtype=torch.int64, device=logits.device)
+    elif out.shape != (B,) or out.dtype != torch.int64 or out.get_device() != dev or not out.is_contiguous():
         raise ValueError("sample_tokens: out must be a contiguous int64 [B] on the logits' device")
-    t, t_row, t_keep = _setting(temperature, torch.float32, B, "temperature", dev)
-    k, k_row, k_keep = _setting(top_k, torch.int32, B, "top_k", dev)
-    p, p_row, p_keep = _setting(top_p, torch.float32, B, "top_p", dev)
-    m, m_row, m_keep = _setting(min_p, torch.float32, B, "min_p", dev)
+    t, k, p, m = temperature, top_k, top_p, min_p
+    t_row = k_row = p_row = m_row = None  # kept until the launch
+    if isinstance(t, torch.Tensor):
+        t_row, t = _setting(t, torch.float32, B, "temperature", dev), 0.0
+    if isinstance(k, torch.Tensor):
+        k_row, k = _setting(k, torch.int32, B, "top_k", dev), 0
+    if isinstance(p, torch.Tensor):
+        p_row, p = _setting(p, torch.float32, B, "top_p", dev), 0.0
+    if isinstance(m, torch.Tensor):
+        m_row, m = _setting(m, torch.float32, B, "min_p", dev), 0.0
     if not (0.0 <= t < math.inf and k >= 0 and 0.0 <= p <= 1.0 and 0.0 <= m <= 1.0):
         raise ValueError(f"sample_tokens: temperature {t} must be >= 0 and finite, top_k {k} >= 0, top_p {p} and "
                          f"min_p {m} in [0, 1]")
     if B == 0:
         return out
-    a = L.SampleArgs(B, V, logits.data_ptr(), _DT_SAMPLE[logits.dtype], logits.stride(0), _ptr(noise),
-                     0 if noise is None else noise.stride(0), 1.0 / t if t > 0 else 0.0, p, m, min(int(k), V), t_row,
-                     p_row, m_row, k_row, out.data_ptr())
-    if dev.index != torch.cuda.current_device():
+    a = L.SampleArgs(B, V, logits.data_ptr(), dt, lst, _ptr(noise), nst, 1.0 / t if t > 0 else 0.0, p, m, min(int(k), V),
+                     _ptr(t_row), _ptr(p_row), _ptr(m_row), _ptr(k_row), out.data_ptr())
+    if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _sample(a, dev, out)
-    return _sample(a, dev, out)
-
-
-def _sample(a, dev, out):
-    L.check(L.lib().ossm_sample_tokens(L.C.byref(a), torch.cuda.current_stream(dev).cuda_stream), "sample_tokens")
+            status = L.lib().ossm_sample_tokens(L.C.byref(a), _raw_stream(dev))
+    else:
+        status = L.lib().ossm_sample_tokens(L.C.byref(a), _raw_stream(dev))
+    if status != L.OSSM_OK:
+        L.check(status, "sample_tokens")
     return out
