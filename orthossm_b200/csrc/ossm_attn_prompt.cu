@@ -146,6 +146,12 @@ struct Sched {
     if (it.end() - pos <= near + kItemCost) return it.end();
     return pos - it.start <= near ? it.start : pos;
   }
+  OSSM_DEV int owner(i64 pos) const {  // the CTA whose part holds a position: the last with cut(c) <= pos
+    int c = (int)min((i64)ncta - 1, pos / max((i64)1, total / ncta));
+    while (c > 0 && cut(c) > pos) --c;
+    while (c + 1 < ncta && cut(c + 1) <= pos) ++c;
+    return c;
+  }
 };
 
 // A CTA's share of one item, as the roles read it.
@@ -496,9 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             c.len = x.n();
             c.start = x.start;
             c.slot = head ? 2 * cta + 1 : 2 * cta;
-            int f = cta;
-            while (f > 0 && sc.cut(f) > x.start) --f;
-            c.first = f;
+            c.first = head ? cta : sc.owner(x.start);
           }
           break;
         }
@@ -854,10 +858,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __threadfence();
       // the last one in joins the pieces in the order of the cut
-      const i64 stop = c.start + c.len;
       float M = -INFINITY, Ls = 0.f;
-      int npieces = 1;
-      while (c.first + npieces < sc.ncta && sc.cut(c.first + npieces) < stop) ++npieces;
+      const int npieces = sc.owner(c.start + c.len - 1) - c.first + 1;
       for (int k = 0; k < npieces; ++k) {
         const float* q = p.part + (size_t)(k ? 2 * (c.first + k) : 2 * c.first + 1) * C::kPartFloats;
         M = fmaxf(M, __ldcg(q + r2));

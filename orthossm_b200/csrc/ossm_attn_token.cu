@@ -99,6 +99,12 @@ struct Line {
     if (it.end() - pos <= near + kItemCost) return it.end();
     return pos - it.start <= near ? it.start : pos;
   }
+  OSSM_DEV int owner(i64 pos) const {  // the CTA whose part holds a position: the last with cut(c) <= pos
+    int c = (int)min((i64)ncta - 1, pos / max((i64)1, total / ncta));
+    while (c > 0 && cut(c) > pos) --c;
+    while (c + 1 < ncta && cut(c + 1) <= pos) ++c;
+    return c;
+  }
 };
 
 template <typename T>
@@ -404,8 +410,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
     int first = 0;
     float* part = nullptr;
     if (split) {
-      first = cta;
-      while (first > 0 && ln.cut(first) > x.start) --first;
+      first = head ? cta : ln.owner(x.start);
       part = p.part + (size_t)(head ? 2 * cta + 1 : 2 * cta) * C::kPartFloats;
     }
     T* out = static_cast<T*>(p.out);
@@ -454,8 +459,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       __syncthreads();
       if (last_in) {
         __threadfence();
-        int np = 1;
-        while (first + np < ln.ncta && ln.cut(first + np) < x.start + x.n) ++np;
+        const int np = ln.owner(x.start + x.n - 1) - first + 1;
         auto piece = [&](int k) { return p.part + (size_t)(k ? 2 * (first + k) : 2 * first + 1) * C::kPartFloats; };
         for (int e = threadIdx.x; e < nrows * CH; e += kThreads) {
           const int r = e / CH, d = (e % CH) * 8;
