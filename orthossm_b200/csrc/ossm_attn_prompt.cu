@@ -1,8 +1,9 @@
 // Attention of many queries a sequence: prompts, pieces of prompts.
 //
-// Work item: two tiles of 128 query rows that share their keys: the same 128
-// queries of two neighbouring heads of a group (an even number of query heads
-// per key head), or 256 queries of one head.  An item walks its range of
+// Work item: two tiles of 128 rows that share their keys.  A row is a query of
+// one of g heads (row = query * g + head), g the largest power of two that
+// divides the heads per key head: one read of K and V serves the group, and a
+// few queries of a large group still fill a tile.  An item walks its range of
 // 128-key tiles once with a running maximum and sum per row.
 //
 // One persistent CTA per SM, three warpgroups:
@@ -58,42 +59,53 @@ constexpr int kBox = kT * 128;      // bytes of a [128 rows x 64 channels] box
 // ---------------------------------------------------------------- schedule
 typedef long long i64;
 
-OSSM_DEV int floor_div(int a, int b) { return a >= 0 ? a / b : -((b - 1 - a) / b); }
-OSSM_DEV int ceil_div(int a, int b) { return -floor_div(-a, b); }
+// Positions are divided by powers of two only: shifts, rounding down.
+constexpr int kLT = 7;  // log2 of a tile's rows and keys
 
-// sum over i < n of max(0, a + s i)
-OSSM_DEV i64 ramp(int n, int a, int s) {
-  const int i0 = a >= 0 ? 0 : (-a + s - 1) / s;
-  const i64 c = max(0, n - i0);
-  return c * a + (i64)s * (c * i0 + c * (c - 1) / 2);
+// sum over i < n of max(0, floor((x + i 2^lq) / 128))
+OSSM_DEV i64 ramp(int n, int x, int lq) {
+  if (lq >= kLT) {  // floor(x / 128) + i s
+    const int a = x >> kLT, ls = lq - kLT;
+    const int i0 = a >= 0 ? 0 : (-a + (1 << ls) - 1) >> ls;
+    const i64 c = max(0, n - i0);
+    return c * a + ((c * i0 + c * (c - 1) / 2) << ls);
+  }
+  const int lr = kLT - lq;  // floor((floor(x / 2^lq) + i) / 2^lr)
+  auto upto = [lr](i64 m) {
+    const i64 t = m > 0 ? m >> lr : 0;
+    return m > 0 ? ((t * (t - 1) / 2) << lr) + (m - (t << lr)) * t : 0;
+  };
+  const i64 c = x >> lq;
+  return upto(c + n) - upto(c);
 }
 
-// A sequence's blocks of s * 128 query rows: block i walks key tiles
-// [max(0, b + i s), min(max(0, a + (i + 1) s), t)).
+// A sequence's blocks of 2 * 128 rows, 2^lq queries each: block i walks key
+// tiles [lo(i), hi(i)).
 struct Shape {
-  int nblk, a, b, t, s;
-  OSSM_DEV int lo(int i) const { return max(0, b + i * s); }
-  OSSM_DEV int hi(int i) const { return min(max(0, a + (i + 1) * s), t); }
+  int nblk, lq, t;  // t: the sequence's key tiles
+  int x_lo, x_hi;   // lo(i) = floor((x_lo + i 2^lq) / 128), hi(i) = floor((x_hi + i 2^lq) / 128), within 0 .. t
+  OSSM_DEV int lo(int i) const { return max(0, (x_lo + (i << lq)) >> kLT); }
+  OSSM_DEV int hi(int i) const { return min(max(0, (x_hi + (i << lq)) >> kLT), t); }
   OSSM_DEV i64 before(int i) const {  // length of the blocks before i
-    return ramp(i, a + s, s) - ramp(i, a + s - t, s) - ramp(i, b, s) + (i64)i * kItemCost;
+    return ramp(i, x_hi, lq) - ramp(i, x_hi - (t << kLT), lq) - ramp(i, x_lo, lq) + (i64)i * kItemCost;
   }
 };
-OSSM_DEV Shape shape_of(const Params& p, const Seq& q, int s) {
-  const int off = q.nk - q.nq;
+OSSM_DEV Shape shape_of(const Params& p, const Seq& s, int lg) {
+  const int off = s.nk - s.nq;
   Shape f;
-  f.s = s;
-  f.nblk = (q.nq + s * kT - 1) / (s * kT);
-  f.a = ceil_div(off, kT);
-  f.t = (q.nk + kT - 1) / kT;
+  f.lq = kLT + 1 - lg;
+  f.nblk = (s.nq + (1 << f.lq) - 1) >> f.lq;
+  f.t = (s.nk + kT - 1) >> kLT;
+  f.x_hi = off + (1 << f.lq) + kT - 1;  // the keys up to the block's last query, in tiles, rounded up
   // no window: the lower edge stays at 0 for every block
-  f.b = p.window ? floor_div(off - p.window + 1, kT) : -(f.nblk * s + 1);
+  f.x_lo = p.window ? off - p.window + 1 : -(f.nblk << f.lq);
   return f;
 }
 
 struct Sched {
   const Params& p;
   const i64* pre;  // [ngroups + 1] length of the line before each group of sequences
-  int ngroups, gsz, s, units;
+  int ngroups, gsz, lg, units;
   i64 total;
   int ncta;
 
@@ -118,7 +130,7 @@ struct Sched {
     i64 one = 0;
     for (int b = lo * gsz;; ++b) {
       it.q = seq_of(p, b);
-      it.f = shape_of(p, it.q, s);
+      it.f = shape_of(p, it.q, lg);
       one = it.f.before(it.f.nblk);
       if (pos < base + one * units || b + 1 >= min(p.B, (lo + 1) * gsz)) break;
       base += one * units;
@@ -157,10 +169,12 @@ struct Sched {
 // A CTA's share of one item, as the roles read it.
 struct Piece {
   int live;                // 0: no more pieces
-  int q0, nq, off, k0, nk; // the sequence
-  int head[2], row0[2];    // of the two tiles; row0: first row in the sequence
+  int q0, off, k0, nk;     // the sequence
+  int nrows;               // its rows
+  int head, row0;          // first head; first row of tile 0 (tile 1: 128 further)
   int j0, j1;              // the piece's key tiles
   int lo[2], hi[2];        // each tile's share of them
+  int w0[2], w1[2];        // key tiles that every row of the tile sees whole
   int split;               // the item has other pieces
   int slot, first, len;    // split: this piece's slot, the CTA with the item's first piece, the item's key tiles
   i64 start;               // split: the item's start on the line
@@ -312,11 +326,6 @@ OSSM_DEV bool meet_any(uint32_t id, uint32_t n, bool pred) {
   return r != 0;
 }
 
-// Does some row of a tile, at positions first to last, miss a key of key tile j?
-OSSM_DEV bool partly(int window, int first, int last, int j) {
-  return j * kT + kT - 1 > first || (window && j * kT <= last - window);
-}
-
 OSSM_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {  // has the phase passed? (may doze off for a moment)
   uint32_t done;
   asm volatile(
@@ -365,7 +374,8 @@ struct Waits {
 template <typename T, int HDP>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_prompt_kernel(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
-                       const __grid_constant__ CUtensorMap mV, const __grid_constant__ Params p, const int pair_heads) {
+                       const __grid_constant__ CUtensorMap mV, const __grid_constant__ Params p,
+                       const int lg) {  // log2 of g
   using C = Cfg<HDP>;
   constexpr int NS = C::kSlots;
   extern __shared__ uint8_t smem_raw[];
@@ -383,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ------------------------------------------------------------ schedule
   const int gsz = (p.B + kGroups - 1) / kGroups, ngroups = (p.B + gsz - 1) / gsz;
-  const int s = pair_heads ? 1 : 2, units = pair_heads ? p.H / 2 : p.H;
+  const int units = p.H >> lg;
   if (threadIdx.x == 0) {
     n_items = 0;
     failed = 0;
@@ -393,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int g = threadIdx.x; g < ngroups; g += kThreads) {
     i64 len = 0;
     for (int b = g * gsz; b < min(p.B, (g + 1) * gsz); ++b) {
-      const Shape f = shape_of(p, seq_of(p, b), s);
+      const Shape f = shape_of(p, seq_of(p, b), lg);
       len += f.before(f.nblk) * units;
       mine += (unsigned long long)f.nblk * units;
     }
@@ -416,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) pre[0] = 0;
   }
   __syncthreads();
-  Sched sc{p, pre, ngroups, gsz, s, units, pre[ngroups], 0};
+  Sched sc{p, pre, ngroups, gsz, lg, units, pre[ngroups], 0};
   // as many CTAs as there are items or pieces of 8 key tiles
   sc.ncta = (int)min((i64)gridDim.x, max((i64)n_items, sc.total / 8));
   if (cta >= sc.ncta) return;
@@ -485,17 +495,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           pos = min(end, x.end());
           if (a >= b && !(head && x.n() == 0)) continue;
           c.live = 1;
-          c.q0 = x.q.q0, c.nq = x.q.nq, c.k0 = x.q.k0, c.nk = x.q.nk, c.off = x.q.nk - x.q.nq;
+          c.q0 = x.q.q0, c.k0 = x.q.k0, c.nk = x.q.nk, c.off = x.q.nk - x.q.nq;
+          c.nrows = x.q.nq << lg;
+          c.head = x.unit << lg;
+          c.row0 = x.blk * 2 * kT;
           const int base = x.f.lo(x.blk);
           c.j0 = base + a, c.j1 = base + b;
           for (int t = 0; t < 2; ++t) {
-            c.head[t] = pair_heads ? 2 * x.unit + t : x.unit;
-            c.row0[t] = pair_heads ? x.blk * kT : (2 * x.blk + t) * kT;
-            const int first = c.row0[t] + c.off, top = min(c.row0[t] + kT, c.nq) - 1 + c.off;
-            int lo = p.window ? max(0, first - p.window + 1) / kT : 0, hi = top < 0 ? 0 : top / kT + 1;
-            if (c.row0[t] >= c.nq) hi = lo = 0;
+            const int row0 = c.row0 + t * kT, first = (row0 >> lg) + c.off;
+            const int top = ((min(row0 + kT, c.nrows) - 1) >> lg) + c.off;
+            int lo = p.window ? max(0, first - p.window + 1) >> kLT : 0, hi = top < 0 ? 0 : (top >> kLT) + 1;
+            if (row0 >= c.nrows) hi = lo = 0;
             c.lo[t] = max(lo, c.j0);
             c.hi[t] = max(c.lo[t], min(hi, c.j1));
+            c.w0[t] = p.window ? ((top - p.window) >> kLT) + 1 : 0;
+            c.w1[t] = (first + 1) >> kLT;
           }
           c.split = b - a < x.n();
           if (c.split) {
@@ -514,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         pieces[sl] = c;
         mbar_arrive(&bars.piece_full[sl]);
         if (!c.live) break;
-        const int kvh = c.head[0] / (p.H / p.Hkv);
+        const int kvh = c.head / (p.H / p.Hkv);
         for (int j = c.j0; j < c.j1 && ok; ++j) {
           if (j == c.j0)
             for (int t = 0; t < 2 && ok; ++t) {
@@ -526,7 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               ++nq[t];
               mbar_expect_tx(&bars.q_full[t], C::kTile);
               for (int x = 0; x < C::kBoxes; ++x)
-                tma_load_3d(smem + t * C::kTile + x * kBox, &mQ, &bars.q_full[t], 64 * x, c.head[t], c.q0 + c.row0[t]);
+                tma_load_3d(smem + t * C::kTile + x * kBox, &mQ, &bars.q_full[t], 64 * x, c.head,
+                            c.q0 + ((c.row0 + t * kT) >> lg));
             }
           ok = ok && load(false, kvh, c.k0 + j * kT) && (j == c.j0 || load(true, kvh, c.k0 + (j - 1) * kT));
         }
@@ -662,8 +677,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Piece& c = pieces[sl];  // given back at the piece's end
       if (!c.live) break;
       const int lo = c.lo[t], hi = c.hi[t], j0 = c.j0;
-      const int first = c.row0[t] + c.off, at = first + row;  // the position of the tile's first row, and of this one
-      const int last = min(c.row0[t] + kT, c.nq) - 1 + c.off;
+      const int row0 = c.row0 + t * kT;
+      int w0 = c.w0[t], w1 = c.w1[t], at = ((row0 + row) >> lg) + c.off;  // the row's position
+      asm volatile("" : "+r"(w0), "+r"(w1), "+r"(at));  // in registers, not worked out again for every tile
       float m = -INFINITY, l = 0.f;
       for (int j = lo; j < hi; ++j) {
         wait(&bars.s_full[t], ns & 1);
@@ -676,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) pin32(x + 32 * i);
         free_scores();
-        const bool part = partly(p.window, first, last, j);
+        const bool part = j < w0 || j >= w1;
         const int k_hi = at - j * kT, k_lo = p.window ? k_hi - p.window + 1 : -1;  // seen: k_lo <= key <= k_hi
         if (part) {
 #pragma unroll
@@ -787,8 +803,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       it += c.j1 - j0;
       settled(ns);
-      const bool mine_row = c.row0[t] + row < c.nq;
-      T* out = static_cast<T*>(p.out) + (i64)(c.q0 + c.row0[t] + row) * p.ost + (i64)c.head[t] * p.osh;
+      const bool mine_row = row0 + row < c.nrows;
+      T* out = static_cast<T*>(p.out) + (i64)(c.q0 + ((row0 + row) >> lg)) * p.ost +
+               (i64)(c.head + ((row0 + row) & ((1 << lg) - 1))) * p.osh;
       if (!c.split) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
@@ -903,15 +920,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0 && failed) atomicExch(&p.hdr->status, (uint32_t)OSSM_ETIMEOUT);
 }
 
-// [rows, heads, hd] as (channel, head, row); box: 128 rows of 64 channels of
-// one head; channels past hd and rows past the end read as zero.
-bool encode(CUtensorMap* map, int dtype, const void* base, int hd, int heads, i64 rows, i64 st, i64 sh) {
+// [rows, heads, hd] as (channel, head, row); box: 64 channels of g heads of
+// 128 / g rows; channels past hd and rows past the end read as zero.
+bool encode(CUtensorMap* map, int dtype, const void* base, int hd, int heads, i64 rows, i64 st, i64 sh, int g) {
   // a single row or head has no stride of its own to respect
   if (heads == 1) sh = hd;
   if (rows == 1) st = std::max(st, (i64)heads * std::max(sh, (i64)hd));
   cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
   cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
-  cuuint32_t box[3] = {64, 1, kT};
+  cuuint32_t box[3] = {64, (cuuint32_t)g, (cuuint32_t)(kT / g)};
   cuuint32_t estr[3] = {1, 1, 1};
   return fast::encode_fn()(map, dtype == OSSM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                            3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -920,13 +937,13 @@ bool encode(CUtensorMap* map, int dtype, const void* base, int hd, int heads, i6
 }
 
 template <typename T, int HDP>
-cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, int grid,
+cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, int lg, int grid,
                    cudaStream_t st) {
   auto kern = attn_prompt_kernel<T, HDP>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(kern, (int)Cfg<HDP>::kSmem, done);
   if (e != cudaSuccess) return e;
-  kern<<<grid, kThreads, Cfg<HDP>::kSmem, st>>>(q, k, v, p, (p.H / p.Hkv) % 2 == 0);
+  kern<<<grid, kThreads, Cfg<HDP>::kSmem, st>>>(q, k, v, p, lg);
   return cudaGetLastError();
 }
 
@@ -935,16 +952,18 @@ size_t prompt_part_floats(int hd) { return 2 * (hd <= 64 ? Cfg<64>::kPartFloats 
 int prompt_forward(const ossm_attn_args* a, const Params& p, int grid, cudaStream_t st) {
   if (!fast::encode_fn()) return OSSM_ELAUNCH;
   CUtensorMap q, k, v;
-  if (!encode(&q, a->dtype, p.q, p.hd, p.H, p.Tq, p.qst, p.qsh) ||
-      !encode(&k, a->dtype, p.k, p.hd, p.Hkv, p.Tk, p.kst, p.ksh) ||
-      !encode(&v, a->dtype, p.v, p.hd, p.Hkv, p.Tk, p.vst, p.vsh))
+  int lg = 0;
+  while (lg < 7 && (p.H / p.Hkv) % (2 << lg) == 0) ++lg;
+  if (!encode(&q, a->dtype, p.q, p.hd, p.H, p.Tq, p.qst, p.qsh, 1 << lg) ||
+      !encode(&k, a->dtype, p.k, p.hd, p.Hkv, p.Tk, p.kst, p.ksh, 1) ||
+      !encode(&v, a->dtype, p.v, p.hd, p.Hkv, p.Tk, p.vst, p.vsh, 1))
     return OSSM_EINVAL;
   const bool bf = a->dtype == OSSM_BF16;
   cudaError_t e;
   if (p.hd <= 64)
-    e = bf ? launch<__nv_bfloat16, 64>(q, k, v, p, grid, st) : launch<__half, 64>(q, k, v, p, grid, st);
+    e = bf ? launch<__nv_bfloat16, 64>(q, k, v, p, lg, grid, st) : launch<__half, 64>(q, k, v, p, lg, grid, st);
   else
-    e = bf ? launch<__nv_bfloat16, 128>(q, k, v, p, grid, st) : launch<__half, 128>(q, k, v, p, grid, st);
+    e = bf ? launch<__nv_bfloat16, 128>(q, k, v, p, lg, grid, st) : launch<__half, 128>(q, k, v, p, lg, grid, st);
   return e == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
 }
 

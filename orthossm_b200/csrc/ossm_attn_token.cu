@@ -34,6 +34,8 @@ constexpr int kGroups = 1024;         // entries of the line's prefix in shared 
 constexpr int kItemCost = 2;          // an item's start and end, in steps
 constexpr int kMinPiece = 4;          // no cut closer to an item's edge
 constexpr int kMinWork = 8;           // no more CTAs than items, or parts of this length
+constexpr int kJoin = 16;             // partial results joined at once
+constexpr int kCounts = 1024;         // counters of the second step follow those of the first
 
 template <int HDP>
 struct Cfg {
@@ -407,12 +409,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
     }
     __syncthreads();
     const bool split = b - a < x.n;
-    int first = 0;
-    float* part = nullptr;
-    if (split) {
-      first = head ? cta : ln.owner(x.start);
-      part = p.part + (size_t)(head ? 2 * cta + 1 : 2 * cta) * C::kPartFloats;
-    }
+    const int first = split ? (head ? cta : ln.owner(x.start)) : cta;
+    auto slot = [&](int c) {  // of CTA c's piece of this item
+      return p.part + (size_t)(c == first ? 2 * c + 1 : 2 * c) * C::kPartFloats;
+    };
+    float* part = slot(cta);
     T* out = static_cast<T*>(p.out);
     auto out_at = [&](int r) {
       return out + (i64)(x.q.q0 + (row0 + r) / G) * p.ost + (i64)(x.kvh * G + (row0 + r) % G) * p.osh;
@@ -449,43 +450,92 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       }
     }
     if (split) {
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const uint32_t done = atomicAdd(p.counts + first, (uint32_t)(b - a)) + (b - a);
-        last_in = done == (uint32_t)x.n;
-        if (last_in) p.counts[first] = 0;  // for the next call
-      }
-      __syncthreads();
-      if (last_in) {
+      const int last = ln.owner(x.start + x.n - 1);
+      // Is this the last of n arrivals at a counter?  Then the others' partial results are there to read.
+      auto arrive = [&](uint32_t* count, int n) {
         __threadfence();
-        const int np = ln.owner(x.start + x.n - 1) - first + 1;
-        auto piece = [&](int k) { return p.part + (size_t)(k ? 2 * (first + k) : 2 * first + 1) * C::kPartFloats; };
-        for (int e = threadIdx.x; e < nrows * CH; e += kThreads) {
-          const int r = e / CH, d = (e % CH) * 8;
-          float M = -INFINITY;
-#pragma unroll 4
-          for (int k = 0; k < np; ++k) M = fmaxf(M, __ldcg(piece(k) + r));
-          const float Ms = M == -INFINITY ? 0.f : M;
-          float acc[8] = {}, L = 0.f;
-#pragma unroll 4
-          for (int k = 0; k < np; ++k) {
-            const float* q = piece(k);
-            const float f = ex2(__ldcg(q + r) - Ms);
-            const float4 u = __ldcg(reinterpret_cast<const float4*>(q + 2 * kRows + r * HDP + d));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(q + 2 * kRows + r * HDP + d) + 1);
-            L = fmaf(f, __ldcg(q + kRows + r), L);
-            acc[0] = fmaf(f, u.x, acc[0]), acc[1] = fmaf(f, u.y, acc[1]);
-            acc[2] = fmaf(f, u.z, acc[2]), acc[3] = fmaf(f, u.w, acc[3]);
-            acc[4] = fmaf(f, v.x, acc[4]), acc[5] = fmaf(f, v.y, acc[5]);
-            acc[6] = fmaf(f, v.z, acc[6]), acc[7] = fmaf(f, v.w, acc[7]);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          last_in = atomicAdd(count, 1u) == (uint32_t)n - 1;
+          if (last_in) *count = 0;  // for the next call
+        }
+        __syncthreads();
+        const bool r = last_in;
+        __threadfence();
+        return r;
+      };
+      // The sum of n partial results, to the output or in place of the first.
+      auto join = [&](auto piece, int n, float* to) {
+        for (int e0 = 0; e0 < nrows * CH; e0 += kThreads) {
+          const int e = e0 + threadIdx.x, r = e / CH, d = (e % CH) * 8;
+          float M = -INFINITY, L = 0.f, acc[8] = {};
+          if (e < nrows * CH) {
+            for (int k0 = 0; k0 < n; k0 += 8) {
+              float pm[8], pl[8];
+              float4 u[8], v[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                pm[k] = -INFINITY, pl[k] = 0.f;
+                u[k] = v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k0 + k < n) {
+                  const float* q = piece(k0 + k);
+                  pm[k] = __ldcg(q + r);
+                  pl[k] = __ldcg(q + kRows + r);
+                  u[k] = __ldcg(reinterpret_cast<const float4*>(q + 2 * kRows + r * HDP + d));
+                  v[k] = __ldcg(reinterpret_cast<const float4*>(q + 2 * kRows + r * HDP + d) + 1);
+                }
+              }
+              float top = M;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) top = fmaxf(top, pm[k]);
+              const float ms = top == -INFINITY ? 0.f : top, f0 = ex2(M - ms);
+              M = top;
+              L *= f0;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) acc[i] *= f0;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float f = ex2(pm[k] - ms);
+                L = fmaf(f, pl[k], L);
+                acc[0] = fmaf(f, u[k].x, acc[0]), acc[1] = fmaf(f, u[k].y, acc[1]);
+                acc[2] = fmaf(f, u[k].z, acc[2]), acc[3] = fmaf(f, u[k].w, acc[3]);
+                acc[4] = fmaf(f, v[k].x, acc[4]), acc[5] = fmaf(f, v[k].y, acc[5]);
+                acc[6] = fmaf(f, v[k].z, acc[6]), acc[7] = fmaf(f, v[k].w, acc[7]);
+              }
+            }
           }
-          if (d < p.hd) {
+          __syncthreads();  // `to` is read by all before it is written
+          if (e >= nrows * CH) continue;
+          if (to) {
+            if (d == 0) {
+              to[r] = M;
+              to[kRows + r] = L;
+            }
+            float4* po = reinterpret_cast<float4*>(to + 2 * kRows + r * HDP + d);
+            po[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            po[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+          } else if (d < p.hd) {
             const float inv = L == 0.f ? 0.f : 1.f / L;
             *reinterpret_cast<uint4*>(out_at(r) + d) =
                 make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
                            pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
           }
+        }
+      };
+      // Many pieces are joined in two steps, groups of neighbouring CTAs first:
+      // one CTA alone would read all of them at its own small share of L2.
+      const int np = last - first + 1;
+      if (np <= kJoin) {
+        if (arrive(p.counts + kCounts + first, np))
+          join([&](int k) { return slot(first + k); }, np, static_cast<float*>(nullptr));
+      } else {
+        const int g0 = max(first, cta / kJoin * kJoin), g1 = min(last, cta / kJoin * kJoin + kJoin - 1);
+        const int ng = last / kJoin - first / kJoin + 1;
+        if (arrive(p.counts + (g0 == first ? 2 * g0 + 1 : 2 * g0), g1 - g0 + 1)) {
+          join([&](int k) { return slot(g0 + k); }, g1 - g0 + 1, slot(g0));
+          if (arrive(p.counts + kCounts + first, ng))
+            join([&](int k) { return slot(k ? (first / kJoin + k) * kJoin : first); }, ng,
+                 static_cast<float*>(nullptr));
         }
       }
     }
