@@ -33,7 +33,7 @@ constexpr int kChunk = kWarps * kWK;  // keys of a CTA's step, the line's unit
 constexpr int kGroups = 1024;         // entries of the line's prefix in shared memory
 constexpr int kItemCost = 2;          // an item's start and end, in steps
 constexpr int kMinPiece = 4;          // no cut closer to an item's edge
-constexpr int kMinWork = 8;           // no more CTAs than items, or parts of this length
+constexpr int kMinWork = 8;           // a CTA for each part of this length at most, and for each item
 constexpr int kJoin = 16;             // partial results joined at once
 constexpr int kCounts = 1024;         // counters of the second step follow those of the first
 
@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
   __shared__ float sm_p[kWarps][kRows][kWK];
   __shared__ int last_in;
+  __shared__ i64 cuts[2];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
   const int G = p.H / p.Hkv;
@@ -196,14 +197,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
   }
   __syncthreads();
   Line ln{p, pre, ngroups, gsz, pre[ngroups], 0};
-  ln.ncta = (int)min((i64)gridDim.x, max((i64)n_items, ln.total / kMinWork));
+  // twice the items: each item's edge is the nearest one to some cut, and short items get a CTA each
+  ln.ncta = (int)min((i64)gridDim.x, max(2 * (i64)n_items, ln.total / kMinWork));
   if (cta >= ln.ncta) return;
+  if (lane == 0 && warp < 2) cuts[warp] = ln.cut(cta + warp);
+  __syncthreads();
 
   const uint32_t ring = smem_u32(smem) + warp * (C::kStages * 2 * C::kTile);
   const uint8_t* ringp = smem + warp * (C::kStages * 2 * C::kTile);
   const int r4 = lane >> 2, c4 = lane & 3;  // this lane's rows r4, r4 + 8 and column pair in the fragments
-  i64 pos = ln.cut(cta);
-  const i64 end = ln.cut(cta + 1);
+  i64 pos = cuts[0];
+  const i64 end = cuts[1];
   while (pos < end) {
     const Line::Item x = ln.at(pos);
     const int a = (int)min(pos - x.start, (i64)x.n), b = (int)min(end - x.start, (i64)x.n);
