@@ -30,7 +30,7 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kRows = 16;             // query rows of an item
 constexpr int kWK = 16;               // keys of a warp's step
 constexpr int kChunk = kWarps * kWK;  // keys of a CTA's step, the line's unit
-constexpr int kGroups = 1024;         // entries of the line's prefix in shared memory
+constexpr int kGroups = 256;          // entries of the line's prefix in shared memory
 constexpr int kItemCost = 2;          // an item's start and end, in steps
 constexpr int kMinPiece = 4;          // no cut closer to an item's edge
 constexpr int kMinWork = 8;           // a CTA for each part of this length at most, and for each item
