@@ -29,11 +29,11 @@ typedef long long i64;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kRows = 16;             // query rows of an item
 constexpr int kWK = 16;               // keys of a warp's step
-constexpr int kChunk = kWarps * kWK;  // keys of a CTA's step, the line's unit
 constexpr int kGroups = 256;          // entries of the line's prefix in shared memory
 constexpr int kItemCost = 2;          // an item's start and end, in steps
 constexpr int kMinPiece = 4;          // no cut closer to an item's edge
 constexpr int kMinWork = 8;           // a CTA for each part of this length at most, and for each item
+constexpr int kPairFrom = 32;         // steps a CTA from which items take two heads
 constexpr int kJoin = 16;             // partial results joined at once
 constexpr int kCounts = 1024;         // counters of the second step follow those of the first
 
@@ -43,12 +43,19 @@ struct Cfg {
   static constexpr int kCtas = HDP == 64 ? 3 : 2;             // resident CTAs an SM
   static constexpr int kTile = kWK * HDP * 2;                 // bytes of a warp's K or V tile
   static constexpr int kSmem = kWarps * kStages * 2 * kTile;  // also holds the warps' outputs at the end
-  static constexpr size_t kPartFloats = kRows * (HDP + 2);
+  static constexpr int kHeads = HDP == 64 ? 2 : 1;            // key heads of an item, at most
+  static constexpr int kPart = kHeads * kRows;                // rows of a partial result
+  static constexpr size_t kPartFloats = kPart * (HDP + 2);
   static_assert(kSmem >= kWarps * kRows * HDP * 4, "outputs of the warps");
 };
 
+// An item takes `hp` neighbouring key heads, a warp one of them: with 64
+// channels one head's row is 128 bytes, and reading the heads of a token far
+// apart in time cost a sixth of the bandwidth (1048576 keys, 8 heads: 392 us,
+// head-major 340 us).
 struct Line {
   const Params& p;
+  int hp;
   const i64* pre;
   int ngroups, gsz;
   i64 total;
@@ -56,7 +63,7 @@ struct Line {
 
   struct Item {
     Seq q;
-    int rb, kvh, n;  // row block, key head, steps
+    int rb, kvh, n;  // row block, first key head, steps
     i64 start;
     OSSM_DEV i64 end() const { return start + n + kItemCost; }
   };
@@ -64,11 +71,10 @@ struct Line {
   static OSSM_DEV int first_key(const Params& p, const Seq& q) {
     return p.window ? max(0, q.nk - q.nq - p.window + 1) : 0;
   }
-  static OSSM_DEV int steps(const Params& p, const Seq& q) {
-    return max(1, (q.nk - first_key(p, q) + kChunk - 1) / kChunk);
-  }
-  static OSSM_DEV int blocks(const Params& p, const Seq& q) {  // row blocks times key heads
-    return (int)(((i64)q.nq * (p.H / p.Hkv) + kRows - 1) / kRows) * p.Hkv;
+  OSSM_DEV int chunk() const { return kWarps * kWK / hp; }  // keys of a CTA's step, the line's unit
+  OSSM_DEV int steps(const Seq& q) const { return max(1, (q.nk - first_key(p, q) + chunk() - 1) / chunk()); }
+  OSSM_DEV int blocks(const Seq& q) const {  // row blocks times groups of key heads
+    return (int)(((i64)q.nq * (p.H / p.Hkv) + kRows - 1) / kRows) * (p.Hkv / hp);
   }
   OSSM_DEV Item at(i64 pos) const {
     int lo = 0, hi = ngroups;
@@ -80,14 +86,14 @@ struct Line {
     Item it;
     for (int b = lo * gsz;; ++b) {
       it.q = seq_of(p, b);
-      it.n = steps(p, it.q);
-      const i64 len = (i64)blocks(p, it.q) * (it.n + kItemCost);
+      it.n = steps(it.q);
+      const i64 len = (i64)blocks(it.q) * (it.n + kItemCost);
       if (pos < base + len || b + 1 >= min(p.B, (lo + 1) * gsz)) break;
       base += len;
     }
     const int u = (int)((pos - base) / (it.n + kItemCost));
-    it.rb = u / p.Hkv;
-    it.kvh = u % p.Hkv;
+    it.rb = u / (p.Hkv / hp);
+    it.kvh = u % (p.Hkv / hp) * hp;
     it.start = base + (i64)u * (it.n + kItemCost);
     return it;
   }
@@ -166,37 +172,46 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
   const int G = p.H / p.Hkv;
   const int gsz = (p.B + kGroups - 1) / kGroups, ngroups = (p.B + gsz - 1) / gsz;
-  if (threadIdx.x == 0) n_items = 0;
-  __syncthreads();
-  unsigned long long mine = 0;
-  for (int g = threadIdx.x; g < ngroups; g += kThreads) {
-    i64 len = 0;
-    for (int b = g * gsz; b < min(p.B, (g + 1) * gsz); ++b) {
-      const Seq q = seq_of(p, b);
-      const int nb = Line::blocks(p, q);
-      len += (i64)nb * (Line::steps(p, q) + kItemCost);
-      mine += nb;
-    }
-    pre[g + 1] = len;
-  }
-  if (mine) atomicAdd(&n_items, mine);
-  __syncthreads();
-  if (warp == 0) {
-    i64 run = 0;
-    for (int g0 = 0; g0 < ngroups; g0 += 32) {
-      i64 v = g0 + lane < ngroups ? pre[g0 + lane + 1] : 0;
-#pragma unroll
-      for (int w = 1; w < 32; w *= 2) {
-        const i64 u = __shfl_up_sync(~0u, v, w);
-        if (lane >= w) v += u;
+  // One head an item; two where the line is long for the GPU, as they halve the
+  // items (32 streams with a window of 512: 14 us with one, 23 us with two).
+  Line ln{p, 1, pre, ngroups, gsz, 0, 0};
+  for (;;) {
+    if (threadIdx.x == 0) n_items = 0;
+    __syncthreads();
+    unsigned long long mine = 0;
+    for (int g = threadIdx.x; g < ngroups; g += kThreads) {
+      i64 len = 0;
+      for (int b = g * gsz; b < min(p.B, (g + 1) * gsz); ++b) {
+        const Seq q = seq_of(p, b);
+        const int nb = ln.blocks(q);
+        len += (i64)nb * (ln.steps(q) + kItemCost);
+        mine += nb;
       }
-      if (g0 + lane < ngroups) pre[g0 + lane + 1] = run + v;
-      run += __shfl_sync(~0u, v, 31);
+      pre[g + 1] = len;
     }
-    if (lane == 0) pre[0] = 0;
+    if (mine) atomicAdd(&n_items, mine);
+    __syncthreads();
+    if (warp == 0) {
+      i64 run = 0;
+      for (int g0 = 0; g0 < ngroups; g0 += 32) {
+        i64 v = g0 + lane < ngroups ? pre[g0 + lane + 1] : 0;
+#pragma unroll
+        for (int w = 1; w < 32; w *= 2) {
+          const i64 u = __shfl_up_sync(~0u, v, w);
+          if (lane >= w) v += u;
+        }
+        if (g0 + lane < ngroups) pre[g0 + lane + 1] = run + v;
+        run += __shfl_sync(~0u, v, 31);
+      }
+      if (lane == 0) pre[0] = 0;
+    }
+    __syncthreads();
+    ln.total = pre[ngroups];
+    if (C::kHeads == 1 || ln.hp == 2 || p.Hkv % 2 || ln.total < (i64)kPairFrom * gridDim.x) break;
+    ln.hp = 2;
+    __syncthreads();
   }
-  __syncthreads();
-  Line ln{p, pre, ngroups, gsz, pre[ngroups], 0};
+  const int hp = ln.hp, sub = warp & (hp - 1), kw = warp / hp, nkw = kWarps / hp;  // head, place among its warps
   // twice the items: each item's edge is the nearest one to some cut, and short items get a CTA each
   ln.ncta = (int)min((i64)gridDim.x, max(2 * (i64)n_items, ln.total / kMinWork));
   if (cta >= ln.ncta) return;
@@ -215,7 +230,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
     pos = min(end, x.end());
     if (a >= b) continue;
     const int off = x.q.nk - x.q.nq, lo = Line::first_key(p, x.q);
-    const int kbeg = lo + a * kChunk, kend = min(x.q.nk, lo + b * kChunk);
+    const int kbeg = lo + a * ln.chunk(), kend = min(x.q.nk, lo + b * ln.chunk());
+    const int kvh = x.kvh + sub;
     const int row0 = x.rb * kRows, nrows = (int)min((i64)kRows, (i64)x.q.nq * G - row0);
     const int i_first = row0 / G, i_last = (row0 + nrows - 1) / G;
     // positions of this lane's rows (rows past the block repeat its last)
@@ -227,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
     uint32_t qf[KS][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = r4 + 8 * h, i = (row0 + r) / G, hd_ = x.kvh * G + (row0 + r) % G;
+      const int r = r4 + 8 * h, i = (row0 + r) / G, hd_ = kvh * G + (row0 + r) % G;
       const T* q = static_cast<const T*>(p.q) + (i64)(x.q.q0 + i) * p.qst + (i64)hd_ * p.qsh;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
@@ -244,15 +260,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    // this warp's tiles: kbeg + (warp + kWarps u) * 16
-    const int nt = kend > kbeg ? ((kend - kbeg + kWK - 1) / kWK - warp + kWarps - 1) / kWarps : 0;
+    // this warp's tiles: kbeg + (kw + nkw u) * 16
+    const int nt = kend > kbeg ? ((kend - kbeg + kWK - 1) / kWK - kw + nkw - 1) / nkw : 0;
     constexpr int RP = 32 / CH;  // rows a warp copies at once
     const int cr = lane / CH, cc = lane % CH;
-    const T* kg = static_cast<const T*>(p.k) + (i64)x.q.k0 * p.kst + (i64)x.kvh * p.ksh + cc * 8;
-    const T* vg = static_cast<const T*>(p.v) + (i64)x.q.k0 * p.vst + (i64)x.kvh * p.vsh + cc * 8;
+    const T* kg = static_cast<const T*>(p.k) + (i64)x.q.k0 * p.kst + (i64)kvh * p.ksh + cc * 8;
+    const T* vg = static_cast<const T*>(p.v) + (i64)x.q.k0 * p.vst + (i64)kvh * p.vsh + cc * 8;
     auto load = [&](int u) {
       if (u < nt) {
-        const int key = kbeg + (warp + kWarps * u) * kWK + cr;
+        const int key = kbeg + (kw + nkw * u) * kWK + cr;
         const uint32_t kd = ring + (u % C::kStages) * (2 * C::kTile), vd = kd + C::kTile;
         const T *ks = kg + (i64)key * p.kst, *vs = vg + (i64)key * p.vst;
 #pragma unroll
@@ -271,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       __syncwarp();
       load(u + C::kStages - 1);
       const uint32_t kd = ring + (u % C::kStages) * (2 * C::kTile), vd = kd + C::kTile;
-      const int key0 = kbeg + (warp + kWarps * u) * kWK;
+      const int key0 = kbeg + (kw + nkw * u) * kWK;
       float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -419,18 +435,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
     };
     float* part = slot(cta);
     T* out = static_cast<T*>(p.out);
-    auto out_at = [&](int r) {
-      return out + (i64)(x.q.q0 + (row0 + r) / G) * p.ost + (i64)(x.kvh * G + (row0 + r) % G) * p.osh;
+    // rows of the item's heads one after the other
+    auto out_at = [&](int rr) {
+      const int h = rr / nrows, r = row0 + rr % nrows;
+      return out + (i64)(x.q.q0 + r / G) * p.ost + (i64)((x.kvh + h) * G + r % G) * p.osh;
     };
-    for (int e = threadIdx.x; e < nrows * CH; e += kThreads) {
-      const int r = e / CH, d = (e % CH) * 8;
-      float M = sm_m[0][r];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+    const int nout = nrows * hp * CH;
+    for (int e = threadIdx.x; e < nout; e += kThreads) {
+      const int rr = e / CH, r = rr % nrows, h = rr / nrows, d = (e % CH) * 8;
+      float M = -INFINITY;
+      for (int w = h; w < kWarps; w += hp) M = fmaxf(M, sm_m[w][r]);
       const float Ms = M == -INFINITY ? 0.f : M;
       float acc[8] = {}, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = h; w < kWarps; w += hp) {
         if (sm_m[w][r] == -INFINITY && sm_l[w][r] == 0.f) continue;  // a warp that has seen no key
         const float f = ex2(sm_m[w][r] - Ms);
         L += f * sm_l[w][r];
@@ -440,15 +457,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       }
       if (split) {
         if (d == 0) {
-          part[r] = M;
-          part[kRows + r] = L;
+          part[rr] = M;
+          part[C::kPart + rr] = L;
         }
-        float4* po = reinterpret_cast<float4*>(part + 2 * kRows + r * HDP + d);
+        float4* po = reinterpret_cast<float4*>(part + 2 * C::kPart + rr * HDP + d);
         po[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         po[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
       } else if (d < p.hd) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        *reinterpret_cast<uint4*>(out_at(r) + d) =
+        *reinterpret_cast<uint4*>(out_at(rr) + d) =
             make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
                        pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
       }
@@ -470,10 +487,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       };
       // The sum of n partial results, to the output or in place of the first.
       auto join = [&](auto piece, int n, float* to) {
-        for (int e0 = 0; e0 < nrows * CH; e0 += kThreads) {
+        for (int e0 = 0; e0 < nout; e0 += kThreads) {
           const int e = e0 + threadIdx.x, r = e / CH, d = (e % CH) * 8;
           float M = -INFINITY, L = 0.f, acc[8] = {};
-          if (e < nrows * CH) {
+          if (e < nout) {
             for (int k0 = 0; k0 < n; k0 += 8) {
               float pm[8], pl[8];
               float4 u[8], v[8];
@@ -484,9 +501,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
                 if (k0 + k < n) {
                   const float* q = piece(k0 + k);
                   pm[k] = __ldcg(q + r);
-                  pl[k] = __ldcg(q + kRows + r);
-                  u[k] = __ldcg(reinterpret_cast<const float4*>(q + 2 * kRows + r * HDP + d));
-                  v[k] = __ldcg(reinterpret_cast<const float4*>(q + 2 * kRows + r * HDP + d) + 1);
+                  pl[k] = __ldcg(q + C::kPart + r);
+                  u[k] = __ldcg(reinterpret_cast<const float4*>(q + 2 * C::kPart + r * HDP + d));
+                  v[k] = __ldcg(reinterpret_cast<const float4*>(q + 2 * C::kPart + r * HDP + d) + 1);
                 }
               }
               float top = M;
@@ -509,13 +526,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
             }
           }
           __syncthreads();  // `to` is read by all before it is written
-          if (e >= nrows * CH) continue;
+          if (e >= nout) continue;
           if (to) {
             if (d == 0) {
               to[r] = M;
-              to[kRows + r] = L;
+              to[C::kPart + r] = L;
             }
-            float4* po = reinterpret_cast<float4*>(to + 2 * kRows + r * HDP + d);
+            float4* po = reinterpret_cast<float4*>(to + 2 * C::kPart + r * HDP + d);
             po[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
             po[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
           } else if (d < p.hd) {

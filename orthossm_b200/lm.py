@@ -30,6 +30,11 @@ flash-attention's sliding-window kernel (library kernels, the spec's
 "SDPA").  ``local_window_attention_blocked`` restates that attention with
 torch's scaled_dot_product_attention over 2*window-key blocks; the tests check
 the two against each other and against dense masked attention.
+
+``OrthoSSMLM.generate`` serves the model: prompts of different lengths packed
+into one pass, a cache of keys and values per layer, and drawn tokens.  There
+the local attention is this package's ``packed_attention`` (the window reaches
+over call boundaries) and the tokens come from ``sample_tokens``.
 """
 from __future__ import annotations
 
@@ -42,6 +47,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .sdpc_kernel import BASELINE_LAMBDA, cheby_ema_forward, init_chebyshev_coefficients
+from .serving import packed_attention, sample_tokens
 from .state import ChebyStreamState
 
 
@@ -101,6 +107,26 @@ def local_window_attention_blocked(q: torch.Tensor, k: torch.Tensor, v: torch.Te
     return o[:, :S]
 
 
+@dataclasses.dataclass
+class DecodeCache:
+    """What a batch of streams carries between calls of ``OrthoSSMLM.extend``:
+    per layer the keys and values of every token ([B, slots, H, hd]) and the
+    EMA state of the global path ([B, d], None before the first token); the
+    Chebyshev coefficients; the tokens held of each stream, on the host and on
+    the device."""
+    keys: List[torch.Tensor]
+    values: List[torch.Tensor]
+    coeffs: List[torch.Tensor]
+    ema: List[Optional[torch.Tensor]]
+    lengths: List[int]
+    lengths_dev: torch.Tensor   # int32 [B]
+    starts: torch.Tensor        # int32 [B+1]: each stream's first slot
+
+    @property
+    def slots(self) -> int:
+        return self.keys[0].shape[1]
+
+
 class V8Layer(nn.Module):
     def __init__(self, cfg: OrthoLMConfig):
         super().__init__()
@@ -133,6 +159,38 @@ class V8Layer(nn.Module):
         attn = local_window_attention if h.dtype in (torch.bfloat16, torch.float16) else local_window_attention_blocked
         loc = self.o(attn(q, k, v, self.cfg.window).reshape(B, S, d))
         return x + self.out_proj(self.norm_comb(g + loc)), fin
+
+    def extend(self, x: torch.Tensor, news: List[int], cu: torch.Tensor, at: torch.Tensor, kv_lengths: torch.Tensor,
+               li: int, cache: DecodeCache) -> torch.Tensor:
+        """The layer on new tokens of each stream, packed: x [T, d], stream b's
+        news[b] tokens at cu[b]; their keys and values go to the cache rows
+        ``at``.  Unlike ``forward``, the local window reaches back over the
+        calls before."""
+        T, d = x.shape
+        H = self.cfg.n_heads
+        h = self.norm_in(x)
+        opts = dict(lambda_per_head=self.lam(h.device), gate_weight=self.gate.weight.float(),
+                    gate_bias=self.gate.bias.float(), gate_scale=self.cfg.gate_scale, out_dtype=h.dtype)
+        ema = cache.ema[li]
+        if min(news) == max(news):  # streams of equal length are one batch of the global path
+            g, fin = cheby_ema_forward(h.view(len(news), news[0], d), cache.coeffs[li], init_state=ema, **opts)
+            g = g.reshape(T, d)
+        else:
+            g, fin, t = torch.empty_like(h), [], 0
+            for b, n in enumerate(news):
+                gb, fb = cheby_ema_forward(h[t:t + n].unsqueeze(0), cache.coeffs[li][b:b + 1],
+                                           init_state=None if ema is None else ema[b:b + 1], **opts)
+                g[t:t + n] = gb[0]
+                fin.append(fb)
+                t += n
+            fin = torch.cat(fin)
+        cache.ema[li] = fin
+        q, k, v = self.qkv(h).view(T, 3, H, d // H).unbind(1)
+        K, V = (c.view(-1, H, d // H) for c in (cache.keys[li], cache.values[li]))
+        K[at], V[at] = k, v
+        a = packed_attention(q, K, V, cu, cache.starts, max_seqlen_q=max(news), kv_lengths=kv_lengths,
+                             window=self.cfg.window)
+        return x + self.out_proj(self.norm_comb(g + self.o(a.reshape(T, d))))
 
 
 class OrthoSSMLM(nn.Module):
@@ -181,6 +239,72 @@ class OrthoSSMLM(nn.Module):
             new_states.append(dataclasses.replace(st, ema=fin, tokens_seen=st.tokens_seen + S))
         logits = self.lm_head(self.final_norm(x))
         return (logits, new_states) if return_state else logits
+
+
+    # ------------------------------------------------------------------ serving
+    def new_cache(self, batch: int, slots: int, coeffs: Optional[List[torch.Tensor]] = None) -> DecodeCache:
+        """An empty cache for ``batch`` streams of up to ``slots`` tokens;
+        ``coeffs``: the layers' Chebyshev coefficients (default: fresh ones)."""
+        p = self.embedding.weight
+        if p.dtype != torch.bfloat16:
+            raise ValueError(f"serving runs in bf16: cast the model first (parameters are {p.dtype})")
+        cfg = self.cfg
+        if coeffs is None:
+            coeffs = [st.coeffs for st in self.fresh_states(batch, p.device)]
+        kv = [torch.zeros(2, batch, slots, cfg.n_heads, cfg.head_dim, dtype=p.dtype, device=p.device)
+              for _ in range(cfg.n_layers)]
+        return DecodeCache(keys=[t[0] for t in kv], values=[t[1] for t in kv], coeffs=list(coeffs),
+                           ema=[None] * cfg.n_layers, lengths=[0] * batch,
+                           lengths_dev=torch.zeros(batch, dtype=torch.int32, device=p.device),
+                           starts=torch.arange(batch + 1, dtype=torch.int32, device=p.device) * slots)
+
+    @torch.no_grad()
+    def extend(self, tokens: List[torch.Tensor], cache: DecodeCache) -> torch.Tensor:
+        """Appends tokens[b] (at least one each) to stream b: whole prompts,
+        pieces of them, or single tokens.  Returns the logits [B, vocab] after
+        each stream's last token."""
+        news = [int(t.numel()) for t in tokens]
+        if len(news) != len(cache.lengths) or min(news) < 1:
+            raise ValueError("extend: every stream of the cache takes at least one token")
+        if max(n + old for n, old in zip(news, cache.lengths)) > cache.slots:
+            raise ValueError(f"extend: the cache's {cache.slots} slots a stream do not hold the new tokens")
+        dev = cache.lengths_dev.device
+        if max(news) == 1:
+            cu = torch.arange(len(news) + 1, dtype=torch.int32, device=dev)
+            at = (cache.starts[:-1] + cache.lengths_dev).long()
+            grown = cache.lengths_dev + 1
+        else:
+            n = torch.tensor(news, dtype=torch.int32)
+            cu = torch.cat([torch.zeros(1, dtype=torch.int32), n.cumsum(0, dtype=torch.int32)]).to(dev)
+            at = torch.cat([torch.arange(k, dtype=torch.int64) + b * cache.slots + old
+                            for b, (k, old) in enumerate(zip(news, cache.lengths))]).to(dev)
+            grown = cache.lengths_dev + n.to(dev)
+        x = self.embedding(torch.cat([t.reshape(-1) for t in tokens]))
+        for li, layer in enumerate(self.layers):
+            x = layer.extend(x, news, cu, at, grown, li, cache)
+        cache.lengths = [old + k for old, k in zip(cache.lengths, news)]
+        cache.lengths_dev = grown
+        return self.lm_head(self.final_norm(x[(cu[1:] - 1).long()]))
+
+    @torch.no_grad()
+    def generate(self, prompts: List[torch.Tensor], max_new_tokens: int, *, temperature=1.0, top_k=0, top_p=1.0,
+                 min_p=0.0, generator: Optional[torch.Generator] = None,
+                 coeffs: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
+        """Continues each prompt (1-D token ids on the GPU, of any lengths) by
+        ``max_new_tokens`` tokens [B, max_new_tokens], drawn as
+        ``sample_tokens`` does from noise of ``generator``."""
+        B = len(prompts)
+        cache = self.new_cache(B, max(int(t.numel()) for t in prompts) + max_new_tokens, coeffs)
+        dev = cache.lengths_dev.device
+        noise = torch.empty(B, self.cfg.vocab_size, device=dev)
+        out = torch.empty(max_new_tokens, B, dtype=torch.int64, device=dev)
+        tokens = list(prompts)
+        for i in range(max_new_tokens):
+            logits = self.extend(tokens, cache)
+            sample_tokens(logits, noise.exponential_(generator=generator), temperature=temperature, top_k=top_k,
+                          top_p=top_p, min_p=min_p, out=out[i])
+            tokens = list(out[i].split(1))
+        return out.t()
 
 
 def n_params(model: nn.Module) -> int:

@@ -190,6 +190,24 @@ def test_large_scores_and_scale(nq):
     check(out, q, k, v, cu_q, cu_k, scale=0.25)
 
 
+@pytest.mark.parametrize("H,Hkv,hd,nq", [(8, 8, 64, 1), (4, 4, 32, 3), (6, 3, 64, 2), (8, 2, 128, 1)])
+def test_long_caches_of_a_batch(H, Hkv, hd, nq):
+    """A line of keys long enough that each item takes two key heads (where
+    their number is even and a head has up to 64 channels), cut between CTAs."""
+    n, slots = 24, 20000
+    g = torch.Generator(device="cuda").manual_seed(H)
+    lens = [slots - (i * 997) % 9000 for i in range(n)]
+    q = torch.randn(n * nq, H, hd, device="cuda", generator=g).to(torch.bfloat16)
+    k, v = (torch.randn(n * slots, Hkv, hd, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    kv = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    cu_q, cu_k = cum([nq] * n), cum([slots] * n)
+    out = O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq, kv_lengths=kv)
+    for b in (0, 1, 11, n - 1):
+        qs = slice(b * nq, (b + 1) * nq)
+        ks = slice(b * slots, b * slots + lens[b])
+        check(out[qs], q[qs], k[ks], v[ks], torch.tensor([0, nq]), torch.tensor([0, lens[b]]))
+
+
 def test_offsets_beyond_32_bits():
     """A cache of more than 2^32 bytes and 2^31 elements, read at its end."""
     H, hd, slots, n = 4, 128, 1 << 20, 5
