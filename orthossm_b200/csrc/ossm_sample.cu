@@ -58,6 +58,7 @@ OSSM_DEV float to_f(__half v) { return __half2float(v); }
 
 // A NaN or -inf logit is no candidate.
 OSSM_DEV bool live(float l) { return l > -INFINITY; }
+constexpr float kLowest = -3.402823466e38f;  // the lowest candidate
 
 // Larger key: earlier candidate.  -0 and +0 are the same logit.
 OSSM_DEV uint32_t ord(float l) {
@@ -154,6 +155,58 @@ OSSM_DEV void scan(const T* row, int V, int rank, int nrank, F f) {
       float l[N];
       l[0] = fmaxf(to_f(row[i]), -INFINITY);
       f(l, i, 1);
+    }
+  }
+}
+
+// The same with the noise of each logit: f(l, e, i, n).  Both are loaded ahead
+// for several vectors, as the noise comes from HBM.
+template <typename T, typename F>
+OSSM_DEV void scan_noise(const T* row, const float* nz, int V, int rank, int nrank, F f) {
+  constexpr int N = Vec<T>::n, U = 16 / N;
+  const int head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
+  const int nv = (V - head) / N, v0 = (int)((i64)nv * rank / nrank), v1 = (int)((i64)nv * (rank + 1) / nrank);
+  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  const float* nbody = nz + head;
+  const bool aligned = ((uintptr_t)nbody & 15) == 0;
+  for (int v = v0 + threadIdx.x; v < v1; v += U * kThreads) {
+    uint4 u[U];
+    float e[U][N];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int w = v + k * kThreads;
+      if (w >= v1) break;
+      u[k] = __ldg(body + w);
+      if (aligned) {
+#pragma unroll
+        for (int h = 0; h < N; h += 4) {
+          const float4 x = __ldcs(reinterpret_cast<const float4*>(nbody + (size_t)w * N + h));
+          e[k][h] = x.x, e[k][h + 1] = x.y, e[k][h + 2] = x.z, e[k][h + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < N; ++h) e[k][h] = __ldcs(nbody + (size_t)w * N + h);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int w = v + k * kThreads;
+      if (w >= v1) break;
+      float l[N];
+      unpack(u[k], l, T());
+#pragma unroll
+      for (int h = 0; h < N; ++h) l[h] = fmaxf(l[h], -INFINITY);
+      f(l, e[k], head + w * N, N);
+    }
+  }
+  if (rank == 0) {
+    const int tail = V - head - nv * N, t = threadIdx.x;
+    if (t < head + tail) {
+      const int i = t < head ? t : V - tail + (t - head);
+      float l[N], e[N];
+      l[0] = fmaxf(to_f(row[i]), -INFINITY);
+      e[0] = nz[i];
+      f(l, e, i, 1);
     }
   }
 }
@@ -304,8 +357,9 @@ OSSM_DEV u64 select(const Row& r, const T* lg, int V, float m, float lb, u64 flo
   const int tid = threadIdx.x;
   const float scale = m > lb && m - lb < INFINITY ? (kBins - 1) / (m - lb) : 0.f;
   const float c = r.inv_t * 1.44269504f;
-  auto rough = [&](float l) { return l == m ? 1.f : ex2((l - m) * c); };  // weight, to a few 2^-22
-  auto bin_of = [&](float l) { return m == l ? 0 : min(kBins - 1, (int)fminf((m - l) * scale, (float)kBins)); };
+  // (m - l) scale, rounded by adding 2^23: the bin in the low bits
+  auto bin_of = [&](float d) { return __float_as_int(fminf(d * scale, (float)(kBins - 1)) + 8388608.f) & (kBins - 1); };
+  auto below = [&](float l) { return l == m ? 0.f : m - l; };
   // Masses in steps of 2^-28 (the sums are compared with a share of the whole,
   // which is at least 1), in two parts that 2^17 candidates cannot overflow;
   // longer rows take one 64-bit sum, which costs a loop of exchanges.
@@ -315,14 +369,15 @@ OSSM_DEV u64 select(const Row& r, const T* lg, int V, float m, float lb, u64 flo
   __syncthreads();
   for (int i = tid; i < kBins; i += kThreads) wide[i] = 0;
   __syncthreads();
-  const float first = logit_of(floor);  // floor's logit: only there the index decides
+  const float first = floor ? logit_of(floor) : -INFINITY;  // floor's logit: only there the index decides
+  const float low = fmaxf(lb, kLowest);
   scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
 #pragma unroll
     for (int e = 0; e < Vec<T>::n; ++e) {
-      const bool in = e < n && live(l[e]) && l[e] >= lb && (floor == 0 || l[e] > first || key_of(l[e], i + e) >= floor);
-      if (!__any_sync(__activemask(), in)) continue;
-      const int b = bin_of(l[e]);
-      const uint32_t q = __float2uint_rn(rough(l[e]) * 0x1p28f);
+      const bool in = e < n && l[e] >= low && (l[e] > first || key_of(l[e], i + e) >= floor);
+      const float d = below(l[e]);
+      const int b = bin_of(d);
+      const uint32_t q = __float2uint_rn(ex2(-d * c) * 0x1p28f);  // the weight, to a few 2^-22
       if (!in) continue;
       if (count) {
         atomicAdd(part + 2 * b, 1u);
@@ -351,11 +406,14 @@ OSSM_DEV u64 select(const Row& r, const T* lg, int V, float m, float lb, u64 flo
   const int cut = (int)s.sh[0];
   u64 left = target - s.sh[1];  // from the bin itself
   __syncthreads();
+  // the bin's logits lie between these (half a bin wider on both sides)
+  const float from = scale > 0.f ? fmaxf(low, cut == kBins - 1 ? low : m - (cut + 1.f) / scale) : low;
+  const float to = scale > 0.f && cut ? m - (cut - 1.f) / scale : INFINITY;
   auto each = [&](auto f) {  // the keys of the bin
     scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
 #pragma unroll
       for (int e = 0; e < Vec<T>::n; ++e)
-        if (e < n && live(l[e]) && l[e] >= lb && bin_of(l[e]) == cut) {
+        if (e < n && l[e] >= from && l[e] <= to && bin_of(below(l[e])) == cut) {
           const u64 key = key_of(l[e], i + e);
           if (key >= floor) f(key);
         }
@@ -406,36 +464,31 @@ OSSM_DEV u64 select(const Row& r, const T* lg, int V, float m, float lb, u64 flo
   return prefix;
 }
 
-// May the noise of a vector of logits be loaded 16 bytes at a time?
-template <typename T>
-OSSM_DEV bool noise_aligned(const T* lg, const float* nz) {
-  const int head = (int)((16 - ((uintptr_t)lg & 15)) & 15) / (int)sizeof(T);
-  return ((uintptr_t)(nz + head) & 15) == 0;
+OSSM_DEV float lg2(float x) {  // log2, within 2^-22 (of 1, or of its value)
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-// The scores of the candidates `in` of a vector against the best so far.  The
-// logarithm in its fast form is within 2^-22 (of 1, or of its value), far below
-// the slack; the exact score is only taken of those that come that near.
-template <typename T>
-OSSM_DEV void race(const float* l, int i, int n, uint32_t in, const float* nz, bool aligned, float inv_t, Best& b) {
-  float e[Vec<T>::n];
-#pragma unroll
-  for (int k = 0; k < Vec<T>::n; k += 4) {
-    if (!(in >> k & 15u)) continue;
-    if (n > 1 && aligned) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(nz + i + k));
-      e[k] = f.x, e[k + 1] = f.y, e[k + 2] = f.z, e[k + 3] = f.w;
-    } else {
-#pragma unroll
-      for (int h = k; h < k + 4; ++h)
-        if (in >> h & 1u) e[h] = nz[i + h];
-    }
-  }
+// The scores of a vector's logits l >= low that are candidates (stays(l, i))
+// against the best so far.  The logarithm in its fast form is off by far less
+// than the slack; the exact score is only taken of those that come that near to
+// the warp's best, `mark` (a thread's own best is passed by some lane at almost
+// every step).
+template <typename T, typename F>
+OSSM_DEV void race(const float* l, const float* e, int i, int n, float low, F stays, float inv_t, Best& b, float& mark) {
+  const float bar = mark - 1e-4f;
+  uint32_t near = 0;
 #pragma unroll
   for (int k = 0; k < Vec<T>::n; ++k) {
-    const float x = l[k] * inv_t, s = fmaf(-0.693147181f, __log2f(e[k]), x);
-    if ((in >> k & 1u) && (!(s < b.s - (1e-4f + 1e-6f * fabsf(x))) || b.i < 0))
-      better(b, score_of(l[k], inv_t, e[k]), i + k);
+    const float x = l[k] * inv_t, s = fmaf(-0.693147181f, lg2(e[k]), fmaf(1e-6f, fabsf(x), x));
+    near |= k < n && l[k] >= low && !(s < bar) ? 1u << k : 0u;
   }
+  if (near) {
+#pragma unroll
+    for (int k = 0; k < Vec<T>::n; ++k)
+      if ((near >> k & 1u) && stays(l[k], i + k)) better(b, score_of(l[k], inv_t, e[k]), i + k);
+  }
+  mark = logit_of((u64)__reduce_max_sync(__activemask(), ord(b.i < 0 ? -INFINITY : b.s)) << 32);
 }
 
 // What the CTAs of a cluster tell each other.
@@ -462,12 +515,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
 
   if (r.open()) {
     Best b{0.f, -1};
-    const bool aligned = noise_aligned(lg, nz);
-    scan(lg, p.V, rank, nrank, [&](const float* l, int i, int n) {
-      uint32_t in = 0;
-#pragma unroll
-      for (int k = 0; k < Vec<T>::n; ++k) in |= k < n && live(l[k]) ? 1u << k : 0u;
-      race<T>(l, i, n, in, nz, aligned, r.inv_t, b);
+    float mark = -INFINITY;
+    scan_noise(lg, nz, p.V, rank, nrank, [&](const float* l, const float* e, int i, int n) {
+      race<T>(l, e, i, n, kLowest, [](float, int) { return true; }, r.inv_t, b, mark);
     });
     b = block_best(b, bests);
     if (nrank > 1) {
@@ -568,7 +618,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   }
   Told* first = nrank > 1 ? cluster.map_shared_rank(&told, 0) : &told;
   u64* first_list = nrank > 1 ? cluster.map_shared_rank(room.list, 0) : room.list;
-  const float low = bound ? fmaxf(logit_of((u64)bound << 32), -3.402823466e38f) : -3.402823466e38f;
+  const float low = bound ? fmaxf(logit_of((u64)bound << 32), kLowest) : kLowest;
   bool over = false;  // the list is full: its end is found in another way
   scan(lg, p.V, rank, nrank, [&](const float* l, int i, int n) {
     uint32_t in = 0;
@@ -599,6 +649,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     better(b, r.greedy ? 0.f : score_of(logit_of(key), r.inv_t, nz[i]), i);
   };
   if (N > kList) {
+    if (!r.greedy && tid == 0) {  // the last pass reads the noise: on its way to L2 meanwhile
+      const uintptr_t a = ((uintptr_t)nz + 15) & ~(uintptr_t)15, z = (uintptr_t)(nz + p.V) & ~(uintptr_t)15;
+      for (uintptr_t x = a; x < z; x += 32768)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x), "r"((uint32_t)min((u64)32768, (u64)(z - x)))
+                     : "memory");
+    }
     u64 top = 0, keep = 0;  // the first candidate (which stays whatever min_p is), the last one's key
     float least = INFINITY;
     if (r.greedy || r.min_p > 0.f || top_k || !live(lb)) {
@@ -619,25 +675,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
                       whole, room);
     }
     const float end = keep ? logit_of(keep) : -INFINITY;  // the last one's logit: only there the index decides
-    const bool aligned = noise_aligned(lg, nz);
-    scan(lg, p.V, 0, 1, [&](const float* l, int i, int n) {
-      uint32_t in = 0;
-#pragma unroll
-      for (int e = 0; e < Vec<T>::n; ++e)
-        in |= e < n && live(l[e]) && l[e] >= lb && (l[e] > end || (l[e] == end && key_of(l[e], i + e) >= keep))
-                  ? 1u << e : 0u;
-      if (r.min_p > 0.f) {
-#pragma unroll
-        for (int e = 0; e < Vec<T>::n; ++e)
-          if ((in >> e & 1u) && key_of(l[e], i + e) != top && weight(l[e], m, r.inv_t) < r.min_p) in &= ~(1u << e);
-      }
-      if (!in) return;
-      if (r.greedy) {
-        consider(keep);
-        return;
-      }
-      race<T>(l, i, n, in, nz, aligned, r.inv_t, b);
-    });
+    if (r.greedy) {
+      if (tid == 0) consider(keep);
+    } else {
+      float mark = -INFINITY;
+      auto stays = [&](float l, int i) {
+        const u64 key = key_of(l, i);
+        return key >= keep && (!(r.min_p > 0.f) || key == top || weight(l, m, r.inv_t) >= r.min_p);
+      };
+      scan_noise(lg, nz, p.V, 0, 1, [&](const float* l, const float* e, int i, int n) {
+        race<T>(l, e, i, n, fmaxf(fmaxf(end, lb), kLowest), stays, r.inv_t, b, mark);
+      });
+    }
   } else {
     order(room.list, N);
     int n = top_k ? min(top_k, N) : N;
