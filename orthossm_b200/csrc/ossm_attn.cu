@@ -7,6 +7,7 @@
 #include "ossm_attn.cuh"
 
 namespace ossm {
+int device_sms();
 namespace attn {
 
 size_t prompt_part_floats(int hd);
@@ -41,19 +42,24 @@ bool valid(const ossm_attn_args* a) {
 
 using namespace ossm;
 
+// SMs of the current device (asked for once a device).
+int ossm::device_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 namespace {
 
 // Workspace: header, two progress counters a CTA, two partial results a CTA.
 constexpr int kMaxCtas = 1024;
 constexpr int kTokenRows = 16;
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return std::min(n, kMaxCtas / 4);
-}
+int sm_count() { return std::min(device_sms(), kMaxCtas / 4); }
 
 size_t ws_bytes(const ossm_attn_args* a) {
   return sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t) +

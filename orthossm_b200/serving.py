@@ -120,7 +120,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError("packed_attention has no backward pass: call it under torch.no_grad()")
     if out is None:
-        out = torch.empty((Tq, H, hd), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if Tq == 0:
         return out
     layout = []
