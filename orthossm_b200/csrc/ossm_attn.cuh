@@ -80,7 +80,7 @@ OSSM_DEV uint32_t pack2<__half>(float lo, float hi) {
 // An infinity or NaN in either half of a packed pair.
 template <typename T>
 OSSM_DEV bool nonfinite2(uint32_t u) {
-  constexpr uint32_t e = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   return (u & e) == e || (u & (e << 16)) == (e << 16);
 }
 

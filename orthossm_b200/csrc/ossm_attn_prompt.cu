@@ -760,12 +760,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           // zeros, and if another one holds a non-finite value, the product
           // is taken here over the seen keys alone.
           uint4* vr = reinterpret_cast<uint4*>(vring + (g % NS) * C::kTile + row * 128);
-          bool bad = false;
+          uint32_t big = 0;  // the largest magnitudes, as packed integers: NaN and infinities are above all others
           if (j * kT + row < c.nk) {
 #pragma unroll
             for (int i = 0; i < 8 * C::kBoxes; ++i) {  // in an order that spreads the rows over the banks
               const uint4 u = vr[(i >> 3) * (kBox / 16) + ((i ^ row) & 7)];
-              bad |= nonfinite2<T>(u.x) || nonfinite2<T>(u.y) || nonfinite2<T>(u.z) || nonfinite2<T>(u.w);
+              big = __vmaxu2(__vmaxu2(big, u.x & 0x7fff7fffu), u.y & 0x7fff7fffu);
+              big = __vmaxu2(__vmaxu2(big, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu);
             }
           } else {
 #pragma unroll
@@ -773,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               vr[(i >> 3) * (kBox / 16) + ((i ^ row) & 7)] = make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();  // before the tensor core reads them
           }
-          const bool own = meet_any(1 + t, kT, bad);
+          const bool own = meet_any(1 + t, kT, nonfinite2<T>(big));
           if (row == 0) scalar[t] = own;
           if (own) {
             tmem_wait_st();
