@@ -84,6 +84,11 @@ OSSM_DEV bool nonfinite2(uint32_t u) {
   return (u & e) == e || (u & (e << 16)) == (e << 16);
 }
 
+OSSM_DEV unsigned long long warp_sum(unsigned long long v) {
+#pragma unroll
+  for (int w = 16; w; w >>= 1) v += __shfl_xor_sync(~0u, v, w);
+  return v;
+}
 OSSM_DEV float2 add2(float2 a, float2 b) {
   float2 d;
   asm("{\n\t.reg .b64 ra, rb, rd;\n\t"

@@ -166,7 +166,7 @@ struct Sched {
     return cut(c, it, in);
   }
   OSSM_DEV int owner(i64 pos) const {  // the CTA whose part holds a position: the last with cut(c) <= pos
-    int c = (int)min((i64)ncta - 1, pos / max((i64)1, total / ncta));
+    int c = (int)min((i64)ncta - 1, (i64)((double)pos * ncta / (double)total));  // off by the moved cuts only
     while (c > 0 && cut(c) > pos) --c;
     while (c + 1 < ncta && cut(c + 1) <= pos) ++c;
     return c;
@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     pre[g + 1] = len;
   }
-  if (mine) atomicAdd(&n_items, mine);
+  mine = warp_sum(mine);
+  if (lane == 0 && mine) atomicAdd(&n_items, mine);
   __syncthreads();
   if (warp == 0) {  // prefix sums, 32 groups at a time
     i64 run = 0;

@@ -108,7 +108,7 @@ struct Line {
     return pos - it.start <= near ? it.start : pos;
   }
   OSSM_DEV int owner(i64 pos) const {  // the CTA whose part holds a position: the last with cut(c) <= pos
-    int c = (int)min((i64)ncta - 1, pos / max((i64)1, total / ncta));
+    int c = (int)min((i64)ncta - 1, (i64)((double)pos * ncta / (double)total));  // off by the moved cuts only
     while (c > 0 && cut(c) > pos) --c;
     while (c + 1 < ncta && cut(c + 1) <= pos) ++c;
     return c;
@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       }
       pre[g + 1] = len;
     }
-    if (mine) atomicAdd(&n_items, mine);
+    mine = warp_sum(mine);
+    if (lane == 0 && mine) atomicAdd(&n_items, mine);
     __syncthreads();
     if (warp == 0) {
       i64 run = 0;
