@@ -1,21 +1,24 @@
 // Attention of many queries a sequence: prompts, pieces of prompts.
 //
 // Work item: two tiles of 128 rows that share their keys.  A row is a query of
-// one of g heads (row = query * g + head), g the largest power of two that
-// divides the heads per key head: one read of K and V serves the group, and a
-// few queries of a large group still fill a tile.  An item walks its range of
-// 128-key tiles once with a running maximum and sum per row.
+// one of g heads (row = query * g + head), g a power of two that divides the
+// heads per key head, so that a few queries of a large group still fill a
+// tile.  An item walks its range of 128-key tiles once with a running maximum
+// and sum per row.
 //
 // One persistent CTA per SM, three warpgroups:
 //   warps 0-3, 4-7  softmax of tile 0 / 1: a thread owns a row.  Scores from
-//                   tensor memory, mask, maximum, exponentials, weights back
-//                   to tensor memory over the scores; at the end the output
-//                   row out of the accumulator.
-//   warp 8          issues the products S_t = Q_t K^T (tcgen05.mma, both operands
-//                   in shared memory).
-//   warps 10, 11    issue O_t += P_t V for tile 0 / 1 (P_t in tensor memory, V read MN-major, so
-//                   it is never transposed).
+//                   tensor memory, mask, maximum, exponentials, weights to
+//                   tensor memory; at the end the output row out of the
+//                   accumulator.  They also look through the V tiles that some
+//                   row does not see whole (hidden values, below).
+//   warp 8          issues the products S_t = Q_t K^T (tcgen05.mma, both
+//                   operands in shared memory).
 //   warp 9          walks the schedule, loads Q, K and V tiles by TMA.
+//   warps 10, 11    issue O_t += P_t V for tile 0 / 1 (P_t in tensor memory, V
+//                   read MN-major, so it is never transposed).
+// One warp for all products spent its time waiting (16384 causal, 16 heads of
+// 128: 1157 us against 937 us with three).
 // Tensor memory (512 columns): scores, weights P_0 P_1, accumulators O_0 O_1.
 // Up to 64 channels each tile has a score buffer of its own; above that there
 // is room for one, which the tiles use in turn: a softmax takes its scores
@@ -32,6 +35,17 @@
 // cut near an item's edge moves to the edge; an item that stays cut leaves
 // partial sums in the workspace, and whichever CTA finishes it last joins
 // them, in the order of the cut.
+//
+// What bounds it: the exponentials.  A step of an item (two tiles, 128 keys)
+// is 1024 (64 channels) or 2048 cycles (128) of the tensor core and 2048 cycles
+// of the special function unit (16 results a clock and SM); the softmax's
+// other work overlaps with the other tile's exponentials in part.  Measured, at
+// the clock under load: 16384 causal, fp16, 16 heads of 128: 940-995 us, 1105
+// to 1170 TFLOP/s (0.67-0.71 of measured cuBLAS); 8 heads of 64: 435-455 us;
+// 2 x 16384 with a window of 512, 8 heads of 64: 96 us.  Tried and slower:
+// part of the exponentials as a polynomial on the FMA pipe (1 to 4 of 8:
+// +1 to +9 %), the tiles taking turns at them (+3 to +13 %), a row on two
+// threads (16 softmax warps: +25 % at 128 channels).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -347,6 +361,7 @@ constexpr long long kWaitCycles = 1LL << 31;  // about a second
 struct Failed {
   int* flag;
   OSSM_DEV bool one(uint64_t* bar, uint32_t parity) const {  // one thread; true: give up
+    if (mbar_test(bar, parity)) return false;
     const long long t0 = clock64();
     while (!mbar_test(bar, parity))
       if (clock64() - t0 > kWaitCycles) {
@@ -367,6 +382,14 @@ struct Failed {
   }
 };
 
+// An arrival under a predicate, without a branch.
+OSSM_DEV void mbar_arrive_if(uint64_t* bar, bool pred) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"((uint32_t)pred)
+      : "memory");
+}
 // The waits of warps that also meet at named barriers: one that ran out is
 // remembered (dead) and the warp goes on without waiting, so that the others
 // are not left at a barrier; they agree to stop at the next piece.
@@ -374,7 +397,8 @@ struct Waits {
   const Failed& f;
   bool dead;
   OSSM_DEV void operator()(uint64_t* bar, uint32_t parity) {
-    if (!dead) dead = f(bar, parity);
+    if (!dead) dead = f.one(bar, parity);
+    __syncwarp();
   }
 };
 
@@ -396,6 +420,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int failed, last_in[2];
   __shared__ unsigned long long n_items;
   __shared__ i64 cuts[2];
+  __shared__ Sched::Item item;  // the first one, if item_in
+  __shared__ bool item_in;
 
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, cta = blockIdx.x;
 
@@ -440,8 +466,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   // edge is the nearest one to some cut and short items get a CTA each
   sc.ncta = (int)min((i64)gridDim.x, max(2 * (i64)n_items, sc.total / 8));
   if (cta >= sc.ncta) return;
-  Sched::Item item;  // the first one (warp 9)
-  bool item_in = false;
   if (threadIdx.x == 9 * 32) cuts[0] = sc.cut(cta, item, item_in);
   if (threadIdx.x == 10 * 32) cuts[1] = sc.cut(cta + 1);
 
@@ -473,201 +497,203 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tslot;
   const Failed gave_up{&failed};
 
-  // 256 x 200 + 128 x 104 = 384 x 168 registers
+  // 256 x 216 + 128 x 72 = 384 x 168 registers.  With 200 and 104 the softmax
+  // spilled within its loop (16384 causal, 8 heads of 64: 448 us against 388).
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  if (warp == 9) {
-    // ---------------------------------------------------------- schedule and loads
-    if (lane == 0) {
-      prefetch_tmap(&mQ);
-      prefetch_tmap(&mK);
-      prefetch_tmap(&mV);
-      const i64 end = cuts[1];
-      i64 pos = cuts[0];
-      int n = 0, nq[2] = {0, 0};
-      uint32_t ki = 0, vi = 0;  // K and V tiles loaded; V runs one behind
-      bool ok = true;
-      auto load = [&](bool v, int head, int row) {
-        const uint32_t i = v ? vi++ : ki++, r = i % NS;
-        uint64_t* full = v ? &bars.v_full[r] : &bars.k_full[r];
-        if (i >= NS && gave_up.one(v ? &bars.v_empty[r] : &bars.k_empty[r], ((i / NS) & 1) ^ 1)) {
-          --(v ? vi : ki);
-          return false;
-        }
-        mbar_expect_tx(full, C::kTile);
-        for (int x = 0; x < C::kBoxes; ++x)
-          tma_load_3d((v ? vring : kring) + r * C::kTile + x * kBox, v ? &mV : &mK, full, 64 * x, head, row);
-        return true;
-      };
-      for (;; ++n) {
-        Piece c;
-        c.live = 0;
-        while (pos < end) {  // the next piece with work
-          const Sched::Item x = item_in ? item : sc.at(pos);
-          item_in = false;
-          const int a = (int)min(pos - x.start, (i64)x.n()), b = (int)min(end - x.start, (i64)x.n());
-          const bool head = pos == x.start;
-          pos = min(end, x.end());
-          if (a >= b && !(head && x.n() == 0)) continue;
-          c.live = 1;
-          c.q0 = x.q.q0, c.k0 = x.q.k0, c.nk = x.q.nk, c.off = x.q.nk - x.q.nq;
-          c.nrows = x.q.nq << lg;
-          c.head = x.unit << lg;
-          c.row0 = x.blk * 2 * kT;
-          const int base = x.f.lo(x.blk);
-          c.j0 = base + a, c.j1 = base + b;
-          for (int t = 0; t < 2; ++t) {
-            const int row0 = c.row0 + t * kT, first = (row0 >> lg) + c.off;
-            const int top = ((min(row0 + kT, c.nrows) - 1) >> lg) + c.off;
-            int lo = p.window ? max(0, first - p.window + 1) >> kLT : 0, hi = top < 0 ? 0 : (top >> kLT) + 1;
-            if (row0 >= c.nrows) hi = lo = 0;
-            c.lo[t] = max(lo, c.j0);
-            c.hi[t] = max(c.lo[t], min(hi, c.j1));
-            c.w0[t] = p.window ? ((top - p.window) >> kLT) + 1 : 0;
-            c.w1[t] = (first + 1) >> kLT;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 9) {
+      // ---------------------------------------------------------- schedule and loads
+      if (lane == 0) {
+        prefetch_tmap(&mQ);
+        prefetch_tmap(&mK);
+        prefetch_tmap(&mV);
+        const i64 end = cuts[1];
+        i64 pos = cuts[0];
+        int n = 0, nq[2] = {0, 0};
+        uint32_t ki = 0, vi = 0;  // K and V tiles loaded; V runs one behind
+        bool ok = true;
+        auto load = [&](bool v, int head, int row) {
+          const uint32_t i = v ? vi++ : ki++, r = i % NS;
+          uint64_t* full = v ? &bars.v_full[r] : &bars.k_full[r];
+          if (i >= NS && gave_up.one(v ? &bars.v_empty[r] : &bars.k_empty[r], ((i / NS) & 1) ^ 1)) {
+            --(v ? vi : ki);
+            return false;
           }
-          c.split = b - a < x.n();
-          if (c.split) {
-            c.len = x.n();
-            c.start = x.start;
-            c.slot = head ? 2 * cta + 1 : 2 * cta;
-            c.first = head ? cta : sc.owner(x.start);
-          }
-          break;
-        }
-        const int sl = n % kPieces;
-        if (n >= kPieces && gave_up.one(&bars.piece_empty[sl], ((n / kPieces) & 1) ^ 1)) {
-          ok = false;
-          break;
-        }
-        pieces[sl] = c;
-        mbar_arrive(&bars.piece_full[sl]);
-        if (!c.live) break;
-        const int kvh = c.head / (p.H / p.Hkv);
-        for (int j = c.j0; j < c.j1 && ok; ++j) {
-          if (j == c.j0)
-            for (int t = 0; t < 2 && ok; ++t) {
-              if (c.lo[t] >= c.hi[t]) continue;
-              if (nq[t] && gave_up.one(&bars.q_empty[t], (nq[t] & 1) ^ 1)) {
-                ok = false;
-                break;
-              }
-              ++nq[t];
-              mbar_expect_tx(&bars.q_full[t], C::kTile);
-              for (int x = 0; x < C::kBoxes; ++x)
-                tma_load_3d(smem + t * C::kTile + x * kBox, &mQ, &bars.q_full[t], 64 * x, c.head,
-                            c.q0 + ((c.row0 + t * kT) >> lg));
-            }
-          ok = ok && load(false, kvh, c.k0 + j * kT) && (j == c.j0 || load(true, kvh, c.k0 + (j - 1) * kT));
-        }
-        if (c.j0 < c.j1) ok = ok && load(true, kvh, c.k0 + (c.j1 - 1) * kT);
-        if (!ok) break;
-      }
-      if (!ok) {  // no copy may still be landing when the CTA exits
-        for (int t = 0; t < 2; ++t)
-          if (nq[t]) gave_up.one(&bars.q_full[t], (nq[t] & 1) ^ 1);
-        for (uint32_t i = ki > NS ? ki - NS : 0; i < ki; ++i) gave_up.one(&bars.k_full[i % NS], (i / NS) & 1);
-        for (uint32_t i = vi > NS ? vi - NS : 0; i < vi; ++i) gave_up.one(&bars.v_full[i % NS], (i / NS) & 1);
-      }
-    }
-  } else if (warp == 8) {
-    // ---------------------------------------------------------- S_t = Q_t K^T
-    // Scores and outputs are issued by a warp each: one for both was busy with
-    // its waits and left the tensor core idle.  The whole warp walks the loop,
-    // so that operands stay uniform; one lane issues.
-    constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, kT, 0);
-    const bool leader = elect_one();
-    const uint32_t qb = smem_u32(smem), kb = smem_u32(kring);
-    uint32_t nq[2] = {0, 0}, ns[2] = {0, 0}, g = 0;
-    bool ok = true;
-    for (int n = 0; ok; ++n) {
-      const int sl = n % kPieces;
-      if (gave_up(&bars.piece_full[sl], (n / kPieces) & 1)) break;
-      const Piece& c = pieces[sl];
-      if (!c.live) break;
-      const int j1 = c.j1, lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
-      int j = c.j0;
-      __syncwarp();
-      if (leader) mbar_arrive(&bars.piece_empty[sl]);
-      for (; j < j1 && ok; ++j, ++g) {
-        const uint32_t r = g % NS;
-        if (gave_up(&bars.k_full[r], (g / NS) & 1)) {
-          ok = false;
-          break;
-        }
-        const uint64_t kd = sdesc(kb + r * C::kTile, 16);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j < lo[t] || j >= hi[t]) continue;
-          constexpr int kS = C::kS;
-          const int b = t % kS;
-          if ((j == lo[t] && gave_up(&bars.q_full[t], nq[t]++ & 1)) ||
-              (ns[b] && gave_up(&bars.s_free[b], (ns[b] & 1) ^ 1))) {
+          mbar_expect_tx(full, C::kTile);
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_3d((v ? vring : kring) + r * C::kTile + x * kBox, v ? &mV : &mK, full, 64 * x, head, row);
+          return true;
+        };
+        for (;; ++n) {
+          const int sl = n % kPieces;
+          if (n >= kPieces && gave_up.one(&bars.piece_empty[sl], ((n / kPieces) & 1) ^ 1)) {
             ok = false;
             break;
           }
-          ++ns[b];
+          Piece& c = pieces[sl];
+          c.live = 0;
+          while (pos < end) {  // the next piece with work
+            const Sched::Item x = item_in ? item : sc.at(pos);
+            item_in = false;
+            const int a = (int)min(pos - x.start, (i64)x.n()), b = (int)min(end - x.start, (i64)x.n());
+            const bool head = pos == x.start;
+            pos = min(end, x.end());
+            if (a >= b && !(head && x.n() == 0)) continue;
+            c.live = 1;
+            c.q0 = x.q.q0, c.k0 = x.q.k0, c.nk = x.q.nk, c.off = x.q.nk - x.q.nq;
+            c.nrows = x.q.nq << lg;
+            c.head = x.unit << lg;
+            c.row0 = x.blk * 2 * kT;
+            const int base = x.f.lo(x.blk);
+            c.j0 = base + a, c.j1 = base + b;
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+              const int row0 = c.row0 + t * kT, first = (row0 >> lg) + c.off;
+              const int top = ((min(row0 + kT, c.nrows) - 1) >> lg) + c.off;
+              int lo = p.window ? max(0, first - p.window + 1) >> kLT : 0, hi = top < 0 ? 0 : (top >> kLT) + 1;
+              if (row0 >= c.nrows) hi = lo = 0;
+              c.lo[t] = max(lo, c.j0);
+              c.hi[t] = max(c.lo[t], min(hi, c.j1));
+              c.w0[t] = p.window ? ((top - p.window) >> kLT) + 1 : 0;
+              c.w1[t] = (first + 1) >> kLT;
+            }
+            c.split = b - a < x.n();
+            if (c.split) {
+              c.len = x.n();
+              c.start = x.start;
+              c.slot = head ? 2 * cta + 1 : 2 * cta;
+              c.first = head ? cta : sc.owner(x.start);
+            }
+            break;
+          }
+          mbar_arrive(&bars.piece_full[sl]);
+          if (!c.live) break;
+          const int kvh = c.head / (p.H / p.Hkv);
+          for (int j = c.j0; j < c.j1 && ok; ++j) {
+            if (j == c.j0)
+#pragma unroll 1
+              for (int t = 0; t < 2 && ok; ++t) {
+                if (c.lo[t] >= c.hi[t]) continue;
+                if (nq[t] && gave_up.one(&bars.q_empty[t], (nq[t] & 1) ^ 1)) {
+                  ok = false;
+                  break;
+                }
+                ++nq[t];
+                mbar_expect_tx(&bars.q_full[t], C::kTile);
+                for (int x = 0; x < C::kBoxes; ++x)
+                  tma_load_3d(smem + t * C::kTile + x * kBox, &mQ, &bars.q_full[t], 64 * x, c.head,
+                              c.q0 + ((c.row0 + t * kT) >> lg));
+              }
+            ok = ok && load(false, kvh, c.k0 + j * kT) && (j == c.j0 || load(true, kvh, c.k0 + (j - 1) * kT));
+          }
+          if (c.j0 < c.j1) ok = ok && load(true, kvh, c.k0 + (c.j1 - 1) * kT);
+          if (!ok) break;
+        }
+        if (!ok) {  // no copy may still be landing when the CTA exits
+          for (int t = 0; t < 2; ++t)
+            if (nq[t]) gave_up.one(&bars.q_full[t], (nq[t] & 1) ^ 1);
+          for (uint32_t i = ki > NS ? ki - NS : 0; i < ki; ++i) gave_up.one(&bars.k_full[i % NS], (i / NS) & 1);
+          for (uint32_t i = vi > NS ? vi - NS : 0; i < vi; ++i) gave_up.one(&bars.v_full[i % NS], (i / NS) & 1);
+        }
+      }
+    } else if (warp == 8) {
+      // ---------------------------------------------------------- S_t = Q_t K^T
+      // Scores and outputs are issued by a warp each: one for both was busy with
+      // its waits and left the tensor core idle.  The whole warp walks the loop,
+      // so that operands stay uniform; one lane issues.
+      constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, kT, 0);
+      const bool leader = elect_one();
+      const uint32_t qb = smem_u32(smem), kb = smem_u32(kring);
+      uint32_t nq[2] = {0, 0}, ns[2] = {0, 0}, g = 0;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int sl = n % kPieces;
+        if (gave_up(&bars.piece_full[sl], (n / kPieces) & 1)) break;
+        const Piece& c = pieces[sl];
+        if (!c.live) break;
+        const int j1 = c.j1, lo[2] = {c.lo[0], c.lo[1]}, hi[2] = {c.hi[0], c.hi[1]};
+        int j = c.j0;
+        __syncwarp();
+        if (leader) mbar_arrive(&bars.piece_empty[sl]);
+        for (; j < j1 && ok; ++j, ++g) {
+          const uint32_t r = g % NS;
+          if (gave_up(&bars.k_full[r], (g / NS) & 1)) {
+            ok = false;
+            break;
+          }
+          const uint64_t kd = sdesc(kb + r * C::kTile, 16);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j < lo[t] || j >= hi[t]) continue;
+            constexpr int kS = C::kS;
+            const int b = t % kS;
+            if ((j == lo[t] && gave_up(&bars.q_full[t], nq[t]++ & 1)) ||
+                (ns[b] && gave_up(&bars.s_free[b], (ns[b] & 1) ^ 1))) {
+              ok = false;
+              break;
+            }
+            ++ns[b];
+            tc_fence_after();
+            if (leader) {
+              const uint64_t qd = sdesc(qb + t * C::kTile, 16);
+#pragma unroll
+              for (int kk = 0; kk < HDP / 16; ++kk) {
+                const uint32_t o = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+                mma_ss(tmem + b * kT, qd + o, kd + o, id, kk > 0);
+              }
+              mma_commit(&bars.s_full[t]);
+              if (j == hi[t] - 1) mma_commit(&bars.q_empty[t]);
+            }
+          }
+          if (leader) mma_commit(&bars.k_empty[r]);
+        }
+      }
+      if (!ok) failed = 1;
+    } else {
+      // ---------------------------------------------------------- O_t += P_t V
+      constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, HDP, 1);
+      const bool leader = elect_one();
+      const uint32_t vb = smem_u32(vring);
+      const int t = warp - 10;
+      uint32_t np = 0, g = 0;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        const int sl = n % kPieces;
+        if (gave_up(&bars.piece_full[sl], (n / kPieces) & 1)) break;
+        const Piece& c = pieces[sl];
+        if (!c.live) break;
+        const int j1 = c.j1, lo = c.lo[t], hi = c.hi[t];
+        int j = c.j0;
+        __syncwarp();
+        if (leader) mbar_arrive(&bars.piece_empty[sl]);
+        for (; j < j1; ++j, ++g) {
+          const uint32_t r = g % NS;
+          const bool act = j >= lo && j < hi;
+          if (gave_up(&bars.v_full[r], (g / NS) & 1) || (act && gave_up(&bars.p_ready[t], np++ & 1))) {
+            ok = false;
+            break;
+          }
           tc_fence_after();
           if (leader) {
-            const uint64_t qd = sdesc(qb + t * C::kTile, 16);
+            if (act) {
+              if (!*(volatile int*)&scalar[t]) {
+                const uint64_t vd = sdesc(vb + r * C::kTile, kBox);
 #pragma unroll
-            for (int kk = 0; kk < HDP / 16; ++kk) {
-              const uint32_t o = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
-              mma_ss(tmem + b * kT, qd + o, kd + o, id, kk > 0);
+                for (int kk = 0; kk < kT / 16; ++kk)
+                  mma_ts(tmem + C::kO + t * HDP, tmem + C::kP + t * (kT / 2) + kk * 8, vd + kk * (2048 >> 4), id,
+                         kk > 0 || j > lo);
+              }
+              mma_commit(&bars.pv_done[t]);
             }
-            mma_commit(&bars.s_full[t]);
-            if (j == hi[t] - 1) mma_commit(&bars.q_empty[t]);
+            mma_commit(&bars.v_empty[r]);
           }
+          __syncwarp();
         }
-        if (leader) mma_commit(&bars.k_empty[r]);
       }
+      if (!ok) failed = 1;
     }
-    if (!ok) failed = 1;
   } else {
-    // ---------------------------------------------------------- O_t += P_t V
-    constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, HDP, 1);
-    const bool leader = elect_one();
-    const uint32_t vb = smem_u32(vring);
-    const int t = warp - 10;
-    uint32_t np = 0, g = 0;
-    bool ok = true;
-    for (int n = 0; ok; ++n) {
-      const int sl = n % kPieces;
-      if (gave_up(&bars.piece_full[sl], (n / kPieces) & 1)) break;
-      const Piece& c = pieces[sl];
-      if (!c.live) break;
-      const int j1 = c.j1, lo = c.lo[t], hi = c.hi[t];
-      int j = c.j0;
-      __syncwarp();
-      if (leader) mbar_arrive(&bars.piece_empty[sl]);
-      for (; j < j1; ++j, ++g) {
-        const uint32_t r = g % NS;
-        const bool act = j >= lo && j < hi;
-        if (gave_up(&bars.v_full[r], (g / NS) & 1) || (act && gave_up(&bars.p_ready[t], np++ & 1))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (leader) {
-          if (act) {
-            if (!*(volatile int*)&scalar[t]) {
-              const uint64_t vd = sdesc(vb + r * C::kTile, kBox);
-#pragma unroll
-              for (int kk = 0; kk < kT / 16; ++kk)
-                mma_ts(tmem + C::kO + t * HDP, tmem + C::kP + t * (kT / 2) + kk * 8, vd + kk * (2048 >> 4), id,
-                       kk > 0 || j > lo);
-            }
-            mma_commit(&bars.pv_done[t]);
-          }
-          mma_commit(&bars.v_empty[r]);
-        }
-        __syncwarp();
-      }
-    }
-    if (!ok) failed = 1;
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------------------------------------------------- softmax and output
     const int t = warp >> 2, row = threadIdx.x & (kT - 1);
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), tS = tl + (t % C::kS) * kT,
@@ -683,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto free_scores = [&]() {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.s_free[t % C::kS]);
+      mbar_arrive_if(&bars.s_free[t % C::kS], lane == 0);
     };
     for (int n = 0;; ++n) {
       const int sl = n % kPieces;
@@ -713,23 +739,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {  // bit e: key 32 i + e is seen
             const int a = k_lo - 32 * i, b = k_hi - 32 * i;
-            const uint32_t up = b >= 31 ? ~0u : b < 0 ? 0u : (2u << b) - 1u, low = a <= 0 ? ~0u : a > 31 ? 0u : ~0u << a;
-            const uint32_t seen = up & low;
+            const uint32_t up = b >= 31 ? ~0u : b < 0 ? 0u : (2u << b) - 1u;
+            const uint32_t seen = up & (a <= 0 ? ~0u : a > 31 ? 0u : ~0u << a);
 #pragma unroll
             for (int e = 0; e < 32; ++e) x[32 * i + e] = (seen >> e & 1u) ? x[32 * i + e] : -INFINITY;
           }
         }
-        float mx[4];
+        float mx[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          mx[i] = x[32 * i];
+        for (int i = 0; i < 8; ++i) mx[i] = max3(x[16 * i], x[16 * i + 1], x[16 * i + 2]);
 #pragma unroll
-          for (int e = 1; e < 31; e += 2) mx[i] = max3(mx[i], x[32 * i + e], x[32 * i + e + 1]);
-        }
-        mx[0] = max3(mx[0], mx[1], x[31]);
-        mx[1] = max3(mx[2], mx[3], x[63]);
-        mx[0] = max3(mx[0], mx[1], x[95]);
-        const float top = max3(mx[0], x[127], x[127]) * p.scale2;
+        for (int e = 3; e < 15; e += 2)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mx[i] = max3(mx[i], x[16 * i + e], x[16 * i + e + 1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mx[i] = max3(max3(mx[i], mx[i + 4], x[16 * i + 15]), x[16 * i + 79], x[16 * i + 79]);
+        mx[0] = max3(mx[0], mx[1], mx[2]);
+        const float top = max3(mx[0], mx[3], mx[3]) * p.scale2;
         if (!(top < INFINITY)) m = NAN;  // a seen score is NaN or infinite: so is the softmax's sum
         const bool grow = top > m + 8.f;
         if (__any_sync(~0u, grow)) {
@@ -815,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p_ready[t]);
+        mbar_arrive_if(&bars.p_ready[t], lane == 0);
       }
       it += c.j1 - j0;
       settled(ns);

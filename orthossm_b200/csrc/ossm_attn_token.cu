@@ -14,6 +14,11 @@
 //
 // The weights enter the product with V as a sum of two 16-bit terms, so that
 // their rounding does not add to the output's; the reads hide that product.
+//
+// Measured: 64 streams of up to 8192 keys, 32/8 heads of 128: 191 us, 6.3 TB/s
+// (0.97 of measured copy bandwidth); one stream of 1048576 keys, 8 heads of 64:
+// 350 us, 6.1 TB/s; 32 streams with a window of 512: 14 us (5.1 us of reads:
+// bound by the launch, the schedule and one item's chain of loads and merge).
 #include <algorithm>
 
 #include "ossm_attn.cuh"
@@ -118,9 +123,10 @@ struct Line {
 template <typename T>
 OSSM_DEV void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

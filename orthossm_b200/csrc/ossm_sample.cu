@@ -114,7 +114,8 @@ OSSM_DEV void unpack(const uint4& u, float (&l)[4], float) {
 OSSM_DEV void unpack(const uint4& u, float (&l)[8], __nv_bfloat16) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) l[2 * i] = __uint_as_float(w[i] << 16), l[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  for (int i = 0; i < 4; ++i)
+    l[2 * i] = __uint_as_float(w[i] << 16), l[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
 }
 OSSM_DEV void unpack(const uint4& u, float (&l)[8], __half) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -477,7 +478,8 @@ OSSM_DEV float lg2(float x) {  // log2, within 2^-22 (of 1, or of its value)
 // the warp's best, `mark` (a thread's own best is passed by some lane at almost
 // every step).
 template <typename T, typename F>
-OSSM_DEV void race(const float* l, const float* e, int i, int n, float low, F stays, float inv_t, Best& b, float& mark) {
+OSSM_DEV void race(const float* l, const float* e, int i, int n, float low, F stays, float inv_t, Best& b,
+                   float& mark) {
   const float bar = mark - 1e-4f;
   uint32_t near = 0;
 #pragma unroll

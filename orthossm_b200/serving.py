@@ -37,8 +37,11 @@ def _tma_rows(t):
         t.clone(memory_format=torch.contiguous_format)
 
 
+_I32 = torch.int32
+
+
 def _vector(t, n, dev):
-    return t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.get_device() == dev
+    return t.dtype is _I32 and t.shape == (n,) and t.get_device() == dev
 
 
 def _refuse_attention(q, k, v, cu_q, cu_k, kv_lengths, window, scale, out):
@@ -119,30 +122,30 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                           out)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError("packed_attention has no backward pass: call it under torch.no_grad()")
+    ot, oh = H * hd, hd
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        ot, oh, unit = out.stride()
+        if not _rows_ok(ot, oh, unit, Tq, H, out.data_ptr()):
+            _refuse_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, kv_lengths, window, scale_, out)
     if Tq == 0:
         return out
-    layout = []
-    for t, n, heads in ((q, Tq, H), (k, Tk, Hkv), (v, Tk, Hkv), (out, Tq, H)):
-        st, sh, sd = t.stride()
-        ptr = t.data_ptr()
-        if not _rows_ok(st, sh, sd, n, heads, ptr):
-            if t is out:
-                _refuse_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, kv_lengths, window, scale_, out)
-            t = t.clone(memory_format=torch.contiguous_format)
-            st, sh, _ = t.stride()
-            ptr = t.data_ptr()
-        layout.append((t, ptr, st, sh))  # t: kept until the launch
-    (_, qp, qt, qh), (_, kp, kt, kh), (_, vp, vt, vh), (_, op, ot, oh) = layout
+    (qt, qh, qu), (kt, kh, ku), (vt, vh, vu) = q.stride(), k.stride(), v.stride()
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (qu != 1 or ku != 1 or vu != 1 or (qt | qh | kt | kh | vt | vh) & 7 or (qp | kp | vp) & 15
+            or not (qt and qh and kt and kh and vt and vh)):
+        q, k, v = _tma_rows(q), _tma_rows(k), _tma_rows(v)  # copies of what cannot be read as it is
+        (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if not cu_seqlens_q.is_contiguous():
         cu_seqlens_q, cu_k = cu_seqlens_q.contiguous(), cu_k.contiguous()
     elif not cu_k.is_contiguous():
         cu_k = cu_k.contiguous()
     if kv_lengths is not None and not kv_lengths.is_contiguous():
         kv_lengths = kv_lengths.contiguous()
-    a = L.AttnArgs(B, H, Hkv, hd, Tq, Tk, min(int(max_seqlen_q), 0x7fffffff), dt, qp, kp, vp, op, qt, qh, kt, kh, vt,
-                   vh, ot, oh, cu_seqlens_q.data_ptr(), cu_k.data_ptr(),
+    a = L.AttnArgs(B, H, Hkv, hd, Tq, Tk, min(int(max_seqlen_q), 0x7fffffff), dt, qp, kp, vp, out.data_ptr(), qt, qh,
+                   kt, kh, vt, vh, ot, oh, cu_seqlens_q.data_ptr(), cu_k.data_ptr(),
                    None if kv_lengths is None else kv_lengths.data_ptr(),
                    0 if window is None else min(int(window), 0x7fffffff), scale_)
     if dev != torch.cuda.current_device():
@@ -239,8 +242,8 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
                          f"min_p {m} in [0, 1]")
     if B == 0:
         return out
-    a = L.SampleArgs(B, V, logits.data_ptr(), dt, lst, _ptr(noise), nst, 1.0 / t if t > 0 else 0.0, p, m, min(int(k), V),
-                     _ptr(t_row), _ptr(p_row), _ptr(m_row), _ptr(k_row), out.data_ptr())
+    a = L.SampleArgs(B, V, logits.data_ptr(), dt, lst, _ptr(noise), nst, 1.0 / t if t > 0 else 0.0, p, m,
+                     min(int(k), V), _ptr(t_row), _ptr(p_row), _ptr(m_row), _ptr(k_row), out.data_ptr())
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             status = L.lib().ossm_sample_tokens(L.C.byref(a), _raw_stream(dev))

@@ -32,8 +32,8 @@ def packed_attention_ref(q, k, v, cu_q, cu_k, kv_lengths=None, window=None, scal
 
 def bound(ref, mag, dtype, keys, vmax):
     """Elementwise error bound.  Roundings to the type (8 significant bits in
-    bf16, 11 in fp16: to within u = 2^-8 and 2^-11 of the value): the output's, u |o|, and each weight's before the product
-    with v, u sum p|v|.  fp32: the scores (sums of hd products, |s| up to a few
+    bf16, 11 in fp16: to within u = 2^-8 and 2^-11 of the value): the
+    output's, u |o|, and each weight's before the product with v, u sum p|v|.  fp32: the scores (sums of hd products, |s| up to a few
     tens) and the exponential move each weight by less than 2^-12 of itself.
     fp16 weights below 2^-14 of the largest are rounded to steps of 2^-24."""
     u = 2.0 ** (-8 if dtype == torch.bfloat16 else -11)

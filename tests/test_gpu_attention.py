@@ -143,7 +143,8 @@ def test_layouts(nq, nk):
 
 
 @pytest.mark.parametrize("H,Hkv,hd", [(3, 3, 128), (8, 2, 64), (6, 1, 96)])
-@pytest.mark.parametrize("nq,nk,window", [(9000, 9000, None), (7000, 7000, 300), (900, 20000, None), (260, 40000, None)])
+@pytest.mark.parametrize("nq,nk,window",
+                         [(9000, 9000, None), (7000, 7000, 300), (900, 20000, None), (260, 40000, None)])
 def test_long_sequences(H, Hkv, hd, nq, nk, window):
     """Many items a CTA, and items cut between CTAs: rows spread over the
     sequence against the reference."""
