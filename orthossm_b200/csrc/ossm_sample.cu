@@ -35,6 +35,7 @@ namespace smp {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024;
+constexpr int kOpen = 512;     // threads of a CTA where nothing is filtered
 constexpr int kList = 4096;    // candidates that are ordered in shared memory
 constexpr int kRank = 512;     // up to here by counting the larger ones, above by a bitonic sort
 typedef unsigned long long u64;
@@ -163,7 +164,7 @@ OSSM_DEV void scan(const T* row, int V, int rank, int nrank, F f) {
 
 // The same with the noise of each logit: f(l, e, i, n).  Both are loaded ahead
 // for several vectors, as the noise comes from HBM.
-template <typename T, typename F>
+template <int NT, typename T, typename F>
 OSSM_DEV void scan_noise(const T* row, const float* nz, int V, int rank, int nrank, F f) {
   constexpr int N = Vec<T>::n, U = 16 / N;
   const int head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
@@ -171,12 +172,12 @@ OSSM_DEV void scan_noise(const T* row, const float* nz, int V, int rank, int nra
   const uint4* body = reinterpret_cast<const uint4*>(row + head);
   const float* nbody = nz + head;
   const bool aligned = ((uintptr_t)nbody & 15) == 0;
-  for (int v = v0 + threadIdx.x; v < v1; v += U * kThreads) {
+  for (int v = v0 + threadIdx.x; v < v1; v += U * NT) {
     uint4 u[U];
     float e[U][N];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int w = v + k * kThreads;
+      const int w = v + k * NT;
       if (w >= v1) break;
       u[k] = __ldg(body + w);
       if (aligned) {
@@ -192,7 +193,7 @@ OSSM_DEV void scan_noise(const T* row, const float* nz, int V, int rank, int nra
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int w = v + k * kThreads;
+      const int w = v + k * NT;
       if (w >= v1) break;
       float l[N];
       unpack(u[k], l, T());
@@ -226,12 +227,13 @@ OSSM_DEV V block_reduce(V v, V* red, Op op) {  // the result in every thread
   return v;
 }
 
+template <int NT>
 OSSM_DEV Best block_best(Best b, Best* bests) {  // the result in warp 0
   for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) bests[threadIdx.x >> 5] = b;
   __syncthreads();
-  b = bests[threadIdx.x & 31];
+  b = bests[threadIdx.x & (NT / 32 - 1)];
   for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
   return b;
 }
@@ -503,6 +505,45 @@ struct Told {
   Best best;
 };
 
+// A row without filters: the best score of all its candidates.
+template <int NT, typename T>
+OSSM_DEV void open_row(const T* lg, const float* nz, int V, float inv_t, int rank, int nrank, Best* bests, Told& told,
+                       int64_t* out) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
+  Best b{0.f, -1};
+  float mark = -INFINITY;
+  scan_noise<NT>(lg, nz, V, rank, nrank, [&](const float* l, const float* e, int i, int n) {
+    race<T>(l, e, i, n, kLowest, [](float, int) { return true; }, inv_t, b, mark);
+  });
+  b = block_best<NT>(b, bests);
+  if (nrank > 1) {
+    if (tid == 0) told.best = b;
+    cluster.sync();
+    if (rank == 0 && tid < 32) {
+      b = Best{0.f, -1};
+      if (tid < nrank) b = cluster.map_shared_rank(&told, tid)->best;
+      for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
+    }
+    cluster.sync();  // the others' memory is read before they leave
+  }
+  if (rank == 0 && tid == 0) *out = b.i;
+}
+
+// Every row without filters (known on the host).  Two CTAs of 512 threads an SM
+// cover one another's loads and tails: 256 rows of 32000 fp32, 11.9 us (10.0 us
+// of reads; 15.1 us with one CTA of 1024), 256 of 131072 bf16, 35.6 us (30.8
+// of reads).  At 40 registers a thread the loads ahead spill (17 and 38 us).
+template <typename T>
+__global__ void __launch_bounds__(kOpen, 2) open_kernel(const Params p) {
+  __shared__ Best bests[kOpen / 32];
+  __shared__ Told told;
+  const int nrank = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
+  const i64 row = blockIdx.x / nrank;
+  open_row<kOpen>(static_cast<const T*>(p.logits) + row * p.lst, p.noise + row * p.nst, p.V, p.inv_t, rank, nrank, bests,
+                  told, p.out + row);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   __shared__ Room room;
@@ -518,23 +559,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   if (tid == 0) told.count = 0;
 
   if (r.open()) {
-    Best b{0.f, -1};
-    float mark = -INFINITY;
-    scan_noise(lg, nz, p.V, rank, nrank, [&](const float* l, const float* e, int i, int n) {
-      race<T>(l, e, i, n, kLowest, [](float, int) { return true; }, r.inv_t, b, mark);
-    });
-    b = block_best(b, bests);
-    if (nrank > 1) {
-      if (tid == 0) told.best = b;
-      cluster.sync();
-      if (rank == 0 && tid < 32) {
-        b = Best{0.f, -1};
-        if (tid < nrank) b = cluster.map_shared_rank(&told, tid)->best;
-        for (int w = 16; w; w >>= 1) better(b, __shfl_xor_sync(~0u, b.s, w), __shfl_xor_sync(~0u, b.i, w));
-      }
-      cluster.sync();  // the others' memory is read before they leave
-    }
-    if (rank == 0 && tid == 0) p.out[row] = b.i;
+    open_row<kThreads>(lg, nz, p.V, r.inv_t, rank, nrank, bests, told, p.out + row);
     return;
   }
 
@@ -689,7 +714,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
         const u64 key = key_of(l, i);
         return key >= keep && (!(r.min_p > 0.f) || key == top || weight(l, m, r.inv_t) >= r.min_p);
       };
-      scan_noise(lg, nz, p.V, 0, 1, [&](const float* l, const float* e, int i, int n) {
+      scan_noise<kThreads>(lg, nz, p.V, 0, 1, [&](const float* l, const float* e, int i, int n) {
         race<T>(l, e, i, n, fmaxf(fmaxf(end, lb), kLowest), stays, r.inv_t, b, mark);
       });
     }
@@ -706,29 +731,31 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       if (e == 0 || r.greedy || !(r.min_p > 0.f) || weight(logit_of(key), m, r.inv_t) >= r.min_p) consider(key);
     }
   }
-  b = block_best(b, bests);
+  b = block_best<kThreads>(b, bests);
   if (tid == 0) p.out[row] = b.i;
 }
 
 // CTAs a row: as many as fill the GPU about once, with 4096 logits each at
 // least.  One row of 32000 with top-k 50 took 10.4 us with 4 CTAs and 13.7 us
 // with 8 (the bound, of each CTA's own threads, gets weak: 377 candidates are
-// collected instead of 90), 10.7 us with one; unfiltered 6.6, 5.8 and 8.8 us.
+// collected instead of 90), 10.7 us with one.
 template <typename T>
 cudaError_t launch(const Params& p, int B, cudaStream_t st) {
   const int sms = device_sms();
+  const bool open = p.noise && !p.t_row && !p.k_row && !p.p_row && !p.m_row && p.inv_t > 0.f && p.inv_t < INFINITY &&
+                    (p.top_k <= 0 || p.top_k >= p.V) && p.top_p >= 1.f && !(p.min_p > 0.f);
   int c = 1;
-  while (c < 8 && (i64)B * c * 2 <= sms && p.V / (2 * c) >= 4096) c *= 2;
+  while (c < 8 && (i64)B * c * (open ? 1 : 2) <= sms && p.V / (2 * c) >= 4096) c *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)B * c);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(open ? kOpen : kThreads);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = c, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+  return open ? cudaLaunchKernelEx(&cfg, open_kernel<T>, p) : cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
 }
 
 }  // namespace smp
