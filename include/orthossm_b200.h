@@ -407,8 +407,9 @@ typedef struct {
 } ossm_attn_args;
 
 /* Bytes of device workspace (zero-filled once when allocated, then reused by
- * calls ordered on one stream; its first 256 bytes are a header that
- * ossm_workspace_status reads); 0 for invalid arguments. */
+ * calls ordered on one stream, of any arguments that it is large enough for;
+ * its first 256 bytes are a header that ossm_workspace_status reads, and after
+ * OSSM_ETIMEOUT it has to be zero-filled again); 0 for invalid arguments. */
 size_t ossm_attn_workspace_bytes(const ossm_attn_args* a);
 int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream);
 

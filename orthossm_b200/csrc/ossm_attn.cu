@@ -28,7 +28,7 @@ bool valid(const ossm_attn_args* a) {
       a->total_q * a->H > 0x7fffffffLL)
     return false;
   if (a->dtype != OSSM_BF16 && a->dtype != OSSM_F16) return false;
-  if (a->window < 0 || !(a->scale > 0.f) || !std::isfinite(a->scale) || !a->cu_q || !a->cu_k) return false;
+  if (a->window < 0 || !(a->scale > 0.f) || !std::isfinite(a->scale * 1.5f) || !a->cu_q || !a->cu_k) return false;
   if (a->total_q == 0) return true;
   if (!row_ok(a->q, a->q_stride_t, a->q_stride_h, a->total_q, a->H) ||
       !row_ok(a->out, a->out_stride_t, a->out_stride_h, a->total_q, a->H))

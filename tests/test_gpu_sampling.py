@@ -88,6 +88,16 @@ def test_ties_flat_and_peaked_rows(f, V, spread):
     check(l, e, **f)
 
 
+@pytest.mark.parametrize("f", [dict(), dict(top_k=50), dict(top_k=3000, top_p=0.7), dict(top_p=0.95), dict(top_p=0.5),
+                               dict(top_p=0.9, min_p=0.001)],
+                         ids=lambda f: "_".join(f"{k}{v}" for k, v in f.items()) or "open")
+@pytest.mark.parametrize("B,V,spread", [(1, 150001, 1.0), (3, 131072, 2.5), (40, 30011, 1.0)])
+def test_long_rows(f, B, V, spread):
+    """Rows shared by several CTAs, wide prefixes, and rows beyond 2^17 logits."""
+    l, e = inputs(B, V, torch.bfloat16, seed=B, spread=spread)
+    check(l, e, temperature=1.1, **f)
+
+
 def test_all_equal():
     """One logit everywhere: the first k by index."""
     for val in (0.0, -0.0, 3.0, -7.5):
