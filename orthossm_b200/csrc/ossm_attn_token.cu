@@ -102,15 +102,23 @@ struct Line {
     it.start = base + (i64)u * (it.n + kItemCost);
     return it;
   }
-  OSSM_DEV i64 cut(int c) const {  // where CTA c's part begins
-    if (c <= 0) return 0;
+  // Where CTA c's part begins (and the item there, if it is not past the item's end).
+  OSSM_DEV i64 cut(int c, Item& it, bool& in) const {
+    in = false;
     if (c >= ncta) return total;
-    const i64 pos = total / ncta * c + total % ncta * c / ncta;
-    const Item it = at(pos);
+    const i64 pos = c <= 0 ? 0 : total / ncta * c + total % ncta * c / ncta;
+    it = at(pos);
     const i64 near = max((i64)kMinPiece, total / ncta / 16);
+    in = true;
     if (pos - it.start <= near && pos - it.start <= it.end() - pos) return it.start;
-    if (it.end() - pos <= near + kItemCost) return it.end();
+    in = it.end() - pos > near + kItemCost;
+    if (!in) return it.end();
     return pos - it.start <= near ? it.start : pos;
+  }
+  OSSM_DEV i64 cut(int c) const {
+    Item it;
+    bool in;
+    return cut(c, it, in);
   }
   OSSM_DEV int owner(i64 pos) const {  // the CTA whose part holds a position: the last with cut(c) <= pos
     int c = (int)min((i64)ncta - 1, (i64)((double)pos * ncta / (double)total));  // off by the moved cuts only
@@ -174,6 +182,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
   __shared__ float sm_p[kWarps][kRows][kWK];
   __shared__ int last_in;
   __shared__ i64 cuts[2];
+  __shared__ Line::Item item;  // the first one, if item_in
+  __shared__ bool item_in;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
   const int G = p.H / p.Hkv;
@@ -222,8 +232,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
   // twice the items: each item's edge is the nearest one to some cut, and short items get a CTA each
   ln.ncta = (int)min((i64)gridDim.x, max(2 * (i64)n_items, ln.total / kMinWork));
   if (cta >= ln.ncta) return;
-  if (lane == 0 && warp < 2) cuts[warp] = ln.cut(cta + warp);
+  if (lane == 0 && warp < 2) {
+    Line::Item it;
+    bool in;
+    cuts[warp] = ln.cut(cta + warp, it, in);
+    if (warp == 0) {
+      item = it;
+      item_in = in;
+    }
+  }
   __syncthreads();
+  bool known = item_in;
 
   const uint32_t ring = smem_u32(smem) + warp * (C::kStages * 2 * C::kTile);
   const uint8_t* ringp = smem + warp * (C::kStages * 2 * C::kTile);
@@ -231,7 +250,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
   i64 pos = cuts[0];
   const i64 end = cuts[1];
   while (pos < end) {
-    const Line::Item x = ln.at(pos);
+    const Line::Item x = known ? item : ln.at(pos);
+    known = false;
     const int a = (int)min(pos - x.start, (i64)x.n), b = (int)min(end - x.start, (i64)x.n);
     const bool head = pos == x.start;
     pos = min(end, x.end());
@@ -246,20 +266,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
 #pragma unroll
     for (int h = 0; h < 2; ++h) at[h] = (row0 + min(r4 + 8 * h, nrows - 1)) / G + off;
 
-    // Q fragments
-    uint32_t qf[KS][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = r4 + 8 * h, i = (row0 + r) / G, hd_ = kvh * G + (row0 + r) % G;
-      const T* q = static_cast<const T*>(p.q) + (i64)(x.q.q0 + i) * p.qst + (i64)hd_ * p.qsh;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = ks * 16 + e * 8 + c4 * 2;
-          qf[ks][h + 2 * e] = r < nrows && d < p.hd ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
-        }
-    }
     float o[HDP / 8][4];
 #pragma unroll
     for (int i = 0; i < HDP / 8; ++i)
@@ -289,6 +295,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
     };
 #pragma unroll
     for (int u = 0; u < C::kStages - 1; ++u) load(u);
+    // Q fragments
+    uint32_t qf[KS][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = r4 + 8 * h, i = (row0 + r) / G, hd_ = kvh * G + (row0 + r) % G;
+      const T* q = static_cast<const T*>(p.q) + (i64)(x.q.q0 + i) * p.qst + (i64)hd_ * p.qsh;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = ks * 16 + e * 8 + c4 * 2;
+          qf[ks][h + 2 * e] = r < nrows && d < p.hd ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+        }
+    }
     for (int u = 0; u < nt; ++u) {
       asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 2) : "memory");
       __syncwarp();
