@@ -883,8 +883,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* mine_part = p.part + (size_t)c.slot * C::kPartFloats;
       const int r2 = t * kT + row;
       const bool any = hi > lo;
-      mine_part[r2] = m;
-      mine_part[2 * kT + r2] = l;
+      if (mine_row) {
+        mine_part[r2] = m;
+        mine_part[2 * kT + r2] = l;
+      }
       float4* po = reinterpret_cast<float4*>(mine_part + 4 * kT);
 #pragma unroll 1
       for (int i = 0; i < HDP / 32; ++i) {
@@ -894,10 +896,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
           pin32(o);
         }
+        if (mine_row) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          po[(8 * i + e) * 2 * kT + r2] =
-              any ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int e = 0; e < 8; ++e)
+            po[(8 * i + e) * 2 * kT + r2] =
+                any ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        __syncwarp();
       }
       tc_fence_before();
       __threadfence();
@@ -917,37 +922,53 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       __threadfence();
-      // the last one in joins the pieces in the order of the cut
-      float M = -INFINITY, Ls = 0.f;
-      const int npieces = sc.owner(c.start + c.len - 1) - c.first + 1;
-      for (int k = 0; k < npieces; ++k) {
-        const float* q = p.part + (size_t)(k ? 2 * (c.first + k) : 2 * c.first + 1) * C::kPartFloats;
-        M = fmaxf(M, __ldcg(q + r2));
-      }
-      const float Ms = M == -INFINITY ? 0.f : M;
-      for (int k = 0; k < npieces; ++k) {
-        const float* q = p.part + (size_t)(k ? 2 * (c.first + k) : 2 * c.first + 1) * C::kPartFloats;
-        Ls += __ldcg(q + 2 * kT + r2) * ex2(__ldcg(q + r2) - Ms);
-      }
-      const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
-      if (mine_row) {
-#pragma unroll 1
-        for (int e = 0; e < p.hd / 4; e += 2) {
-          float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-          for (int k = 0; k < npieces; ++k) {
-            const float* q = p.part + (size_t)(k ? 2 * (c.first + k) : 2 * c.first + 1) * C::kPartFloats;
-            const float w = ex2(__ldcg(q + r2) - Ms);
-            if (!(w != 0.f)) continue;  // a piece without a seen key
-            const float4* qo = reinterpret_cast<const float4*>(q + 4 * kT);
-            const float4 u = __ldcg(qo + e * 2 * kT + r2), v = __ldcg(qo + (e + 1) * 2 * kT + r2);
-            a = make_float4(fmaf(w, u.x, a.x), fmaf(w, u.y, a.y), fmaf(w, u.z, a.z), fmaf(w, u.w, a.w));
-            b = make_float4(fmaf(w, v.x, b.x), fmaf(w, v.y, b.y), fmaf(w, v.z, b.z), fmaf(w, v.w, b.w));
+      // The last one in joins the pieces in the order of the cut: a thread takes
+      // 8 channels of a row at a time, 8 pieces' worth of loads ahead.
+      const int np = sc.owner(c.start + c.len - 1) - c.first + 1;
+      const int rows = min(kT, c.nrows - row0);
+      for (int e = row; e < rows * (p.hd / 8); e += kT) {
+        const int r = e % rows, d = e / rows * 8, rr = t * kT + r;
+        float M = -INFINITY, L = 0.f, acc[8] = {};
+        for (int k0 = 0; k0 < np; k0 += 8) {
+          float pm[8], pl[8];
+          float4 u[8], v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            pm[k] = -INFINITY, pl[k] = 0.f;
+            u[k] = v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k0 + k < np) {
+              const float* q = p.part + (size_t)(k0 + k ? 2 * (c.first + k0 + k) : 2 * c.first + 1) * C::kPartFloats;
+              const float4* qo = reinterpret_cast<const float4*>(q + 4 * kT) + (d / 4) * 2 * kT + rr;
+              pm[k] = __ldcg(q + rr);
+              pl[k] = __ldcg(q + 2 * kT + rr);
+              u[k] = __ldcg(qo);
+              v[k] = __ldcg(qo + 2 * kT);
+            }
           }
-          uint4 u = make_uint4(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv),
-                               pack2<T>(b.x * inv, b.y * inv), pack2<T>(b.z * inv, b.w * inv));
-          if (Ls == 0.f) u = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(out + 4 * e) = u;
+          float top = M;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top = fmaxf(top, pm[k]);
+          const float ms = top == -INFINITY ? 0.f : top, f0 = ex2(M - ms);
+          M = top;
+          L *= f0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] *= f0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float f = ex2(pm[k] - ms);
+            L = fmaf(f, pl[k], L);
+            acc[0] = fmaf(f, u[k].x, acc[0]), acc[1] = fmaf(f, u[k].y, acc[1]);
+            acc[2] = fmaf(f, u[k].z, acc[2]), acc[3] = fmaf(f, u[k].w, acc[3]);
+            acc[4] = fmaf(f, v[k].x, acc[4]), acc[5] = fmaf(f, v[k].y, acc[5]);
+            acc[6] = fmaf(f, v[k].z, acc[6]), acc[7] = fmaf(f, v[k].w, acc[7]);
+          }
         }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        T* to = static_cast<T*>(p.out) + (i64)(c.q0 + ((row0 + r) >> lg)) * p.ost +
+                (i64)(c.head + ((row0 + r) & ((1 << lg) - 1))) * p.osh;
+        *reinterpret_cast<uint4*>(to + d) =
+            make_uint4(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv),
+                       pack2<T>(acc[4] * inv, acc[5] * inv), pack2<T>(acc[6] * inv, acc[7] * inv));
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.piece_empty[sl]);
