@@ -58,6 +58,44 @@ OSSM_DEV Seq seq_of(const Params& p, int b) {
   return s;
 }
 
+// A line of work items of length `total`, cut into ncta parts.  A cut within
+// `near` of its item's edge moves to the edge (never closer than kMinPiece to
+// the start, or kMinPiece + kItemCost to the end).
+template <int kMinPiece, int kItemCost>
+struct Cuts {
+  long long total;
+  int ncta;
+  OSSM_DEV long long place(int c) const {  // of cut c, before it moves
+    return total / ncta * c + total % ncta * c / ncta;
+  }
+  OSSM_DEV long long moved(long long pos, long long start, long long end) const {  // of a cut in item [start, end)
+    const long long near = max((long long)kMinPiece, total / ncta / 16);
+    if (pos - start <= near && pos - start <= end - pos) return start;
+    if (end - pos <= near + kItemCost) return end;
+    return pos - start <= near ? start : pos;
+  }
+  // The CTA whose part holds the item's start: the last whose cut is there or before.
+  OSSM_DEV int first_of(long long start, long long end) const {
+    int c = min(ncta - 1, (int)((double)start * ncta / (double)total));
+    while (c > 0 && place(c) > start) --c;
+    for (; c + 1 < ncta; ++c) {
+      const long long q = place(c + 1);
+      if (q > start && (q >= end || moved(q, start, end) > start)) break;
+    }
+    return c;
+  }
+  // The CTA whose part holds the item's last step, at `last`.
+  OSSM_DEV int last_of(long long start, long long end, long long last) const {
+    int c = min(ncta - 1, (int)((double)end * ncta / (double)total));
+    while (c > 0 && (place(c) >= end || (place(c) > start && moved(place(c), start, end) > last))) --c;
+    for (; c + 1 < ncta; ++c) {
+      const long long q = place(c + 1);
+      if (q >= end || (q > start && moved(q, start, end) > last)) break;
+    }
+    return c;
+  }
+};
+
 template <typename T>
 OSSM_DEV float2 to_f2(uint32_t u);
 template <>

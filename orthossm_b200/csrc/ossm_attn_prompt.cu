@@ -120,8 +120,7 @@ struct Sched {
   const Params& p;
   const i64* pre;  // [ngroups + 1] length of the line before each group of sequences
   int ngroups, gsz, lg, units;
-  i64 total;
-  int ncta;
+  Cuts<kMinPiece, kItemCost> cuts;
 
   struct Item {
     Seq q;
@@ -164,26 +163,17 @@ struct Sched {
   // Where CTA c's part begins (and the item there, if it is not past the item's end).
   OSSM_DEV i64 cut(int c, Item& it, bool& in) const {
     in = false;
-    if (c >= ncta) return total;
-    const i64 pos = c <= 0 ? 0 : total / ncta * c + total % ncta * c / ncta;
+    if (c >= cuts.ncta) return cuts.total;
+    const i64 pos = c <= 0 ? 0 : cuts.place(c);
     it = at(pos);
-    const i64 near = max((i64)kMinPiece, total / ncta / 16);
-    in = true;
-    if (pos - it.start <= near && pos - it.start <= it.end() - pos) return it.start;
-    in = it.end() - pos > near + kItemCost;
-    if (!in) return it.end();
-    return pos - it.start <= near ? it.start : pos;
+    const i64 to = cuts.moved(pos, it.start, it.end());
+    in = to < it.end();
+    return to;
   }
   OSSM_DEV i64 cut(int c) const {
     Item it;
     bool in;
     return cut(c, it, in);
-  }
-  OSSM_DEV int owner(i64 pos) const {  // the CTA whose part holds a position: the last with cut(c) <= pos
-    int c = (int)min((i64)ncta - 1, (i64)((double)pos * ncta / (double)total));  // off by the moved cuts only
-    while (c > 0 && cut(c) > pos) --c;
-    while (c + 1 < ncta && cut(c + 1) <= pos) ++c;
-    return c;
   }
 };
 
@@ -461,11 +451,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) pre[0] = 0;
   }
   __syncthreads();
-  Sched sc{p, pre, ngroups, gsz, lg, units, pre[ngroups], 0};
+  Sched sc{p, pre, ngroups, gsz, lg, units, {pre[ngroups], 0}};
   // CTAs for pieces of 8 key tiles; and twice the items, so that each item's
   // edge is the nearest one to some cut and short items get a CTA each
-  sc.ncta = (int)min((i64)gridDim.x, max(2 * (i64)n_items, sc.total / 8));
-  if (cta >= sc.ncta) return;
+  sc.cuts.ncta = (int)min((i64)gridDim.x, max(2 * (i64)n_items, sc.cuts.total / 8));
+  if (cta >= sc.cuts.ncta) return;
   if (threadIdx.x == 9 * 32) cuts[0] = sc.cut(cta, item, item_in);
   if (threadIdx.x == 10 * 32) cuts[1] = sc.cut(cta + 1);
 
@@ -562,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               c.len = x.n();
               c.start = x.start;
               c.slot = head ? 2 * cta + 1 : 2 * cta;
-              c.first = head ? cta : sc.owner(x.start);
+              c.first = head ? cta : sc.cuts.first_of(x.start, x.end());
             }
             break;
           }
@@ -924,7 +914,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __threadfence();
       // The last one in joins the pieces in the order of the cut: a thread takes
       // 8 channels of a row at a time, 8 pieces' worth of loads ahead.
-      const int np = sc.owner(c.start + c.len - 1) - c.first + 1;
+      const int np = sc.cuts.last_of(c.start, c.start + c.len + kItemCost, c.start + c.len - 1) - c.first + 1;
       const int rows = min(kT, c.nrows - row0);
       for (int e = row; e < rows * (p.hd / 8); e += kT) {
         const int r = e % rows, d = e / rows * 8, rr = t * kT + r;

@@ -63,8 +63,7 @@ struct Line {
   int hp;
   const i64* pre;
   int ngroups, gsz;
-  i64 total;
-  int ncta;
+  Cuts<kMinPiece, kItemCost> cuts;
 
   struct Item {
     Seq q;
@@ -105,26 +104,17 @@ struct Line {
   // Where CTA c's part begins (and the item there, if it is not past the item's end).
   OSSM_DEV i64 cut(int c, Item& it, bool& in) const {
     in = false;
-    if (c >= ncta) return total;
-    const i64 pos = c <= 0 ? 0 : total / ncta * c + total % ncta * c / ncta;
+    if (c >= cuts.ncta) return cuts.total;
+    const i64 pos = c <= 0 ? 0 : cuts.place(c);
     it = at(pos);
-    const i64 near = max((i64)kMinPiece, total / ncta / 16);
-    in = true;
-    if (pos - it.start <= near && pos - it.start <= it.end() - pos) return it.start;
-    in = it.end() - pos > near + kItemCost;
-    if (!in) return it.end();
-    return pos - it.start <= near ? it.start : pos;
+    const i64 to = cuts.moved(pos, it.start, it.end());
+    in = to < it.end();
+    return to;
   }
   OSSM_DEV i64 cut(int c) const {
     Item it;
     bool in;
     return cut(c, it, in);
-  }
-  OSSM_DEV int owner(i64 pos) const {  // the CTA whose part holds a position: the last with cut(c) <= pos
-    int c = (int)min((i64)ncta - 1, (i64)((double)pos * ncta / (double)total));  // off by the moved cuts only
-    while (c > 0 && cut(c) > pos) --c;
-    while (c + 1 < ncta && cut(c + 1) <= pos) ++c;
-    return c;
   }
 };
 
@@ -190,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
   const int gsz = (p.B + kGroups - 1) / kGroups, ngroups = (p.B + gsz - 1) / gsz;
   // One head an item; two where the line is long for the GPU, as they halve the
   // items (32 streams with a window of 512: 14 us with one, 23 us with two).
-  Line ln{p, 1, pre, ngroups, gsz, 0, 0};
+  Line ln{p, 1, pre, ngroups, gsz, {0, 0}};
   for (;;) {
     if (threadIdx.x == 0) n_items = 0;
     __syncthreads();
@@ -223,15 +213,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       if (lane == 0) pre[0] = 0;
     }
     __syncthreads();
-    ln.total = pre[ngroups];
-    if (C::kHeads == 1 || ln.hp == 2 || p.Hkv % 2 || ln.total < (i64)kPairFrom * gridDim.x) break;
+    ln.cuts.total = pre[ngroups];
+    if (C::kHeads == 1 || ln.hp == 2 || p.Hkv % 2 || ln.cuts.total < (i64)kPairFrom * gridDim.x) break;
     ln.hp = 2;
     __syncthreads();
   }
   const int hp = ln.hp, sub = warp & (hp - 1), kw = warp / hp, nkw = kWarps / hp;  // head, place among its warps
   // twice the items: each item's edge is the nearest one to some cut, and short items get a CTA each
-  ln.ncta = (int)min((i64)gridDim.x, max(2 * (i64)n_items, ln.total / kMinWork));
-  if (cta >= ln.ncta) return;
+  ln.cuts.ncta = (int)min((i64)gridDim.x, max(2 * (i64)n_items, ln.cuts.total / kMinWork));
+  if (cta >= ln.cuts.ncta) return;
   if (lane == 0 && warp < 2) {
     Line::Item it;
     bool in;
@@ -456,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
     }
     __syncthreads();
     const bool split = b - a < x.n;
-    const int first = split ? (head ? cta : ln.owner(x.start)) : cta;
+    const int first = split ? (head ? cta : ln.cuts.first_of(x.start, x.end())) : cta;
     auto slot = [&](int c) {  // of CTA c's piece of this item
       return p.part + (size_t)(c == first ? 2 * c + 1 : 2 * c) * C::kPartFloats;
     };
@@ -498,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       }
     }
     if (split) {
-      const int last = ln.owner(x.start + x.n - 1);
+      const int last = ln.cuts.last_of(x.start, x.end(), x.start + x.n - 1);
       // Is this the last of n arrivals at a counter?  Then the others' partial results are there to read.
       auto arrive = [&](uint32_t* count, int n) {
         __threadfence();
