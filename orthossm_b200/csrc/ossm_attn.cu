@@ -57,8 +57,7 @@ namespace {
 
 // Workspace: header, two progress counters a CTA, two partial results a CTA.
 constexpr int kMaxCtas = 1024;
-constexpr int kTokenRows = 16;            // of the token kernel's items
-constexpr int64_t kL2Bytes = 96ll << 20;  // K and V that stay in L2 (126 MB) between two reads
+constexpr int kTokenRows = 16;  // of the token kernel's items
 
 int sm_count() { return std::min(device_sms(), kMaxCtas / 4); }
 
@@ -86,16 +85,15 @@ extern "C" int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size
                        reinterpret_cast<float*>(w + sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t))};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // Rows that share a key head.  Up to 16, one item of the token kernel holds
-  // them and K and V are read once (32 streams of 8192 keys, 32/8 heads of 128,
-  // 1 new token: 171 us, 220 us on the prompt kernel; 64 of 1000, 16/4 of 64:
-  // 23 and 35 us).  Up to 32 they are read twice: still ahead where L2 serves
-  // the second read (8 of 2000, 8/8 of 128, 32 rows: 34 and 48 us) or a row is
-  // short (32 of 8192, 8/8 of 64: 140 and 181 us), but not for long caches of
-  // 128 channels (32 of 8192, 32/8 of 128: 330 and 226 us).  Beyond, the prompt
-  // kernel's tile of 128 rows.
+  // them and K and V are read once (8 streams of 2000 keys, 8/8 heads of 128,
+  // 16 new tokens: 23 us, 28 us on the prompt kernel; 32 of 8192, 32/8 of 128,
+  // 1 token: 167 and 180 us; 64 of 1000, 16/4 of 64, 1 token: 19 and 34 us).
+  // Up to 32 they are read twice, which still pays at 64 channels (32 of 8192,
+  // 8/8 of 64, 32 tokens: 133 and 160 us; 64 of 1000, 16/4, 8: 31 and 34 us) and
+  // not above (8 of 2000, 8/8 of 128, 32 tokens: 31 and 28 us; 32 of 8192, 32/8
+  // of 128, 8: 330 and 187 us).  Beyond, the prompt kernel's tile of 128 rows.
   const int64_t rows = (int64_t)a->max_seqlen_q * (a->H / a->H_kv);
-  const int64_t kv_bytes = 4 * a->total_k * a->H_kv * a->head_dim;
-  const bool twice = a->head_dim <= 64 || kv_bytes <= kL2Bytes;
-  if (a->total_k == 0 || rows <= (twice ? 2 : 1) * kTokenRows) return attn::token_forward(a, p, sm_count(), st);
+  if (a->total_k == 0 || rows <= (a->head_dim <= 64 ? 2 : 1) * kTokenRows)
+    return attn::token_forward(a, p, sm_count(), st);
   return attn::prompt_forward(a, p, sm_count(), st);
 }

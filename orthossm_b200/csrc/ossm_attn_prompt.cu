@@ -36,16 +36,15 @@
 // partial sums in the workspace, and whichever CTA finishes it last joins
 // them, in the order of the cut.
 //
-// What bounds it: the exponentials.  A step of an item (two tiles, 128 keys)
-// is 1024 (64 channels) or 2048 cycles (128) of the tensor core and 2048 cycles
-// of the special function unit (16 results a clock and SM); the softmax's
-// other work overlaps with the other tile's exponentials in part.  Measured, at
-// the clock under load: 16384 causal, fp16, 16 heads of 128: 940-995 us, 1105
-// to 1170 TFLOP/s (0.67-0.71 of measured cuBLAS); 8 heads of 64: 435-455 us;
-// 2 x 16384 with a window of 512, 8 heads of 64: 96 us.  Tried and slower:
-// part of the exponentials as a polynomial on the FMA pipe (1 to 4 of 8:
-// +1 to +9 %), the tiles taking turns at them (+3 to +13 %), a row on two
-// threads (16 softmax warps: +25 % at 128 channels).
+// What bounds it: a step of an item (two tiles, 128 keys) is 1024 (64 channels)
+// or 2048 cycles (128) of the tensor core and 2048 of the special function unit
+// (16 exponentials a clock and SM); of the softmax's other work a part overlaps
+// with the other tile's exponentials.  Measured: 16384 causal, fp16, 16 heads
+// of 128: 886 us, 1242 TFLOP/s (0.76 of measured cuBLAS); 8 heads of 64: 375 us;
+// 2 x 16384 with a window of 512, 8 heads of 64: 89 us; 3 x 4096, 32/8 heads of
+// 128: 351 us.  Tried and slower: part of the exponentials as a polynomial on
+// the FMA pipe (1 to 3 pairs of 8: +3 to +11 %), the tiles taking turns at them
+// (+3 to +13 %), a row on two threads (16 softmax warps: +25 % at 128 channels).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -1007,9 +1006,9 @@ int prompt_forward(const ossm_attn_args* a, const Params& p, int grid, cudaStrea
   if (!fast::encode_fn()) return OSSM_ELAUNCH;
   CUtensorMap q, k, v;
   // Two heads a tile where there are two, more only as far as the queries do
-  // not fill the item's rows: 3 x 4096 causal, 32/8 heads of 128, took 381 us
-  // with 2 and 393 us with 4; 32 x 5 new tokens against 8192, 229 us with 4
-  // and 487 us with one a tile.
+  // not fill the item's rows: 3 x 4096 causal, 32/8 heads of 128, was 3 % faster
+  // with 2 than with 4; 32 x 5 new tokens against 8192 took 229 us with 4 and
+  // 487 us with one a tile.
   int lg = 0;
   while (lg < 7 && (p.H / p.Hkv) % (2 << lg) == 0 && (lg == 0 || ((int64_t)a->max_seqlen_q << lg) < 2 * kT)) ++lg;
   if (!encode(&q, a->dtype, p.q, p.hd, p.H, p.Tq, p.qst, p.qsh, 1 << lg) ||
