@@ -7,13 +7,19 @@
 // A row is shared by a cluster of up to 8 CTAs.  One pass over the logits finds
 // the largest and the sum of the weights, from which follows a logit that the
 // prefix cannot reach below (Bound); a second pass, out of L2, collects the
-// candidates above it into the first CTA's shared memory, where they are
-// ordered and the prefix and its best score are found.  The noise is read for
-// the prefix alone.  Where too many candidates are collected (wide or nearly
-// flat rows) the first CTA finds the prefix's end in a histogram of the logits
-// instead, and orders the candidates of one bin.
+// candidates above it into the first CTA's shared memory, where the prefix's end
+// and its best score are found: a few candidates in order, of more a histogram
+// first.  The noise is read for the prefix alone.  In wide rows the bound is
+// guessed from a sample and the guess checked by the mass collected.  Where too
+// many candidates are collected all the same (nearly flat rows) the first CTA
+// goes over the row instead of the list.
 // Masses that are compared are 64-bit fixed-point sums, which do not depend on
 // the order of the additions.
+// Measured: 1 x 32000 bf16, top-k 50 and top-p 0.95: 10.8 us; 128 x 131072 bf16,
+// top-k 50: 17 us (5.1 us of reads), min-p 0.01: 21 us, top-p 0.72 (4000 stay):
+// 41 us, top-p 0.92 (18000 stay): 61 us.  What bounds it there: one CTA an SM
+// works through steps that wait for one another; of 41 us, 8 are the first
+// pass (5 of reads), 5 the sample, 16 the collection, 8 the prefix's end.
 //
 // Without filters the score of every candidate is needed: one pass over logits
 // and noise.  The logarithm is first taken in its fast form, and exactly only
@@ -36,8 +42,10 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024;
 constexpr int kOpen = 512;     // threads of a CTA where nothing is filtered
-constexpr int kList = 4096;    // candidates that are ordered in shared memory
-constexpr int kRank = 512;     // up to here by counting the larger ones, above by a bitonic sort
+constexpr int kList = 24576;   // candidates that shared memory holds
+constexpr int kRank = 256;     // candidates that are put in order
+constexpr int kBins = 1024;
+constexpr int kGuess = 16384;  // logits a CTA from which on a guess of the bound pays
 typedef unsigned long long u64;
 typedef long long i64;
 
@@ -72,6 +80,8 @@ OSSM_DEV float logit_of(u64 key) {
   const uint32_t o = (uint32_t)(key >> 32);
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
+
+OSSM_DEV int index_of(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
 
 // Probability relative to the first candidate (logit m): 1 at l == m, also
 // where both are +inf.
@@ -127,15 +137,29 @@ OSSM_DEV void unpack(const uint4& u, float (&l)[8], __half) {
   }
 }
 
+// This CTA's share of a row: vectors v0 to v1 of 16 aligned bytes from logit
+// `head` on.
+template <typename T>
+struct Share {
+  const uint4* body;
+  int head, nv, v0, v1;
+  OSSM_DEV Share(const T* row, int V, int rank, int nrank) {
+    head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
+    nv = (V - head) / Vec<T>::n;
+    v0 = (int)((i64)nv * rank / nrank), v1 = (int)((i64)nv * (rank + 1) / nrank);
+    body = reinterpret_cast<const uint4*>(row + head);
+  }
+};
+
 // This CTA's share of a row: f(l, i, n) for the n logits from index i on, 16
 // aligned bytes at a time; the row's unaligned ends go to the first CTA, one by
 // one.  What is not a candidate (NaN) arrives as -inf.
 template <typename T, typename F>
 OSSM_DEV void scan(const T* row, int V, int rank, int nrank, F f) {
   constexpr int N = Vec<T>::n;
-  const int head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
-  const int nv = (V - head) / N, v0 = (int)((i64)nv * rank / nrank), v1 = (int)((i64)nv * (rank + 1) / nrank);
-  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  const Share<T> own(row, V, rank, nrank);
+  const int head = own.head, nv = own.nv, v0 = own.v0, v1 = own.v1;
+  const uint4* body = own.body;
   for (int v = v0 + threadIdx.x; v < v1; v += 4 * kThreads) {
     uint4 u[4];
 #pragma unroll
@@ -167,9 +191,9 @@ OSSM_DEV void scan(const T* row, int V, int rank, int nrank, F f) {
 template <int NT, typename T, typename F>
 OSSM_DEV void scan_noise(const T* row, const float* nz, int V, int rank, int nrank, F f) {
   constexpr int N = Vec<T>::n, U = 16 / N;
-  const int head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
-  const int nv = (V - head) / N, v0 = (int)((i64)nv * rank / nrank), v1 = (int)((i64)nv * (rank + 1) / nrank);
-  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  const Share<T> own(row, V, rank, nrank);
+  const int head = own.head, nv = own.nv, v0 = own.v0, v1 = own.v1;
+  const uint4* body = own.body;
   const float* nbody = nz + head;
   const bool aligned = ((uintptr_t)nbody & 15) == 0;
   for (int v = v0 + threadIdx.x; v < v1; v += U * NT) {
@@ -242,7 +266,7 @@ OSSM_DEV Best block_best(Best b, Best* bests) {  // the result in warp 0
 struct Row {
   float inv_t, top_p, min_p;
   int top_k;     // 0: off
-  bool greedy;
+  bool greedy;   // the first candidate alone
   OSSM_DEV bool open() const { return !greedy && top_k == 0 && top_p >= 1.f && !(min_p > 0.f); }
 };
 OSSM_DEV Row row_of(const Params& p, int row) {
@@ -253,51 +277,36 @@ OSSM_DEV Row row_of(const Params& p, int row) {
   r.min_p = p.m_row ? p.m_row[row] : p.min_p;
   if (r.top_k <= 0 || r.top_k >= p.V) r.top_k = 0;
   if (!(r.top_p >= 0.f)) r.top_p = 0.f;
-  r.greedy = !p.noise || !(r.inv_t > 0.f) || r.inv_t == INFINITY;
+  r.greedy = !p.noise || !(r.inv_t > 0.f) || r.inv_t == INFINITY || r.min_p > 1.f;
   return r;
 }
 
 // Shared memory of the work on one row.
 struct Room {
   u64 list[kList];
+  u64 bins[kBins];
+  u64 few[kRank];
   u64 red[32];
   u64 sh[4];
 };
-constexpr int kPer = kList / kThreads;
-constexpr int kBins = 1024;
 
-// The N keys of the list in descending order.
-OSSM_DEV void order(u64* list, int N) {
+// The n <= kRank keys of a list in descending order: a key's position is the
+// number of larger ones; parts of the count by neighbouring threads.
+OSSM_DEV void order(u64* list, int n) {
   const int tid = threadIdx.x;
-  if (N <= kRank) {
-    // a key's position is the number of larger ones; parts of the count by neighbouring threads
-    int parts = 1;
-    while (parts < 32 && N * parts * 2 <= kThreads) parts *= 2;
-    const int e = tid / parts, q = tid % parts;
-    u64 key = 0;
-    int larger = 0;
-    if (e < N) {
-      key = list[e];
+  int parts = 1;
+  while (parts < 32 && n * parts * 2 <= kThreads) parts *= 2;
+  const int e = tid / parts, q = tid % parts;
+  u64 key = 0;
+  int larger = 0;
+  if (e < n) {
+    key = list[e];
 #pragma unroll 8
-      for (int k = q; k < N; k += parts) larger += list[k] > key;
-    }
-    for (int w = 1; w < parts; w *= 2) larger += __shfl_xor_sync(~0u, larger, w);
-    __syncthreads();
-    if (e < N && q == 0) list[larger] = key;
-  } else {
-    int size = 1024;
-    while (size < N) size *= 2;
-    for (int k = N + tid; k < size; k += kThreads) list[k] = 0;
-    for (int k = 2; k <= size; k *= 2)
-      for (int j = k / 2; j; j /= 2) {
-        __syncthreads();
-        for (int e = tid; e < size / 2; e += kThreads) {
-          const int a = 2 * j * (e / j) + e % j, o = a + j;
-          const u64 x = list[a], y = list[o];
-          if ((x < y) == ((a & k) == 0)) list[a] = y, list[o] = x;
-        }
-      }
+    for (int k = q; k < n; k += parts) larger += list[k] > key;
   }
+  for (int w = 1; w < parts; w *= 2) larger += __shfl_xor_sync(~0u, larger, w);
+  __syncthreads();
+  if (e < n && q == 0) list[larger] = key;
   __syncthreads();
 }
 
@@ -322,66 +331,157 @@ OSSM_DEV u64 block_scan(u64 v, u64* red, u64& all) {
   return before + v;
 }
 
-// Mass of the ordered list's first n keys up to and including this thread's
-// positions tid + k kThreads; the sum over all.
-OSSM_DEV u64 masses(Room& s, int n, float m, float inv_t, u64 (&own)[kPer], u64 (&upto)[kPer]) {
-  u64 base = 0;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int e = threadIdx.x + k * kThreads;
-    own[k] = upto[k] = 0;
-    if (k * kThreads >= n) continue;
-    if (e < n) own[k] = mass_of(weight(logit_of(s.list[e]), m, inv_t));
-    u64 all;
-    upto[k] = base + block_scan(own[k], s.red, all);
-    base += all;
-  }
-  return base;
-}
-// How many of them the prefix holds that reaches `target` (at least one).
-OSSM_DEV int reaching(int n, const u64 (&own)[kPer], const u64 (&upto)[kPer], u64 target) {
-  int stay = 0;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k)
-    if (k * kThreads < n)
-      stay += __syncthreads_count((int)threadIdx.x + k * kThreads < n && upto[k] - own[k] < target);
-  return max(1, stay);
-}
 OSSM_DEV u64 share(float top_p, u64 whole) {  // the mass that a prefix has to reach
   return max((u64)1, (u64)__double2ull_ru((double)top_p * (double)whole));
 }
-
-// The smallest key of the prefix of the candidates at or above `floor` that
-// holds `count` of them, or (count == 0) the share top_p of their mass; `whole`:
-// that mass where it is known, else 0.  Candidates below logit lb are known to
-// lie behind the prefix.  One CTA: a histogram of the logits between lb and the
-// largest, m; the keys of the bin where the prefix ends, in order; if they are
-// too many, radix passes of 8 bits over them.
-template <typename T>
-OSSM_DEV u64 select(const Row& r, const T* lg, int V, float m, float lb, u64 floor, u64 count, u64 whole, Room& s) {
+// How many of n <= kRank keys in order the prefix holds (at least one) whose
+// mass reaches `target`, or (target == 0) the share top_p of theirs; n + 1: they
+// do not reach it.
+OSSM_DEV int reaching(const u64* list, int n, float m, const Row& r, u64 target, u64* red) {
   const int tid = threadIdx.x;
-  const float scale = m > lb && m - lb < INFINITY ? (kBins - 1) / (m - lb) : 0.f;
+  const u64 own = tid < n ? mass_of(weight(logit_of(list[tid]), m, r.inv_t)) : 0;
+  u64 all;
+  const u64 upto = block_scan(own, red, all);
+  if (target == 0) target = share(r.top_p, all);
+  const int stay = max(1, __syncthreads_count(tid < n && upto - own < target));
+  return all < target ? n + 1 : stay;
+}
+
+// A 64-bit sum in shared memory of 32-bit atomics: one with a result, a second
+// where it carries or q has a high part.  (A 64-bit one is a loop of exchanges.)
+OSSM_DEV void add64(u64* to, u64 q) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(to);
+  const uint32_t lo = (uint32_t)q, old = atomicAdd(w, lo), hi = (uint32_t)(q >> 32) + (old + lo < old);
+  if (hi) atomicAdd(w + 1, hi);
+}
+
+OSSM_DEV void clear_bins(Room& s) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins[i] = 0;
+  __syncthreads();
+}
+// The bin in which the sums of s.bins, from the first on, reach `target`, or
+// (target == 0) the share top_p of them all; -1: none.  left: what of it the bin
+// itself has to give.
+OSSM_DEV int find_bin(Room& s, u64 target, float top_p, u64& left) {
+  static_assert(kBins == kThreads, "a bin a thread");
+  __syncthreads();
+  const u64 own = s.bins[threadIdx.x];
+  u64 all;
+  const u64 upto = block_scan(own, s.red, all);
+  if (target == 0) target = share(top_p, all);
+  if (threadIdx.x == 0) s.sh[0] = ~(u64)0;
+  __syncthreads();
+  if (upto - own < target && target <= upto) {
+    s.sh[0] = threadIdx.x;
+    s.sh[1] = target - (upto - own);
+  }
+  __syncthreads();
+  const int bin = (int)s.sh[0];
+  left = s.sh[1];
+  __syncthreads();
+  return bin;
+}
+
+// The smallest key of the prefix of a set of keys that holds `left` of them
+// (count) or of their mass; each(f) calls f for every key of the set.  As long
+// as more than kRank are between the bounds, their range is cut into bins and
+// narrowed to the one where the prefix ends; keys differ, so that ends.
+template <typename Each>
+OSSM_DEV u64 narrow(const Row& r, Each each, bool count, u64 left, float m, Room& s) {
+  u64 lo = 0, hi = ~(u64)0;
+  int* fill = reinterpret_cast<int*>(&s.sh[3]);
+  for (;;) {
+    __syncthreads();
+    if (threadIdx.x == 0) *fill = 0;
+    __syncthreads();
+    u64 least = ~(u64)0, most = 0;
+    int at = 0;
+    each([&](u64 key) {
+      if (key < lo || key > hi) return;
+      if (at < kRank && (at = atomicAdd(fill, 1)) < kRank) s.few[at] = key;
+      least = min(least, key), most = max(most, key);
+    });
+    __syncthreads();
+    const int n = *fill;
+    if (n <= kRank) {
+      order(s.few, n);
+      return s.few[(count ? (int)left : min(n, reaching(s.few, n, m, r, left, s.red))) - 1];
+    }
+    lo = block_reduce(least, s.red, [](u64 a, u64 b) { return min(a, b); });
+    hi = block_reduce(most, s.red, [](u64 a, u64 b) { return max(a, b); });
+    const int shift = max(0, 54 - __clzll((long long)(hi - lo)));
+    clear_bins(s);
+    each([&](u64 key) {
+      if (key >= lo && key <= hi)
+        add64(s.bins + ((hi - key) >> shift), count ? 1 : mass_of(weight(logit_of(key), m, r.inv_t)));
+    });
+    const int bin = find_bin(s, left, 1.f, left);
+    if (bin < 0) return lo;
+    hi -= (u64)bin << shift;
+    const u64 width = ((u64)1 << shift) - 1;
+    lo = max(lo, hi > width ? hi - width : 0);
+  }
+}
+
+// A logit's bin between the largest, m, and lb: (m - l) scale, rounded by adding
+// 2^23, in the low bits.
+struct Bins {
+  float m, scale;
+  OSSM_DEV Bins(float m, float lb) : m(m), scale(m > lb && m - lb < INFINITY ? (kBins - 1) / (m - lb) : 0.f) {}
+  OSSM_DEV float below(float l) const { return l == m ? 0.f : m - l; }
+  OSSM_DEV int of(float d) const {
+    return __float_as_int(fminf(d * scale, (float)(kBins - 1)) + 8388608.f) & (kBins - 1);
+  }
+};
+
+// The smallest key of the prefix of the list's N candidates at or above `floor`
+// that holds `count` of them, or (count == 0) the mass `target` (0: the share
+// top_p of theirs); `floor` where they do not reach it.
+OSSM_DEV u64 select_list(const Row& r, int N, float m, u64 floor, int count, u64 target, Room& s) {
+  auto all = [&](auto f) {
+    for (int e = threadIdx.x; e < N; e += kThreads)
+      if (s.list[e] >= floor) f(s.list[e]);
+  };
+  u64 least = ~(u64)0;
+  all([&](u64 key) { least = min(least, key); });
+  const Bins bins(m, logit_of(block_reduce(least, s.red, [](u64 a, u64 b) { return min(a, b); })));
+  clear_bins(s);
+  all([&](u64 key) {
+    const float l = logit_of(key);
+    add64(s.bins + bins.of(bins.below(l)), count ? 1 : mass_of(weight(l, m, r.inv_t)));
+  });
+  u64 left;
+  const int cut = find_bin(s, count ? (u64)count : target, r.top_p, left);
+  if (cut < 0) return floor;  // all of them stay
+  auto each = [&](auto f) {
+    all([&](u64 key) {
+      if (bins.of(bins.below(logit_of(key))) == cut) f(key);
+    });
+  };
+  return narrow(r, each, count != 0, left, m, s);
+}
+
+// The same of all the row's candidates, by one CTA; `whole`: their mass where it
+// is known, else 0.  Candidates below logit lb are known to lie behind the
+// prefix.
+template <typename T>
+OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, float m, float lb, u64 floor, int count, u64 whole, Room& s) {
+  const Bins bins(m, lb);
   const float c = r.inv_t * 1.44269504f;
-  // (m - l) scale, rounded by adding 2^23: the bin in the low bits
-  auto bin_of = [&](float d) { return __float_as_int(fminf(d * scale, (float)(kBins - 1)) + 8388608.f) & (kBins - 1); };
-  auto below = [&](float l) { return l == m ? 0.f : m - l; };
-  // Masses in steps of 2^-28 (the sums are compared with a share of the whole,
-  // which is at least 1), in two parts that 2^17 candidates cannot overflow;
-  // longer rows take one 64-bit sum, which costs a loop of exchanges.
-  const bool two = V <= (1 << 17);
-  uint32_t* part = reinterpret_cast<uint32_t*>(s.list);  // low 14 bits, high 15 bits; or the count
-  u64* wide = s.list;
-  __syncthreads();
-  for (int i = tid; i < kBins; i += kThreads) wide[i] = 0;
-  __syncthreads();
   const float first = floor ? logit_of(floor) : -INFINITY;  // floor's logit: only there the index decides
   const float low = fmaxf(lb, kLowest);
+  // Masses in steps of 2^-28 (the sums are compared with a share of the whole,
+  // which is at least 1), in two parts that 2^17 candidates cannot overflow.
+  const bool two = V <= (1 << 17);
+  uint32_t* part = reinterpret_cast<uint32_t*>(s.bins);  // low 14 bits, high 15 bits; or the count
+  clear_bins(s);
   scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
 #pragma unroll
     for (int e = 0; e < Vec<T>::n; ++e) {
       const bool in = e < n && l[e] >= low && (l[e] > first || key_of(l[e], i + e) >= floor);
-      const float d = below(l[e]);
-      const int b = bin_of(d);
+      const float d = bins.below(l[e]);
+      const int b = bins.of(d);
       const uint32_t q = __float2uint_rn(ex2(-d * c) * 0x1p28f);  // the weight, to a few 2^-22
       if (!in) continue;
       if (count) {
@@ -390,83 +490,139 @@ OSSM_DEV u64 select(const Row& r, const T* lg, int V, float m, float lb, u64 flo
         atomicAdd(part + 2 * b, q & 0x3fffu);
         atomicAdd(part + 2 * b + 1, q >> 14);
       } else {
-        atomicAdd(wide + b, (u64)q);
+        add64(s.bins + b, q);
       }
     }
   });
-  __syncthreads();
-  static_assert(kBins == kThreads, "a bin a thread");
-  const u64 own = count ? part[2 * tid] : two ? part[2 * tid] + ((u64)part[2 * tid + 1] << 14) : wide[tid];
-  u64 all;
-  const u64 upto = block_scan(own, s.red, all);
-  const u64 target = count ? count : share(r.top_p, whole ? whole >> 12 : all);
-  if (tid == 0) s.sh[0] = ~(u64)0;
-  __syncthreads();
-  if (upto - own < target && target <= upto) {
-    s.sh[0] = tid;
-    s.sh[1] = upto - own;
+  if (!count && two) {
+    __syncthreads();
+    s.bins[threadIdx.x] = part[2 * threadIdx.x] + ((u64)part[2 * threadIdx.x + 1] << 14);
   }
-  __syncthreads();
-  if (s.sh[0] == ~(u64)0) return floor;  // all of them stay
-  const int cut = (int)s.sh[0];
-  u64 left = target - s.sh[1];  // from the bin itself
-  __syncthreads();
+  u64 left;
+  const int cut = find_bin(s, count ? (u64)count : whole ? share(r.top_p, whole >> 12) : 0, r.top_p, left);
+  if (cut < 0) return floor;  // all of them stay
+  if (!count) left <<= 12;    // as masses of single candidates are: 2^-40
   // the bin's logits lie between these (half a bin wider on both sides)
+  const float scale = bins.scale;
   const float from = scale > 0.f ? fmaxf(low, cut == kBins - 1 ? low : m - (cut + 1.f) / scale) : low;
   const float to = scale > 0.f && cut ? m - (cut - 1.f) / scale : INFINITY;
   auto each = [&](auto f) {  // the keys of the bin
     scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
 #pragma unroll
       for (int e = 0; e < Vec<T>::n; ++e)
-        if (e < n && l[e] >= from && l[e] <= to && bin_of(below(l[e])) == cut) {
+        if (e < n && l[e] >= from && l[e] <= to && bins.of(bins.below(l[e])) == cut) {
           const u64 key = key_of(l[e], i + e);
           if (key >= floor) f(key);
         }
     });
-    __syncthreads();
   };
-  if (!count) left <<= 12;  // as masses of single candidates are: 2^-40
-  int* fill = reinterpret_cast<int*>(&s.sh[3]);
-  if (tid == 0) *fill = 0;
+  int* fill = reinterpret_cast<int*>(&s.sh[2]);
+  if (threadIdx.x == 0) *fill = 0;
   __syncthreads();
+  int at = 0;
   each([&](u64 key) {
-    const int at = atomicAdd(fill, 1);
-    if (at < kList) s.list[at] = key;
+    if (at < kList && (at = atomicAdd(fill, 1)) < kList) s.list[at] = key;
   });
+  __syncthreads();
   const int size = *fill;
-  if (size <= kList) {
-    order(s.list, size);
-    int at = (int)left;
-    if (!count) {
-      u64 o[kPer], u[kPer];
-      masses(s, size, m, r.inv_t, o, u);
-      at = reaching(size, o, u, left);
+  if (size > kList) return narrow(r, each, count != 0, left, m, s);
+  auto listed = [&](auto f) {
+    for (int e = threadIdx.x; e < size; e += kThreads) f(s.list[e]);
+  };
+  return narrow(r, listed, count != 0, left, m, s);
+}
+
+// The candidates of this CTA's share from logit `low` on, into a list; *count may
+// pass the list's end, which is then found in another way.  A thread's four
+// vectors take their places with one addition (a row of 131072 with 18000
+// candidates: 17 us with one for each vector).
+template <typename T>
+OSSM_DEV void collect(const T* row, int V, int rank, int nrank, float low, int* count, u64* list) {
+  constexpr int N = Vec<T>::n, U = 4;
+  const Share<T> own(row, V, rank, nrank);
+  bool over = false;
+  for (int v = own.v0 + threadIdx.x; v < own.v1 && !over; v += U * kThreads) {
+    uint4 u[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v + k * kThreads < own.v1) u[k] = __ldg(own.body + v + k * kThreads);
+    uint32_t in = 0;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (v + k * kThreads >= own.v1) break;
+      float l[N];
+      unpack(u[k], l, T());
+#pragma unroll
+      for (int e = 0; e < N; ++e) in |= l[e] >= low ? 1u << (k * N + e) : 0u;  // a NaN is not
     }
-    const u64 key = s.list[at - 1];
-    __syncthreads();
-    return key;
-  }
-  u64 prefix = 0;
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    __syncthreads();
-    if (tid < 256) s.list[tid] = 0;
-    __syncthreads();
-    each([&](u64 key) {
-      if (shift == 56 || (key >> (shift + 8)) == prefix)
-        atomicAdd(s.list + ((key >> shift) & 255), count ? (u64)1 : mass_of(weight(logit_of(key), m, r.inv_t)));
-    });
-    if (tid == 0) {
-      int d = 255;
-      for (; d > 0 && s.list[d] < left; --d) left -= s.list[d];
-      s.sh[0] = left;
-      s.sh[1] = (prefix << 8) | d;
+    if (!in) continue;
+    int at = atomicAdd(count, __popc(in));
+    over = at >= kList;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (!(in >> (k * N) & ((1u << N) - 1))) continue;
+      float l[N];
+      unpack(u[k], l, T());
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (in >> (k * N + e) & 1u) {
+          if (at < kList) list[at] = key_of(l[e], own.head + (v + k * kThreads) * N + e);
+          ++at;
+        }
     }
-    __syncthreads();
-    left = s.sh[0];
-    prefix = s.sh[1];
-    __syncthreads();
   }
-  return prefix;
+  if (rank == 0) {
+    const int tail = V - own.head - own.nv * N, e = threadIdx.x;
+    if (e < own.head + tail) {
+      const int i = e < own.head ? e : V - tail + (e - own.head);
+      const float l = to_f(row[i]);
+      if (l >= low) {
+        const int at = atomicAdd(count, 1);
+        if (at < kList) list[at] = key_of(l, i);
+      }
+    }
+  }
+}
+
+// A guess of the logit below which this CTA's share of the row holds `tail` of
+// mass: from up to 16 logits a thread, spread over the share, a histogram
+// between lb (known to lie below) and m.  In whole steps, so that the guess does
+// not depend on the order of the additions either.
+template <typename T>
+OSSM_DEV float guess_bound(const T* lg, int V, int rank, int nrank, float m, float lb, float c, float tail, Room& s) {
+  constexpr int N = Vec<T>::n, U = 16 / N;
+  const Bins bins(m, lb);
+  const Share<T> own(lg, V, rank, nrank);
+  const int nv = own.v1 - own.v0, read = min(nv, U * kThreads);
+  uint32_t* part = reinterpret_cast<uint32_t*>(s.bins);
+  clear_bins(s);
+  const float scale = 0x1p22f * ((float)nv / read) / tail;  // the sums: 2^22 where the sample's tail is reached
+  uint32_t last = 0;
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int at = threadIdx.x + k * kThreads;
+    if (at >= read) continue;
+    float l[N];
+    unpack(__ldg(own.body + own.v0 + (int)((i64)at * nv / read)), l, T());
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float d = bins.below(fmaxf(l[e], -INFINITY));
+      // at most 2^17 each, of 2^14 logits: a sum of 32 bits holds them
+      const uint32_t q = __float2uint_rn(fminf(ex2(-d * c) * scale, 0x1p17f));
+      const int b = bins.of(d);
+      if (b == kBins - 1)
+        last += q;  // most of them, perhaps
+      else
+        atomicAdd(part + 2 * b, q);
+    }
+  }
+  last = __reduce_add_sync(~0u, last);
+  if ((threadIdx.x & 31) == 0) atomicAdd(part + 2 * (kBins - 1), last);
+  __syncthreads();
+  u64 all;
+  const u64 upto = block_scan(part[2 * threadIdx.x], s.red, all);
+  const int bin = __syncthreads_count(all - upto > (u64)(0.9f * 0x1p22f));
+  return bin >= kBins - 1 ? lb : fmaxf(lb, m - (bin + 0.5f) / bins.scale);
 }
 
 OSSM_DEV float lg2(float x) {  // log2, within 2^-22 (of 1, or of its value)
@@ -501,6 +657,7 @@ OSSM_DEV void race(const float* l, const float* e, int i, int n, float low, F st
 struct Told {
   float m, z;      // largest logit; sum of the weights relative to it
   uint32_t tk;     // order bits that at least top_k candidates reach
+  float guess;     // where its part of the tail begins
   int count;       // candidates collected (the first CTA's)
   Best best;
 };
@@ -540,13 +697,14 @@ __global__ void __launch_bounds__(kOpen, 2) open_kernel(const Params p) {
   __shared__ Told told;
   const int nrank = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
   const i64 row = blockIdx.x / nrank;
-  open_row<kOpen>(static_cast<const T*>(p.logits) + row * p.lst, p.noise + row * p.nst, p.V, p.inv_t, rank, nrank, bests,
-                  told, p.out + row);
+  open_row<kOpen>(static_cast<const T*>(p.logits) + row * p.lst, p.noise + row * p.nst, p.V, p.inv_t, rank, nrank,
+                  bests, told, p.out + row);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
-  __shared__ Room room;
+  extern __shared__ u64 dynamic[];
+  Room& room = *reinterpret_cast<Room*>(dynamic);
   __shared__ float redf[32];
   __shared__ Best bests[32];
   __shared__ Told told;
@@ -637,35 +795,40 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   // logarithms' and the products' roundings are covered by the slack.
   uint32_t bound = tk;
   float lb = -INFINITY;  // the same as a logit, of the bounds by mass
+  bool guessed = need_z && p.V / nrank >= kGuess;
   if (!(top_k && by_mass)) {
     float y = -INFINITY;
     if (need_z) y = logf((1.f - r.top_p) * z / (float)p.V);
-    if (!r.greedy && r.min_p > 0.f) y = fmaxf(y, logf(fminf(r.min_p, 1.f)));
+    if (!r.greedy && r.min_p > 0.f) {
+      const float by_min = logf(fminf(r.min_p, 1.f));
+      guessed = guessed && by_min < y + 2.f;  // else min_p leaves a few
+      y = fmaxf(y, by_min);
+    }
     if (y > -INFINITY && m < INFINITY) {
       lb = m + (y - 1e-3f - 1e-5f * fabsf(y)) / r.inv_t;
       lb = fminf(lb - 1e-5f * (fabsf(m) + fabsf(lb)), m);
       bound = max(bound, ord(lb));
     }
   }
+  // That bound by mass leaves many more than the prefix in wide rows (30000 of
+  // 131072 where it holds 4000).  A guess leaves fewer; whether the prefix ends
+  // above it shows in the mass collected.
+  guessed = guessed && lb > -INFINITY && lb < m;
+  if (guessed) {
+    float g = guess_bound(lg, p.V, rank, nrank, m, lb, c, (1.f - r.top_p) * z / (float)nrank, room);
+    if (nrank > 1) {  // the lowest of the CTAs'
+      if (tid == 0) told.guess = g;
+      cluster.sync();
+      g = cluster.map_shared_rank(&told, min(tid & 31, nrank - 1))->guess;
+#pragma unroll
+      for (int w = 16; w; w >>= 1) g = fminf(g, __shfl_xor_sync(~0u, g, w));
+    }
+    bound = max(bound, ord(g));
+  }
   Told* first = nrank > 1 ? cluster.map_shared_rank(&told, 0) : &told;
   u64* first_list = nrank > 1 ? cluster.map_shared_rank(room.list, 0) : room.list;
   const float low = bound ? fmaxf(logit_of((u64)bound << 32), kLowest) : kLowest;
-  bool over = false;  // the list is full: its end is found in another way
-  scan(lg, p.V, rank, nrank, [&](const float* l, int i, int n) {
-    uint32_t in = 0;
-#pragma unroll
-    for (int e = 0; e < Vec<T>::n; ++e) in |= e < n && l[e] >= low ? 1u << e : 0u;
-    if (in && !over) {
-      int at = atomicAdd(&first->count, __popc(in));
-      over = at >= kList;
-#pragma unroll
-      for (int e = 0; e < Vec<T>::n; ++e)
-        if (in >> e & 1u) {
-          if (at < kList) first_list[at] = key_of(l[e], i + e);
-          ++at;
-        }
-    }
-  });
+  collect(lg, p.V, rank, nrank, low, &first->count, first_list);
   if (nrank > 1)
     cluster.sync();
   else
@@ -675,20 +838,56 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   // ---------------------------------------------------------------- the prefix and its best score
   const int N = told.count;
   Best b{0.f, -1};
-  auto consider = [&](u64 key) {
-    const int i = (int)(0xffffffffu - (uint32_t)key);
-    better(b, r.greedy ? 0.f : score_of(logit_of(key), r.inv_t, nz[i]), i);
-  };
-  if (N > kList) {
+  u64 keep = 0;  // the prefix's last key
+  bool by_list = N <= kList;
+  if (by_list && r.greedy) {
+    for (int e = tid; e < N; e += kThreads) keep = max(keep, room.list[e]);
+    keep = block_reduce(keep, room.red, [](u64 a, u64 b) { return max(a, b); });
+  } else if (by_list) {
+    const u64 target = whole ? share(r.top_p, whole) : 0;
+    if (N <= kRank && (top_k || by_mass)) {
+      order(room.list, N);
+      int n = top_k ? min(top_k, N) : N;
+      if (by_mass) {
+        const int stay = reaching(room.list, n, m, r, target, room.red);
+        by_list = !(guessed && stay > n);
+        n = min(n, stay);
+      }
+      if (n) keep = room.list[n - 1];
+    } else {
+      if (top_k && top_k < N) keep = select_list(r, N, m, 0, top_k, 0, room);
+      if (by_mass) keep = select_list(r, N, m, keep, 0, target, room);
+      by_list = !(guessed && keep == 0);  // 0: the guess was too high
+    }
+  }
+  if (by_list && r.greedy) {
+    if (tid == 0) better(b, 0.f, index_of(keep));
+  } else if (by_list) {
+    constexpr int U = 4;  // noises on their way at a time
+    for (int e = tid; e < N; e += U * kThreads) {
+      u64 key[U];
+      float x[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        key[k] = e + k * kThreads < N ? room.list[e + k * kThreads] : 0;
+        if (key[k] < keep || (r.min_p > 0.f && weight(logit_of(key[k]), m, r.inv_t) < r.min_p)) key[k] = 0;
+        if (key[k]) x[k] = nz[index_of(key[k])];
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (key[k]) better(b, score_of(logit_of(key[k]), r.inv_t, x[k]), index_of(key[k]));
+    }
+  } else {
     if (!r.greedy && tid == 0) {  // the last pass reads the noise: on its way to L2 meanwhile
       const uintptr_t a = ((uintptr_t)nz + 15) & ~(uintptr_t)15, z = (uintptr_t)(nz + p.V) & ~(uintptr_t)15;
       for (uintptr_t x = a; x < z; x += 32768)
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x), "r"((uint32_t)min((u64)32768, (u64)(z - x)))
                      : "memory");
     }
-    u64 top = 0, keep = 0;  // the first candidate (which stays whatever min_p is), the last one's key
+    u64 top = 0;
+    keep = 0;
     float least = INFINITY;
-    if (r.greedy || r.min_p > 0.f || top_k || !live(lb)) {
+    if (r.greedy || top_k || !live(lb)) {
       scan(lg, p.V, 0, 1, [&](const float* l, int i, int n) {
 #pragma unroll
         for (int e = 0; e < Vec<T>::n; ++e)
@@ -700,35 +899,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     if (r.greedy) {
       keep = top;
     } else {
-      if (top_k) keep = select(r, lg, p.V, m, least, 0, (u64)top_k, 0, room);
+      if (top_k) keep = select_row(r, lg, p.V, m, least, 0, top_k, 0, room);
       if (by_mass)
-        keep = select(r, lg, p.V, m, live(lb) ? lb : top_k ? logit_of(keep) : least, keep, 0,
-                      whole, room);
+        keep = select_row(r, lg, p.V, m, live(lb) ? lb : top_k ? logit_of(keep) : least, keep, 0, whole, room);
     }
     const float end = keep ? logit_of(keep) : -INFINITY;  // the last one's logit: only there the index decides
     if (r.greedy) {
-      if (tid == 0) consider(keep);
+      if (tid == 0) better(b, 0.f, index_of(keep));
     } else {
       float mark = -INFINITY;
       auto stays = [&](float l, int i) {
         const u64 key = key_of(l, i);
-        return key >= keep && (!(r.min_p > 0.f) || key == top || weight(l, m, r.inv_t) >= r.min_p);
+        return key >= keep && (!(r.min_p > 0.f) || weight(l, m, r.inv_t) >= r.min_p);
       };
       scan_noise<kThreads>(lg, nz, p.V, 0, 1, [&](const float* l, const float* e, int i, int n) {
         race<T>(l, e, i, n, fmaxf(fmaxf(end, lb), kLowest), stays, r.inv_t, b, mark);
       });
-    }
-  } else {
-    order(room.list, N);
-    int n = top_k ? min(top_k, N) : N;
-    if (by_mass) {
-      u64 own[kPer], upto[kPer];
-      const u64 all = masses(room, n, m, r.inv_t, own, upto);
-      n = reaching(n, own, upto, share(r.top_p, whole ? whole : all));
-    }
-    for (int e = tid; e < n; e += kThreads) {
-      const u64 key = room.list[e];
-      if (e == 0 || r.greedy || !(r.min_p > 0.f) || weight(logit_of(key), m, r.inv_t) >= r.min_p) consider(key);
     }
   }
   b = block_best<kThreads>(b, bests);
@@ -755,7 +941,11 @@ cudaError_t launch(const Params& p, int B, cudaStream_t st) {
   at[0].val.clusterDim.x = c, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return open ? cudaLaunchKernelEx(&cfg, open_kernel<T>, p) : cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+  if (open) return cudaLaunchKernelEx(&cfg, open_kernel<T>, p);
+  cfg.dynamicSmemBytes = sizeof(Room);
+  const cudaError_t e =
+      cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Room));
+  return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
 }
 
 }  // namespace smp
