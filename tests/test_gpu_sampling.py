@@ -98,6 +98,21 @@ def test_long_rows(f, B, V, spread):
     check(l, e, temperature=1.1, **f)
 
 
+@pytest.mark.parametrize("f", [dict(top_p=0.8), dict(top_p=0.97, min_p=1e-4), dict(top_p=0.3, min_p=0.02)],
+                         ids=lambda f: "_".join(f"{k}{v}" for k, v in f.items()))
+@pytest.mark.parametrize("period", [2, 3, 8])
+@pytest.mark.parametrize("high", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_uneven_rows(dtype, high, period, f):
+    """Rows whose large and small logits alternate in blocks of 16 bytes, so that
+    what a few blocks show of the tail can be far from the whole row's."""
+    V, block = 32768, 16 // dtype.itemsize
+    l, e = inputs(76, V, torch.float32, seed=period, spread=1.0)
+    every = (torch.arange(V, device="cuda") // block) % period == 0
+    l[:, every if not high else ~every] -= 25.0
+    check(l.to(dtype), e, **f)
+
+
 def test_all_equal():
     """One logit everywhere: the first k by index."""
     for val in (0.0, -0.0, 3.0, -7.5):
