@@ -16,10 +16,10 @@
 // Masses that are compared are 64-bit fixed-point sums, which do not depend on
 // the order of the additions.
 // Measured: 1 x 32000 bf16, top-k 50 and top-p 0.95: 10.8 us; 128 x 131072 bf16,
-// top-k 50: 17 us (5.1 us of reads), min-p 0.01: 21 us, top-p 0.72 (4000 stay):
-// 41 us, top-p 0.92 (18000 stay): 61 us.  What bounds it there: one CTA an SM
-// works through steps that wait for one another; of 41 us, 8 are the first
-// pass (5 of reads), 5 the sample, 16 the collection, 8 the prefix's end.
+// top-k 50: 17 us (5.1 us of reads), min-p 0.01: 19 us, top-p 0.72 (4000 stay):
+// 37 us, top-p 0.92 (18000 stay): 59 us.  What bounds it there: one CTA an SM
+// works through steps that wait for one another; of 37 us, 8 are the first
+// pass (5 of reads), 5 the sample, 9 the collection, 7 the prefix's end.
 //
 // Without filters the score of every candidate is needed: one pass over logits
 // and noise.  The logarithm is first taken in its fast form, and exactly only
@@ -135,6 +135,19 @@ OSSM_DEV void unpack(const uint4& u, float (&l)[8], __half) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
     l[2 * i] = f.x, l[2 * i + 1] = f.y;
   }
+}
+
+// Number e of a vector.
+OSSM_DEV float pick(const uint4& u, int e, float) {
+  return __uint_as_float(e & 2 ? (e & 1 ? u.w : u.z) : (e & 1 ? u.y : u.x));
+}
+OSSM_DEV uint32_t half_of(const uint4& u, int e) {
+  const uint32_t w = e & 4 ? (e & 2 ? u.w : u.z) : (e & 2 ? u.y : u.x);
+  return e & 1 ? w >> 16 : w & 0xffffu;
+}
+OSSM_DEV float pick(const uint4& u, int e, __nv_bfloat16) { return __uint_as_float(half_of(u, e) << 16); }
+OSSM_DEV float pick(const uint4& u, int e, __half) {
+  return __half2float(__ushort_as_half((unsigned short)half_of(u, e)));
 }
 
 // This CTA's share of a row: vectors v0 to v1 of 16 aligned bytes from logit
@@ -533,15 +546,18 @@ OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, float m, float lb, u64
 }
 
 // The candidates of this CTA's share from logit `low` on, into a list; *count may
-// pass the list's end, which is then found in another way.  A thread's four
-// vectors take their places with one addition (a row of 131072 with 18000
-// candidates: 17 us with one for each vector).
+// pass the list's end, which is then found in another way.  A warp's four
+// vectors take their places with one addition, and the candidates are walked
+// by the bits set: code for each of the 32 logits of a thread ran in every warp
+// that had one candidate (128 rows of 131072, 4000 candidates each: 43 us, so 37).
 template <typename T>
 OSSM_DEV void collect(const T* row, int V, int rank, int nrank, float low, int* count, u64* list) {
   constexpr int N = Vec<T>::n, U = 4;
   const Share<T> own(row, V, rank, nrank);
+  const int lane = threadIdx.x & 31;
   bool over = false;
-  for (int v = own.v0 + threadIdx.x; v < own.v1 && !over; v += U * kThreads) {
+  for (int first = own.v0; first < own.v1 && !over; first += U * kThreads) {
+    const int v = first + threadIdx.x;
     uint4 u[U];
 #pragma unroll
     for (int k = 0; k < U; ++k)
@@ -555,21 +571,23 @@ OSSM_DEV void collect(const T* row, int V, int rank, int nrank, float low, int* 
 #pragma unroll
       for (int e = 0; e < N; ++e) in |= l[e] >= low ? 1u << (k * N + e) : 0u;  // a NaN is not
     }
-    if (!in) continue;
-    int at = atomicAdd(count, __popc(in));
-    over = at >= kList;
+    if (!__any_sync(~0u, in)) continue;
+    int upto = __popc(in);
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (!(in >> (k * N) & ((1u << N) - 1))) continue;
-      float l[N];
-      unpack(u[k], l, T());
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (in >> (k * N + e) & 1u) {
-          if (at < kList) list[at] = key_of(l[e], own.head + (v + k * kThreads) * N + e);
-          ++at;
-        }
+    for (int w = 1; w < 32; w *= 2) {
+      const int x = __shfl_up_sync(~0u, upto, w);
+      if (lane >= w) upto += x;
     }
+    int at = lane == 31 ? atomicAdd(count, upto) : 0;
+    at = __shfl_sync(~0u, at, 31);
+    over = at >= kList;
+    at += upto - __popc(in);
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      for (uint32_t left = in >> (k * N) & ((1u << N) - 1); left; left &= left - 1, ++at) {
+        const int e = __ffs(left) - 1;
+        if (at < kList) list[at] = key_of(pick(u[k], e, T()), own.head + (v + k * kThreads) * N + e);
+      }
   }
   if (rank == 0) {
     const int tail = V - own.head - own.nv * N, e = threadIdx.x;
