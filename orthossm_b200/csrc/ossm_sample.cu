@@ -16,7 +16,7 @@
 // Masses that are compared are 64-bit fixed-point sums, which do not depend on
 // the order of the additions.
 // Measured: 1 x 32000 bf16, top-k 50 and top-p 0.95: 10.8 us; 128 x 131072 bf16,
-// top-k 50: 17 us (5.1 us of reads), min-p 0.01: 19 us, top-p 0.72 (4000 stay):
+// top-k 50: 16 us (5.1 us of reads), min-p 0.01: 18 us, top-p 0.72 (4000 stay):
 // 37 us, top-p 0.92 (18000 stay): 59 us.  What bounds it there: one CTA an SM
 // works through steps that wait for one another; of 37 us, 8 are the first
 // pass (5 of reads), 5 the sample, 9 the collection, 7 the prefix's end.
@@ -45,7 +45,7 @@ constexpr int kOpen = 512;     // threads of a CTA where nothing is filtered
 constexpr int kList = 24576;   // candidates that shared memory holds
 constexpr int kRank = 256;     // candidates that are put in order
 constexpr int kBins = 1024;
-constexpr int kGuess = 16384;  // logits a CTA from which on a guess of the bound pays
+constexpr int kGuess = 4096;   // logits a CTA from which on a guess of the bound pays
 typedef unsigned long long u64;
 typedef long long i64;
 
@@ -819,7 +819,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     if (need_z) y = logf((1.f - r.top_p) * z / (float)p.V);
     if (!r.greedy && r.min_p > 0.f) {
       const float by_min = logf(fminf(r.min_p, 1.f));
-      guessed = guessed && by_min < y + 2.f;  // else min_p leaves a few
+      guessed = guessed && by_min < y + 2.f;
       y = fmaxf(y, by_min);
     }
     if (y > -INFINITY && m < INFINITY) {
@@ -830,7 +830,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   }
   // That bound by mass leaves many more than the prefix in wide rows (30000 of
   // 131072 where it holds 4000).  A guess leaves fewer; whether the prefix ends
-  // above it shows in the mass collected.
+  // above it shows in the mass collected.  top-p 0.9, with and without: 1 x 32000
+  // (4 CTAs) 20 and 24 us, 64 x 50257 27 and 36 us, 128 x 32000 23 and 27 us.
+  // Where min_p's bound is the higher one by far it leaves few anyhow.  Up to a
+  // factor of e^2: 128 rows with top-p and a small min-p of their own, V = 131072,
+  // 56 us, only where it is the lower one 79 us (V = 50257: 31 and 28 us); up to
+  // e^4, where prefixes end below it and the row is gone over, 40 us (50257).
   guessed = guessed && lb > -INFINITY && lb < m;
   if (guessed) {
     float g = guess_bound(lg, p.V, rank, nrank, m, lb, c, (1.f - r.top_p) * z / (float)nrank, room);
@@ -841,6 +846,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
 #pragma unroll
       for (int w = 16; w; w >>= 1) g = fminf(g, __shfl_xor_sync(~0u, g, w));
     }
+    guessed = g > lb;
     bound = max(bound, ord(g));
   }
   Told* first = nrank > 1 ? cluster.map_shared_rank(&told, 0) : &told;
