@@ -247,10 +247,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
     pos = min(end, x.end());
     if (a >= b) continue;
     const int off = x.q.nk - x.q.nq, lo = Line::first_key(p, x.q);
-    const int kbeg = lo + a * ln.chunk(), kend = min(x.q.nk, lo + b * ln.chunk());
     const int kvh = x.kvh + sub;
     const int row0 = x.rb * kRows, nrows = (int)min((i64)kRows, (i64)x.q.nq * G - row0);
     const int i_first = row0 / G, i_last = (row0 + nrows - 1) / G;
+    // the piece's keys that some row sees: the item's are those of the whole
+    // sequence, whose other queries begin earlier or end later
+    const int kbeg = max(lo + a * ln.chunk(), p.window ? i_first + off - p.window + 1 : 0);
+    const int kend = min(min(x.q.nk, lo + b * ln.chunk()), i_last + off + 1);
     // positions of this lane's rows (rows past the block repeat its last)
     int at[2];
 #pragma unroll
@@ -367,9 +370,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
             l[h] += s[nb][2 * h + e];
           }
       }
-      // A weight of 0 times a non-finite value is NaN.  Keys outside the piece
-      // were loaded as zeros; where rows see different keys of the tile and one
-      // of its values is not finite, the product is taken key by key.
+      // A weight of 0 times a non-finite value is NaN.  Keys outside [kbeg, kend),
+      // which no row sees, were loaded as zeros; where rows see different keys of
+      // the tile and one of its values is not finite, the product is taken key by
+      // key.  Rows of one query all see every key loaded.
       bool bad = false;
       if (part && i_first != i_last) {
         const uint8_t* vt = ringp + (u % C::kStages) * (2 * C::kTile) + C::kTile;

@@ -123,6 +123,36 @@ def test_hidden_values_do_not_matter(what, hd, nq, nk):
         assert bool(got[seen][:, 1, hd - 1].isnan().all())
 
 
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+@pytest.mark.parametrize("G,hd,nq,window,most", [(16, 64, 2, None, 2), (16, 64, 2, 40, 2), (8, 64, 3, 40, 3),
+                                                 (4, 64, 5, 40, 5), (2, 64, 9, 40, 9), (1, 64, 17, 40, 17),
+                                                 (3, 32, 6, 17, 6), (16, 128, 5, 40, 1), (24, 80, 4, None, 1),
+                                                 (1, 128, 40, 33, 1)])
+def test_hidden_values_of_grouped_heads(G, hd, nq, window, most, what):
+    """One key at a time is not finite: the newest ones, which only the last
+    queries see, and the oldest within a window, which only the first ones see.
+    With many heads on one key head a block of rows is a single query of the
+    sequence; ``max_seqlen_q`` (most) is no bound."""
+    dtype, Hkv, nk = torch.bfloat16, 2, 150
+    g = torch.Generator(device="cuda").manual_seed(G)
+    q = torch.randn(nq, G * Hkv, hd, device="cuda", generator=g).to(dtype)
+    k, v = (torch.randn(nk, Hkv, hd, device="cuda", generator=g).to(dtype) for _ in range(2))
+    cu_q, cu_k = cum([nq]), cum([nk])
+    ref, mag, _ = packed_attention_ref(q, k, v, cu_q, cu_k, window=window)
+    lim = bound(ref, mag, dtype, nk, 6.0)
+    at = torch.arange(nq) + nk - nq
+    places = {nk - 1, nk - nq // 2} | ({nk - nq - window + 1, nk - window - 1} if window else set())
+    for j in places:
+        seen = (at >= j) & ((at - j < window) if window else True)
+        assert 0 < int(seen.sum()) < nq
+        kj, vj = k.clone(), v.clone()
+        kj[j], vj[j] = what, what
+        for kk, vv in ((k, vj), (kj, vj), (kj, v)):
+            out = O.packed_attention(q, kk, vv, cu_q, cu_k, max_seqlen_q=most, window=window).double().cpu()
+            assert bool(((out - ref).abs() <= lim)[~seen].all()), j
+            assert kk is kj or not bool(torch.isfinite(out[seen]).any()), j
+
+
 @pytest.mark.parametrize("nq,nk", [(1, 300), (200, 300)])
 def test_layouts(nq, nk):
     """Head-major tensors, odd strides (copied), a shared head of stride zero, a given output with gaps."""
