@@ -93,8 +93,15 @@ OSSM_DEV float ex2(float x) {  // 2^x, relative error 2^-22
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^-40 steps: a row's sum stays below 2^63 for V < 2^23 equal candidates.
-OSSM_DEV u64 mass_of(float w) { return (u64)__float2ull_rn(w * 0x1p40f); }
+// A weight (0 to 1) in steps of 2^-40, to the nearest: a row's sum stays below
+// 2^63 for V < 2^23 equal candidates.  Two additions round off the steps of
+// 2^-17 and then what is left in steps of 2^-40, exactly.
+OSSM_DEV u64 mass_of(float w) {
+  const float h = __fadd_rn(w, 64.f), r = __fsub_rn(w, __fsub_rn(h, 64.f));
+  const int hi = __float_as_int(h) - __float_as_int(64.f);
+  const int lo = __float_as_int(__fadd_rn(r, 0x1.8p-17f)) - __float_as_int(0x1.8p-17f);
+  return ((u64)hi << 23) + (i64)lo;
+}
 
 // The product and the difference are rounded one after the other (no fused
 // multiply-add), so that a caller can recompute a score exactly.  A NaN (from
@@ -484,10 +491,7 @@ OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, float m, float lb, u64
   const float c = r.inv_t * 1.44269504f;
   const float first = floor ? logit_of(floor) : -INFINITY;  // floor's logit: only there the index decides
   const float low = fmaxf(lb, kLowest);
-  // Masses in steps of 2^-28 (the sums are compared with a share of the whole,
-  // which is at least 1), in two parts that 2^17 candidates cannot overflow.
-  const bool two = V <= (1 << 17);
-  uint32_t* part = reinterpret_cast<uint32_t*>(s.bins);  // low 14 bits, high 15 bits; or the count
+  uint32_t* part = reinterpret_cast<uint32_t*>(s.bins);  // counts: the low half of a bin's sum
   clear_bins(s);
   scan(lg, V, 0, 1, [&](const float* l, int i, int n) {
 #pragma unroll
@@ -495,26 +499,17 @@ OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, float m, float lb, u64
       const bool in = e < n && l[e] >= low && (l[e] > first || key_of(l[e], i + e) >= floor);
       const float d = bins.below(l[e]);
       const int b = bins.of(d);
-      const uint32_t q = __float2uint_rn(ex2(-d * c) * 0x1p28f);  // the weight, to a few 2^-22
+      const u64 q = mass_of(ex2(-d * c));
       if (!in) continue;
-      if (count) {
+      if (count)
         atomicAdd(part + 2 * b, 1u);
-      } else if (two) {
-        atomicAdd(part + 2 * b, q & 0x3fffu);
-        atomicAdd(part + 2 * b + 1, q >> 14);
-      } else {
+      else
         add64(s.bins + b, q);
-      }
     }
   });
-  if (!count && two) {
-    __syncthreads();
-    s.bins[threadIdx.x] = part[2 * threadIdx.x] + ((u64)part[2 * threadIdx.x + 1] << 14);
-  }
   u64 left;
-  const int cut = find_bin(s, count ? (u64)count : whole ? share(r.top_p, whole >> 12) : 0, r.top_p, left);
+  const int cut = find_bin(s, count ? (u64)count : whole ? share(r.top_p, whole) : 0, r.top_p, left);
   if (cut < 0) return floor;  // all of them stay
-  if (!count) left <<= 12;    // as masses of single candidates are: 2^-40
   // the bin's logits lie between these (half a bin wider on both sides)
   const float scale = bins.scale;
   const float from = scale > 0.f ? fmaxf(low, cut == kBins - 1 ? low : m - (cut + 1.f) / scale) : low;

@@ -113,6 +113,25 @@ def test_uneven_rows(dtype, high, period, f):
     check(l.to(dtype), e, **f)
 
 
+@pytest.mark.parametrize("V,low,p,B", [(131072, -20.2, 0.9999, 3), (131072, -20.2, 0.9999, 80),
+                                       (1 << 20, -21.5, 0.9998, 2), ((1 << 22) + 5, -22.5, 0.99965, 1)])
+def test_peak_over_a_flat_tail(V, low, p, B):
+    """Candidates of less than 2^-29 of the first one's weight, so many that
+    together they decide where the nucleus ends: half of them stay."""
+    l = torch.full((1, V), low, device="cuda")
+    l[:, 0] = 0.0
+    w = math.exp(low)
+    whole = 1.0 + (V - 1) * w
+    stay = 1 + (p * whole - 1.0) / w  # so many stay
+    assert V / 4 < stay < 3 * V / 4
+    off = 2.0 ** -18 * whole / w      # the masses' and the sums' fp32 roundings, in candidates
+    for i in (int(stay - off - 2), int(stay + off + 2)):
+        e = torch.ones(1, V, device="cuda")
+        e[:, i] = 1e-30  # wins if it stays
+        got = O.sample_tokens(l.expand(B, V), e.expand(B, V), top_p=p)
+        assert got.tolist() == [i if i < stay else 0] * B
+
+
 def test_all_equal():
     """One logit everywhere: the first k by index."""
     for val in (0.0, -0.0, 3.0, -7.5):
