@@ -406,10 +406,13 @@ typedef struct {
   float scale;                       /* positive, finite */
 } ossm_attn_args;
 
-/* Bytes of device workspace (zero-filled once when allocated, then reused by
- * calls ordered on one stream, of any arguments that it is large enough for;
- * its first 256 bytes are a header that ossm_workspace_status reads, and after
- * OSSM_ETIMEOUT it has to be zero-filled again); 0 for invalid arguments. */
+/* Bytes of device workspace, the same for all valid arguments on a device (0
+ * for invalid ones).  Its first OSSM_ATTN_WS_ZERO bytes, a header that
+ * ossm_workspace_status reads and counters, are zero-filled once when it is
+ * allocated, and again after OSSM_ETIMEOUT; then it is reused by calls ordered
+ * on one stream.  A captured graph needs one that outlives it, and that no call
+ * outside the graph uses while it replays. */
+#define OSSM_ATTN_WS_ZERO 16384
 size_t ossm_attn_workspace_bytes(const ossm_attn_args* a);
 int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream);
 
@@ -445,6 +448,10 @@ typedef struct {
 } ossm_sample_args;
 
 int ossm_sample_tokens(const ossm_sample_args* a, ossm_stream_t stream);
+
+/* The capture that a stream's calls are recorded into (unique in the process),
+ * 0 if they run: for callers that keep a workspace for each graph. */
+int ossm_stream_capture_id(ossm_stream_t stream, uint64_t* id);
 
 /* Library metadata. */
 const char* ossm_version(void);

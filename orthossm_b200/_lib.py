@@ -13,6 +13,7 @@ from . import build as _build
 
 OSSM_OK, OSSM_EINVAL, OSSM_ELAUNCH, OSSM_ETIMEOUT, OSSM_ECOMM, OSSM_EWORKSPACE = range(6)
 OSSM_F32, OSSM_BF16, OSSM_F16 = 0, 1, 2
+OSSM_ATTN_WS_ZERO = 16384
 OSSM_EVAL_CLENSHAW, OSSM_EVAL_LUT, OSSM_EVAL_CLENSHAW_DEG4 = 0, 1, 2
 OSSM_F_FASTPATH = 1 << 2
 OSSM_F_PRECISE = 1 << 3
@@ -31,7 +32,7 @@ EXPORTED = (
     "ossm_ttt_workspace_bytes", "ossm_ttt_wpred_step", "ossm_sizeof_bwd_args", "ossm_bwd_workspace_bytes",
     "ossm_cheby_ema_bwd", "ossm_ttt_run_workspace_bytes", "ossm_ttt_wpred_run", "ossm_sizeof_ttt_run_args",
     "ossm_attn_workspace_bytes", "ossm_attention_fwd", "ossm_sizeof_attn_args",
-    "ossm_sample_tokens", "ossm_sizeof_sample_args",
+    "ossm_sample_tokens", "ossm_sizeof_sample_args", "ossm_stream_capture_id",
 )
 
 _vp = C.c_void_p
@@ -172,6 +173,8 @@ def _declare(lib):
     lib.ossm_attention_fwd.argtypes = [C.POINTER(AttnArgs), _vp, C.c_size_t, _vp]
     lib.ossm_sample_tokens.restype = C.c_int
     lib.ossm_sample_tokens.argtypes = [C.POINTER(SampleArgs), _vp]
+    lib.ossm_stream_capture_id.restype = C.c_int
+    lib.ossm_stream_capture_id.argtypes = [_vp, C.POINTER(C.c_uint64)]
     lib.ossm_sizeof_attn_args.restype = C.c_size_t
     lib.ossm_sizeof_sample_args.restype = C.c_size_t
     if lib.ossm_sizeof_attn_args() != C.sizeof(AttnArgs) or lib.ossm_sizeof_sample_args() != C.sizeof(SampleArgs):

@@ -61,19 +61,24 @@ constexpr int kTokenRows = 16;  // of the token kernel's items
 
 int sm_count() { return std::min(device_sms(), kMaxCtas / 4); }
 
-size_t ws_bytes(const ossm_attn_args* a) {
-  return sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t) +
-         (size_t)sm_count() * std::max(attn::prompt_part_floats(a->head_dim), attn::token_part_floats(a->head_dim)) * 4;
+// One size for all arguments: a workspace never has to be replaced by a larger
+// one while a captured graph still points to it.
+size_t ws_bytes() {
+  size_t part = 0;
+  for (int hd : {64, attn::kMaxHD})
+    part = std::max({part, attn::prompt_part_floats(hd), attn::token_part_floats(hd)});
+  return sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t) + (size_t)sm_count() * part * sizeof(float);
 }
+static_assert(sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t) <= OSSM_ATTN_WS_ZERO, "header and counters");
 
 }  // namespace
 
-extern "C" size_t ossm_attn_workspace_bytes(const ossm_attn_args* a) { return attn::valid(a) ? ws_bytes(a) : 0; }
+extern "C" size_t ossm_attn_workspace_bytes(const ossm_attn_args* a) { return attn::valid(a) ? ws_bytes() : 0; }
 
 extern "C" int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size_t workspace_bytes,
                                   ossm_stream_t stream) {
   if (!attn::valid(a)) return OSSM_EINVAL;
-  if (!workspace || workspace_bytes < ws_bytes(a) || (uintptr_t)workspace % 256) return OSSM_EWORKSPACE;
+  if (!workspace || workspace_bytes < ws_bytes() || (uintptr_t)workspace % 256) return OSSM_EWORKSPACE;
   if (a->total_q == 0) return OSSM_OK;
   char* w = static_cast<char*>(workspace);
   const attn::Params p{a->B, a->H, a->H_kv, a->head_dim, (int)a->total_q, (int)a->total_k, a->q, a->k, a->v, a->out,

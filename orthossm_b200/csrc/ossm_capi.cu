@@ -20,5 +20,13 @@ extern "C" size_t ossm_sizeof_lion_args(void) { return sizeof(ossm_lion_args); }
 extern "C" size_t ossm_sizeof_ttt_args(void) { return sizeof(ossm_ttt_args); }
 extern "C" size_t ossm_sizeof_bwd_args(void) { return sizeof(ossm_bwd_args); }
 extern "C" size_t ossm_sizeof_ttt_run_args(void) { return sizeof(ossm_ttt_run_args); }
+extern "C" int ossm_stream_capture_id(ossm_stream_t stream, uint64_t* id) {
+  cudaStreamCaptureStatus on = cudaStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  if (!id || cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &on, &n) != cudaSuccess)
+    return OSSM_EINVAL;
+  *id = on == cudaStreamCaptureStatusActive ? n : 0;
+  return OSSM_OK;
+}
 extern "C" size_t ossm_sizeof_attn_args(void) { return sizeof(ossm_attn_args); }
 extern "C" size_t ossm_sizeof_sample_args(void) { return sizeof(ossm_sample_args); }

@@ -124,12 +124,35 @@ def _workspace(device, stream, nbytes, host=False, cache=None):
     return ws
 
 
+# Workspaces of captured calls: (what for, device, stream) -> (capture, workspace),
+# of the stream's latest capture.  An earlier one stays in its graph's memory pool.
+_WS_CAPTURED: dict = {}
+
+
+def _captured_workspace(what, device, sptr, nbytes, zero):
+    """A workspace of the graph being captured on the stream, shared by its
+    calls there: its first ``zero`` bytes are zero-filled by the graph itself,
+    at every replay, so no other call may use it."""
+    capture = L.C.c_uint64(0)
+    L.check(L.lib().ossm_stream_capture_id(sptr, L.C.byref(capture)), "stream capture")
+    key = (what, device, sptr)
+    with _WS_LOCK:
+        held, ws = _WS_CAPTURED.get(key, (None, None))
+        if held != capture.value or ws.numel() < nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            ws[:zero].zero_()
+            _WS_CAPTURED[key] = capture.value, ws
+    return ws
+
+
 def workspace_status(device=None, clear=True):
     """Sticky device status over every workspace of a device (0 = ok,
-    3 = a look-back wait timed out).  Synchronises each workspace's stream."""
+    3 = a look-back wait timed out), those of the latest graph captured on a
+    stream among them.  Synchronises each workspace's stream."""
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     worst = 0
-    for (d, sptr), ws in list(_WS.items()) + list(_WS_HOST.items()) + list(_WS_ATTN.items()):
+    captured = [(key[1:], ws) for key, (_, ws) in list(_WS_CAPTURED.items())]
+    for (d, sptr), ws in list(_WS.items()) + list(_WS_HOST.items()) + list(_WS_ATTN.items()) + captured:
         if d != device:
             continue
         st = L._i32(0)

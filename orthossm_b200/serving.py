@@ -16,14 +16,17 @@ from typing import Optional, Union
 import torch
 
 from . import _lib as L
-from .sdpc_kernel import _WS_ATTN, _need_cuda, _ptr, _workspace
+from .sdpc_kernel import _WS_ATTN, _captured_workspace, _need_cuda, _ptr, _workspace
 
 _DT_ATTN = {torch.bfloat16: L.OSSM_BF16, torch.float16: L.OSSM_F16}
 _DT_SAMPLE = {torch.float32: L.OSSM_F32, torch.bfloat16: L.OSSM_BF16, torch.float16: L.OSSM_F16}
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a Stream object (2 us)
-_ATTN_WS: dict = {}  # (device index, stream) -> (workspace address, bytes), of the tensors in _WS_ATTN
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+# (device index, stream) -> (workspace address, bytes) of the tensors in _WS_ATTN: one size fits all
+# arguments, so none is ever replaced
+_ATTN_WS: dict = {}
 
 
 def _rows_ok(st, sh, sd, n, heads, ptr):
@@ -156,20 +159,30 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     return out
 
 
+def _attn_workspace(device, stream, nbytes, capturing):
+    """The stream's workspace, or under capture one of the graph's own: a graph
+    may be replayed beside calls on the stream that it was captured on."""
+    if capturing:
+        return _captured_workspace("attention", device, stream.cuda_stream, nbytes, L.OSSM_ATTN_WS_ZERO)
+    return _workspace(device, stream, nbytes, cache=_WS_ATTN)
+
+
 def _attention(a, dev):
     lib = L.lib()
     stream = _raw_stream(dev)
     ref = L.C.byref(a)
-    ws = _ATTN_WS.get((dev, stream))
-    status = L.OSSM_EWORKSPACE if ws is None else lib.ossm_attention_fwd(ref, ws[0], ws[1], stream)
-    if status == L.OSSM_EWORKSPACE:  # the first call on this stream, or one that needs more
+    capturing = _capturing()
+    ws = None if capturing else _ATTN_WS.get((dev, stream))
+    if ws is None:
         nbytes = lib.ossm_attn_workspace_bytes(ref)
         if nbytes == 0:
             L.check(L.OSSM_EINVAL, "packed_attention (argument check)")
         device = torch.device("cuda", dev)
-        t = _workspace(device, torch.cuda.current_stream(device), nbytes, cache=_WS_ATTN)
-        _ATTN_WS[dev, stream] = (t.data_ptr(), t.numel())
-        status = lib.ossm_attention_fwd(ref, t.data_ptr(), t.numel(), stream)
+        t = _attn_workspace(device, torch.cuda.current_stream(device), nbytes, capturing)
+        ws = t.data_ptr(), t.numel()
+        if not capturing:
+            _ATTN_WS[dev, stream] = ws
+    status = lib.ossm_attention_fwd(ref, ws[0], ws[1], stream)
     if status != L.OSSM_OK:
         L.check(status, "packed_attention")
 

@@ -108,3 +108,58 @@ def test_host_workspace_size_and_validation():
         assert lib.ossm_fwd_host_workspace_bytes(C.byref(a), pieces) == 0
     assert lib.ossm_cheby_ema_fwd_host(C.byref(_args(**base)), 8, None, 0, None) == L.OSSM_EWORKSPACE
     assert lib.ossm_cheby_ema_fwd_host(C.byref(_args(**dict(base, tanh_out=4096))), 8, None, 0, None) == L.OSSM_EINVAL
+
+
+def _attn(**kw):
+    a = dict(B=1, H=4, H_kv=2, head_dim=64, total_q=8, total_k=8, max_seqlen_q=8, dtype=L.OSSM_BF16, q=4096, k=4096,
+             v=4096, out=4096, q_stride_t=256, q_stride_h=64, k_stride_t=128, k_stride_h=64, v_stride_t=128,
+             v_stride_h=64, out_stride_t=256, out_stride_h=64, cu_q=4096, cu_k=4096, scale=1.0)
+    a.update(kw)
+    return L.AttnArgs(**a)
+
+
+def test_attention_workspace_has_one_size():
+    """A larger one for some arguments would replace the one that captured
+    graphs point to."""
+    lib = L.lib()
+    sizes = {lib.ossm_attn_workspace_bytes(C.byref(_attn(**kw)))
+             for kw in (dict(), dict(head_dim=8), dict(head_dim=128, q_stride_h=128, k_stride_h=128, v_stride_h=128,
+                                                       out_stride_h=128), dict(H=2, total_q=1, max_seqlen_q=1))}
+    assert len(sizes) == 1 and sizes.pop() > L.OSSM_ATTN_WS_ZERO
+    assert lib.ossm_attn_workspace_bytes(C.byref(_attn(head_dim=136))) == 0
+    src = open(os.path.join(ROOT, "include", "orthossm_b200.h")).read()
+    assert int(re.search(r"#define OSSM_ATTN_WS_ZERO (\d+)", src).group(1)) == L.OSSM_ATTN_WS_ZERO
+    assert lib.ossm_stream_capture_id(None, None) == L.OSSM_EINVAL
+
+
+def test_attention_workspace_under_capture(monkeypatch):
+    """One workspace a stream outside captures, kept for good; one a graph and
+    stream within, zero-filled in the graph."""
+    import types
+
+    import torch
+
+    from orthossm_b200 import sdpc_kernel, serving
+    now = [0]
+
+    class Lib:
+        def ossm_stream_capture_id(self, stream, ref):
+            ref._obj.value = now[0]
+            return L.OSSM_OK
+
+    monkeypatch.setattr(L, "lib", Lib)
+    for d in (sdpc_kernel._WS_ATTN, sdpc_kernel._WS_CAPTURED):
+        for key in [k for k in d if torch.device("cpu") in k]:
+            del d[key]
+    s, t = types.SimpleNamespace(cuda_stream=1), types.SimpleNamespace(cuda_stream=2)
+    get = lambda st, c: serving._attn_workspace(torch.device("cpu"), st, 1 << 17, c)  # noqa: E731
+    own = get(s, False)
+    assert get(s, False) is own and get(t, False) is not own and int(own.sum()) == 0
+    now[0] = 5
+    first, side = get(s, True), get(t, True)
+    assert first is not own and side is not first and get(s, True) is first
+    assert int(first[:L.OSSM_ATTN_WS_ZERO].sum()) == 0
+    now[0] = 6
+    second = get(s, True)
+    assert second is not first and second is not own and get(s, True) is second
+    assert get(s, False) is own

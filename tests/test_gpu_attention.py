@@ -299,6 +299,84 @@ def test_repeats_streams_and_graphs(nq, nk):
     assert O.workspace_status() == 0
 
 
+def _waste(nbytes=1 << 28):
+    """Fills memory that is free with a pattern that no counter has."""
+    x = [torch.full((nbytes // 4,), 0x5a5a5a5a, dtype=torch.int32, device="cuda") for _ in range(4)]
+    del x
+
+
+def _pieces(hd):
+    """A call of each kernel whose items are cut between CTAs: (call(out), out, check())."""
+    r = []
+    for nq, nk in ((1, 40000), (300, 9000)):
+        H = 4
+        q = torch.randn(nq, H, hd, device="cuda").to(torch.bfloat16)
+        k, v = (torch.randn(nk, H, hd, device="cuda").to(torch.bfloat16) for _ in range(2))
+        cu_q, cu_k = cum([nq]), cum([nk])
+        out = torch.empty_like(q)
+
+        def call(q=q, k=k, v=v, cu_q=cu_q, cu_k=cu_k, nq=nq, out=out):
+            return O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq, out=out)
+        r.append((call, out, call().clone()))
+    return r
+
+
+def test_graphs_and_larger_heads_after_them():
+    """Calls captured at 64 channels, replayed after calls at 128 and with the
+    freed memory overwritten."""
+    calls = _pieces(64)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for call, _, _ in calls:
+            call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for call, _, _ in calls:
+            call()
+    with torch.cuda.stream(side):
+        large = _pieces(128)
+        _waste()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for _, out, _ in calls:
+            out.zero_()
+        graph.replay()
+        for call, out, want in large:
+            assert torch.equal(call(), want)
+        torch.cuda.synchronize()
+        for _, out, want in calls:
+            assert torch.equal(out, want)
+    assert O.workspace_status() == 0
+
+
+def test_graphs_without_a_call_before():
+    """Two graphs captured on a stream that has seen no call, the second one
+    replayed first, and calls on that stream beside them."""
+    calls = _pieces(64)
+    side = torch.cuda.Stream()
+    graphs = []
+    for call, _, _ in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            call()
+        graphs.append(g)
+    _waste()
+    for i in (1, 0, 1, 1, 0):
+        call, out, want = calls[i]
+        out.zero_()
+        torch.cuda.synchronize()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        with torch.cuda.stream(side):
+            assert torch.equal(call(), want)
+        torch.cuda.synchronize()
+    del graphs
+    assert O.workspace_status() == 0
+
+
 def test_refusals():
     q = torch.zeros(4, 4, 64, device="cuda", dtype=torch.bfloat16)
     k = torch.zeros(4, 2, 64, device="cuda", dtype=torch.bfloat16)
