@@ -111,17 +111,29 @@ _WS_ATTN: dict = {}  # packed_attention: partial sums inside, never shared with 
 _WS_LOCK = threading.Lock()
 
 
+_WS_IN_GRAPHS: list = []  # of those above, the ones that captured graphs use: kept when a larger one replaces them
+_is_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
 def _workspace(device, stream, nbytes, host=False, cache=None):
+    """The stream's workspace, zero-filled once (ticket / epoch / flags start at
+    0).  A captured call that finds none that is large enough gets one in its
+    graph's memory: a zero fill under capture runs at that graph's replays only."""
     key = (device, stream.cuda_stream)
+    capturing = cache is None and _is_capturing()  # a cache of its own: the caller sees to captures
     if cache is None:
         cache = _WS_HOST if host else _WS
     with _WS_LOCK:
         ws = cache.get(key)
-        if ws is None or ws.numel() < nbytes:
-            # zero-filled once: ticket / epoch / flags start at 0
-            ws = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
-            cache[key] = ws
-    return ws
+        if ws is not None and ws.numel() >= nbytes:
+            if capturing and not any(w is ws for w in _WS_IN_GRAPHS):
+                _WS_IN_GRAPHS.append(ws)
+            return ws
+        nbytes = max(nbytes, 1 << 16)
+        if not capturing:
+            ws = cache[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            return ws
+    return _captured_workspace("host" if host else "ops", device, stream.cuda_stream, nbytes, nbytes)
 
 
 # Workspaces of captured calls: (what for, device, stream) -> (capture, workspace),

@@ -163,3 +163,39 @@ def test_attention_workspace_under_capture(monkeypatch):
     second = get(s, True)
     assert second is not first and second is not own and get(s, True) is second
     assert get(s, False) is own
+
+
+def test_workspaces_that_graphs_use_are_kept(monkeypatch):
+    """The other operators' workspaces grow: one that a captured call was given
+    stays alive, and captured calls without one get their graph's own."""
+    import types
+
+    import torch
+
+    from orthossm_b200 import sdpc_kernel as K
+    on = [False]
+
+    class Lib:
+        def ossm_stream_capture_id(self, stream, ref):
+            ref._obj.value = 9
+            return L.OSSM_OK
+
+    monkeypatch.setattr(L, "lib", Lib)
+    monkeypatch.setattr(K, "_is_capturing", lambda: on[0])
+    monkeypatch.setattr(K, "_WS", {})
+    monkeypatch.setattr(K, "_WS_CAPTURED", {})
+    monkeypatch.setattr(K, "_WS_IN_GRAPHS", [])
+    s, t = types.SimpleNamespace(cuda_stream=1), types.SimpleNamespace(cuda_stream=2)
+    get = lambda st, n: K._workspace(torch.device("cpu"), st, n)  # noqa: E731
+    small = get(s, 1 << 17)
+    on[0] = True
+    assert get(s, 1 << 17) is small and get(s, 1 << 16) is small
+    larger = get(s, 1 << 18)  # within the capture
+    fresh = get(t, 1 << 16)
+    assert larger is not small and get(s, 1 << 18) is larger and get(t, 1 << 16) is fresh
+    assert int(larger.sum()) == 0
+    on[0] = False
+    grown = get(s, 1 << 19)
+    assert grown is not small and grown is not larger and get(s, 1 << 17) is grown
+    assert len(K._WS_IN_GRAPHS) == 1 and K._WS_IN_GRAPHS[0] is small
+    assert get(t, 1 << 16) is not fresh

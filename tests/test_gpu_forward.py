@@ -336,3 +336,37 @@ def test_long_single_sequence_runs_as_two_ranges(gate):
     head = 4 * 512 * 32
     assert torch.equal(out[:, :head], o1[:, :head])
     assert O.workspace_status() == 0
+
+
+def test_graph_outlives_a_larger_workspace():
+    """A captured forward, replayed after a longer one on the same stream has
+    taken a larger workspace and the freed memory was overwritten; and one
+    captured on a stream that has seen no call."""
+    import orthossm_b200 as O
+    mk = lambda S: torch.randn(2, S, 512, device="cuda").to(torch.bfloat16)  # noqa: E731
+    x, far = mk(4096), mk(65536)
+    c = O.init_chebyshev_coefficients(2, 8, 8, 64, "cuda")
+    gate = dict(lambda_per_head=T(R.BASELINE_LAMBDA), gate_weight=torch.randn(8, 512, device="cuda") * 0.02,
+                gate_bias=torch.zeros(8, device="cuda"))
+    want, fin = O.cheby_ema_forward(x, c, **gate)
+    for before in (True, False):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        if before:
+            with torch.cuda.stream(side):
+                O.cheby_ema_forward(x, c, **gate)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out, f = O.cheby_ema_forward(x, c, **gate)
+        with torch.cuda.stream(side):
+            O.cheby_ema_forward(far, c, **gate)
+            waste = [torch.full((1 << 26,), 0x5a5a5a5a, dtype=torch.int32, device="cuda") for _ in range(4)]
+        torch.cuda.synchronize()
+        del waste
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(f, fin)
+    assert O.workspace_status() == 0
