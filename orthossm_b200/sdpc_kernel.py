@@ -160,17 +160,23 @@ def _captured_workspace(what, device, sptr, nbytes, zero):
 def workspace_status(device=None, clear=True):
     """Sticky device status over every workspace of a device (0 = ok,
     3 = a look-back wait timed out), those of the latest graph captured on a
-    stream among them.  Synchronises each workspace's stream."""
+    stream among them.  Synchronises each workspace's stream.  With ``clear`` a
+    status that was set is reset, and of packed_attention's workspaces the
+    progress counters that the call left behind."""
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     worst = 0
-    captured = [(key[1:], ws) for key, (_, ws) in list(_WS_CAPTURED.items())]
-    for (d, sptr), ws in list(_WS.items()) + list(_WS_HOST.items()) + list(_WS_ATTN.items()) + captured:
+    captured = [(key[1:], ws) for key, (_, ws) in list(_WS_CAPTURED.items())]  # zeroed by their graphs
+    attention = list(_WS_ATTN.items())
+    for (d, sptr), ws in list(_WS.items()) + list(_WS_HOST.items()) + captured + attention:
         if d != device:
             continue
         st = L._i32(0)
         L.check(L.lib().ossm_workspace_status(ws.data_ptr(), int(clear), sptr, L.C.byref(st)),
                 "workspace_status")
         worst = max(worst, int(st.value))
+        if st.value and clear and any(ws is w for _, w in attention):
+            with torch.cuda.stream(torch.cuda.ExternalStream(sptr, device=d)):
+                ws[:L.OSSM_ATTN_WS_ZERO].zero_()
     return worst
 
 

@@ -321,6 +321,28 @@ def _pieces(hd):
     return r
 
 
+@pytest.mark.parametrize("side", [False, True])
+def test_workspace_after_a_timeout(side):
+    """What a call that gave up leaves, its status and counters that are not 0,
+    is gone once the status has been read."""
+    from orthossm_b200 import sdpc_kernel
+    calls = _pieces(64)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream() if side else torch.cuda.current_stream()):
+        for call, _, want in calls:
+            assert torch.equal(call(), want)
+        stream = torch.cuda.current_stream()
+        words = sdpc_kernel._WS_ATTN[(stream.device, stream.cuda_stream)].view(torch.int32)
+        words[64:64 + 2048] = 1  # the counters follow a header of 256 bytes
+        words[2] = 3             # its status word
+        stream.synchronize()
+        assert O.workspace_status(clear=False) == 3 and O.workspace_status() == 3 and O.workspace_status() == 0
+        for _ in range(2):
+            for call, _, want in calls:
+                assert torch.equal(call(), want)
+        stream.synchronize()
+
+
 def test_graphs_and_larger_heads_after_them():
     """Calls captured at 64 channels, replayed after calls at 128 and with the
     freed memory overwritten."""
