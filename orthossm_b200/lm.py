@@ -292,7 +292,9 @@ class OrthoSSMLM(nn.Module):
                  coeffs: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
         """Continues each prompt (1-D token ids on the GPU, of any lengths) by
         ``max_new_tokens`` tokens [B, max_new_tokens], drawn as
-        ``sample_tokens`` does from noise of ``generator``."""
+        ``sample_tokens`` does from noise of ``generator``.  A stream that has no
+        token left to draw (its logits are all NaN or -inf) has ended: its tokens
+        are -1 from there on; the others go on."""
         B = len(prompts)
         cache = self.new_cache(B, max(int(t.numel()) for t in prompts) + max_new_tokens, coeffs)
         dev = cache.lengths_dev.device
@@ -303,7 +305,9 @@ class OrthoSSMLM(nn.Module):
             logits = self.extend(tokens, cache)
             sample_tokens(logits, noise.exponential_(generator=generator), temperature=temperature, top_k=top_k,
                           top_p=top_p, min_p=min_p, out=out[i])
-            tokens = list(out[i].split(1))
+            if i:
+                out[i].masked_fill_(out[i - 1] < 0, -1)
+            tokens = list(out[i].clamp(min=0).split(1))  # -1 is no row of the embedding
         return out.t()
 
 

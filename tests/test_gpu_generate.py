@@ -83,6 +83,21 @@ def test_generate():
     assert torch.equal(draw(1), draw(1)) and not torch.equal(draw(1), draw(2))
 
 
+@pytest.mark.parametrize("f", [dict(temperature=0.0), dict(temperature=0.9, top_k=40), dict()])
+def test_a_stream_without_a_token_ends_alone(f):
+    """One stream's logits are NaN: its tokens are -1 and the other streams'
+    those that they are without it."""
+    model, coeffs = model_and_coeffs(3)
+    prompts = [ids(40), ids(3), ids(90)]
+    draw = lambda c: model.generate(prompts, 6, coeffs=c, **f,  # noqa: E731
+                                    generator=torch.Generator("cuda").manual_seed(5))
+    want = draw(coeffs)
+    coeffs[0][1] = float("nan")
+    got = draw(coeffs)
+    assert got[1].tolist() == [-1] * 6 and int(want.min()) >= 0
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+
+
 def test_refusals():
     model, coeffs = model_and_coeffs(2)
     cache = model.new_cache(2, 16, coeffs)
