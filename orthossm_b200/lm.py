@@ -40,7 +40,7 @@ from __future__ import annotations
 
 import dataclasses
 import math
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -161,11 +161,11 @@ class V8Layer(nn.Module):
         return x + self.out_proj(self.norm_comb(g + loc)), fin
 
     def extend(self, x: torch.Tensor, news: List[int], cu: torch.Tensor, at: torch.Tensor, kv_lengths: torch.Tensor,
-               li: int, cache: DecodeCache) -> torch.Tensor:
+               li: int, cache: DecodeCache) -> Tuple[torch.Tensor, torch.Tensor]:
         """The layer on new tokens of each stream, packed: x [T, d], stream b's
         news[b] tokens at cu[b]; their keys and values go to the cache rows
         ``at``.  Unlike ``forward``, the local window reaches back over the
-        calls before."""
+        calls before.  Returns the output and the global path's new EMA state."""
         T, d = x.shape
         H = self.cfg.n_heads
         h = self.norm_in(x)
@@ -184,13 +184,12 @@ class V8Layer(nn.Module):
                 fin.append(fb)
                 t += n
             fin = torch.cat(fin)
-        cache.ema[li] = fin
         q, k, v = self.qkv(h).view(T, 3, H, d // H).unbind(1)
         K, V = (c.view(-1, H, d // H) for c in (cache.keys[li], cache.values[li]))
         K[at], V[at] = k, v
         a = packed_attention(q, K, V, cu, cache.starts, max_seqlen_q=max(news), kv_lengths=kv_lengths,
                              window=self.cfg.window)
-        return x + self.out_proj(self.norm_comb(g + self.o(a.reshape(T, d))))
+        return x + self.out_proj(self.norm_comb(g + self.o(a.reshape(T, d)))), fin
 
 
 class OrthoSSMLM(nn.Module):
@@ -262,7 +261,8 @@ class OrthoSSMLM(nn.Module):
     def extend(self, tokens: List[torch.Tensor], cache: DecodeCache) -> torch.Tensor:
         """Appends tokens[b] (at least one each) to stream b: whole prompts,
         pieces of them, or single tokens.  Returns the logits [B, vocab] after
-        each stream's last token."""
+        each stream's last token.  A call that raises leaves the streams where
+        they were (what it wrote behind them is written again)."""
         news = [int(t.numel()) for t in tokens]
         if len(news) != len(cache.lengths) or min(news) < 1:
             raise ValueError("extend: every stream of the cache takes at least one token")
@@ -280,11 +280,15 @@ class OrthoSSMLM(nn.Module):
                             for b, (k, old) in enumerate(zip(news, cache.lengths))]).to(dev)
             grown = cache.lengths_dev + n.to(dev)
         x = self.embedding(torch.cat([t.reshape(-1) for t in tokens]))
+        ema = []
         for li, layer in enumerate(self.layers):
-            x = layer.extend(x, news, cu, at, grown, li, cache)
+            x, fin = layer.extend(x, news, cu, at, grown, li, cache)
+            ema.append(fin)
+        logits = self.lm_head(self.final_norm(x[(cu[1:] - 1).long()]))
+        cache.ema = ema
         cache.lengths = [old + k for old, k in zip(cache.lengths, news)]
         cache.lengths_dev = grown
-        return self.lm_head(self.final_norm(x[(cu[1:] - 1).long()]))
+        return logits
 
     @torch.no_grad()
     def generate(self, prompts: List[torch.Tensor], max_new_tokens: int, *, temperature=1.0, top_k=0, top_p=1.0,

@@ -65,6 +65,30 @@ def test_pieces_and_single_tokens_continue_the_stream():
     assert at == [169, 150]
 
 
+@pytest.mark.parametrize("where", [1, "head"])
+def test_a_call_that_raises_leaves_the_streams(where, monkeypatch):
+    model, coeffs = model_and_coeffs(2)
+    cache = model.new_cache(2, 128, coeffs)
+    first, then = [ids(20), ids(33)], [ids(5), ids(1)]
+    model.extend(first, cache)
+    ema = [e.clone() for e in cache.ema]
+
+    def fail(*a, **kw):
+        raise MemoryError("on purpose")
+
+    with monkeypatch.context() as m:
+        m.setattr(model.lm_head if where == "head" else model.layers[where],
+                  "forward" if where == "head" else "extend", fail)
+        with pytest.raises(MemoryError):
+            model.extend([ids(7), ids(9)], cache)
+    assert cache.lengths == [20, 33] and cache.lengths_dev.tolist() == [20, 33]
+    assert all(torch.equal(a, b) for a, b in zip(cache.ema, ema))
+    got = model.extend(then, cache)
+    other = model.new_cache(2, 128, coeffs)
+    model.extend(first, other)
+    assert torch.equal(got, model.extend(then, other))
+
+
 def test_generate():
     model, coeffs = model_and_coeffs(3)
     prompts = [ids(40), ids(3), ids(90)]
