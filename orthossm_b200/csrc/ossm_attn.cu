@@ -13,7 +13,6 @@ namespace attn {
 size_t prompt_part_floats(int hd);
 int prompt_forward(const ossm_attn_args* a, const Params& p, int grid, cudaStream_t st);
 size_t token_part_floats(int hd);
-int token_ctas(int hd);
 int token_forward(const ossm_attn_args* a, const Params& p, int sms, cudaStream_t st);
 
 bool row_ok(const void* ptr, long long st, long long sh, long long rows, int heads) {
@@ -55,11 +54,10 @@ int ossm::device_sms() {
 
 namespace {
 
-// Workspace: header, two progress counters a CTA, two partial results a CTA.
-constexpr int kMaxCtas = 1024;
+// Workspace: header, progress counters, two partial results a CTA.
 constexpr int kTokenRows = 16;  // of the token kernel's items
 
-int sm_count() { return std::min(device_sms(), kMaxCtas / 4); }
+int sm_count() { return std::min(device_sms(), attn::kMaxSms); }
 
 // One size for all arguments: a workspace never has to be replaced by a larger
 // one while a captured graph still points to it.
@@ -67,9 +65,9 @@ size_t ws_bytes() {
   size_t part = 0;
   for (int hd : {64, attn::kMaxHD})
     part = std::max({part, attn::prompt_part_floats(hd), attn::token_part_floats(hd)});
-  return sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t) + (size_t)sm_count() * part * sizeof(float);
+  return sizeof(WsHeader) + attn::kCounters * sizeof(uint32_t) + (size_t)sm_count() * part * sizeof(float);
 }
-static_assert(sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t) <= OSSM_ATTN_WS_ZERO, "header and counters");
+static_assert(sizeof(WsHeader) + attn::kCounters * sizeof(uint32_t) <= OSSM_ATTN_WS_ZERO, "header and counters");
 
 }  // namespace
 
@@ -87,7 +85,7 @@ extern "C" int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size
                        a->window >= a->total_k ? 0 : a->window,  // as wide as all keys: none
                        a->scale * 1.4426950408889634f, reinterpret_cast<WsHeader*>(w),
                        reinterpret_cast<uint32_t*>(w + sizeof(WsHeader)),
-                       reinterpret_cast<float*>(w + sizeof(WsHeader) + 2 * kMaxCtas * sizeof(uint32_t))};
+                       reinterpret_cast<float*>(w + sizeof(WsHeader) + attn::kCounters * sizeof(uint32_t))};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // Rows that share a key head.  Up to 16, one item of the token kernel holds
   // them and K and V are read once (8 streams of 2000 keys, 8/8 heads of 128,

@@ -15,6 +15,9 @@ namespace attn {
 
 constexpr int kMaxSeqs = 16384;
 constexpr int kMaxHD = 128;
+constexpr int kMaxSms = 256;             // SMs that are used, at most
+constexpr int kMaxCtas = 4 * kMaxSms;    // of a kernel's grid, at most
+constexpr int kCounters = 3 * kMaxCtas;  // two a CTA, then one a CTA (the token kernel's second step)
 constexpr long long kMaxRows = 1LL << 30;  // positions and their differences stay within 32 bits
 
 // Lets a kernel have `bytes` of dynamic shared memory, once a device.
@@ -40,7 +43,7 @@ struct Params {
   int window;      // 0: none
   float scale2;    // scale * log2(e): the softmax runs on base-2 exponents
   WsHeader* hdr;
-  uint32_t* counts;  // per CTA and tile: progress of the item that its last piece belongs to (0 between calls)
+  uint32_t* counts;  // [kCounters] progress of the items that are cut (0 between calls)
   float* part;       // per CTA two partial results
 };
 

@@ -40,7 +40,7 @@ constexpr int kMinPiece = 4;          // no cut closer to an item's edge
 constexpr int kMinWork = 8;           // a CTA for each part of this length at most, and for each item
 constexpr int kPairFrom = 32;         // steps a CTA from which items take two heads
 constexpr int kJoin = 16;             // partial results joined at once
-constexpr int kCounts = 1024;         // counters of the second step follow those of the first
+constexpr int kSecond = 2 * kMaxCtas;  // the second step's counters, one a CTA, follow those of the first
 
 template <int HDP>
 struct Cfg {
@@ -51,6 +51,7 @@ struct Cfg {
   static constexpr int kHeads = HDP == 64 ? 2 : 1;            // key heads of an item, at most
   static constexpr int kPart = kHeads * kRows;                // rows of a partial result
   static constexpr size_t kPartFloats = kPart * (HDP + 2);
+  static_assert(kMaxSms * kCtas <= kMaxCtas && kSecond + kMaxCtas <= kCounters, "a counter of its own for each");
   static_assert(kSmem >= kWarps * kRows * HDP * 4, "outputs of the warps");
 };
 
@@ -568,14 +569,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
       // one CTA alone would read all of them at its own small share of L2.
       const int np = last - first + 1;
       if (np <= kJoin) {
-        if (arrive(p.counts + kCounts + first, np))
+        if (arrive(p.counts + kSecond + first, np))
           join([&](int k) { return slot(first + k); }, np, static_cast<float*>(nullptr));
       } else {
         const int g0 = max(first, cta / kJoin * kJoin), g1 = min(last, cta / kJoin * kJoin + kJoin - 1);
         const int ng = last / kJoin - first / kJoin + 1;
         if (arrive(p.counts + (g0 == first ? 2 * g0 + 1 : 2 * g0), g1 - g0 + 1)) {
           join([&](int k) { return slot(g0 + k); }, g1 - g0 + 1, slot(g0));
-          if (arrive(p.counts + kCounts + first, ng))
+          if (arrive(p.counts + kSecond + first, ng))
             join([&](int k) { return slot(k ? (first / kJoin + k) * kJoin : first); }, ng,
                  static_cast<float*>(nullptr));
         }
@@ -603,7 +604,6 @@ size_t token_part_floats(int hd) {
   return hd <= 64 ? 2 * tok::Cfg<64>::kCtas * tok::Cfg<64>::kPartFloats
                   : 2 * tok::Cfg<128>::kCtas * tok::Cfg<128>::kPartFloats;
 }
-int token_ctas(int hd) { return hd <= 64 ? tok::Cfg<64>::kCtas : tok::Cfg<128>::kCtas; }
 
 int token_forward(const ossm_attn_args* a, const Params& p, int sms, cudaStream_t st) {
   const bool bf = a->dtype == OSSM_BF16;

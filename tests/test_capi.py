@@ -199,3 +199,12 @@ def test_workspaces_that_graphs_use_are_kept(monkeypatch):
     assert grown is not small and grown is not larger and get(s, 1 << 17) is grown
     assert len(K._WS_IN_GRAPHS) == 1 and K._WS_IN_GRAPHS[0] is small
     assert get(t, 1 << 16) is not fresh
+
+
+def test_attention_counters_do_not_overlap():
+    """Two counters a CTA and one for the second step, of up to 4 CTAs on each
+    of the SMs that are used, within what the caller zero-fills."""
+    src = open(os.path.join(ROOT, "orthossm_b200", "csrc", "ossm_attn.cuh")).read()
+    sms = int(re.search(r"kMaxSms = (\d+)", src).group(1))
+    assert sms >= 148 and 256 + 3 * 4 * sms * 4 <= L.OSSM_ATTN_WS_ZERO
+    assert L.lib().ossm_attn_workspace_bytes(C.byref(_attn())) > 256 + 3 * 4 * sms * 4
