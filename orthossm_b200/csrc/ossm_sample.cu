@@ -13,8 +13,10 @@
 // guessed from a sample and the guess checked by the mass collected.  Where too
 // many candidates are collected all the same (nearly flat rows) the first CTA
 // goes over the row instead of the list.
-// Masses that are compared are 64-bit fixed-point sums, which do not depend on
-// the order of the additions.
+// Masses that are compared, the whole row's among them, are 64-bit fixed-point
+// sums of one function of the logit: they do not depend on the order of the
+// additions, nor on how many CTAs a row gets.  (The fp32 sum of the first pass
+// gives the bound and the guess alone.)
 // Measured: 1 x 32000 bf16, top-k 50 and top-p 0.95: 10.8 us; 128 x 131072 bf16,
 // top-k 50: 16 us (5.1 us of reads), min-p 0.01: 18 us, top-p 0.72 (4000 stay):
 // 37 us, top-p 0.92 (18000 stay): 59 us.  What bounds it there: one CTA an SM
@@ -93,15 +95,54 @@ OSSM_DEV float ex2(float x) {  // 2^x, relative error 2^-22
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// A weight (0 to 1) in steps of 2^-40, to the nearest: a row's sum stays below
-// 2^63 for V < 2^23 equal candidates.  Two additions round off the steps of
-// 2^-17 and then what is left in steps of 2^-40, exactly.
-OSSM_DEV u64 mass_of(float w) {
-  const float h = __fadd_rn(w, 64.f), r = __fsub_rn(w, __fsub_rn(h, 64.f));
-  const int hi = __float_as_int(h) - __float_as_int(64.f);
-  const int lo = __float_as_int(__fadd_rn(r, 0x1.8p-17f)) - __float_as_int(0x1.8p-17f);
-  return ((u64)hi << 23) + (i64)lo;
-}
+OSSM_DEV float2 add2(float2 a, float2 b) { return fma2(a, make_float2(1.f, 1.f), b); }
+// Masses: the candidates' weights (0 to 1, relative to the row's largest logit m)
+// in steps of 2^-40, to the nearest; a row's sum stays below 2^63 for V < 2^23
+// equal candidates.  Everything that is compared is a sum of these, the whole
+// row's mass too, so that the prefix's end does not depend on how a row is
+// divided, nor on which of the ways below finds it.
+constexpr float kRound = 64.f, kRound2 = 0x1.8p-17f;  // numbers next to these are 2^-17 and 2^-40 apart
+struct Masses {
+  float m, c, c_lo, least;  // c + c_lo = log2(e) / temperature; logits further below m weigh nothing
+  OSSM_DEV Masses(float m, float inv_t) : m(m) {
+    constexpr float kL = 1.44269504f, kL_lo = 1.92596303e-8f;  // log2(e)
+    const float x = inv_t * kL;
+    c = fminf(x, 3e38f);
+    c_lo = x == c ? fmaf(inv_t, kL_lo, fmaf(inv_t, kL, -x)) : 0.f;
+    least = fmaxf(-64.f / c, kLowest);
+  }
+  // The steps of 2^-17 are rounded off by one addition, then what is left in
+  // steps of 2^-40 by a second: exact.
+  OSSM_DEV u64 of(float l) const {
+    const float d = l == m ? 0.f : fmaxf(__fsub_rn(l, m), least);
+    const float w = ex2(__fmaf_rn(d, c, __fmul_rn(d, c_lo)));
+    const float h = __fadd_rn(w, kRound), y = __fadd_rn(__fsub_rn(w, __fsub_rn(h, kRound)), kRound2);
+    const int hi = __float_as_int(h) - __float_as_int(kRound), lo = __float_as_int(y) - __float_as_int(kRound2);
+    return ((u64)hi << 23) + (i64)lo;
+  }
+  // The sum over N logits (m finite; what is no candidate weighs nothing),
+  // added to h and y: the two roundings' bits, kRound's and kRound2's included.
+  template <int N>
+  OSSM_DEV void add(const float (&l)[N], uint32_t& h, uint32_t& y) const {
+    const float2 m2 = make_float2(m, m), c2 = make_float2(c, c), lo2 = make_float2(c_lo, c_lo);
+    const float2 r1 = make_float2(kRound, kRound), r2 = make_float2(kRound2, kRound2);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      float2 d = sub2(make_float2(l[e], l[e + 1]), m2);
+      d = make_float2(fmaxf(d.x, least), fmaxf(d.y, least));  // a NaN operand loses
+      d = fma2(d, c2, mul2(d, lo2));
+      const float2 w = make_float2(ex2(d.x), ex2(d.y));
+      const float2 a = add2(w, r1), b = add2(sub2(w, sub2(a, r1)), r2);
+      h += __float_as_uint(a.x) + __float_as_uint(a.y);
+      y += __float_as_uint(b.x) + __float_as_uint(b.y);
+    }
+  }
+  static OSSM_DEV u64 sum(uint32_t h, uint32_t y, int n) {  // of n logits added, n <= 2^8
+    h -= n * __float_as_uint(kRound);
+    y -= n * __float_as_uint(kRound2);
+    return ((u64)h << 23) + (i64)(int)y;
+  }
+};
 
 // The product and the difference are rounded one after the other (no fused
 // multiply-add), so that a caller can recompute a score exactly.  A NaN (from
@@ -357,9 +398,9 @@ OSSM_DEV u64 share(float top_p, u64 whole) {  // the mass that a prefix has to r
 // How many of n <= kRank keys in order the prefix holds (at least one) whose
 // mass reaches `target`, or (target == 0) the share top_p of theirs; n + 1: they
 // do not reach it.
-OSSM_DEV int reaching(const u64* list, int n, float m, const Row& r, u64 target, u64* red) {
+OSSM_DEV int reaching(const u64* list, int n, const Masses& ms, const Row& r, u64 target, u64* red) {
   const int tid = threadIdx.x;
-  const u64 own = tid < n ? mass_of(weight(logit_of(list[tid]), m, r.inv_t)) : 0;
+  const u64 own = tid < n ? ms.of(logit_of(list[tid])) : 0;
   u64 all;
   const u64 upto = block_scan(own, red, all);
   if (target == 0) target = share(r.top_p, all);
@@ -408,7 +449,7 @@ OSSM_DEV int find_bin(Room& s, u64 target, float top_p, u64& left) {
 // as more than kRank are between the bounds, their range is cut into bins and
 // narrowed to the one where the prefix ends; keys differ, so that ends.
 template <typename Each>
-OSSM_DEV u64 narrow(const Row& r, Each each, bool count, u64 left, float m, Room& s) {
+OSSM_DEV u64 narrow(const Row& r, Each each, bool count, u64 left, const Masses& ms, Room& s) {
   u64 lo = 0, hi = ~(u64)0;
   int* fill = reinterpret_cast<int*>(&s.sh[3]);
   for (;;) {
@@ -426,7 +467,7 @@ OSSM_DEV u64 narrow(const Row& r, Each each, bool count, u64 left, float m, Room
     const int n = *fill;
     if (n <= kRank) {
       order(s.few, n);
-      return s.few[(count ? (int)left : min(n, reaching(s.few, n, m, r, left, s.red))) - 1];
+      return s.few[(count ? (int)left : min(n, reaching(s.few, n, ms, r, left, s.red))) - 1];
     }
     lo = block_reduce(least, s.red, [](u64 a, u64 b) { return min(a, b); });
     hi = block_reduce(most, s.red, [](u64 a, u64 b) { return max(a, b); });
@@ -434,7 +475,7 @@ OSSM_DEV u64 narrow(const Row& r, Each each, bool count, u64 left, float m, Room
     clear_bins(s);
     each([&](u64 key) {
       if (key >= lo && key <= hi)
-        add64(s.bins + ((hi - key) >> shift), count ? 1 : mass_of(weight(logit_of(key), m, r.inv_t)));
+        add64(s.bins + ((hi - key) >> shift), count ? 1 : ms.of(logit_of(key)));
     });
     const int bin = find_bin(s, left, 1.f, left);
     if (bin < 0) return lo;
@@ -458,18 +499,18 @@ struct Bins {
 // The smallest key of the prefix of the list's N candidates at or above `floor`
 // that holds `count` of them, or (count == 0) the mass `target` (0: the share
 // top_p of theirs); `floor` where they do not reach it.
-OSSM_DEV u64 select_list(const Row& r, int N, float m, u64 floor, int count, u64 target, Room& s) {
+OSSM_DEV u64 select_list(const Row& r, int N, const Masses& ms, u64 floor, int count, u64 target, Room& s) {
   auto all = [&](auto f) {
     for (int e = threadIdx.x; e < N; e += kThreads)
       if (s.list[e] >= floor) f(s.list[e]);
   };
   u64 least = ~(u64)0;
   all([&](u64 key) { least = min(least, key); });
-  const Bins bins(m, logit_of(block_reduce(least, s.red, [](u64 a, u64 b) { return min(a, b); })));
+  const Bins bins(ms.m, logit_of(block_reduce(least, s.red, [](u64 a, u64 b) { return min(a, b); })));
   clear_bins(s);
   all([&](u64 key) {
     const float l = logit_of(key);
-    add64(s.bins + bins.of(bins.below(l)), count ? 1 : mass_of(weight(l, m, r.inv_t)));
+    add64(s.bins + bins.of(bins.below(l)), count ? 1 : ms.of(l));
   });
   u64 left;
   const int cut = find_bin(s, count ? (u64)count : target, r.top_p, left);
@@ -479,16 +520,17 @@ OSSM_DEV u64 select_list(const Row& r, int N, float m, u64 floor, int count, u64
       if (bins.of(bins.below(logit_of(key))) == cut) f(key);
     });
   };
-  return narrow(r, each, count != 0, left, m, s);
+  return narrow(r, each, count != 0, left, ms, s);
 }
 
 // The same of all the row's candidates, by one CTA; `whole`: their mass where it
 // is known, else 0.  Candidates below logit lb are known to lie behind the
 // prefix.
 template <typename T>
-OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, float m, float lb, u64 floor, int count, u64 whole, Room& s) {
+OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, const Masses& ms, float lb, u64 floor, int count, u64 whole,
+                        Room& s) {
+  const float m = ms.m;
   const Bins bins(m, lb);
-  const float c = r.inv_t * 1.44269504f;
   const float first = floor ? logit_of(floor) : -INFINITY;  // floor's logit: only there the index decides
   const float low = fmaxf(lb, kLowest);
   uint32_t* part = reinterpret_cast<uint32_t*>(s.bins);  // counts: the low half of a bin's sum
@@ -497,14 +539,12 @@ OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, float m, float lb, u64
 #pragma unroll
     for (int e = 0; e < Vec<T>::n; ++e) {
       const bool in = e < n && l[e] >= low && (l[e] > first || key_of(l[e], i + e) >= floor);
-      const float d = bins.below(l[e]);
-      const int b = bins.of(d);
-      const u64 q = mass_of(ex2(-d * c));
+      const int b = bins.of(bins.below(l[e]));
       if (!in) continue;
       if (count)
         atomicAdd(part + 2 * b, 1u);
       else
-        add64(s.bins + b, q);
+        add64(s.bins + b, ms.of(l[e]));
     }
   });
   u64 left;
@@ -533,11 +573,11 @@ OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, float m, float lb, u64
   });
   __syncthreads();
   const int size = *fill;
-  if (size > kList) return narrow(r, each, count != 0, left, m, s);
+  if (size > kList) return narrow(r, each, count != 0, left, ms, s);
   auto listed = [&](auto f) {
     for (int e = threadIdx.x; e < size; e += kThreads) f(s.list[e]);
   };
-  return narrow(r, listed, count != 0, left, m, s);
+  return narrow(r, listed, count != 0, left, ms, s);
 }
 
 // The candidates of this CTA's share from logit `low` on, into a list; *count may
@@ -545,19 +585,23 @@ OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, float m, float lb, u64
 // vectors take their places with one addition, and the candidates are walked
 // by the bits set: code for each of the 32 logits of a thread ran in every warp
 // that had one candidate (128 rows of 131072, 4000 candidates each: 43 us, so 37).
+// With `sum` it also returns the mass that this thread has seen of the share.
 template <typename T>
-OSSM_DEV void collect(const T* row, int V, int rank, int nrank, float low, int* count, u64* list) {
+OSSM_DEV u64 collect(const T* row, int V, int rank, int nrank, float low, bool sum, const Masses& ms, int* count,
+                     u64* list) {
   constexpr int N = Vec<T>::n, U = 4;
   const Share<T> own(row, V, rank, nrank);
   const int lane = threadIdx.x & 31;
   bool over = false;
-  for (int first = own.v0; first < own.v1 && !over; first += U * kThreads) {
+  u64 mass = 0;
+  for (int first = own.v0; first < own.v1 && !(over && !sum); first += U * kThreads) {
     const int v = first + threadIdx.x;
     uint4 u[U];
 #pragma unroll
     for (int k = 0; k < U; ++k)
       if (v + k * kThreads < own.v1) u[k] = __ldg(own.body + v + k * kThreads);
-    uint32_t in = 0;
+    uint32_t in = 0, h = 0, y = 0;
+    int n = 0;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       if (v + k * kThreads >= own.v1) break;
@@ -565,8 +609,11 @@ OSSM_DEV void collect(const T* row, int V, int rank, int nrank, float low, int* 
       unpack(u[k], l, T());
 #pragma unroll
       for (int e = 0; e < N; ++e) in |= l[e] >= low ? 1u << (k * N + e) : 0u;  // a NaN is not
+      if (sum) ms.add(l, h, y);
+      n += N;
     }
-    if (!__any_sync(~0u, in)) continue;
+    if (sum) mass += Masses::sum(h, y, n);
+    if (over || !__any_sync(~0u, in)) continue;
     int upto = __popc(in);
 #pragma unroll
     for (int w = 1; w < 32; w *= 2) {
@@ -593,8 +640,10 @@ OSSM_DEV void collect(const T* row, int V, int rank, int nrank, float low, int* 
         const int at = atomicAdd(count, 1);
         if (at < kList) list[at] = key_of(l, i);
       }
+      if (sum && live(l)) mass += ms.of(l);
     }
   }
+  return mass;
 }
 
 // A guess of the logit below which this CTA's share of the row holds `tail` of
@@ -668,7 +717,8 @@ OSSM_DEV void race(const float* l, const float* e, int i, int n, float low, F st
 
 // What the CTAs of a cluster tell each other.
 struct Told {
-  float m, z;      // largest logit; sum of the weights relative to it
+  float m, z;      // largest logit; sum of the weights relative to it, in fp32
+  u64 whole;       // the row's mass (the first CTA's)
   uint32_t tk;     // order bits that at least top_k candidates reach
   float guess;     // where its part of the tail begins
   int count;       // candidates collected (the first CTA's)
@@ -727,7 +777,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   const T* lg = static_cast<const T*>(p.logits) + row * p.lst;
   const float* nz = p.noise ? p.noise + row * p.nst : nullptr;
   const Row r = row_of(p, row);
-  if (tid == 0) told.count = 0;
+  if (tid == 0) told.count = 0, told.whole = 0;
 
   if (r.open()) {
     open_row<kThreads>(lg, nz, p.V, r.inv_t, rank, nrank, bests, told, p.out + row);
@@ -738,7 +788,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   const int top_k = r.greedy ? 1 : r.top_k;
   const bool by_mass = !r.greedy && r.top_p < 1.f;
   const bool need_z = by_mass && top_k == 0;
-  const float c = r.inv_t * 1.44269504f;
+  const float c = fminf(r.inv_t * 1.44269504f, 3e38f);
   float m = -INFINITY, z = 0.f;
   scan(lg, p.V, rank, nrank, [&](const float* l, int, int n) {
     float top = l[0];
@@ -798,8 +848,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     if (rank == 0 && tid == 0) p.out[row] = -1;
     return;
   }
-  // next to an infinite logit nothing else has weight; the sum is taken over the candidates then
-  const u64 whole = need_z && m < INFINITY ? (u64)((double)z * 0x1p40) : 0;
+  const Masses ms(m, r.inv_t);
 
   // ---------------------------------------------------------------- Bound, and the candidates above it
   // With top_k: its own bound alone, as its mass counts for top_p.  Without:
@@ -847,7 +896,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   Told* first = nrank > 1 ? cluster.map_shared_rank(&told, 0) : &told;
   u64* first_list = nrank > 1 ? cluster.map_shared_rank(room.list, 0) : room.list;
   const float low = bound ? fmaxf(logit_of((u64)bound << 32), kLowest) : kLowest;
-  collect(lg, p.V, rank, nrank, low, &first->count, first_list);
+  // next to an infinite logit nothing else has weight; the sum is taken over the candidates then
+  const bool sum = need_z && m < INFINITY;
+  u64 whole = collect(lg, p.V, rank, nrank, low, sum, ms, &first->count, first_list);
+  if (sum) {
+#pragma unroll
+    for (int w = 16; w; w >>= 1) whole += __shfl_xor_sync(~0u, whole, w);
+    if ((tid & 31) == 0) add64(&first->whole, whole);
+  }
   if (nrank > 1)
     cluster.sync();
   else
@@ -856,6 +912,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
 
   // ---------------------------------------------------------------- the prefix and its best score
   const int N = told.count;
+  whole = told.whole;
   Best b{0.f, -1};
   u64 keep = 0;  // the prefix's last key
   bool by_list = N <= kList;
@@ -868,14 +925,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
       order(room.list, N);
       int n = top_k ? min(top_k, N) : N;
       if (by_mass) {
-        const int stay = reaching(room.list, n, m, r, target, room.red);
+        const int stay = reaching(room.list, n, ms, r, target, room.red);
         by_list = !(guessed && stay > n);
         n = min(n, stay);
       }
       if (n) keep = room.list[n - 1];
     } else {
-      if (top_k && top_k < N) keep = select_list(r, N, m, 0, top_k, 0, room);
-      if (by_mass) keep = select_list(r, N, m, keep, 0, target, room);
+      if (top_k && top_k < N) keep = select_list(r, N, ms, 0, top_k, 0, room);
+      if (by_mass) keep = select_list(r, N, ms, keep, 0, target, room);
       by_list = !(guessed && keep == 0);  // 0: the guess was too high
     }
   }
@@ -918,9 +975,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     if (r.greedy) {
       keep = top;
     } else {
-      if (top_k) keep = select_row(r, lg, p.V, m, least, 0, top_k, 0, room);
+      if (top_k) keep = select_row(r, lg, p.V, ms, least, 0, top_k, 0, room);
       if (by_mass)
-        keep = select_row(r, lg, p.V, m, live(lb) ? lb : top_k ? logit_of(keep) : least, keep, 0, whole, room);
+        keep = select_row(r, lg, p.V, ms, live(lb) ? lb : top_k ? logit_of(keep) : least, keep, 0, whole, room);
     }
     const float end = keep ? logit_of(keep) : -INFINITY;  // the last one's logit: only there the index decides
     if (r.greedy) {

@@ -132,6 +132,36 @@ def test_peak_over_a_flat_tail(V, low, p, B):
         assert got.tolist() == [i if i < stay else 0] * B
 
 
+@pytest.mark.parametrize("V,spread,dtype", [(131072, 0.5, torch.float32), (50257, 1.5, torch.float32),
+                                            (131072, 1.0, torch.bfloat16), (9001, 1.0, torch.float16)])
+def test_prefix_end_in_any_batch(V, spread, dtype):
+    """Noise that makes the last candidate of the prefix win, so that the token
+    shows where it ends: the same for a row alone and in batches of any size,
+    and where float64 has it, as far as fp32 weights can tell."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    l = (torch.randn(1, V, device="cuda", generator=g) * spread).to(dtype)
+    order = torch.sort(l[0].double(), descending=True, stable=True).indices
+    T = 0.9
+    e = torch.empty(1, V, device="cuda")  # the score of the candidate in place r is r * 80 / V
+    e[0, order] = (l[0].double()[order] / T - 80.0 / V * torch.arange(V, device="cuda")).exp().float()
+    rank = torch.empty(V, dtype=torch.long, device="cuda")
+    rank[order] = torch.arange(V, device="cuda")
+    n = 160
+    p = torch.linspace(0.35, 0.97, n, device="cuda")
+    f = lambda b, **kw: O.sample_tokens(l.expand(b, V), e.expand(b, V), temperature=T, **kw)  # noqa: E731
+    many = f(n, top_p=p)
+    some = torch.cat([f(40, top_p=x) for x in p.split(40)])
+    one = torch.cat([f(1, top_p=x) for x in p.split(1)])
+    x = l[0].double()[order] / T
+    w = (x - x[0]).exp()
+    upto = w.cumsum(0)
+    for b in range(n):
+        end = int((upto - w < float(p[b]) * upto[-1]).sum()) - 1
+        off = 2.0 ** -18 * float(upto[-1] / w[end]) + 1
+        assert abs(int(rank[many[b]]) - end) <= off, (b, int(rank[many[b]]), end)
+    assert torch.equal(many, some) and torch.equal(many, one)
+
+
 def test_all_equal():
     """One logit everywhere: the first k by index."""
     for val in (0.0, -0.0, 3.0, -7.5):
