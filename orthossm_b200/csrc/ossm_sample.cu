@@ -247,8 +247,9 @@ OSSM_DEV void scan(const T* row, int V, int rank, int nrank, F f) {
   }
 }
 
-// The same with the noise of each logit: f(l, e, i, n).  Both are loaded ahead
-// for several vectors, as the noise comes from HBM.
+// The same with the noise of each logit: f(l, e, i, n), by all lanes of a warp
+// together (n = 0: nothing for this lane).  Both are loaded ahead for several
+// vectors, as the noise comes from HBM.
 template <int NT, typename T, typename F>
 OSSM_DEV void scan_noise(const T* row, const float* nz, int V, int rank, int nrank, F f) {
   constexpr int N = Vec<T>::n, U = 16 / N;
@@ -257,12 +258,13 @@ OSSM_DEV void scan_noise(const T* row, const float* nz, int V, int rank, int nra
   const uint4* body = own.body;
   const float* nbody = nz + head;
   const bool aligned = ((uintptr_t)nbody & 15) == 0;
-  for (int v = v0 + threadIdx.x; v < v1; v += U * NT) {
+  const int lane = threadIdx.x & 31;
+  for (int v = v0 + (threadIdx.x - lane); v < v1; v += U * NT) {  // of the warp's first lane
     uint4 u[U];
     float e[U][N];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int w = v + k * NT;
+      const int w = v + lane + k * NT;
       if (w >= v1) break;
       u[k] = __ldg(body + w);
       if (aligned) {
@@ -278,24 +280,21 @@ OSSM_DEV void scan_noise(const T* row, const float* nz, int V, int rank, int nra
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int w = v + k * NT;
-      if (w >= v1) break;
+      if (v + k * NT >= v1) break;
+      const int w = v + lane + k * NT;
       float l[N];
       unpack(u[k], l, T());
 #pragma unroll
       for (int h = 0; h < N; ++h) l[h] = fmaxf(l[h], -INFINITY);
-      f(l, e[k], head + w * N, N);
+      f(l, e[k], head + w * N, w < v1 ? N : 0);
     }
   }
-  if (rank == 0) {
-    const int tail = V - head - nv * N, t = threadIdx.x;
-    if (t < head + tail) {
-      const int i = t < head ? t : V - tail + (t - head);
-      float l[N], e[N];
-      l[0] = fmaxf(to_f(row[i]), -INFINITY);
-      e[0] = nz[i];
-      f(l, e, i, 1);
-    }
+  if (rank == 0 && threadIdx.x < 32) {  // the ends: fewer than 16 logits
+    const int tail = V - head - nv * N, n = lane < head + tail ? 1 : 0;
+    const int i = lane < head ? lane : V - tail + (lane - head);
+    float l[N], e[N];
+    if (n) l[0] = fmaxf(to_f(row[i]), -INFINITY), e[0] = nz[i];
+    f(l, e, i, n);
   }
 }
 
@@ -712,7 +711,7 @@ OSSM_DEV void race(const float* l, const float* e, int i, int n, float low, F st
     for (int k = 0; k < Vec<T>::n; ++k)
       if ((near >> k & 1u) && stays(l[k], i + k)) better(b, score_of(l[k], inv_t, e[k]), i + k);
   }
-  mark = logit_of((u64)__reduce_max_sync(__activemask(), ord(b.i < 0 ? -INFINITY : b.s)) << 32);
+  mark = logit_of((u64)__reduce_max_sync(~0u, ord(b.i < 0 ? -INFINITY : b.s)) << 32);
 }
 
 // What the CTAs of a cluster tell each other.

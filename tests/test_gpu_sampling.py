@@ -162,6 +162,19 @@ def test_prefix_end_in_any_batch(V, spread, dtype):
     assert torch.equal(many, some) and torch.equal(many, one)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_open_rows_of_every_length(dtype):
+    """Unfiltered rows that end at any lane of a warp, at odd alignments."""
+    for V in [*range(1, 20), 127, 128, 129, 255, 256, 257, 511, 513, 2047, 4095, 4097, 8191, 16383, 16385, 40001]:
+        l, e = inputs(5, V, dtype, seed=V)
+        s = l.double() - e.double().log()
+        best = s.argmax(-1)
+        second = s.scatter(1, best[:, None], -INF).amax(-1) if V > 1 else torch.full_like(s[:, 0], -INF)
+        clear = s.amax(-1) - second > 2.0 ** -18 * (s.amax(-1).abs() + 1)
+        got = O.sample_tokens(l, e)
+        assert bool((got == best)[clear].all()), V
+
+
 def test_all_equal():
     """One logit everywhere: the first k by index."""
     for val in (0.0, -0.0, 3.0, -7.5):
