@@ -331,7 +331,11 @@ struct Row {
 };
 OSSM_DEV Row row_of(const Params& p, int row) {
   Row r;
-  r.inv_t = p.t_row ? 1.0f / p.t_row[row] : p.inv_t;
+  r.inv_t = p.inv_t;
+  if (p.t_row) {  // not below the least fp32 number: 0 is the largest logit alone
+    const float t = p.t_row[row];
+    r.inv_t = t > 0.f ? fmaxf(1.0f / t, 0x1p-149f) : 0.f;
+  }
   r.top_k = p.k_row ? p.k_row[row] : p.top_k;
   r.top_p = p.p_row ? p.p_row[row] : p.top_p;
   r.min_p = p.m_row ? p.m_row[row] : p.min_p;

@@ -212,8 +212,9 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
 
     ``noise=None`` or a temperature of 0 takes the largest logit.  Each
     setting is a number or a tensor [B] on the device (float32; top_k int32),
-    one value a row; a tensor's temperature that is not positive is 0.  NaN
-    and -inf logits are never drawn; a row that has nothing else gives -1.
+    one value a row; a tensor's temperature that is not positive is 0, and an
+    infinite one makes all candidates equally likely.  NaN and -inf logits are
+    never drawn; a row that has nothing else gives -1.
     Returns int64 [B] (``out`` if given)."""
     _need_cuda(logits, noise, out)
     dt = _DT_SAMPLE.get(logits.dtype)
@@ -255,7 +256,7 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
                          f"min_p {m} in [0, 1]")
     if B == 0:
         return out
-    a = L.SampleArgs(B, V, logits.data_ptr(), dt, lst, _ptr(noise), nst, 1.0 / t if t > 0 else 0.0, p, m,
+    a = L.SampleArgs(B, V, logits.data_ptr(), dt, lst, _ptr(noise), nst, max(1.0 / t, 2.0 ** -149) if t > 0 else 0.0, p, m,
                      min(int(k), V), _ptr(t_row), _ptr(p_row), _ptr(m_row), _ptr(k_row), out.data_ptr())
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):

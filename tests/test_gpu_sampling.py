@@ -221,6 +221,17 @@ def test_greedy():
     assert O.sample_tokens(l, e, temperature=t, top_k=7).tolist() == want
 
 
+def test_endless_temperature():
+    """A temperature so high that its inverse is 0: every candidate is as likely."""
+    l, e = inputs(4, 3000, torch.float32, seed=11)
+    l[:, 7] = -INF
+    e[:, 7] = 1e-30
+    t = torch.tensor([INF, 3e38, 1.0, INF], device="cuda")
+    for f in (dict(), dict(top_k=50), dict(min_p=0.5), dict(top_p=0.5)):
+        check(l, e, temperature=t, **f)
+        check(l, e, temperature=1e300, **f)
+
+
 @pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 32000), (torch.float32, 4001)])
 def test_settings_of_each_row(dtype, V):
     B = 24
