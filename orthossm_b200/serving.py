@@ -187,11 +187,14 @@ def _attention(a, dev):
         L.check(status, "packed_attention")
 
 
-def _setting(x, dtype, B, what, dev):
-    """A setting given as a tensor [B], in the kernel's type."""
+def _setting(x, dtype, B, what, dev, most=None):
+    """A setting given as a tensor [B], in the kernel's type; of counts, ``most``
+    and more are the same."""
     if x.dim() != 1 or x.shape[0] != B or x.get_device() != dev:
         raise ValueError(f"sample_tokens: {what} must be a number or a vector of {B} on the logits' device")
-    return x if x.dtype == dtype and x.is_contiguous() else x.to(dtype).contiguous()
+    if x.dtype != dtype:
+        x = (x if most is None else x.clamp(0, most)).to(dtype)  # a larger type's counts do not wrap
+    return x.contiguous()
 
 
 def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
@@ -246,7 +249,7 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
     if isinstance(t, torch.Tensor):
         t_row, t = _setting(t, torch.float32, B, "temperature", dev), 0.0
     if isinstance(k, torch.Tensor):
-        k_row, k = _setting(k, torch.int32, B, "top_k", dev), 0
+        k_row, k = _setting(k, torch.int32, B, "top_k", dev, V), 0
     if isinstance(p, torch.Tensor):
         p_row, p = _setting(p, torch.float32, B, "top_p", dev), 0.0
     if isinstance(m, torch.Tensor):

@@ -252,6 +252,15 @@ def test_settings_of_each_row(dtype, V):
     check(l, e, temperature=t)
 
 
+def test_counts_of_a_wider_type():
+    l, e = inputs(5, 3000, torch.float32, seed=12)
+    want = O.sample_tokens(l, e).tolist()
+    k = torch.tensor([2 ** 32 + 1, 2 ** 31, 2 ** 40, -2 ** 33 + 1, 1], device="cuda")
+    got = O.sample_tokens(l, e, top_k=k).tolist()
+    assert got[:4] == want[:4] and got[4] == int(l[4].argmax())
+    assert O.sample_tokens(l, e, top_k=k.clamp(-9, 9)).tolist()[3] == want[3]
+
+
 def test_layouts_and_output():
     l, e = inputs(6, 3001, torch.bfloat16, seed=5)
     want = O.sample_tokens(l, e, top_k=20, top_p=0.9).tolist()
