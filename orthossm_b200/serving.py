@@ -14,6 +14,7 @@ import math
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from .sdpc_kernel import _WS_ATTN, _captured_workspace, _need_cuda, _ptr, _workspace
@@ -125,6 +126,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                           out)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError("packed_attention has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v)):
+        raise NotImplementedError("packed_attention has no forward-mode derivative")
     ot, oh = H * hd, hd
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)

@@ -424,3 +424,17 @@ def test_refusals():
         f(q.requires_grad_(), k, k, cu, **ok)
     with torch.no_grad():
         f(q, k, k, cu, **ok)
+
+
+def test_forward_mode_is_refused():
+    """A tangent of q, k or v must not be dropped in silence."""
+    q, k, v = (torch.randn(4, 2, 64, device="cuda").to(torch.bfloat16) for _ in range(3))
+    cu = cum([4])
+    want = O.packed_attention(q, k, v, cu, max_seqlen_q=4)
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(3):
+            x = [q, k, v]
+            x[i] = torch.autograd.forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(NotImplementedError), torch.no_grad():
+                O.packed_attention(*x, cu, max_seqlen_q=4)
+        assert torch.equal(O.packed_attention(q, k, v, cu, max_seqlen_q=4), want)
