@@ -432,7 +432,7 @@ int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size_t workspac
  * No counterpart in the reference, which stops at the logits (model.py:23-187).
  * ------------------------------------------------------------------------ */
 typedef struct {
-  int32_t B, V;
+  int32_t B, V;                      /* V below 2^23 (the mass of a row is held in 63 bits), B at most 2^27 */
   const void* logits;                /* [B, V], unit stride along V */
   int32_t dtype;                     /* OSSM_F32, OSSM_BF16 or OSSM_F16 */
   int64_t logits_stride;             /* row strides in elements */

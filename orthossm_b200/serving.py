@@ -204,7 +204,8 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
                   temperature: Union[float, torch.Tensor] = 1.0, top_k: Union[int, torch.Tensor] = 0,
                   top_p: Union[float, torch.Tensor] = 1.0, min_p: Union[float, torch.Tensor] = 0.0,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The next token of each row of logits [B, V] (fp32, bf16 or fp16, CUDA).
+    """The next token of each row of logits [B, V] (fp32, bf16 or fp16, CUDA;
+    V below 2^23, B at most 2^27).
 
     Candidates are ordered by logit, at equal logits by index.  The first
     ``top_k`` stay (0: all); of these the shortest prefix whose probability
@@ -229,8 +230,8 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
                          f"{logits.dtype}")
     B, V = logits.shape
     dev = logits.get_device()
-    if V < 1:
-        raise ValueError("sample_tokens: no candidates")
+    if not 1 <= V < 1 << 23 or B > 1 << 27:
+        raise ValueError(f"sample_tokens: 1 to 2^23 - 1 candidates in at most 2^27 rows, got {V} in {B}")
     lst, unit = logits.stride()
     if unit != 1:
         logits = logits.contiguous()

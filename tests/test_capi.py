@@ -208,3 +208,15 @@ def test_attention_counters_do_not_overlap():
     sms = int(re.search(r"kMaxSms = (\d+)", src).group(1))
     assert sms >= 148 and 256 + 3 * 4 * sms * 4 <= L.OSSM_ATTN_WS_ZERO
     assert L.lib().ossm_attn_workspace_bytes(C.byref(_attn())) > 256 + 3 * 4 * sms * 4
+
+
+def test_sampling_limits():
+    """Refused before any CUDA call."""
+    lib = L.lib()
+    f = lambda **kw: lib.ossm_sample_tokens(C.byref(L.SampleArgs(  # noqa: E731
+        **{**dict(B=1, V=8, logits=4096, dtype=L.OSSM_F32, logits_stride=8, inv_temperature=1.0, top_p=1.0,
+                  out=4096), **kw})), None)
+    for bad in (dict(V=1 << 23), dict(V=0), dict(B=(1 << 27) + 1), dict(B=-1), dict(logits=0), dict(logits=4097),
+                dict(out=4), dict(dtype=7), dict(top_p=-0.5), dict(min_p=float("nan")), dict(top_k=-1)):
+        assert f(**bad) == L.OSSM_EINVAL, bad
+    assert f(B=0) == L.OSSM_OK

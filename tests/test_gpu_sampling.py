@@ -252,6 +252,19 @@ def test_settings_of_each_row(dtype, V):
     check(l, e, temperature=t)
 
 
+def test_widest_row():
+    l = torch.zeros(2, 1 << 23, device="cuda")
+    for f in (dict(), dict(top_p=0.5)):
+        with pytest.raises(ValueError, match="candidates"):
+            O.sample_tokens(l, l, **f)
+    V = (1 << 23) - 1
+    l, e = l[:, :V], torch.ones(2, V, device="cuda")
+    e[0, V // 2 - 1], e[0, V // 2 + 1], e[1, V - 1] = 1e-20, 1e-30, 1e-30
+    assert O.sample_tokens(l, e, top_p=0.5).tolist() == [V // 2 - 1, 0]
+    assert O.sample_tokens(l, e).tolist() == [V // 2 + 1, V - 1]
+    assert O.sample_tokens(l, e, top_k=V // 2).tolist() == [V // 2 - 1, 0]
+
+
 def test_counts_of_a_wider_type():
     l, e = inputs(5, 3000, torch.float32, seed=12)
     want = O.sample_tokens(l, e).tolist()
