@@ -438,3 +438,29 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError), torch.no_grad():
                 O.packed_attention(*x, cu, max_seqlen_q=4)
         assert torch.equal(O.packed_attention(q, k, v, cu, max_seqlen_q=4), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("G,hd,nq", [(1, 64, 1), (4, 128, 1), (8, 64, 2), (2, 80, 3)])
+def test_weights_of_few_queries_are_not_rounded(G, hd, nq, dtype):
+    """Values of one size and either sign, so that outputs are differences of
+    weights: the form for few queries keeps these to fp32.  Bound: the output's
+    rounding, u |o|; the weights' two 16-bit parts, u^2, and their fp32 errors:
+    scores off by hd 2^-24 sum |q k| scale (below 2^-14 here), the rest by a
+    few 2^-22.  Weights rounded to the type would not pass."""
+    n, Hkv = 150, 2
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    lk = [nq + i % 9 for i in range(n)]
+    q = torch.randn(n * nq, G * Hkv, hd, device="cuda", generator=g).to(dtype)
+    k = torch.randn(sum(lk), Hkv, hd, device="cuda", generator=g).to(dtype)
+    v = torch.randint(0, 2, (sum(lk), Hkv, hd), device="cuda", generator=g).mul(2).sub(1).to(dtype)
+    cu_q, cu_k = cum([nq] * n), cum(lk)
+    out = O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=nq).double().cpu()
+    ref, mag, _ = packed_attention_ref(q, k, v, cu_q, cu_k)
+    u = 2.0 ** (-8 if dtype == torch.bfloat16 else -11)
+    lim = u * ref.abs() + (2.0 ** -13 + u * u) * mag + 1e-6
+    assert bool(((out - ref).abs() <= lim).all())
+    # a pair of weights p, 1 - p in the type: their difference off by more than the bound
+    p = torch.rand(4000, dtype=torch.float64, generator=torch.Generator().manual_seed(1))
+    d, r = p.to(dtype).double() - (1 - p).to(dtype).double(), 2 * p - 1
+    assert bool(((d - r).abs() > u * r.abs() + 2.0 ** -13 + u * u + 1e-6).any())
