@@ -404,7 +404,11 @@ typedef struct {
   const int32_t* kv_len;             /* [B] on the device, or NULL */
   int32_t window;                    /* 0: every earlier key */
   float scale;                       /* positive, finite */
+  uint32_t flags;                    /* OSSM_ATTN_NO_CAPTURE or 0 */
 } ossm_attn_args;
+/* The workspace is for calls that run: OSSM_EWORKSPACE if the stream's calls
+ * are being recorded into a graph. */
+#define OSSM_ATTN_NO_CAPTURE 1u
 
 /* Bytes of device workspace, the same for all valid arguments on a device (0
  * for invalid ones).  Its first OSSM_ATTN_WS_ZERO bytes, a header that

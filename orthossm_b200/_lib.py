@@ -14,6 +14,7 @@ from . import build as _build
 OSSM_OK, OSSM_EINVAL, OSSM_ELAUNCH, OSSM_ETIMEOUT, OSSM_ECOMM, OSSM_EWORKSPACE = range(6)
 OSSM_F32, OSSM_BF16, OSSM_F16 = 0, 1, 2
 OSSM_ATTN_WS_ZERO = 16384
+OSSM_ATTN_NO_CAPTURE = 1
 OSSM_EVAL_CLENSHAW, OSSM_EVAL_LUT, OSSM_EVAL_CLENSHAW_DEG4 = 0, 1, 2
 OSSM_F_FASTPATH = 1 << 2
 OSSM_F_PRECISE = 1 << 3
@@ -106,6 +107,7 @@ class AttnArgs(C.Structure):
         ("q_stride_t", _i64), ("q_stride_h", _i64), ("k_stride_t", _i64), ("k_stride_h", _i64),
         ("v_stride_t", _i64), ("v_stride_h", _i64), ("out_stride_t", _i64), ("out_stride_h", _i64),
         ("cu_q", _vp), ("cu_k", _vp), ("kv_len", _vp), ("window", _i32), ("scale", _f32),
+        ("flags", C.c_uint32),
     ]
 
 

@@ -27,6 +27,7 @@ bool valid(const ossm_attn_args* a) {
       a->total_q * a->H > 0x7fffffffLL)
     return false;
   if (a->dtype != OSSM_BF16 && a->dtype != OSSM_F16) return false;
+  if (a->flags & ~OSSM_ATTN_NO_CAPTURE) return false;
   if (a->window < 0 || !(a->scale > 0.f) || !std::isfinite(a->scale * 1.5f) || !a->cu_q || !a->cu_k) return false;
   if (a->total_q == 0) return true;
   if (!row_ok(a->q, a->q_stride_t, a->q_stride_h, a->total_q, a->H) ||
@@ -78,6 +79,12 @@ extern "C" int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size
   if (!attn::valid(a)) return OSSM_EINVAL;
   if (!workspace || workspace_bytes < ws_bytes() || (uintptr_t)workspace % 256) return OSSM_EWORKSPACE;
   if (a->total_q == 0) return OSSM_OK;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a->flags & OSSM_ATTN_NO_CAPTURE) {
+    cudaStreamCaptureStatus on = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &on) != cudaSuccess) return OSSM_ELAUNCH;
+    if (on != cudaStreamCaptureStatusNone) return OSSM_EWORKSPACE;
+  }
   char* w = static_cast<char*>(workspace);
   const attn::Params p{a->B, a->H, a->H_kv, a->head_dim, (int)a->total_q, (int)a->total_k, a->q, a->k, a->v, a->out,
                        a->q_stride_t, a->q_stride_h, a->k_stride_t, a->k_stride_h, a->v_stride_t, a->v_stride_h,
@@ -86,7 +93,6 @@ extern "C" int ossm_attention_fwd(const ossm_attn_args* a, void* workspace, size
                        a->scale * 1.4426950408889634f, reinterpret_cast<WsHeader*>(w),
                        reinterpret_cast<uint32_t*>(w + sizeof(WsHeader)),
                        reinterpret_cast<float*>(w + sizeof(WsHeader) + attn::kCounters * sizeof(uint32_t))};
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // Rows that share a key head.  Up to 16, one item of the token kernel holds
   // them and K and V are read once (8 streams of 2000 keys, 8/8 heads of 128,
   // 16 new tokens: 23 us, 28 us on the prompt kernel; 32 of 8192, 32/8 of 128,

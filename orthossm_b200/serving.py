@@ -24,7 +24,6 @@ _DT_SAMPLE = {torch.float32: L.OSSM_F32, torch.bfloat16: L.OSSM_BF16, torch.floa
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a Stream object (2 us)
-_capturing = torch._C._cuda_isCurrentStreamCapturing
 # (device index, stream) -> (workspace address, bytes) of the tensors in _WS_ATTN: one size fits all
 # arguments, so none is ever replaced
 _ATTN_WS: dict = {}
@@ -153,7 +152,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     a = L.AttnArgs(B, H, Hkv, hd, Tq, Tk, min(int(max_seqlen_q), 0x7fffffff), dt, qp, kp, vp, out.data_ptr(), qt, qh,
                    kt, kh, vt, vh, ot, oh, cu_seqlens_q.data_ptr(), cu_k.data_ptr(),
                    None if kv_lengths is None else kv_lengths.data_ptr(),
-                   0 if window is None else min(int(window), 0x7fffffff), scale_)
+                   0 if window is None else min(int(window), 0x7fffffff), scale_, L.OSSM_ATTN_NO_CAPTURE)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             _attention(a, dev)
@@ -174,18 +173,20 @@ def _attention(a, dev):
     lib = L.lib()
     stream = _raw_stream(dev)
     ref = L.C.byref(a)
-    capturing = _capturing()
-    ws = None if capturing else _ATTN_WS.get((dev, stream))
-    if ws is None:
+    ws = _ATTN_WS.get((dev, stream))
+    status = L.OSSM_EWORKSPACE if ws is None else lib.ossm_attention_fwd(ref, ws[0], ws[1], stream)
+    if status == L.OSSM_EWORKSPACE:  # the first call on this stream, or one that is captured
         nbytes = lib.ossm_attn_workspace_bytes(ref)
         if nbytes == 0:
             L.check(L.OSSM_EINVAL, "packed_attention (argument check)")
         device = torch.device("cuda", dev)
+        capturing = torch.cuda.is_current_stream_capturing()
         t = _attn_workspace(device, torch.cuda.current_stream(device), nbytes, capturing)
-        ws = t.data_ptr(), t.numel()
-        if not capturing:
-            _ATTN_WS[dev, stream] = ws
-    status = lib.ossm_attention_fwd(ref, ws[0], ws[1], stream)
+        if capturing:
+            a.flags = 0
+        else:
+            _ATTN_WS[dev, stream] = t.data_ptr(), t.numel()
+        status = lib.ossm_attention_fwd(ref, t.data_ptr(), t.numel(), stream)
     if status != L.OSSM_OK:
         L.check(status, "packed_attention")
 

@@ -220,3 +220,11 @@ def test_sampling_limits():
                 dict(out=4), dict(dtype=7), dict(top_p=-0.5), dict(min_p=float("nan")), dict(top_k=-1)):
         assert f(**bad) == L.OSSM_EINVAL, bad
     assert f(B=0) == L.OSSM_OK
+
+
+def test_attention_flags():
+    lib = L.lib()
+    src = open(os.path.join(ROOT, "include", "orthossm_b200.h")).read()
+    assert int(re.search(r"#define OSSM_ATTN_NO_CAPTURE (\d+)u", src).group(1)) == L.OSSM_ATTN_NO_CAPTURE
+    assert lib.ossm_attn_workspace_bytes(C.byref(_attn(flags=1))) > 0
+    assert lib.ossm_attn_workspace_bytes(C.byref(_attn(flags=2))) == 0
