@@ -589,9 +589,8 @@ OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, const Masses& ms, floa
 // by the bits set: code for each of the 32 logits of a thread ran in every warp
 // that had one candidate (128 rows of 131072, 4000 candidates each: 43 us, so 37).
 // With `sum` it also returns the mass that this thread has seen of the share.
-template <typename T>
-OSSM_DEV u64 collect(const T* row, int V, int rank, int nrank, float low, bool sum, const Masses& ms, int* count,
-                     u64* list) {
+template <bool sum, typename T>
+OSSM_DEV u64 collect(const T* row, int V, int rank, int nrank, float low, const Masses& ms, int* count, u64* list) {
   constexpr int N = Vec<T>::n, U = 4;
   const Share<T> own(row, V, rank, nrank);
   const int lane = threadIdx.x & 31;
@@ -901,8 +900,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   const float low = bound ? fmaxf(logit_of((u64)bound << 32), kLowest) : kLowest;
   // next to an infinite logit nothing else has weight; the sum is taken over the candidates then
   const bool sum = need_z && m < INFINITY;
-  u64 whole = collect(lg, p.V, rank, nrank, low, sum, ms, &first->count, first_list);
-  if (sum) {
+  u64 whole;
+  if (!sum) {
+    collect<false>(lg, p.V, rank, nrank, low, ms, &first->count, first_list);
+  } else {
+    whole = collect<true>(lg, p.V, rank, nrank, low, ms, &first->count, first_list);
 #pragma unroll
     for (int w = 16; w; w >>= 1) whole += __shfl_xor_sync(~0u, whole, w);
     if ((tid & 31) == 0) add64(&first->whole, whole);
