@@ -317,8 +317,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::kCtas) attn_token_kernel(c
         mma16816<T>(s[0], qf[ks], f[0], f[1]);
         mma16816<T>(s[1], qf[ks], f[2], f[3]);
       }
-      // some row does not see the whole tile
-      const bool part = key0 + kWK - 1 > i_first + off || (p.window && key0 <= i_last + off - p.window);
+      // some row does not see the whole tile, or it reaches past the piece
+      const bool part = key0 + kWK - 1 > i_first + off || key0 + kWK > kend ||
+                        (p.window && key0 <= i_last + off - p.window);
       uint32_t seen = 0xffu;  // bit 4 h + 2 nb + e: row r4 + 8 h, key 8 nb + 2 c4 + e
       if (part) {
         seen = 0;

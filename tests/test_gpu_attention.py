@@ -153,6 +153,19 @@ def test_hidden_values_of_grouped_heads(G, hd, nq, window, most, what):
             assert kk is kj or not bool(torch.isfinite(out[seen]).any()), j
 
 
+@pytest.mark.parametrize("G,hd", [(1, 64), (3, 128), (8, 64)])
+@pytest.mark.parametrize("nq,nk,window", [(700, 700, 100), (700, 1200, 33), (700, 732, None), (333, 5000, 900)])
+def test_many_queries_in_the_form_for_few(nq, nk, window, G, hd):
+    """max_seqlen_q far too small: blocks whose windows begin and end anywhere
+    within the pieces that their keys are cut into."""
+    dtype = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(nk)
+    q = torch.randn(nq, G, hd, device="cuda", generator=g).to(dtype)
+    k, v = (torch.randn(nk, 1, hd, device="cuda", generator=g).to(dtype) for _ in range(2))
+    cu_q, cu_k = cum([nq]), cum([nk])
+    check(O.packed_attention(q, k, v, cu_q, cu_k, max_seqlen_q=1, window=window), q, k, v, cu_q, cu_k, window=window)
+
+
 @pytest.mark.parametrize("nq,nk", [(1, 300), (200, 300)])
 def test_layouts(nq, nk):
     """Head-major tensors, odd strides (copied), a shared head of stride zero, a given output with gaps."""
