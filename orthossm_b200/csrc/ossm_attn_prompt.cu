@@ -25,6 +25,12 @@
 // into registers at once and frees the buffer, and the next ones are formed
 // while it computes.
 //
+// The weights enter the product rounded to the inputs' 16 bits, as the tensor
+// core takes them (their sum is of the fp32 values): outputs are 1.2 to 1.4 times
+// as far from float64 as with fp32 weights (a window of 512, bf16: 2.2e-3 and
+// 1.6e-3 of their norm; 16384 causal, fp16: 2.4e-4 and 1.9e-4).  As two 16-bit
+// parts they would take the product with V twice, on the pipe that bounds it.
+//
 // The maximum that the exponents are taken against follows the true one only
 // when a row has grown by more than 2^8 since: the weights then stay below
 // 2^8 and the accumulator is rescaled in a few tiles of a row instead of all.
@@ -39,12 +45,15 @@
 // What bounds it: a step of an item (two tiles, 128 keys) is 1024 (64 channels)
 // or 2048 cycles (128) of the tensor core and 2048 of the special function unit
 // (16 exponentials a clock and SM); of the softmax's other work a part overlaps
-// with the other tile's exponentials.  Measured: 16384 causal, fp16, 16 heads
-// of 128: 886 us, 1242 TFLOP/s (0.76 of measured cuBLAS); 8 heads of 64: 375 us;
-// 2 x 16384 with a window of 512, 8 heads of 64: 89 us; 3 x 4096, 32/8 heads of
-// 128: 351 us.  Tried and slower: part of the exponentials as a polynomial on
-// the FMA pipe (1 to 3 pairs of 8: +3 to +11 %), the tiles taking turns at them
-// (+3 to +13 %), a row on two threads (16 softmax warps: +25 % at 128 channels).
+// with the other tile's exponentials.  Measured in bursts of 10 calls: 16384
+// causal, fp16, 16 heads of 128: 910 us, 1209 TFLOP/s (0.74 of measured cuBLAS;
+// 886 us on another GPU; called for longer, at the power cap, 1056 us, 1041
+// TFLOP/s, 0.76 of cuBLAS under it); 8 heads of 64: 376 us; 2 x 16384 with a
+// window of 512, 8 heads of 64: 88 us; 3 x 4096, 32/8 heads of 128: 365 us.  64
+// bytes a thread are spilled.  Tried and slower: part of the exponentials as a
+// polynomial on the FMA pipe (1 to 3 pairs of 8: +3 to +11 %), the tiles taking
+// turns at them (+3 to +13 %), a row on two threads (16 softmax warps: +25 % at
+// 128 channels).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

@@ -15,10 +15,11 @@
 // The weights enter the product with V as a sum of two 16-bit terms, so that
 // their rounding does not add to the output's; the reads hide that product.
 //
-// Measured: 64 streams of up to 8192 keys, 32/8 heads of 128: 188 us, 6.4 TB/s
-// (0.98 of measured copy bandwidth); one stream of 1048576 keys, 8 heads of 64:
-// 350 us, 6.1 TB/s; 32 streams with a window of 512: 13.4 us (5.1 us of reads:
-// bound by the launch, the schedule and one item's chain of loads and merge).
+// Measured as calls among others: 64 streams of up to 8192 keys, 32/8 heads of
+// 128: 189 us, 6.4 TB/s (0.98 of measured copy bandwidth); one stream of 1048576
+// keys, 8 heads of 64: 359 to 378 us, 6.0 to 5.7 TB/s on different GPUs; 32
+// streams with a window of 512: 14.4 us (5.1 us of reads: bound by the launch, the
+// schedule and one item's chain of loads and merge).
 #include <algorithm>
 
 #include "ossm_attn.cuh"

@@ -17,11 +17,14 @@
 // sums of one function of the logit: they do not depend on the order of the
 // additions, nor on how many CTAs a row gets.  (The fp32 sum of the first pass
 // gives the bound and the guess alone.)
-// Measured: 1 x 32000 bf16, top-k 50 and top-p 0.95: 10.8 us; 128 x 131072 bf16,
-// top-k 50: 16 us (5.1 us of reads), min-p 0.01: 18 us, top-p 0.72 (4000 stay):
-// 37 us, top-p 0.92 (18000 stay): 59 us.  What bounds it there: one CTA an SM
-// works through steps that wait for one another; of 37 us, 8 are the first
-// pass (5 of reads), 5 the sample, 9 the collection, 7 the prefix's end.
+// Measured back to back, replayed from a graph (a call among others takes 1 to 2
+// us more): 1 x 32000 bf16, top-k 50 and top-p 0.95: 11.2 us; 128 x 131072 bf16,
+// top-k 50: 16.5 us (5.1 us of reads), min-p 0.01: 18.7 us, top-p 0.72 (4000
+// stay): 42 us, top-p 0.92 (18000 stay): 63 us.  What bounds it there: one CTA an
+// SM works through steps that wait for one another; of 49 us of a row whose list
+// is 12000 long, 7.5 are the first pass (5 of reads), 5 the sample, 16 the
+// collection with the row's mass (6 of them the mass), 11 the prefix's end, 6 the
+// noise.  64 registers a thread, with 32 (fp32) to 52 bytes spilled.
 //
 // Without filters the score of every candidate is needed: one pass over logits
 // and noise.  The logarithm is first taken in its fast form, and exactly only
@@ -587,7 +590,7 @@ OSSM_DEV u64 select_row(const Row& r, const T* lg, int V, const Masses& ms, floa
 // pass the list's end, which is then found in another way.  A warp's four
 // vectors take their places with one addition, and the candidates are walked
 // by the bits set: code for each of the 32 logits of a thread ran in every warp
-// that had one candidate (128 rows of 131072, 4000 candidates each: 43 us, so 37).
+// that had one candidate (128 rows of 131072, 4000 candidates each, before the masses were added up here: 43 us, so 37).
 // With `sum` it also returns the mass that this thread has seen of the share.
 template <bool sum, typename T>
 OSSM_DEV u64 collect(const T* row, int V, int rank, int nrank, float low, const Masses& ms, int* count, u64* list) {
@@ -753,9 +756,10 @@ OSSM_DEV void open_row(const T* lg, const float* nz, int V, float inv_t, int ran
 }
 
 // Every row without filters (known on the host).  Two CTAs of 512 threads an SM
-// cover one another's loads and tails: 256 rows of 32000 fp32, 11.9 us (10.0 us
-// of reads; 15.1 us with one CTA of 1024), 256 of 131072 bf16, 35.6 us (30.8
-// of reads).  At 40 registers a thread the loads ahead spill (17 and 38 us).
+// cover one another's loads and tails: 256 rows of 32000 fp32, 11.6 us back to
+// back (10.0 us of reads; 15.1 us with one CTA of 1024; 14.4 us as a call among
+// others), 256 of 131072 bf16, 33.5 us (30.8 of reads).  At 40 registers a
+// thread the loads ahead spill (17 and 38 us).
 template <typename T>
 __global__ void __launch_bounds__(kOpen, 2) open_kernel(const Params p) {
   __shared__ Best bests[kOpen / 32];
@@ -877,11 +881,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
   // That bound by mass leaves many more than the prefix in wide rows (30000 of
   // 131072 where it holds 4000).  A guess leaves fewer; whether the prefix ends
   // above it shows in the mass collected.  top-p 0.9, with and without: 1 x 32000
-  // (4 CTAs) 20 and 24 us, 64 x 50257 27 and 36 us, 128 x 32000 23 and 27 us.
+  // (4 CTAs) 21 and 26 us, 64 x 50257 28 and 38 us, 128 x 32000 24 and 28 us.
   // Where min_p's bound is the higher one by far it leaves few anyhow.  Up to a
   // factor of e^2: 128 rows with top-p and a small min-p of their own, V = 131072,
-  // 56 us, only where it is the lower one 79 us (V = 50257: 31 and 28 us); up to
-  // e^4, where prefixes end below it and the row is gone over, 40 us (50257).
+  // 52 to 63 us over three inputs, only where it is the lower one 52 to 100 us (V =
+  // 50257: 27 and 30 us); up to e^4, where prefixes end below it and the row is
+  // gone over, 43 us (50257).
   guessed = guessed && lb > -INFINITY && lb < m;
   if (guessed) {
     float g = guess_bound(lg, p.V, rank, nrank, m, lb, c, (1.f - r.top_p) * z / (float)nrank, room);

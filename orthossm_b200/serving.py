@@ -216,7 +216,8 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor] = None, *,
     ``logit / temperature - log(noise)``, ties to the lowest index: with
     ``noise`` [B, V] fp32 from the standard exponential distribution
     (``torch.empty(B, V).exponential_()``) it is drawn from the softmax over
-    the candidates, and the same noise gives the same token.
+    the candidates, and the same row and noise give the same token, alone or
+    in any batch.
 
     ``noise=None`` or a temperature of 0 takes the largest logit.  Each
     setting is a number or a tensor [B] on the device (float32; top_k int32),
