@@ -47,8 +47,8 @@
 // (16 exponentials a clock and SM); of the softmax's other work a part overlaps
 // with the other tile's exponentials.  Measured in bursts of 10 calls: 16384
 // causal, fp16, 16 heads of 128: 910 us, 1209 TFLOP/s (0.74 of measured cuBLAS;
-// 886 us on another GPU; called for longer, at the power cap, 1056 us, 1041
-// TFLOP/s, 0.76 of cuBLAS under it); 8 heads of 64: 376 us; 2 x 16384 with a
+// 886 us on another GPU; called for longer, at the power cap, 1026 to 1070 us,
+// 0.78 to 0.75 of cuBLAS under it); 8 heads of 64: 376 us; 2 x 16384 with a
 // window of 512, 8 heads of 64: 88 us; 3 x 4096, 32/8 heads of 128: 365 us.  64
 // bytes a thread are spilled.  Tried and slower: part of the exponentials as a
 // polynomial on the FMA pipe (1 to 3 pairs of 8: +3 to +11 %), the tiles taking
