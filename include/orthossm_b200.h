@@ -47,7 +47,7 @@ enum ossm_status {
   OSSM_EWORKSPACE = 5 /* workspace missing or too small */
 };
 
-enum ossm_dtype { OSSM_F32 = 0, OSSM_BF16 = 1, OSSM_F16 = 2 /* attention and sampling only */ };
+enum ossm_dtype { OSSM_F32 = 0, OSSM_BF16 = 1, OSSM_F16 = 2 /* serving and training operators only */ };
 
 /* Chebyshev evaluation mode (low 2 bits of flags). */
 #define OSSM_EVAL_CLENSHAW 0u      /* exact degree-K Clenshaw (sdpc_kernel.py:1147-1156) */
@@ -453,6 +453,125 @@ typedef struct {
 
 int ossm_sample_tokens(const ossm_sample_args* a, ossm_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Training: the language-model loss from hidden states, without the logits.
+ *
+ *   z_tv = hidden_t . weight_v,  lse_t = log sum_v exp z_tv
+ *   loss_t = lse_t - z_t,target + z_loss lse_t^2
+ * A token whose target is ignore_index has no loss (0) and no gradient, and no
+ * part in any product, whatever its state holds.  Another target outside 0 ..
+ * vocab - 1 makes its loss, and the gradients it reaches, NaN.  reduction: the losses [tokens], their sum, or
+ * their mean over the tokens that have a target (0 if none has).
+ * Backward from grad_loss ([tokens], or one value for a sum or mean):
+ *   dz_tv = g_t ((1 + 2 z_loss lse_t) exp(z_tv - lse_t) - [v = target])
+ *   grad_hidden = dz weight,  grad_weight = dz^T hidden
+ * with the logits computed again, a piece of the vocabulary at a time; dz is
+ * rounded to the inputs' type, as the tensor core takes it.  Sums are fp32 or
+ * wider and their order depends on the arguments alone.
+ * No counterpart in the reference, whose training script takes
+ * F.cross_entropy of whole logits (model.py:23-187 returns them).
+ * ------------------------------------------------------------------------ */
+enum ossm_loss_reduction { OSSM_LOSS_NONE = 0, OSSM_LOSS_MEAN = 1, OSSM_LOSS_SUM = 2 };
+typedef struct {
+  int64_t tokens;                    /* 1 to 2^27 */
+  int32_t dim, vocab;                /* dim a multiple of 8, at most 65536; vocab at most 2^27 */
+  int32_t dtype;                     /* OSSM_BF16 or OSSM_F16: hidden, weight, their gradients */
+  const void* hidden;                /* [tokens, dim], 16-byte aligned, unit channel stride */
+  int64_t hidden_stride;             /* row strides in elements, multiples of 8 */
+  const void* weight;                /* [vocab, dim], the same */
+  int64_t weight_stride;
+  const int64_t* targets;            /* [tokens] on the device */
+  int64_t ignore_index;
+  float z_loss;                      /* not negative */
+  int32_t reduction;                 /* enum ossm_loss_reduction */
+  float* loss;                       /* forward: [tokens], or one value */
+  float* lse;                        /* [tokens]: written forward (0 where ignored), read backward */
+  const float* grad_loss;            /* backward: [tokens], or one value */
+  void* grad_hidden;                 /* [tokens, dim] contiguous, 16-byte aligned, or NULL */
+  void* grad_weight;                 /* [vocab, dim] contiguous, 16-byte aligned, or NULL */
+  uint32_t* status;                  /* a device word that a wait that ran out sets to OSSM_ETIMEOUT, or NULL */
+} ossm_lce_args;
+
+/* Bytes of device workspace (0 for invalid arguments), 256-byte aligned, with
+ * nothing to be kept or zeroed between calls. */
+size_t ossm_lce_workspace_bytes(const ossm_lce_args* a, int backward);
+int ossm_lce_fwd(const ossm_lce_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream);
+int ossm_lce_bwd(const ossm_lce_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Training: token embeddings, and their gradient by sorted tokens.
+ *   out_t = scale weight[ids_t], 0 where ids_t is no row of the weight
+ *   grad_weight_v = scale sum over t with ids_t = v of grad_out_t (0 if none)
+ * Sums are fp32, in an order that depends on the arguments alone.
+ * The reference's model looks its tokens up with torch.nn.Embedding
+ * (model.py:23-187).
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  int64_t tokens;                    /* below 2^31 */
+  int32_t dim, vocab;                /* dim at most 65536, vocab below 2^27 */
+  int32_t dtype;                     /* of all float tensors */
+  const int64_t* ids;                /* [tokens] on the device */
+  const void* weight;                /* [vocab, dim], unit channel stride */
+  int64_t weight_stride;
+  float scale;
+  void* out;                         /* [tokens, dim] contiguous */
+  const void* grad_out;              /* backward: [tokens, dim], unit channel stride */
+  int64_t grad_out_stride;
+  void* grad_weight;                 /* backward: [vocab, dim] contiguous */
+} ossm_embed_args;
+
+int ossm_embed_fwd(const ossm_embed_args* a, ossm_stream_t stream);
+size_t ossm_embed_workspace_bytes(const ossm_embed_args* a); /* of the backward; as for ossm_lce */
+int ossm_embed_bwd(const ossm_embed_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Training: a block's residual with the norms on its two sides.
+ *   n = post_norm(y),  r = x + scale gate n,  h = norm(r)
+ * rms: v w / sqrt(mean v^2 + eps) (+ b); layer: the same of v less its mean.
+ * gate: none, a value per channel [dim], per token [tokens], or of y's shape.
+ * y == NULL: r is x (not written), h its norm.  h is of the unrounded r.
+ * Statistics and sums are fp32, in an order that depends on the arguments
+ * alone.  Backward from grad_r and grad_h (either may be NULL: zeros).  It
+ * reads x and y where there is a gate or a post_norm, otherwise r alone (with
+ * x_stride; x itself where y was NULL).
+ * The reference composes nn.RMSNorm, a product and a sum
+ * (sdpc_engine.py:420-426).
+ * ------------------------------------------------------------------------ */
+enum ossm_norm_kind { OSSM_NORM_NONE = 0, OSSM_NORM_RMS = 1, OSSM_NORM_LAYER = 2 };
+enum ossm_gate_kind { OSSM_GATE_NONE = 0, OSSM_GATE_CHANNEL = 1, OSSM_GATE_TOKEN = 2, OSSM_GATE_FULL = 3 };
+typedef struct {
+  int64_t tokens;                    /* below 2^31 */
+  int32_t dim;                       /* at most 16384 */
+  int32_t stream_dtype, dtype;       /* of x, r and of y, h: the same, or fp32 and a 16-bit type */
+  const void* x;                     /* [tokens, dim], unit channel stride */
+  int64_t x_stride;                  /* row strides in elements */
+  const void* y;                     /* or NULL */
+  int64_t y_stride;
+  const void* gate;
+  int32_t gate_kind, gate_dtype;     /* enum ossm_gate_kind */
+  int64_t gate_stride;               /* of a gate of y's shape */
+  float scale;
+  int32_t norm, post_norm;           /* enum ossm_norm_kind; norm is not NONE */
+  float eps, post_eps;
+  const void *weight, *bias, *post_weight, *post_bias; /* [dim] or NULL (ones, zeros) */
+  int32_t weight_dtype, bias_dtype, post_weight_dtype, post_bias_dtype;
+  void* r;                           /* contiguous (forward output) */
+  void* h;
+  float* stats;                      /* [4][tokens], or [2][tokens] without post_norm: written forward (or NULL), read backward */
+  const void* grad_r;                /* backward: [tokens, dim], unit channel stride, x's type, or NULL */
+  int64_t grad_r_stride;
+  const void* grad_h;                /* the same of y's type */
+  int64_t grad_h_stride;
+  void* grad_x;                      /* contiguous, or NULL */
+  void* grad_y;
+  void* grad_gate;                   /* of the gate's shape and type, or NULL */
+  void *grad_weight, *grad_bias, *grad_post_weight, *grad_post_bias; /* of the parameters' types, or NULL */
+} ossm_norm_args;
+
+int ossm_residual_norm_fwd(const ossm_norm_args* a, ossm_stream_t stream);
+size_t ossm_norm_workspace_bytes(const ossm_norm_args* a); /* of the backward; as for ossm_lce */
+int ossm_residual_norm_bwd(const ossm_norm_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream);
+
 /* The capture that a stream's calls are recorded into (unique in the process),
  * 0 if they run: for callers that keep a workspace for each graph. */
 int ossm_stream_capture_id(ossm_stream_t stream, uint64_t* id);
@@ -468,6 +587,9 @@ size_t ossm_sizeof_bwd_args(void);
 size_t ossm_sizeof_ttt_run_args(void);
 size_t ossm_sizeof_attn_args(void);
 size_t ossm_sizeof_sample_args(void);
+size_t ossm_sizeof_lce_args(void);
+size_t ossm_sizeof_embed_args(void);
+size_t ossm_sizeof_norm_args(void);
 
 #ifdef __cplusplus
 }

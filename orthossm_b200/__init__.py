@@ -14,5 +14,6 @@ from .sdpc_kernel import (  # noqa: F401
 
 from .serving import packed_attention, sample_tokens  # noqa: F401
 from .state import ChebyStreamState, StreamingChebyRKV  # noqa: F401
+from .training import embed_tokens, linear_cross_entropy, residual_norm  # noqa: F401
 
 __version__ = "0.1.0"

@@ -15,6 +15,9 @@ OSSM_OK, OSSM_EINVAL, OSSM_ELAUNCH, OSSM_ETIMEOUT, OSSM_ECOMM, OSSM_EWORKSPACE =
 OSSM_F32, OSSM_BF16, OSSM_F16 = 0, 1, 2
 OSSM_ATTN_WS_ZERO = 16384
 OSSM_ATTN_NO_CAPTURE = 1
+OSSM_LOSS_NONE, OSSM_LOSS_MEAN, OSSM_LOSS_SUM = range(3)
+OSSM_NORM_NONE, OSSM_NORM_RMS, OSSM_NORM_LAYER = range(3)
+OSSM_GATE_NONE, OSSM_GATE_CHANNEL, OSSM_GATE_TOKEN, OSSM_GATE_FULL = range(4)
 OSSM_EVAL_CLENSHAW, OSSM_EVAL_LUT, OSSM_EVAL_CLENSHAW_DEG4 = 0, 1, 2
 OSSM_F_FASTPATH = 1 << 2
 OSSM_F_PRECISE = 1 << 3
@@ -34,6 +37,9 @@ EXPORTED = (
     "ossm_cheby_ema_bwd", "ossm_ttt_run_workspace_bytes", "ossm_ttt_wpred_run", "ossm_sizeof_ttt_run_args",
     "ossm_attn_workspace_bytes", "ossm_attention_fwd", "ossm_sizeof_attn_args",
     "ossm_sample_tokens", "ossm_sizeof_sample_args", "ossm_stream_capture_id",
+    "ossm_lce_workspace_bytes", "ossm_lce_fwd", "ossm_lce_bwd", "ossm_sizeof_lce_args",
+    "ossm_embed_fwd", "ossm_embed_workspace_bytes", "ossm_embed_bwd", "ossm_sizeof_embed_args",
+    "ossm_residual_norm_fwd", "ossm_norm_workspace_bytes", "ossm_residual_norm_bwd", "ossm_sizeof_norm_args",
 )
 
 _vp = C.c_void_p
@@ -120,6 +126,36 @@ class SampleArgs(C.Structure):
     ]
 
 
+class LceArgs(C.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("dim", _i32), ("vocab", _i32), ("dtype", _i32), ("hidden", _vp), ("hidden_stride", _i64),
+        ("weight", _vp), ("weight_stride", _i64), ("targets", _vp), ("ignore_index", _i64), ("z_loss", _f32),
+        ("reduction", _i32), ("loss", _vp), ("lse", _vp), ("grad_loss", _vp), ("grad_hidden", _vp),
+        ("grad_weight", _vp), ("status", _vp),
+    ]
+
+
+class EmbedArgs(C.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("dim", _i32), ("vocab", _i32), ("dtype", _i32), ("ids", _vp), ("weight", _vp),
+        ("weight_stride", _i64), ("scale", _f32), ("out", _vp), ("grad_out", _vp), ("grad_out_stride", _i64),
+        ("grad_weight", _vp),
+    ]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("dim", _i32), ("stream_dtype", _i32), ("dtype", _i32), ("x", _vp), ("x_stride", _i64),
+        ("y", _vp), ("y_stride", _i64), ("gate", _vp), ("gate_kind", _i32), ("gate_dtype", _i32),
+        ("gate_stride", _i64), ("scale", _f32), ("norm", _i32), ("post_norm", _i32), ("eps", _f32),
+        ("post_eps", _f32), ("weight", _vp), ("bias", _vp), ("post_weight", _vp), ("post_bias", _vp),
+        ("weight_dtype", _i32), ("bias_dtype", _i32), ("post_weight_dtype", _i32), ("post_bias_dtype", _i32),
+        ("r", _vp), ("h", _vp), ("stats", _vp), ("grad_r", _vp), ("grad_r_stride", _i64), ("grad_h", _vp),
+        ("grad_h_stride", _i64), ("grad_x", _vp), ("grad_y", _vp), ("grad_gate", _vp), ("grad_weight", _vp),
+        ("grad_bias", _vp), ("grad_post_weight", _vp), ("grad_post_bias", _vp),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -177,6 +213,20 @@ def _declare(lib):
     lib.ossm_sample_tokens.argtypes = [C.POINTER(SampleArgs), _vp]
     lib.ossm_stream_capture_id.restype = C.c_int
     lib.ossm_stream_capture_id.argtypes = [_vp, C.POINTER(C.c_uint64)]
+    for name, args in (("lce", LceArgs), ("embed", EmbedArgs), ("norm", NormArgs)):
+        size = getattr(lib, f"ossm_sizeof_{name}_args")
+        size.restype = C.c_size_t
+        if size() != C.sizeof(args):
+            raise RuntimeError("orthossm_b200: ctypes struct layout does not match the C ABI")
+        getattr(lib, f"ossm_{name}_workspace_bytes").restype = C.c_size_t
+        getattr(lib, f"ossm_{name}_workspace_bytes").argtypes = \
+            [C.POINTER(args), C.c_int] if name == "lce" else [C.POINTER(args)]
+    for name, args, ws in (("lce_fwd", LceArgs, True), ("lce_bwd", LceArgs, True), ("embed_fwd", EmbedArgs, False),
+                           ("embed_bwd", EmbedArgs, True), ("residual_norm_fwd", NormArgs, False),
+                           ("residual_norm_bwd", NormArgs, True)):
+        f = getattr(lib, "ossm_" + name)
+        f.restype = C.c_int
+        f.argtypes = [C.POINTER(args), _vp, C.c_size_t, _vp] if ws else [C.POINTER(args), _vp]
     lib.ossm_sizeof_attn_args.restype = C.c_size_t
     lib.ossm_sizeof_sample_args.restype = C.c_size_t
     if lib.ossm_sizeof_attn_args() != C.sizeof(AttnArgs) or lib.ossm_sizeof_sample_args() != C.sizeof(SampleArgs):

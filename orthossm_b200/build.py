@@ -18,9 +18,9 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIBDIR = os.path.join(PKG, "_lib")
 LIBNAME = "liborthossm_b200.so"
-SOURCES = ["ossm_attn.cu", "ossm_attn_prompt.cu", "ossm_attn_token.cu", "ossm_capi.cu", "ossm_forward.cu",
-           "ossm_forward_3p.cu", "ossm_forward_grp.cu", "ossm_host.cu", "ossm_lion.cu", "ossm_noalloc.cu",
-           "ossm_reverse.cu", "ossm_sample.cu", "ossm_ttt.cu"]
+SOURCES = ["ossm_attn.cu", "ossm_attn_prompt.cu", "ossm_attn_token.cu", "ossm_capi.cu", "ossm_embed.cu",
+           "ossm_forward.cu", "ossm_forward_3p.cu", "ossm_forward_grp.cu", "ossm_host.cu", "ossm_lce.cu",
+           "ossm_lion.cu", "ossm_noalloc.cu", "ossm_norm.cu", "ossm_reverse.cu", "ossm_sample.cu", "ossm_ttt.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

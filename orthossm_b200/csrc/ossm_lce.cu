@@ -1,0 +1,876 @@
+// The language-model loss from hidden states: softmax cross entropy over the
+// vocabulary of the logits z = H W^T, and its gradients, without keeping z.
+//
+//   lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_t,target + zl lse_t^2
+//   dz_tv = g_t ((1 + 2 zl lse_t) exp(z_tv - lse_t) - [v = target]),
+//   dH = dZ W,  dW = dZ^T H
+//
+// Forward: rows (which tokens have a target, their states side by side), stats
+// (logits tile by tile on the tensor core, a running maximum and sum a row),
+// finish (joins the sums, the losses and their sum).  Backward: rows, then for
+// each piece of the vocabulary gradz (the logits again, dz rounded to the
+// inputs' type into the workspace) and prod (dW of the piece, dH).
+//
+// Tokens without a target have no part in any product: their states are not
+// read, so NaN there harms nothing, and they cost nothing.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "ossm_attn.cuh"
+#include "ossm_sm100.cuh"
+
+namespace ossm {
+int device_sms();
+namespace fast {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
+}
+namespace lce {
+
+using namespace sm100;
+using attn::allow_smem;
+using attn::ex2;
+using attn::pack2;
+typedef long long i64;
+
+constexpr int kM = 128, kN = 256, kK = 64;  // a tile, and the depth of one load
+constexpr int kStages = 4;
+constexpr int kThreads = 320;               // 8 warps read tensor memory, one loads, one issues products
+constexpr int kABytes = kM * kK * 2, kBBytes = kN * kK * 2, kStage = kABytes + kBBytes;
+constexpr int kOut = 8 * 32 * 128;          // a [32 rows x 64 columns] box a warp
+constexpr size_t kSmem = kStages * (size_t)kStage + kOut + 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRowThreads = 256;
+constexpr int kMaxBlocks = 1024;
+
+struct Head {      // of the workspace
+  int n;           // tokens that have a target
+  float unit;      // backward: what dz in the workspace is in units of
+  uint32_t count;  // finished blocks
+};
+// dz is written in units that bring the largest factor of a row to kDzScale:
+// probabilities down to 2^-28 stay out of fp16's subnormals, whatever the loss
+// was multiplied by.  (bf16 has the exponents, but one rule does.)
+constexpr float kDzScale = 16384.f;
+
+struct Params {
+  i64 T;
+  int Tpad, d, V;
+  const void* hidden;
+  i64 hst;
+  const int64_t* targets;
+  i64 ignore;
+  float zl;
+  int reduction;
+  float *loss, *lse;
+  const float* g;
+  void *dh, *dw;
+  Head* head;
+  int *rows, *tgt;   // [n] token and target of each row
+  float *lse2, *fa, *fb;  // [n] lse log2(e), factors of the softmax and of the target
+  void* hc;          // [Tpad, d] states of the rows side by side, where tokens were left out
+  float2* part;      // [Tpad, 2 * panels] maximum (base 2) and sum of a row over a panel's half columns
+  float* zt;         // [Tpad] the target's logit
+  double* sums;      // [kMaxBlocks]
+  float* dh32;       // [tiles] sums of dH over the pieces, in the order of tensor memory
+  int panels, pan;   // panels of `pan` tiles of columns
+  int v0, vp;        // the piece: columns v0 .. v0 + vp
+  int first, last;   // the piece is the first, the last
+  uint32_t* status;
+};
+
+// ---------------------------------------------------------------- waits
+OSSM_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+constexpr i64 kWaitCycles = 1LL << 31;  // about a second
+// True: it ran out.  The role then goes on without waiting (readers of tensor
+// memory) or ends; the others run out in turn.
+OSSM_DEV bool gave_up(uint64_t* bar, uint32_t parity, int* failed) {
+  if (mbar_test(bar, parity)) return false;
+  const i64 t0 = clock64();
+  while (!mbar_test(bar, parity))
+    if (clock64() - t0 > kWaitCycles) {
+      *failed = 1;
+      return true;
+    }
+  return false;
+}
+
+OSSM_DEV void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+OSSM_DEV void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+OSSM_DEV void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// Instruction descriptor: fp32 accumulator, 16-bit operands (0 = fp16, 1 =
+// bf16), bits 15 and 16: A, B are MN-major, N/8 from bit 17, M/16 from bit 24.
+__host__ __device__ constexpr uint32_t idesc(int fmt, int a_mn, int b_mn, int n) {
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
+}
+// Shared-memory descriptor, 128-byte swizzle.  K-major: groups of 8 rows 1024
+// bytes apart.  MN-major: groups of 8 steps of K 1024 bytes apart, the next 64
+// of M or N a box of 64 x 64 further.
+constexpr int kBox = 64 * 128;
+OSSM_DEV uint64_t sdesc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(kBox >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+OSSM_DEV void mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(ad), "l"(bd), "r"(id), "r"(acc)
+      : "memory");
+}
+OSSM_DEV void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+OSSM_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+OSSM_DEV void tmem_ld32_nowait(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+// Orders uses of v after the wait before it.
+OSSM_DEV void pin32(float* v) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+}
+
+// ---------------------------------------------------------------- what the tensor-core kernels share
+struct Shared {
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int failed, last_in;
+};
+
+// Barriers, tensor memory: all threads, before the roles part.
+OSSM_DEV void setup(Shared& s, int warp) {
+  if (threadIdx.x == 0) {
+    s.failed = 0;
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.acc_full[i], 1);
+      mbar_init(&s.acc_empty[i], 8);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(&s.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+}
+OSSM_DEV void teardown(Shared& s, int warp, uint32_t* status) {
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(s.tmem, 512);
+  }
+  if (threadIdx.x == 0 && s.failed && status) atomicExch(status, (uint32_t)OSSM_ETIMEOUT);
+}
+
+// The ring of loaded stages, on the loading side.
+struct Loader {
+  Shared& s;
+  uint8_t* ring;
+  uint32_t i;
+  OSSM_DEV uint8_t* next(uint32_t bytes, uint64_t*& bar) {  // NULL: give up
+    const uint32_t r = i % kStages;
+    if (i >= kStages && gave_up(&s.empty[r], ((i / kStages) & 1) ^ 1, &s.failed)) return nullptr;
+    ++i;
+    bar = &s.full[r];
+    mbar_expect_tx(bar, bytes);
+    return ring + r * kStage;
+  }
+  OSSM_DEV void drain() {  // no copy may still be landing when the CTA exits
+    for (uint32_t j = i > kStages ? i - kStages : 0; j < i; ++j) gave_up(&s.full[j % kStages], (j / kStages) & 1, &s.failed);
+  }
+};
+
+// One tile's products: `steps` stages into the accumulator at column `acc`.
+// a_step, b_step: bytes between the starts of two 16-deep products.
+struct Issuer {
+  Shared& s;
+  uint32_t ring, i, tiles;
+  OSSM_DEV bool tile(int steps, uint32_t id, uint32_t a_step, uint32_t b_step, bool leader) {
+    const uint32_t b = tiles & 1;
+    if (tiles >= 2 && __any_sync(~0u, gave_up(&s.acc_empty[b], ((tiles >> 1) & 1) ^ 1, &s.failed))) return false;
+    tc_fence_after();
+    for (int k = 0; k < steps; ++k, ++i) {
+      const uint32_t r = i % kStages;
+      if (__any_sync(~0u, gave_up(&s.full[r], (i / kStages) & 1, &s.failed))) return false;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t ad = sdesc(ring + r * kStage), bd = sdesc(ring + r * kStage + kABytes);
+#pragma unroll
+        for (int kk = 0; kk < kK / 16; ++kk)
+          mma(s.tmem + b * kN, ad + kk * (a_step >> 4), bd + kk * (b_step >> 4), id, k > 0 || kk > 0);
+        mma_commit(&s.empty[r]);
+      }
+      __syncwarp();
+    }
+    if (leader) mma_commit(&s.acc_full[b]);
+    __syncwarp();
+    ++tiles;
+    return true;
+  }
+};
+
+// ---------------------------------------------------------------- logits
+enum { STATS, GRADZ };
+
+// Items of the logits kernels: a block of 128 rows by a panel of columns.  Of
+// 16 blocks of rows all take a panel before the next one, so that the CTAs at
+// work read the same columns of W and a few blocks of rows, which L2 keeps.
+struct Walk {
+  int blocks, panels, items;
+  OSSM_DEV Walk(const Params& p) {
+    blocks = max(1, (p.head->n + kM - 1) / kM);
+    panels = p.panels;
+    items = blocks * panels;
+  }
+  OSSM_DEV void at(int it, int& block, int& panel) const {
+    const int g = it / (16 * panels), r = it - g * 16 * panels, rows = min(16, blocks - 16 * g);
+    panel = r / rows;
+    block = 16 * g + r % rows;
+  }
+};
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+    lce_logits_kernel(const __grid_constant__ CUtensorMap mH, const __grid_constant__ CUtensorMap mHc,
+                      const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mZ,
+                      const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ Shared s;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  setup(s, warp);
+  const int n = p.head->n;
+  const Walk walk(p);
+  const int ktiles = (p.d + kK - 1) / kK;
+  const int ntiles = (min(p.vp, p.V - p.v0) + kN - 1) / kN;  // of the piece
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const CUtensorMap* a = n == p.T ? &mH : &mHc;
+      Loader ld{s, smem, 0};
+      bool ok = true;
+      for (int it = blockIdx.x; it < walk.items && ok; it += gridDim.x) {
+        int block, panel;
+        walk.at(it, block, panel);
+        for (int nt = panel * p.pan; nt < min(ntiles, (panel + 1) * p.pan) && ok; ++nt)
+          for (int k = 0; k < ktiles; ++k) {
+            uint64_t* bar;
+            uint8_t* to = ld.next(kStage, bar);
+            if (!to) {
+              ok = false;
+              break;
+            }
+            tma_load_2d(to, a, bar, k * kK, block * kM);
+            tma_load_2d(to + kABytes, &mW, bar, k * kK, p.v0 + nt * kN);
+          }
+      }
+      if (!ok) ld.drain();
+    }
+  } else if (warp == 9) {
+    const bool leader = elect_one();
+    Issuer mm{s, smem_u32(smem), 0, 0};
+    constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, 0, 0, kN);
+    bool ok = true;
+    for (int it = blockIdx.x; it < walk.items && ok; it += gridDim.x) {
+      int block, panel;
+      walk.at(it, block, panel);
+      for (int nt = panel * p.pan; nt < min(ntiles, (panel + 1) * p.pan) && ok; ++nt)
+        ok = mm.tile(ktiles, id, 32, 32, leader);
+    }
+  } else {
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t tl = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
+    uint8_t* box = smem + kStages * kStage + warp * 4096;
+    uint32_t tiles = 0;
+    bool dead = false;
+    for (int it = blockIdx.x; it < walk.items; it += gridDim.x) {
+      int block, panel;
+      walk.at(it, block, panel);
+      const int r = block * kM + row;
+      const bool live = r < n;
+      const int tcol = live ? __ldg(p.tgt + r) - p.v0 : -1;
+      float ms = -INFINITY, l = 0.f;              // STATS
+      float lse2 = 0.f, fa = 0.f, fb = 0.f;       // GRADZ
+      if (MODE == GRADZ && live) lse2 = __ldg(p.lse2 + r), fa = __ldg(p.fa + r), fb = __ldg(p.fb + r);
+      for (int nt = panel * p.pan; nt < min(ntiles, (panel + 1) * p.pan); ++nt, ++tiles) {
+        const uint32_t b = tiles & 1;
+        if (!dead) dead = gave_up(&s.acc_full[b], (tiles >> 1) & 1, &s.failed);
+        __syncwarp();
+        tc_fence_after();
+        float x[128];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld32_nowait(tl + b * kN + 32 * i, x + 32 * i);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pin32(x + 32 * i);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+        const int c0 = nt * kN + half * 128;
+        const int cols = min(p.V - p.v0, p.vp) - c0;  // that exist
+        const int at = tcol - c0;                     // the target's place
+        const bool here = __any_sync(~0u, at >= 0 && at < 128);
+        if (MODE == STATS) {
+          if (cols < 128) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) x[i] = i < cols ? x[i] : -INFINITY;
+          }
+          if (here) {
+            float z = 0.f;
+#pragma unroll
+            for (int i = 0; i < 128; ++i) z = i == at ? x[i] : z;
+            if (at >= 0 && at < 128) p.zt[r] = z;
+          }
+          float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int i = 4; i < 128; i += 4) {
+            mx[0] = fmaxf(mx[0], x[i]), mx[1] = fmaxf(mx[1], x[i + 1]);
+            mx[2] = fmaxf(mx[2], x[i + 2]), mx[3] = fmaxf(mx[3], x[i + 3]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
+          if (top > ms + 8.f) {  // the reference follows the maximum in steps, so that few tiles rescale
+            l *= ex2(ms - top);
+            ms = top;
+          }
+          const float off = ms == -INFINITY ? 0.f : ms;
+          const float2 c2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-off, -off);
+          float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), c2, m2);
+            y = make_float2(ex2(y.x), ex2(y.y));
+            if (i & 1) s1 = attn::add2(s1, y); else s0 = attn::add2(s0, y);
+          }
+          s0 = attn::add2(s0, s1);
+          l += s0.x + s0.y;
+        } else {
+          const float2 c2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-lse2, -lse2);
+          const float2 a2 = make_float2(fa, fa);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 32 * h; i < 32 * h + 32; ++i) {
+              float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), c2, m2);
+              y = mul2(make_float2(ex2(y.x), ex2(y.y)), a2);
+              x[2 * i] = y.x, x[2 * i + 1] = y.y;
+            }
+            if (here) {
+#pragma unroll
+              for (int i = 64 * h; i < 64 * h + 64; ++i) x[i] = i == at ? x[i] - fb : x[i];
+            }
+            if (cols < 128 || !live) {
+#pragma unroll
+              for (int i = 64 * h; i < 64 * h + 64; ++i) x[i] = live && i < cols ? x[i] : 0.f;
+            }
+            if (lane == 0) bulk_wait_read0();
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float* y = x + 64 * h + 8 * i;
+              *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                  make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&mZ, box, c0 + 64 * h, block * kM + (warp & 3) * 32);
+              bulk_commit();
+            }
+          }
+        }
+      }
+      if (MODE == STATS && live) p.part[(i64)r * 2 * p.panels + 2 * panel + half] = make_float2(ms, l);
+    }
+    if (MODE == GRADZ && lane == 0) bulk_wait0();
+  }
+  teardown(s, warp, p.status);
+}
+
+// ---------------------------------------------------------------- dW = dZ^T H of the piece, dH += dZ W
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    lce_prod_kernel(const __grid_constant__ CUtensorMap mZm, const __grid_constant__ CUtensorMap mZk,
+                    const __grid_constant__ CUtensorMap mH, const __grid_constant__ CUtensorMap mHc,
+                    const __grid_constant__ CUtensorMap mW, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ Shared s;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  setup(s, warp);
+  const int n = p.head->n, nn = max(n, 1);
+  const int cols = min(p.vp, p.V - p.v0);
+  const int nt = (p.d + kN - 1) / kN;
+  const int tw = p.dw ? (cols + kM - 1) / kM * nt : 0;  // tiles of dW, then those of dH
+  const int th = p.dh ? (nn + kM - 1) / kM * nt : 0;
+  const int kw = (nn + kK - 1) / kK, kh = (cols + kK - 1) / kK;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const CUtensorMap* hm = n == p.T ? &mH : &mHc;
+      Loader ld{s, smem, 0};
+      bool ok = true;
+      for (int t = blockIdx.x; t < tw + th && ok; t += gridDim.x) {
+        const bool w = t < tw;
+        const int u = w ? t : t - tw, m0 = u / nt * kM, n0 = u % nt * kN;
+        const int boxes = min(4, (p.d - n0 + 63) / 64), steps = w ? kw : kh;
+        for (int k = 0; k < steps; ++k) {
+          uint64_t* bar;
+          uint8_t* to = ld.next(kABytes + boxes * kBox, bar);
+          if (!to) {
+            ok = false;
+            break;
+          }
+          if (w) {
+            tma_load_2d(to, &mZm, bar, m0, k * kK);
+            tma_load_2d(to + kBox, &mZm, bar, m0 + 64, k * kK);
+            for (int i = 0; i < boxes; ++i) tma_load_2d(to + kABytes + i * kBox, hm, bar, n0 + 64 * i, k * kK);
+          } else {
+            tma_load_2d(to, &mZk, bar, k * kK, m0);
+            for (int i = 0; i < boxes; ++i)
+              tma_load_2d(to + kABytes + i * kBox, &mW, bar, n0 + 64 * i, p.v0 + k * kK);
+          }
+        }
+      }
+      if (!ok) ld.drain();
+    }
+  } else if (warp == 9) {
+    const bool leader = elect_one();
+    constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
+    Issuer mm{s, smem_u32(smem), 0, 0};
+    bool ok = true;
+    for (int t = blockIdx.x; t < tw + th && ok; t += gridDim.x) {
+      const bool w = t < tw;
+      const int u = w ? t : t - tw, n0 = u % nt * kN, N = min(kN, (p.d - n0 + 63) / 64 * 64);
+      ok = mm.tile(w ? kw : kh, idesc(fmt, w, 1, N), w ? 2048 : 32, 2048, leader);
+    }
+  } else {
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t tl = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
+    const float unit = p.head->unit;
+    uint32_t tiles = 0;
+    bool dead = false;
+    for (int t = blockIdx.x; t < tw + th; t += gridDim.x, ++tiles) {
+      const bool w = t < tw;
+      const int u = w ? t : t - tw, m0 = u / nt * kM, n0 = u % nt * kN + half * 128;
+      const uint32_t b = tiles & 1;
+      if (!dead) dead = gave_up(&s.acc_full[b], (tiles >> 1) & 1, &s.failed);
+      __syncwarp();
+      tc_fence_after();
+      const int r = m0 + row;
+      T* to = nullptr;
+      if (w) {
+        if (r < cols) to = static_cast<T*>(p.dw) + (i64)(p.v0 + r) * p.d + n0;
+      } else if (r < n) {
+        to = static_cast<T*>(p.dh) + (i64)__ldg(p.rows + r) * p.d + n0;
+      }
+      float4* sum = w ? nullptr : reinterpret_cast<float4*>(p.dh32) + ((i64)u * 2 + half) * 32 * kM + row;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        if (n0 + 32 * i >= p.d) break;
+        float x[32];
+        tmem_ld32_nowait(tl + b * kN + 32 * i, x);
+        tmem_wait_ld();
+        pin32(x);
+        if (!w && !p.first) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 y = sum[(8 * i + e) * kM];
+            x[4 * e] += y.x, x[4 * e + 1] += y.y, x[4 * e + 2] += y.z, x[4 * e + 3] += y.w;
+          }
+        }
+        if (!w && !p.last) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            sum[(8 * i + e) * kM] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        } else if (to) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (n0 + 32 * i + 8 * e >= p.d) break;
+            const float* y = x + 8 * e;
+            *reinterpret_cast<uint4*>(to + 32 * i + 8 * e) =
+                make_uint4(pack2<T>(y[0] * unit, y[1] * unit), pack2<T>(y[2] * unit, y[3] * unit),
+                           pack2<T>(y[4] * unit, y[5] * unit), pack2<T>(y[6] * unit, y[7] * unit));
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+    }
+  }
+  teardown(s, warp, p.status);
+}
+
+// ---------------------------------------------------------------- rows
+template <typename V, typename F>
+OSSM_DEV V block_reduce(V v, V* warps, F f) {  // of kRowThreads threads, the same in all of them
+#pragma unroll
+  for (int w = 16; w; w >>= 1) v = f(v, __shfl_xor_sync(~0u, v, w));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = warps[0];
+#pragma unroll
+  for (int i = 1; i < kRowThreads / 32; ++i) v = f(v, warps[i]);
+  return v;
+}
+
+// Which tokens have a target: their numbers in order, their targets, and, if
+// some have none, their states side by side.  Backward: the factors of each
+// row's gradient, zeros in dH where there is no target.  Every block counts
+// the tokens before its own (they are in L2), so that none waits for another.
+template <bool BWD>
+__global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_constant__ Params p) {
+  __shared__ i64 wi[kRowThreads / 32];
+  __shared__ float wf[kRowThreads / 32];
+  __shared__ int places[kRowThreads], total[kRowThreads / 32];
+  const i64 chunk = (p.T + gridDim.x - 1) / gridDim.x, c0 = min(p.T, chunk * blockIdx.x), c1 = min(p.T, c0 + chunk);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  i64 before = 0, all = 0;
+  float top = 0.f;
+  for (i64 t = threadIdx.x; t < p.T; t += kRowThreads) {
+    const bool has = __ldg(p.targets + t) != p.ignore;
+    all += has;
+    before += has && t < c0;
+    if (BWD && has) {
+      const float f = p.reduction ? 1.f : fabsf(__ldg(p.g + t));
+      top = fmaxf(top, f * fmaxf(1.f, fabsf(1.f + 2.f * p.zl * __ldg(p.lse + t))));
+    }
+  }
+  auto plus = [](i64 a, i64 b) { return a + b; };
+  all = block_reduce(all, wi, plus);
+  before = block_reduce(before, wi, plus);
+  const int n = (int)all;
+  float scale = 1.f;
+  if (BWD) {
+    top = block_reduce(top, wf, [](float a, float b) { return fmaxf(a, b); });
+    if (p.reduction) scale = __ldg(p.g) / (p.reduction == 1 ? (float)max(n, 1) : 1.f);
+  }
+  const float inv = top > 0.f ? fminf(kDzScale / top, 0x1p120f) : 0.f;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.head->n = n;
+    p.head->unit = inv > 0.f ? scale / inv : 0.f;
+    p.head->count = 0;
+  }
+  const bool gather = all < p.T;
+  const int vecs = p.d / 8;
+  i64 base = before;
+  for (i64 t0 = c0; t0 < c1; t0 += kRowThreads) {
+    const i64 t = t0 + threadIdx.x;
+    const i64 target = t < c1 ? __ldg(p.targets + t) : 0;
+    const bool has = t < c1 && target != p.ignore;
+    const uint32_t votes = __ballot_sync(~0u, has);
+    __syncthreads();
+    if (lane == 0) total[warp] = __popc(votes);
+    __syncthreads();
+    int at = __popc(votes & ((1u << lane) - 1)), count = 0;
+    for (int i = 0; i < kRowThreads / 32; ++i) {
+      if (i < warp) at += total[i];
+      count += total[i];
+    }
+    const i64 place = base + at;
+    base += count;
+    places[threadIdx.x] = has ? (int)place : -1;
+    const bool known = target >= 0 && target < p.V;
+    if (has) {
+      p.rows[place] = (int)t;
+      p.tgt[place] = known ? (int)target : -1;
+      if (BWD) {
+        const float lse = __ldg(p.lse + t), g = p.reduction ? 1.f : __ldg(p.g + t);
+        // a target outside the vocabulary: NaN, as its loss
+        const float f = known ? g * inv : NAN;
+        p.lse2[place] = lse * kLog2e;
+        p.fa[place] = f * (1.f + 2.f * p.zl * lse);
+        p.fb[place] = f;
+      }
+    } else if (!BWD && t < c1) {
+      p.lse[t] = 0.f;
+      if (!p.reduction) p.loss[t] = 0.f;
+    }
+    if (!gather) continue;
+    __syncthreads();
+    for (int i = warp; i < (int)min((i64)kRowThreads, c1 - t0); i += kRowThreads / 32) {
+      const int to = places[i];
+      if (to >= 0) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.hidden) + (t0 + i) * p.hst);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.hc) + (i64)to * p.d);
+        for (int e = lane; e < vecs; e += 32) dst[e] = __ldg(src + e);
+      } else if (BWD && p.dh) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dh) + (t0 + i) * p.d);
+        for (int e = lane; e < vecs; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  if (gather && blockIdx.x == gridDim.x - 1) {  // the last block of rows is read whole
+    const int to = (max(n, 1) + kM - 1) / kM * kM;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.hc) + (i64)n * p.d);
+    for (i64 e = threadIdx.x; e < (i64)(to - n) * vecs; e += kRowThreads) dst[e] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------- losses
+// A warp a row joins the partial sums; block sums in float64, added in order by
+// the last block.
+__global__ void __launch_bounds__(kRowThreads) lce_finish_kernel(const __grid_constant__ Params p) {
+  __shared__ double ws[kRowThreads / 32];
+  __shared__ bool last;
+  const int n = p.head->n, lane = threadIdx.x & 31, warps = gridDim.x * (kRowThreads / 32);
+  double sum = 0.0;
+  for (int r = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5); r < n; r += warps) {
+    const float2* q = p.part + (i64)r * 2 * p.panels;
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < 2 * p.panels; i += 32) {
+      const float2 v = q[i];
+      const float top = fmaxf(m, v.x), ref = top == -INFINITY ? 0.f : top;
+      l = l * ex2(m - ref) + v.y * ex2(v.x - ref);
+      m = top;
+    }
+#pragma unroll
+    for (int w = 16; w; w >>= 1) {
+      const float m2 = __shfl_xor_sync(~0u, m, w), l2 = __shfl_xor_sync(~0u, l, w);
+      const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
+      l = l * ex2(m - ref) + l2 * ex2(m2 - ref);
+      m = top;
+    }
+    if (lane == 0) {
+      const int t = p.rows[r];
+      const double lse = ((double)m + log2((double)l)) * 0.6931471805599453;
+      double loss = lse - (double)p.zt[r] + (double)p.zl * lse * lse;
+      if (p.tgt[r] < 0) loss = NAN;
+      p.lse[t] = (float)lse;
+      if (!p.reduction) p.loss[t] = (float)loss;
+      sum += loss;
+    }
+  }
+  if (!p.reduction) return;
+  auto plus = [](double a, double b) { return a + b; };
+  sum = block_reduce(sum, ws, plus);
+  if (threadIdx.x == 0) {
+    p.sums[blockIdx.x] = sum;
+    __threadfence();
+    last = atomicAdd(&p.head->count, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double all = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kRowThreads) all += __ldcg(p.sums + i);
+  all = block_reduce(all, ws, plus);
+  if (threadIdx.x == 0) *p.loss = (float)(p.reduction == 1 ? all / max(n, 1) : all);
+}
+
+// ---------------------------------------------------------------- host
+bool valid(const ossm_lce_args* a, bool bwd) {
+  if (!a || a->tokens < 1 || a->tokens > (1 << 27) || a->vocab < 1 || a->vocab > (1 << 27)) return false;
+  if (a->dim < 8 || a->dim % 8 || a->dim > (1 << 16)) return false;
+  if (a->dtype != OSSM_BF16 && a->dtype != OSSM_F16) return false;
+  if (a->reduction < OSSM_LOSS_NONE || a->reduction > OSSM_LOSS_SUM) return false;
+  if (!(a->z_loss >= 0.f) || !std::isfinite(a->z_loss)) return false;
+  auto rows_ok = [&](const void* q, i64 st) { return q && (uintptr_t)q % 16 == 0 && st % 8 == 0 && st >= a->dim; };
+  if (!rows_ok(a->hidden, a->hidden_stride) || !rows_ok(a->weight, a->weight_stride)) return false;
+  if (!a->targets || !a->lse) return false;
+  if (!bwd) return a->loss != nullptr;
+  return a->grad_loss && (uintptr_t)a->grad_hidden % 16 == 0 && (uintptr_t)a->grad_weight % 16 == 0;
+}
+
+struct Plan {
+  int Tpad, Vpad, sms, ntiles, pan, panels, vp;
+  size_t at[12], bytes;
+};
+// The workspace, and how the vocabulary is cut.
+Plan plan_of(const ossm_lce_args* a, bool bwd) {
+  Plan q{};
+  q.sms = device_sms();
+  q.Tpad = (int)((a->tokens + 255) / 256 * 256);
+  q.Vpad = (a->vocab + kN - 1) / kN * kN;
+  const i64 blocks = (a->tokens + kM - 1) / kM;
+  // Backward: dZ of a piece takes at most 512 MB, but has 4096 columns at
+  // least: each piece reads and writes dH's fp32 sums once.
+  q.vp = bwd ? (int)std::min<i64>(q.Vpad, std::max<i64>(4096, (1LL << 28) / q.Tpad / kN * kN)) : q.Vpad;
+  q.ntiles = q.vp / kN;
+  // A row's sums stay in registers over a panel: up to 8 tiles, fewer where
+  // there would not be 6 panels for each CTA to even out.
+  q.pan = bwd ? 1 : (int)std::min<i64>(8, std::max<i64>(1, blocks * q.ntiles / (6 * q.sms)));
+  q.panels = (q.ntiles + q.pan - 1) / q.pan;
+  size_t at = 0;
+  int k = 0;
+  auto take = [&](size_t bytes) {
+    q.at[k++] = at;
+    at += (bytes + 255) / 256 * 256;
+  };
+  const size_t T = q.Tpad, d = a->dim;
+  take(sizeof(Head));
+  take(4 * T);              // rows
+  take(4 * T);              // targets
+  take(2 * T * d);          // states side by side
+  if (!bwd) {
+    take(8 * T * 2 * q.panels);
+    take(4 * T);
+    take(8 * kMaxBlocks);
+  } else {
+    take(4 * T);
+    take(4 * T);
+    take(4 * T);
+    take(2 * T * (size_t)q.vp);  // dz
+    const size_t nt = (d + kN - 1) / kN;
+    take(a->grad_hidden && q.vp < q.Vpad ? 4 * T * nt * kN : 0);
+  }
+  q.bytes = at;
+  return q;
+}
+
+// [rows, inner] with 128-byte swizzle, box [brows, 64].
+bool encode(CUtensorMap* map, int dtype, const void* base, i64 inner, i64 rows, i64 stride, int brows) {
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)brows}, estr[2] = {1, 1};
+  return fast::encode_fn()(map, dtype == OSSM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+Params params_of(const ossm_lce_args* a, const Plan& q, char* w, bool bwd) {
+  Params p{};
+  p.T = a->tokens, p.Tpad = q.Tpad, p.d = a->dim, p.V = a->vocab;
+  p.hidden = a->hidden, p.hst = a->hidden_stride;
+  p.targets = a->targets, p.ignore = a->ignore_index, p.zl = a->z_loss, p.reduction = a->reduction;
+  p.loss = a->loss, p.lse = a->lse, p.g = a->grad_loss, p.dh = a->grad_hidden, p.dw = a->grad_weight;
+  p.head = reinterpret_cast<Head*>(w + q.at[0]);
+  p.rows = reinterpret_cast<int*>(w + q.at[1]);
+  p.tgt = reinterpret_cast<int*>(w + q.at[2]);
+  p.hc = w + q.at[3];
+  if (!bwd) {
+    p.part = reinterpret_cast<float2*>(w + q.at[4]);
+    p.zt = reinterpret_cast<float*>(w + q.at[5]);
+    p.sums = reinterpret_cast<double*>(w + q.at[6]);
+  } else {
+    p.lse2 = reinterpret_cast<float*>(w + q.at[4]);
+    p.fa = reinterpret_cast<float*>(w + q.at[5]);
+    p.fb = reinterpret_cast<float*>(w + q.at[6]);
+    p.dh32 = reinterpret_cast<float*>(w + q.at[8]);
+  }
+  p.panels = q.panels, p.pan = q.pan, p.vp = q.vp;
+  p.status = a->status;
+  return p;
+}
+
+int row_blocks(const Plan& q, i64 T) { return (int)std::min<i64>(q.sms, (T + kRowThreads - 1) / kRowThreads); }
+
+template <typename T>
+int forward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
+  Params p = params_of(a, q, w, false);
+  CUtensorMap mh, mc, mw;
+  if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kM) ||
+      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kM) ||
+      !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kN))
+    return OSSM_EINVAL;
+  lce_rows_kernel<false><<<row_blocks(q, a->tokens), kRowThreads, 0, st>>>(p);
+  static std::atomic<uint64_t> done{0};
+  auto kern = lce_logits_kernel<T, STATS>;
+  if (allow_smem(kern, (int)kSmem, done) != cudaSuccess) return OSSM_ELAUNCH;
+  const i64 items = (a->tokens + kM - 1) / kM * q.panels;
+  kern<<<(int)std::min<i64>(q.sms, items), kThreads, kSmem, st>>>(mh, mc, mw, mw, p);
+  const int blocks = (int)std::min<i64>(kMaxBlocks, (a->tokens + kRowThreads / 32 - 1) / (kRowThreads / 32));
+  lce_finish_kernel<<<blocks, kRowThreads, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
+}
+
+template <typename T>
+int backward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
+  Params p = params_of(a, q, w, true);
+  void* dz = w + q.at[7];
+  CUtensorMap mh, mc, mw, ms, mzm, mzk, hm, hcm, wm;
+  if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kM) ||
+      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kM) ||
+      !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kN) ||
+      !encode(&ms, a->dtype, dz, q.vp, q.Tpad, q.vp, 32) || !encode(&mzm, a->dtype, dz, q.vp, q.Tpad, q.vp, 64) ||
+      !encode(&mzk, a->dtype, dz, q.vp, q.Tpad, q.vp, kM) ||
+      !encode(&hm, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, 64) ||
+      !encode(&hcm, a->dtype, p.hc, a->dim, q.Tpad, a->dim, 64) ||
+      !encode(&wm, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, 64))
+    return OSSM_EINVAL;
+  lce_rows_kernel<true><<<row_blocks(q, a->tokens), kRowThreads, 0, st>>>(p);
+  static std::atomic<uint64_t> done_z{0}, done_p{0};
+  auto gradz = lce_logits_kernel<T, GRADZ>;
+  auto prod = lce_prod_kernel<T>;
+  if (allow_smem(gradz, (int)kSmem, done_z) != cudaSuccess || allow_smem(prod, (int)kSmem, done_p) != cudaSuccess)
+    return OSSM_ELAUNCH;
+  for (int v0 = 0; v0 < a->vocab; v0 += q.vp) {
+    p.v0 = v0, p.first = v0 == 0, p.last = v0 + q.vp >= a->vocab;
+    gradz<<<q.sms, kThreads, kSmem, st>>>(mh, mc, mw, ms, p);
+    prod<<<q.sms, kThreads, kSmem, st>>>(mzm, mzk, hm, hcm, wm, p);
+  }
+  return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
+}
+
+}  // namespace lce
+}  // namespace ossm
+
+using namespace ossm;
+
+extern "C" size_t ossm_lce_workspace_bytes(const ossm_lce_args* a, int backward) {
+  return lce::valid(a, backward != 0) ? lce::plan_of(a, backward != 0).bytes : 0;
+}
+
+static int lce_call(const ossm_lce_args* a, void* workspace, size_t bytes, ossm_stream_t stream, bool bwd) {
+  if (!lce::valid(a, bwd)) return OSSM_EINVAL;
+  const lce::Plan q = lce::plan_of(a, bwd);
+  if (!workspace || bytes < q.bytes || (uintptr_t)workspace % 256) return OSSM_EWORKSPACE;
+  if (bwd && !a->grad_hidden && !a->grad_weight) return OSSM_OK;
+  if (!fast::encode_fn()) return OSSM_ELAUNCH;
+  char* w = static_cast<char*>(workspace);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool bf = a->dtype == OSSM_BF16;
+  if (bwd) return bf ? lce::backward<__nv_bfloat16>(a, q, w, st) : lce::backward<__half>(a, q, w, st);
+  return bf ? lce::forward<__nv_bfloat16>(a, q, w, st) : lce::forward<__half>(a, q, w, st);
+}
+
+extern "C" int ossm_lce_fwd(const ossm_lce_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream) {
+  return lce_call(a, workspace, workspace_bytes, stream, false);
+}
+extern "C" int ossm_lce_bwd(const ossm_lce_args* a, void* workspace, size_t workspace_bytes, ossm_stream_t stream) {
+  return lce_call(a, workspace, workspace_bytes, stream, true);
+}
+extern "C" size_t ossm_sizeof_lce_args(void) { return sizeof(ossm_lce_args); }

@@ -35,6 +35,11 @@ the two against each other and against dense masked attention.
 into one pass, a cache of keys and values per layer, and drawn tokens.  There
 the local attention is this package's ``packed_attention`` (the window reaches
 over call boundaries) and the tokens come from ``sample_tokens``.
+
+``OrthoSSMLM.loss`` trains it, or scores text, without the logits: the same
+network with ``embed_tokens``, ``residual_norm`` (each block's residual with the
+next one's norm, and the combine's sum with its LayerNorm) and
+``linear_cross_entropy``.
 """
 from __future__ import annotations
 
@@ -49,6 +54,7 @@ import torch.nn.functional as F
 from .sdpc_kernel import BASELINE_LAMBDA, cheby_ema_forward, init_chebyshev_coefficients
 from .serving import packed_attention, sample_tokens
 from .state import ChebyStreamState
+from .training import embed_tokens, linear_cross_entropy, residual_norm
 
 
 @dataclasses.dataclass
@@ -148,16 +154,19 @@ class V8Layer(nn.Module):
             t = self._lam[device] = torch.tensor(self.cfg.lambda_per_head, dtype=torch.float32, device=device)
         return t
 
-    def forward(self, x: torch.Tensor, coeffs: torch.Tensor, ema: Optional[torch.Tensor]):
-        B, S, d = x.shape
+    def paths(self, h: torch.Tensor, coeffs: torch.Tensor, ema: Optional[torch.Tensor]):
+        """The global and the local path on the normed input, and the new EMA state."""
+        B, S, d = h.shape
         H = self.cfg.n_heads
-        h = self.norm_in(x)
         g, fin = cheby_ema_forward(h, coeffs, lambda_per_head=self.lam(h.device), gate_weight=self.gate.weight.float(),
                                    gate_bias=self.gate.bias.float(), gate_scale=self.cfg.gate_scale,
                                    init_state=ema, out_dtype=h.dtype)
         q, k, v = self.qkv(h).view(B, S, 3, H, d // H).unbind(2)
         attn = local_window_attention if h.dtype in (torch.bfloat16, torch.float16) else local_window_attention_blocked
-        loc = self.o(attn(q, k, v, self.cfg.window).reshape(B, S, d))
+        return g, self.o(attn(q, k, v, self.cfg.window).reshape(B, S, d)), fin
+
+    def forward(self, x: torch.Tensor, coeffs: torch.Tensor, ema: Optional[torch.Tensor]):
+        g, loc, fin = self.paths(self.norm_in(x), coeffs, ema)
         return x + self.out_proj(self.norm_comb(g + loc)), fin
 
     def extend(self, x: torch.Tensor, news: List[int], cu: torch.Tensor, at: torch.Tensor, kv_lengths: torch.Tensor,
@@ -239,6 +248,38 @@ class OrthoSSMLM(nn.Module):
         logits = self.lm_head(self.final_norm(x))
         return (logits, new_states) if return_state else logits
 
+    def loss(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None,
+             states: Optional[List[ChebyStreamState]] = None, *, ignore_index: int = -100, z_loss: float = 0.0,
+             reduction: str = "mean", return_state: bool = False):
+        """Cross entropy of the logits after each token [B, S] against
+        ``targets`` (default: the next token, none after the last), without the
+        logits; arguments and reductions as ``linear_cross_entropy`` has them.
+        Differentiable as ``forward`` is (the decay gates are constants).  A
+        position that holds -1 is padding: its embedding is zero."""
+        p = self.embedding.weight
+        if p.dtype != torch.bfloat16:
+            raise ValueError(f"loss runs in bf16: cast the model first (parameters are {p.dtype})")
+        B, S = input_ids.shape
+        if targets is None:
+            targets = torch.full_like(input_ids, ignore_index)
+            targets[:, :-1] = input_ids[:, 1:]
+            targets.masked_fill_(targets == -1, ignore_index)
+        if states is None:
+            states = self.fresh_states(B, input_ids.device)
+        norms = [layer.norm_in for layer in self.layers] + [self.final_norm]
+        eps = [torch.finfo(torch.float32).eps if n.eps is None else n.eps for n in norms]  # nn.RMSNorm's default
+        x = embed_tokens(input_ids, p)
+        x, h = residual_norm(x, None, norms[0].weight, eps=eps[0])
+        new_states = []
+        for i, (layer, st) in enumerate(zip(self.layers, states)):
+            g, loc, fin = layer.paths(h, st.coeffs, st.ema)
+            comb = layer.norm_comb
+            _, c = residual_norm(g, loc, comb.weight, comb.bias, norm="layer", eps=comb.eps)
+            x, h = residual_norm(x, layer.out_proj(c), norms[i + 1].weight, eps=eps[i + 1])
+            new_states.append(dataclasses.replace(st, ema=fin, tokens_seen=st.tokens_seen + S))
+        loss = linear_cross_entropy(h, self.lm_head.weight, targets, ignore_index=ignore_index, z_loss=z_loss,
+                                    reduction=reduction)
+        return (loss, new_states) if return_state else loss
 
     # ------------------------------------------------------------------ serving
     def new_cache(self, batch: int, slots: int, coeffs: Optional[List[torch.Tensor]] = None) -> DecodeCache:

@@ -108,6 +108,7 @@ def init_chebyshev_coefficients(batch, n_heads, degree, head_dim, device):
 _WS: dict = {}
 _WS_HOST: dict = {}  # host-buffer calls: staging buffers inside, never shared with the others
 _WS_ATTN: dict = {}  # packed_attention: partial sums inside, never shared with the others
+_WS_TRAIN: dict = {}  # training operators: a header alone (their workspaces are a call's own)
 _WS_LOCK = threading.Lock()
 
 
@@ -167,7 +168,7 @@ def workspace_status(device=None, clear=True):
     worst = 0
     captured = [(key[1:], ws) for key, (_, ws) in list(_WS_CAPTURED.items())]  # zeroed by their graphs
     attention = list(_WS_ATTN.items())
-    for (d, sptr), ws in list(_WS.items()) + list(_WS_HOST.items()) + captured + attention:
+    for (d, sptr), ws in list(_WS.items()) + list(_WS_HOST.items()) + list(_WS_TRAIN.items()) + captured + attention:
         if d != device:
             continue
         st = L._i32(0)
