@@ -566,6 +566,7 @@ typedef struct {
   void* grad_y;
   void* grad_gate;                   /* of the gate's shape and type, or NULL */
   void *grad_weight, *grad_bias, *grad_post_weight, *grad_post_bias; /* of the parameters' types, or NULL */
+  uint32_t* status;                  /* as for ossm_lce */
 } ossm_norm_args;
 
 int ossm_residual_norm_fwd(const ossm_norm_args* a, ossm_stream_t stream);

@@ -152,7 +152,7 @@ class NormArgs(C.Structure):
         ("weight_dtype", _i32), ("bias_dtype", _i32), ("post_weight_dtype", _i32), ("post_bias_dtype", _i32),
         ("r", _vp), ("h", _vp), ("stats", _vp), ("grad_r", _vp), ("grad_r_stride", _i64), ("grad_h", _vp),
         ("grad_h_stride", _i64), ("grad_x", _vp), ("grad_y", _vp), ("grad_gate", _vp), ("grad_weight", _vp),
-        ("grad_bias", _vp), ("grad_post_weight", _vp), ("grad_post_bias", _vp),
+        ("grad_bias", _vp), ("grad_post_weight", _vp), ("grad_post_bias", _vp), ("status", _vp),
     ]
 
 

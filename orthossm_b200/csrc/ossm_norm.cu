@@ -17,11 +17,13 @@
 #include <cmath>
 
 #include "ossm_attn.cuh"
+#include "ossm_sm100.cuh"
 
 namespace ossm {
 int device_sms();
 namespace nrm {
 
+using attn::allow_smem;
 using attn::pack2;
 using attn::to_f2;
 typedef long long i64;
@@ -37,12 +39,12 @@ OSSM_DEV void put1(__half* p, float v) { *p = __float2half_rn(v); }
 // A thread's 8 N channels of a row that R threads share: N runs of eight, or,
 // where a row does not start on 16 bytes or is no whole number of runs, every
 // R-th channel.
-template <int N>
+template <int N, bool VEC>
 struct Own {
+  static constexpr bool vec = VEC;
   int R, t, d;
-  bool vec;
-  OSSM_DEV int at(int i) const { return vec ? ((i >> 3) * R + t) * 8 + (i & 7) : i * R + t; }
-  OSSM_DEV bool has(int i) const { return at(i) < d; }
+  OSSM_DEV int at(int i) const { return VEC ? ((i >> 3) * R + t) * 8 + (i & 7) : i * R + t; }
+  OSSM_DEV bool has(int i) const { return VEC ? ((i >> 3) * R + t) * 8 < d : at(i) < d; }  // whole runs of eight
 };
 template <typename T>
 OSSM_DEV void vec8(const T* p, float* v) {
@@ -65,9 +67,9 @@ OSSM_DEV void put8<float>(float* p, const float* v) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
-template <typename T, int N>
-OSSM_DEV void load(const Own<N>& o, const T* row, float (&v)[8 * N]) {  // 0 past the row's end
-  if (o.vec) {
+template <typename T, int N, bool VEC>
+OSSM_DEV void load(const Own<N, VEC>& o, const T* row, float (&v)[8 * N]) {  // 0 past the row's end
+  if (VEC) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (o.has(8 * i)) {
@@ -82,9 +84,9 @@ OSSM_DEV void load(const Own<N>& o, const T* row, float (&v)[8 * N]) {  // 0 pas
     for (int i = 0; i < 8 * N; ++i) v[i] = o.has(i) ? get1(row + o.at(i)) : 0.f;
   }
 }
-template <typename T, int N>
-OSSM_DEV void store(const Own<N>& o, T* row, const float (&v)[8 * N]) {
-  if (o.vec) {
+template <typename T, int N, bool VEC>
+OSSM_DEV void store(const Own<N, VEC>& o, T* row, const float (&v)[8 * N]) {
+  if (VEC) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (o.has(8 * i)) put8<T>(row + o.at(8 * i), v + 8 * i);
@@ -94,22 +96,26 @@ OSSM_DEV void store(const Own<N>& o, T* row, const float (&v)[8 * N]) {
       if (o.has(i)) put1(row + o.at(i), v[i]);
   }
 }
-// A vector of parameters, of any of the three types; `none` where there is none.
+// A vector of parameters, of any of the three types.  The kernels keep a copy in
+// fp32 in shared memory where it fits beside the rows.
 struct Param {
   const void* p;
   int dtype;
+  const float* shared;  // a copy in shared memory, or NULL
   OSSM_DEV float one(i64 i) const {
     return dtype == OSSM_F32    ? get1(static_cast<const float*>(p) + i)
            : dtype == OSSM_BF16 ? get1(static_cast<const __nv_bfloat16*>(p) + i)
                                 : get1(static_cast<const __half*>(p) + i);
   }
 };
-template <int N>
-OSSM_DEV void load(const Own<N>& o, const Param& q, i64 from, bool vec, float none, float (&v)[8 * N]) {
+template <int N, bool VEC>
+OSSM_DEV void load(const Own<N, VEC>& o, const Param& q, i64 from, bool vec, float none, float (&v)[8 * N]) {
   if (!q.p) {
 #pragma unroll
-    for (int i = 0; i < 8 * N; ++i) v[i] = none;
-  } else if (o.vec && !vec) {
+    for (int i = 0; i < 8 * N; ++i) v[i] = o.has(i) ? none : 0.f;
+  } else if (q.shared) {
+    load<float>(o, q.shared, v);
+  } else if (VEC && !vec) {
 #pragma unroll
     for (int i = 0; i < 8 * N; ++i) v[i] = o.has(i) ? q.one(from + o.at(i)) : 0.f;
   } else if (q.dtype == OSSM_F32) {
@@ -146,46 +152,111 @@ struct Params {
   void *dx, *dy, *dgate;  // or NULL; dgate: of token and full gates
   int dgate_dtype;
   float* part;    // [blocks][sums][d]
+  int stages, stage_bytes;  // of the ring of a row's threads
+  bool shared;              // parameters are copied to shared memory, behind the rows
+  uint32_t* status;
 };
 
-// Sums over the threads of a row, the same in all of them.
-template <int K>
-OSSM_DEV void row_sum(float (&v)[K], int R, float (*warps)[K]) {
+// The rows of up to four tensors on their way to the threads that share them.
+// Where rows are whole 16-byte pieces, bulk copies bring them into a ring in
+// shared memory several rows ahead; otherwise they are read where they are used.
+// (A row ahead in registers kept 48 KB an SM on its way and cost 24 to 48 of
+// them: 131072 x 512 bf16, backward: 119 us.)
+constexpr int kMaxStages = 8;
+struct Tensor {
+  const char* p;  // NULL: not there
+  i64 stride;     // in bytes
+  int bytes, at;  // of a row; where in a stage
+};
+template <bool VEC>
+struct Rows {
+  Tensor t[4];
+  char* ring;          // of this row's threads
+  uint64_t* full;
+  int stages, stage_bytes, R, lane;
+  i64 step, T;
+  uint32_t* status;
+  uint32_t slot, turn;  // of the row at hand
+  OSSM_DEV void fetch(i64 row, uint32_t slot) {  // one thread
+    sm100::mbar_expect_tx(full + slot, stage_bytes);
 #pragma unroll
-  for (int w = 16; w; w >>= 1)
+    for (int i = 0; i < 4; ++i)
+      if (t[i].p) sm100::bulk_load(ring + slot * stage_bytes + t[i].at, t[i].p + row * t[i].stride, t[i].bytes, full + slot);
+  }
+  OSSM_DEV void begin(i64 first) {
+    if (!VEC) return;
+    if (lane == 0) {
+      for (int i = 0; i < stages; ++i) sm100::mbar_init(full + i, 1);
+      sm100::fence_mbar_init();
+      for (int i = 0; i < stages && first + i * step < T; ++i) fetch(first + i * step, i);
+    }
+    meet();
+  }
+  OSSM_DEV void meet() const {
+    if (R == 32) __syncwarp(); else __syncthreads();
+  }
+  OSSM_DEV void wait() const {
+    if (VEC && !sm100::mbar_wait(full + slot, turn) && status) atomicExch(status, (uint32_t)OSSM_ETIMEOUT);
+  }
+  // Tensor i's row `row`, the row at hand.
+  template <typename E, int N>
+  OSSM_DEV void get(const Own<N, VEC>& o, int i, i64 row, float (&v)[8 * N]) const {
+    load<E>(o, reinterpret_cast<const E*>(VEC ? ring + slot * stage_bytes + t[i].at : t[i].p + row * t[i].stride), v);
+  }
+  OSSM_DEV void taken(i64 row) {  // all threads have met since they got what they need of it
+    if (VEC && R == 32) __syncwarp();
+    if (VEC && lane == 0 && row + stages * step < T) fetch(row + stages * step, slot);
+    if (++slot == stages) slot = 0, turn ^= 1;
+  }
+};
+
+// Sums over the threads of a row, the same in all of them.  Rows of several
+// warps take the two buffers in turn, so that one barrier a sum is enough.
+struct RowSum {
+  float (*buf)[32][2];
+  int R, turn;
+  template <int K>
+  OSSM_DEV void operator()(float (&v)[K]) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(~0u, v[k], w);
-  if (R == 32) return;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0)
+    for (int w = 16; w; w >>= 1)
 #pragma unroll
-    for (int k = 0; k < K; ++k) warps[threadIdx.x >> 5][k] = v[k];
-  __syncthreads();
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(~0u, v[k], w);
+    if (R == 32) return;
+    if ((threadIdx.x & 31) == 0)
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = 0.f;
-  for (int i = 0; i < R / 32; ++i)
+      for (int k = 0; k < K; ++k) buf[turn][threadIdx.x >> 5][k] = v[k];
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += warps[i][k];
-}
+    for (int k = 0; k < K; ++k) v[k] = lane < R / 32 ? buf[turn][lane][k] : 0.f;
+    for (int w = R > 256 ? 16 : 4; w; w >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(~0u, v[k], w);
+    if (R <= 256)  // eight warps' sums, in the first lanes of each eight
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = __shfl_sync(~0u, v[k], 0);
+    turn ^= 1;
+  }
+};
 
 // Mean and inverse deviation of a row; v becomes the normed values.
-template <int N>
-OSSM_DEV void normalise(const Own<N>& o, float (&v)[8 * N], int kind, float eps, float inv_d, float& mean, float& inv,
-                        float (*warps)[2]) {
+template <int N, bool VEC>
+OSSM_DEV void normalise(const Own<N, VEC>& o, float (&v)[8 * N], int kind, float eps, float inv_d, float& mean, float& inv,
+                        RowSum& sum) {
   mean = 0.f;
   if (kind == N_LAYER) {
-    float s[2] = {0.f, 0.f};
+    float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < 8 * N; ++i) s[0] += v[i];
-    row_sum<2>(s, o.R, warps);
+    sum(s);
     mean = s[0] * inv_d;
 #pragma unroll
     for (int i = 0; i < 8 * N; ++i) v[i] = o.has(i) ? v[i] - mean : 0.f;
   }
-  float s[2] = {0.f, 0.f};
+  float s[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < 8 * N; ++i) s[0] = fmaf(v[i], v[i], s[0]);
-  row_sum<2>(s, o.R, warps);
+  sum(s);
   inv = 1.f / sqrtf(fmaf(s[0], inv_d, eps));
 #pragma unroll
   for (int i = 0; i < 8 * N; ++i) v[i] *= inv;
@@ -193,62 +264,94 @@ OSSM_DEV void normalise(const Own<N>& o, float (&v)[8 * N], int kind, float eps,
 
 constexpr int kWarpRows = 8;  // rows of a block where a warp takes one
 
+// The parameters that all rows share, copied to shared memory.
+struct Shares {
+  Param w, b, pw, pb, gate;
+  OSSM_DEV Shares(const Params& p, char* ring, int per) : w(p.w), b(p.b), pw(p.pw), pb(p.pb), gate(p.gate) {
+    if (!p.shared) return;
+    float* to = reinterpret_cast<float*>(ring + (i64)per * p.stages * p.stage_bytes);
+    auto copy = [&](Param& q) {
+      if (!q.p) return;
+      for (int i = threadIdx.x; i < p.d; i += blockDim.x) to[i] = q.one(i);
+      q.shared = to;
+      to += p.d;
+    };
+    copy(w), copy(b), copy(pw), copy(pb);
+    if (p.gate_kind == G_CHANNEL) copy(gate);
+    __syncthreads();
+  }
+};
+
 // ---------------------------------------------------------------- forward
 // MAXT: the most threads of a block; a block is one row, or 8 rows of a warp each.
-template <typename TX, typename TY, int N, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ Params p) {
-  __shared__ float warps[MAXT / 32][2];
-  const int per = blockDim.x / p.R;
-  const i64 t = (i64)blockIdx.x * per + threadIdx.x / p.R;
-  if (t >= p.T) return;
-  const Own<N> o{p.R, (int)(threadIdx.x % p.R), p.d, p.vec};
-  float v[8 * N], u[8 * N];
-  load<TX>(o, static_cast<const TX*>(p.x) + t * p.xst, v);
-  float mean, inv, pmean = 0.f, pinv = 1.f;
-  if (p.y) {
-    load<TY>(o, static_cast<const TY*>(p.y) + t * p.yst, u);
-    if (p.post) {
-      normalise(o, u, p.post, p.post_eps, p.inv_d, pmean, pinv, warps);
-      float a[8 * N];
-      load(o, p.pw, 0, p.pw_vec, 1.f, a);
+template <typename TX, typename TY, int N, bool VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 3 : 1) norm_fwd_kernel(const __grid_constant__ Params p) {
+  __shared__ float buf[2][32][2];
+  __shared__ uint64_t full[kWarpRows][kMaxStages];
+  extern __shared__ __align__(16) char ring[];
+  RowSum sum{buf, p.R, 0};
+  const int per = blockDim.x / p.R, mine = threadIdx.x / p.R;
+  const i64 step = (i64)gridDim.x * per;
+  i64 t = (i64)blockIdx.x * per + mine;
+  const Own<N, VEC> o{p.R, (int)(threadIdx.x % p.R), p.d};
+  constexpr int SX = sizeof(TX), SY = sizeof(TY);
+  Rows<VEC> rows{{{static_cast<const char*>(p.x), p.xst * SX, p.d * SX, 0},
+                  {static_cast<const char*>(p.y), p.yst * SY, p.d * SY, p.d * SX}},
+                 ring + mine * p.stages * p.stage_bytes, full[mine], p.stages, p.stage_bytes, p.R, o.t, step, p.T,
+                 p.status, 0, 0};
+  rows.begin(t);
+  const Shares own(p, ring, per);
+  for (; t < p.T; t += step) {
+    float v[8 * N], u[8 * N];
+    rows.wait();
+    rows.template get<TX>(o, 0, t, v);
+    if (p.y) rows.template get<TY>(o, 1, t, u);
+    float mean, inv, pmean = 0.f, pinv = 1.f;
+    if (p.y) {
+      if (p.post) {
+        normalise(o, u, p.post, p.post_eps, p.inv_d, pmean, pinv, sum);
+        float a[8 * N];
+        load(o, own.pw, 0, p.pw_vec, 1.f, a);
 #pragma unroll
-      for (int i = 0; i < 8 * N; ++i) u[i] *= a[i];
-      if (p.pb.p) {
-        load(o, p.pb, 0, p.pb_vec, 0.f, a);
+        for (int i = 0; i < 8 * N; ++i) u[i] *= a[i];
+        if (p.pb.p) {
+          load(o, own.pb, 0, p.pb_vec, 0.f, a);
 #pragma unroll
-        for (int i = 0; i < 8 * N; ++i) u[i] += a[i];
+          for (int i = 0; i < 8 * N; ++i) u[i] += a[i];
+        }
       }
+      if (p.gate_kind == G_TOKEN) {
+        const float g = p.gate.one(t);
+#pragma unroll
+        for (int i = 0; i < 8 * N; ++i) u[i] *= g;
+      } else if (p.gate_kind) {
+        float a[8 * N];
+        load(o, own.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, a);
+#pragma unroll
+        for (int i = 0; i < 8 * N; ++i) u[i] *= a[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8 * N; ++i) v[i] = fmaf(p.scale, u[i], v[i]);
+      store<TX>(o, static_cast<TX*>(p.r) + t * p.d, v);
     }
-    if (p.gate_kind == G_TOKEN) {
-      const float g = p.gate.one(t);
+    normalise(o, v, p.norm, p.eps, p.inv_d, mean, inv, sum);
+    rows.taken(t);
+    load(o, own.w, 0, p.w_vec, 1.f, u);
 #pragma unroll
-      for (int i = 0; i < 8 * N; ++i) u[i] *= g;
-    } else if (p.gate_kind) {
-      float a[8 * N];
-      load(o, p.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, a);
+    for (int i = 0; i < 8 * N; ++i) v[i] *= u[i];
+    if (p.b.p) {
+      load(o, own.b, 0, p.b_vec, 0.f, u);
 #pragma unroll
-      for (int i = 0; i < 8 * N; ++i) u[i] *= a[i];
+      for (int i = 0; i < 8 * N; ++i) v[i] += u[i];
     }
-#pragma unroll
-    for (int i = 0; i < 8 * N; ++i) v[i] = fmaf(p.scale, u[i], v[i]);
-    if (p.r) store<TX>(o, static_cast<TX*>(p.r) + t * p.d, v);
-  }
-  normalise(o, v, p.norm, p.eps, p.inv_d, mean, inv, warps);
-  load(o, p.w, 0, p.w_vec, 1.f, u);
-#pragma unroll
-  for (int i = 0; i < 8 * N; ++i) v[i] *= u[i];
-  if (p.b.p) {
-    load(o, p.b, 0, p.b_vec, 0.f, u);
-#pragma unroll
-    for (int i = 0; i < 8 * N; ++i) v[i] += u[i];
-  }
-  store<TY>(o, static_cast<TY*>(p.h) + t * p.d, v);
-  if (p.stats && o.t == 0) {
-    p.stats[t] = mean;
-    p.stats[p.T + t] = inv;
-    if (p.post) {
-      p.stats[2 * p.T + t] = pmean;
-      p.stats[3 * p.T + t] = pinv;
+    store<TY>(o, static_cast<TY*>(p.h) + t * p.d, v);
+    if (p.stats && o.t == 0) {
+      p.stats[t] = mean;
+      p.stats[p.T + t] = inv;
+      if (p.post) {
+        p.stats[2 * p.T + t] = pmean;
+        p.stats[3 * p.T + t] = pinv;
+      }
     }
   }
 }
@@ -256,100 +359,136 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------- backward
 enum { S_W, S_B, S_GATE, S_PW, S_PB, kSums };  // sums over the rows
 
-// FULL: the block's output has a norm or a gate, so y is read.
-template <typename TX, typename TY, int N, bool FULL, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const __grid_constant__ Params p) {
-  constexpr int kHere = FULL ? (int)kSums : 2;
-  __shared__ float warps[MAXT / 32][2];
-  extern __shared__ float smem[];  // to join the sums of a block's rows
+// SUMS: how many of the sums are kept: the weight's, the bias's too, or all,
+// where the block's output has a norm or a gate, so that y is read.
+template <typename TX, typename TY, int N, bool VEC, int SUMS, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2 : 1)
+    norm_bwd_kernel(const __grid_constant__ Params p) {
+  constexpr bool FULL = SUMS == (int)kSums;
+  __shared__ float buf[2][32][2];
+  __shared__ uint64_t full[kWarpRows][kMaxStages];
+  extern __shared__ __align__(16) char ring[];
+  RowSum row_sum{buf, p.R, 0};
   const int per = blockDim.x / p.R, mine = threadIdx.x / p.R;
-  const Own<N> o{p.R, (int)(threadIdx.x % p.R), p.d, p.vec};
-  float sum[kHere][8 * N];
+  const i64 step = (i64)gridDim.x * per;
+  const Own<N, VEC> o{p.R, (int)(threadIdx.x % p.R), p.d};
+  float sum[SUMS][8 * N];
 #pragma unroll
-  for (int k = 0; k < kHere; ++k)
+  for (int k = 0; k < SUMS; ++k)
 #pragma unroll
     for (int i = 0; i < 8 * N; ++i) sum[k][i] = 0.f;
-  for (i64 t = (i64)blockIdx.x * per + mine; t < p.T; t += (i64)gridDim.x * per) {
-    float v[8 * N], g[8 * N], n[8 * N], a[8 * N];  // normed r; gradient of r; block's output
-    const float inv = p.stats[p.T + t], mean = p.norm == N_LAYER ? p.stats[t] : 0.f;
-    if (FULL) {
-      load<TX>(o, static_cast<const TX*>(p.x) + t * p.xst, v);
-      load<TY>(o, static_cast<const TY*>(p.y) + t * p.yst, n);
+  i64 t = (i64)blockIdx.x * per + mine;
+  constexpr int SX = sizeof(TX), SY = sizeof(TY);
+  // r (or x), its gradient, the gradient of h, y
+  const int at1 = p.d * SX, at2 = at1 + (p.dr ? p.d * SX : 0), at3 = at2 + (p.dh ? p.d * SY : 0);
+  Rows<VEC> rows{{{static_cast<const char*>(FULL ? p.x : p.r), p.xst * SX, p.d * SX, 0},
+                  {static_cast<const char*>(p.dr), p.drst * SX, p.d * SX, at1},
+                  {static_cast<const char*>(p.dh), p.dhst * SY, p.d * SY, at2},
+                  {static_cast<const char*>(FULL ? p.y : nullptr), p.yst * SY, p.d * SY, at3}},
+                 ring + mine * p.stages * p.stage_bytes, full[mine], p.stages, p.stage_bytes, p.R, o.t, step, p.T,
+                 p.status, 0, 0};
+  rows.begin(t);
+  const Shares own(p, ring, per);
+  float inv_a = 0.f, mean_a = 0.f, pinv_a = 1.f, pmean_a = 0.f;  // of the next row
+  auto stats = [&](i64 row) {
+    if (row >= p.T) return;
+    inv_a = __ldg(p.stats + p.T + row);
+    if (p.norm == N_LAYER) mean_a = __ldg(p.stats + row);
+    if (FULL && p.post) {
+      pinv_a = __ldg(p.stats + 3 * p.T + row);
+      if (p.post == N_LAYER) pmean_a = __ldg(p.stats + 2 * p.T + row);
+    }
+  };
+  stats(t);
+  for (; t < p.T; t += step) {
+    // past the row's end e and a are 0, and nothing else of there is used
+    float v[8 * N], g[8 * N], e[8 * N], n[FULL ? 8 * N : 1], a[FULL ? 8 * N : 1];
+    const float inv = inv_a, mean = mean_a, pinv = pinv_a, pmean = pmean_a;
+    stats(t + step);
+    rows.wait();
+    rows.template get<TX>(o, 0, t, v);
+    if (p.dr) {
+      rows.template get<TX>(o, 1, t, g);
     } else {
-      load<TX>(o, static_cast<const TX*>(p.r) + t * p.xst, v);
-    }
-    float pinv = 1.f, pmean = 0.f, gt = 1.f;
-    if (FULL) {
-      if (p.post) {
-        pinv = p.stats[3 * p.T + t];
-        if (p.post == N_LAYER) pmean = p.stats[2 * p.T + t];
-      }
-      if (p.gate_kind == G_TOKEN) gt = p.gate.one(t);
-      // r again: x + scale gate (pv pw + pb)
-      float c[8 * N];
-      load(o, p.pw, 0, p.pw_vec, 1.f, a);
-      if (p.gate_kind == G_CHANNEL || p.gate_kind == G_FULL)
-        load(o, p.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, c);
-      else
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) c[i] = gt;
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) a[i] *= (n[i] - pmean) * pinv;
-      if (p.pb.p) {
-        load(o, p.pb, 0, p.pb_vec, 0.f, g);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) a[i] += g[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) v[i] = fmaf(p.scale, c[i] * a[i], v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8 * N; ++i) v[i] = o.has(i) ? (v[i] - mean) * inv : 0.f;
-    if (p.dr)
-      load<TX>(o, static_cast<const TX*>(p.dr) + t * p.drst, g);
-    else
 #pragma unroll
       for (int i = 0; i < 8 * N; ++i) g[i] = 0.f;
+    }
+    if (p.dh) rows.template get<TY>(o, 2, t, e);
+    if constexpr (FULL) rows.template get<TY>(o, 3, t, n);
+    float gt = 1.f;
+    if constexpr (FULL) {
+      // n becomes y normed (or y); a: the block's output after that; v: r again
+      if (p.post) {
+#pragma unroll
+        for (int i = 0; i < 8 * N; ++i) n[i] = (n[i] - pmean) * pinv;
+      }
+      float c[8 * N];
+      load(o, own.pw, 0, p.pw_vec, 1.f, a);
+#pragma unroll
+      for (int i = 0; i < 8 * N; ++i) a[i] *= n[i];
+      if (p.pb.p) {
+        load(o, own.pb, 0, p.pb_vec, 0.f, c);
+#pragma unroll
+        for (int i = 0; i < 8 * N; ++i) a[i] += c[i];
+      }
+      if (p.gate_kind == G_TOKEN) gt = p.gate.one(t);
+      if (p.gate_kind == G_CHANNEL || p.gate_kind == G_FULL) {
+        load(o, own.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, c);
+#pragma unroll
+        for (int i = 0; i < 8 * N; ++i) v[i] = fmaf(p.scale, c[i] * a[i], v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8 * N; ++i) v[i] = fmaf(p.scale, gt * a[i], v[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8 * N; ++i) v[i] = (v[i] - mean) * inv;
     if (p.dh) {
-      float e[8 * N], f[8 * N];
-      load<TY>(o, static_cast<const TY*>(p.dh) + t * p.dhst, e);
-      load(o, p.w, 0, p.w_vec, 1.f, f);
       float s[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < 8 * N; ++i) {
         sum[S_W][i] = fmaf(e[i], v[i], sum[S_W][i]);
-        sum[S_B][i] += e[i];
-        e[i] *= f[i];
+        if (SUMS > 1) sum[SUMS > 1 ? S_B : 0][i] += e[i];
+      }
+      if (own.w.p) {
+        float f[8 * N];
+        load(o, own.w, 0, p.w_vec, 1.f, f);
+#pragma unroll
+        for (int i = 0; i < 8 * N; ++i) e[i] *= f[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8 * N; ++i) {
         s[0] = fmaf(e[i], v[i], s[0]);
         s[1] += e[i];
       }
-      row_sum<2>(s, p.R, warps);
+      row_sum(s);
+      rows.taken(t);
       const float m0 = s[0] * p.inv_d, m1 = p.norm == N_LAYER ? s[1] * p.inv_d : 0.f;
 #pragma unroll
       for (int i = 0; i < 8 * N; ++i) g[i] = fmaf(inv, e[i] - m1 - v[i] * m0, g[i]);
+    } else {
+      rows.meet();
+      rows.taken(t);
     }
     if (p.dx) store<TX>(o, static_cast<TX*>(p.dx) + t * p.d, g);
-    if (!FULL) {
+    if constexpr (!FULL) {
       if (p.dy) {
 #pragma unroll
         for (int i = 0; i < 8 * N; ++i) g[i] *= p.scale;
         store<TY>(o, static_cast<TY*>(p.dy) + t * p.d, g);
       }
-      continue;
-    }
-    if (FULL) {
-      // a: the block's output after its norm; g: the gradient of r
+    } else {
       float s[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < 8 * N; ++i) {
         g[i] *= p.scale;
-        a[i] = o.has(i) ? a[i] * g[i] : 0.f;  // the gate's gradient
+        a[i] *= g[i];  // the gate's gradient
         s[0] += a[i];
         sum[S_GATE][i] += a[i];
       }
       if (p.gate_kind == G_TOKEN) {
         if (p.dgate) {
-          row_sum<2>(s, p.R, warps);
+          row_sum(s);
           if (o.t == 0) {
             if (p.dgate_dtype == OSSM_F32) put1(static_cast<float*>(p.dgate) + t, s[0]);
             else if (p.dgate_dtype == OSSM_BF16) put1(static_cast<__nv_bfloat16*>(p.dgate) + t, s[0]);
@@ -364,24 +503,25 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const __grid_constant__ 
           else if (p.dgate_dtype == OSSM_BF16) store<__nv_bfloat16>(o, static_cast<__nv_bfloat16*>(p.dgate) + t * p.d, a);
           else store<__half>(o, static_cast<__half*>(p.dgate) + t * p.d, a);
         }
-        float c[8 * N];
-        load(o, p.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, c);
+        load(o, own.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, a);
 #pragma unroll
-        for (int i = 0; i < 8 * N; ++i) g[i] *= c[i];
+        for (int i = 0; i < 8 * N; ++i) g[i] *= a[i];
       }
       if (p.post) {
-        load(o, p.pw, 0, p.pw_vec, 1.f, a);
         s[0] = s[1] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8 * N; ++i) {
-          n[i] = o.has(i) ? (n[i] - pmean) * pinv : 0.f;
           sum[S_PW][i] = fmaf(g[i], n[i], sum[S_PW][i]);
           sum[S_PB][i] += g[i];
-          g[i] = o.has(i) ? g[i] * a[i] : 0.f;
+        }
+        load(o, own.pw, 0, p.pw_vec, 1.f, a);
+#pragma unroll
+        for (int i = 0; i < 8 * N; ++i) {
+          g[i] *= a[i];
           s[0] = fmaf(g[i], n[i], s[0]);
           s[1] += g[i];
         }
-        row_sum<2>(s, p.R, warps);
+        row_sum(s);
         const float m0 = s[0] * p.inv_d, m1 = p.post == N_LAYER ? s[1] * p.inv_d : 0.f;
 #pragma unroll
         for (int i = 0; i < 8 * N; ++i) g[i] = pinv * (g[i] - m1 - n[i] * m0);
@@ -390,10 +530,11 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const __grid_constant__ 
     }
   }
   if (!p.part) return;
+  float* smem = reinterpret_cast<float*>(ring);  // the rows are through
   // the block's sums, its rows' threads in order
 #pragma unroll
-  for (int k = 0; k < kHere; ++k) {
-    float* to = p.part + ((i64)blockIdx.x * kHere + k) * p.d;
+  for (int k = 0; k < SUMS; ++k) {
+    float* to = p.part + ((i64)blockIdx.x * SUMS + k) * p.d;
     if (per == 1) {
 #pragma unroll
       for (int i = 0; i < 8 * N; ++i)
@@ -416,20 +557,21 @@ struct Outs {
   void* to[kSums];
   int dtype[kSums];
 };
-// Adds the blocks' sums up in order: 32 channels a block, 8 runs of blocks side by side.
-__global__ void __launch_bounds__(256) norm_sums_kernel(const float* part, int blocks, int sums, int d, const __grid_constant__ Outs outs) {
-  __shared__ float s[8][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5, k = blockIdx.y;
+// Adds the blocks' sums up in order: 32 channels a block, 32 runs of blocks side by side.
+__global__ void __launch_bounds__(1024)
+    norm_sums_kernel(const float* part, int blocks, int sums, int d, const __grid_constant__ Outs outs) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, run = threadIdx.x >> 5, k = blockIdx.y;
   if (!outs.to[k]) return;
-  const int each = (blocks + 7) / 8;
+  const int each = (blocks + 31) / 32;
   float a = 0.f;
   if (c < d)
 #pragma unroll 8
     for (int b = run * each; b < min(blocks, (run + 1) * each); ++b) a += __ldg(part + ((i64)b * sums + k) * d + c);
-  s[run][threadIdx.x & 31] = a;
+  s[run][lane] = a;
   __syncthreads();
   if (run || c >= d) return;
-  for (int i = 1; i < 8; ++i) a += s[i][threadIdx.x];
+  for (int i = 1; i < 32; ++i) a += s[i][lane];
   if (outs.dtype[k] == OSSM_F32) put1(static_cast<float*>(outs.to[k]) + c, a);
   else if (outs.dtype[k] == OSSM_BF16) put1(static_cast<__nv_bfloat16*>(outs.to[k]) + c, a);
   else put1(static_cast<__half*>(outs.to[k]) + c, a);
@@ -468,24 +610,34 @@ bool valid(const ossm_norm_args* a, bool bwd) {
 }
 
 struct Plan {
-  int R, N, per, blocks, sums;
-  bool full;
+  int R, N, per, at_once, blocks, sums;
   size_t bytes;
 };
-// Threads of a row: a warp up to 512 channels, then as many as make 16 channels each.
+constexpr int kRingBytes = 208 << 10;
+// Threads of a row: a warp up to 512 channels (8 rows a block), beyond that a
+// block with 16 channels a thread; backward, which keeps up to five sums a
+// channel in registers, 8 channels up to 2048.  (16384 x 2048, fp32 stream, two
+// norms and a gate: 103 us forward with 8 channels a thread, 86 us with 16;
+// 197 and 219 us backward.)
 Plan plan_of(const ossm_norm_args* a, bool bwd) {
   Plan q{};
-  q.full = a->post_norm || a->gate_kind;
   const int runs = (a->dim + 7) / 8;
-  q.N = runs <= 32 ? 1 : 2;
-  q.R = runs <= 64 ? 32 : (runs + 63) / 64 * 32;
-  q.per = q.R == 32 ? kWarpRows : 1;
-  const i64 rows = std::max<i64>(1, (a->tokens + q.per - 1) / q.per);
-  q.sums = q.full ? (int)kSums : 2;
-  if (bwd) {
-    q.blocks = (int)std::min<i64>(rows, 4LL * device_sms());
-    q.bytes = (size_t)q.blocks * q.sums * a->dim * 4;
+  const bool full = a->post_norm || a->gate_kind;
+  if (runs <= 64) {
+    q.N = runs <= 32 ? 1 : 2;
+    q.R = 32;
+    q.per = kWarpRows;
+  } else {
+    q.N = bwd && runs <= 256 ? 1 : 2;
+    q.R = ((runs + q.N - 1) / q.N + 31) / 32 * 32;
+    q.per = 1;
   }
+  const i64 rows = std::max<i64>(1, (a->tokens + q.per - 1) / q.per);
+  q.sums = full ? (int)kSums : a->grad_bias ? 2 : 1;
+  // blocks that are at work at once: 512 threads an SM backward, 768 forward
+  q.at_once = std::max(1, (bwd ? 512 : 768) / (q.R * q.per));
+  q.blocks = (int)std::min<i64>(rows, (i64)q.at_once * device_sms());
+  if (bwd) q.bytes = (size_t)q.blocks * q.sums * a->dim * 4;
   return q;
 }
 
@@ -498,7 +650,7 @@ Params params_of(const ossm_norm_args* a, const Plan& q, bool bwd) {
   };
   rows(a->x, a->x_stride, sx);
   rows(a->y, a->y_stride, sy);
-  rows(a->r, bwd && !q.full ? a->x_stride : a->dim, sx);
+  rows(a->r, bwd && q.sums < (int)kSums ? a->x_stride : a->dim, sx);
   if (bwd) {
     rows(a->grad_r, a->grad_r_stride, sx);
     rows(a->grad_h, a->grad_h_stride, sy);
@@ -510,10 +662,10 @@ Params params_of(const ossm_norm_args* a, const Plan& q, bool bwd) {
   }
   p.T = a->tokens, p.d = a->dim, p.R = q.R, p.vec = vec;
   p.x = a->x, p.y = a->y, p.xst = a->x_stride, p.yst = a->y_stride;
-  p.gate_kind = a->gate_kind, p.gate = {a->gate, a->gate_dtype}, p.gst = a->gate_stride;
+  p.gate_kind = a->gate_kind, p.gate = {a->gate, a->gate_dtype, nullptr}, p.gst = a->gate_stride;
   p.scale = a->scale, p.post = a->post_norm, p.norm = a->norm;
-  p.w = {a->weight, a->weight_dtype}, p.b = {a->bias, a->bias_dtype};
-  p.pw = {a->post_weight, a->post_weight_dtype}, p.pb = {a->post_bias, a->post_bias_dtype};
+  p.w = {a->weight, a->weight_dtype, nullptr}, p.b = {a->bias, a->bias_dtype, nullptr};
+  p.pw = {a->post_weight, a->post_weight_dtype, nullptr}, p.pb = {a->post_bias, a->post_bias_dtype, nullptr};
   auto aligned = [](const void* ptr) { return (uintptr_t)ptr % 16 == 0; };
   p.gate_vec = aligned(a->gate) && (a->gate_kind != OSSM_GATE_FULL || a->gate_stride * size_of(a->gate_dtype) % 16 == 0);
   p.w_vec = aligned(a->weight), p.b_vec = aligned(a->bias);
@@ -521,20 +673,57 @@ Params params_of(const ossm_norm_args* a, const Plan& q, bool bwd) {
   p.post_eps = a->post_eps, p.eps = a->eps, p.inv_d = 1.f / a->dim;
   p.r = a->r, p.h = a->h, p.stats = a->stats;
   p.dr = a->grad_r, p.dh = a->grad_h, p.drst = a->grad_r_stride, p.dhst = a->grad_h_stride;
+  p.status = a->status;
   p.dx = a->grad_x, p.dy = a->grad_y, p.dgate = a->grad_gate, p.dgate_dtype = a->gate_dtype;
   return p;
+}
+
+// The ring's stages, and the shared memory of a block: up to 8 rows ahead in
+// what the blocks of an SM share.  Rows of which no two fit take the scalar path.
+size_t ring_of(Params& p, const Plan& q, bool bwd) {
+  const size_t rows = (size_t)p.stage_bytes * q.per, most = kRingBytes / q.at_once;
+  size_t shared = 4 * (size_t)p.d * ((p.w.p != nullptr) + (p.b.p != nullptr) + (p.pw.p != nullptr) +
+                                     (p.pb.p != nullptr) + (p.gate_kind == G_CHANNEL));
+  p.shared = shared + (p.vec ? 2 * rows : 0) <= most;
+  if (!p.shared) shared = 0;
+  if (2 * rows > kRingBytes) p.vec = false;
+  p.stages = p.vec ? (int)std::max<size_t>(2, std::min<size_t>(kMaxStages, (most - std::min(most, shared)) / rows)) : 0;
+  return std::max(p.stages * rows + shared, bwd && q.per > 1 ? (size_t)q.per * 8 * q.N * q.R * 4 : 0);
 }
 
 template <typename TX, typename TY>
 int forward(const ossm_norm_args* a, cudaStream_t st) {
   const Plan q = plan_of(a, false);
-  const Params p = params_of(a, q, false);
-  const unsigned grid = (unsigned)((a->tokens + q.per - 1) / q.per);
-  auto kern = q.N == 1     ? norm_fwd_kernel<TX, TY, 1, 256>
-              : q.R <= 256 ? norm_fwd_kernel<TX, TY, 2, 256>
-                           : norm_fwd_kernel<TX, TY, 2, 1024>;
-  kern<<<grid, q.R * q.per, 0, st>>>(p);
+  Params p = params_of(a, q, false);
+  p.stage_bytes = a->dim * (int)(sizeof(TX) + (a->y ? sizeof(TY) : 0));
+  const size_t smem = ring_of(p, q, false);
+  auto kern = p.vec ? (q.N == 1     ? norm_fwd_kernel<TX, TY, 1, true, 256>
+                       : q.R <= 256 ? norm_fwd_kernel<TX, TY, 2, true, 256>
+                                    : norm_fwd_kernel<TX, TY, 2, true, 1024>)
+                    : (q.N == 1 ? norm_fwd_kernel<TX, TY, 1, false, 256> : norm_fwd_kernel<TX, TY, 2, false, 1024>);
+  static std::atomic<uint64_t> done[5];
+  if (allow_smem(kern, kRingBytes, done[p.vec ? (q.N == 1 ? 0 : q.R <= 256 ? 1 : 2) : 2 + q.N]) != cudaSuccess)
+    return OSSM_ELAUNCH;
+  kern<<<q.blocks, q.R * q.per, smem, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
+}
+
+// N and MAXT by the plan.
+template <typename TX, typename TY, int SUMS>
+bool launch_bwd(const Plan& q, Params& p, cudaStream_t st) {
+  p.stage_bytes = p.d * (int)(sizeof(TX) + (p.dr ? sizeof(TX) : 0) + (p.dh ? sizeof(TY) : 0) +
+                              (SUMS == (int)kSums ? sizeof(TY) : 0));
+  const size_t smem = ring_of(p, q, true);
+  auto kern = p.vec ? (q.N == 1     ? norm_bwd_kernel<TX, TY, 1, true, SUMS, 256>
+                       : q.R <= 256 ? norm_bwd_kernel<TX, TY, 2, true, SUMS, 256>
+                                    : norm_bwd_kernel<TX, TY, 2, true, SUMS, 1024>)
+                    : (q.N == 1 ? norm_bwd_kernel<TX, TY, 1, false, SUMS, 256>
+                                : norm_bwd_kernel<TX, TY, 2, false, SUMS, 1024>);
+  static std::atomic<uint64_t> done[5];
+  if (allow_smem(kern, kRingBytes, done[p.vec ? (q.N == 1 ? 0 : q.R <= 256 ? 1 : 2) : 2 + q.N]) != cudaSuccess)
+    return false;
+  kern<<<q.blocks, q.R * q.per, smem, st>>>(p);
+  return true;
 }
 
 template <typename TX, typename TY>
@@ -544,15 +733,10 @@ int backward(const ossm_norm_args* a, const Plan& q, float* part, cudaStream_t s
                     (a->gate_kind == OSSM_GATE_CHANNEL && a->grad_gate);
   p.part = sums ? part : nullptr;
   if (a->gate_kind == OSSM_GATE_CHANNEL) p.dgate = nullptr;
-  const bool big = q.R > 256;
-  auto kern = q.full ? (q.N == 1 ? norm_bwd_kernel<TX, TY, 1, true, 256>
-                        : big    ? norm_bwd_kernel<TX, TY, 2, true, 1024>
-                                 : norm_bwd_kernel<TX, TY, 2, true, 256>)
-                     : (q.N == 1 ? norm_bwd_kernel<TX, TY, 1, false, 256>
-                        : big    ? norm_bwd_kernel<TX, TY, 2, false, 1024>
-                                 : norm_bwd_kernel<TX, TY, 2, false, 256>);
-  const size_t smem = q.per > 1 ? (size_t)q.per * 8 * q.N * q.R * 4 : 0;
-  kern<<<q.blocks, q.R * q.per, smem, st>>>(p);
+  if (!(q.sums == 1   ? launch_bwd<TX, TY, 1>(q, p, st)
+        : q.sums == 2 ? launch_bwd<TX, TY, 2>(q, p, st)
+                      : launch_bwd<TX, TY, kSums>(q, p, st)))
+    return OSSM_ELAUNCH;
   if (sums) {
     Outs o{};
     o.to[S_W] = a->grad_weight, o.dtype[S_W] = a->weight_dtype;
@@ -560,7 +744,7 @@ int backward(const ossm_norm_args* a, const Plan& q, float* part, cudaStream_t s
     if (a->gate_kind == OSSM_GATE_CHANNEL) o.to[S_GATE] = a->grad_gate, o.dtype[S_GATE] = a->gate_dtype;
     o.to[S_PW] = a->grad_post_weight, o.dtype[S_PW] = a->post_weight_dtype;
     o.to[S_PB] = a->grad_post_bias, o.dtype[S_PB] = a->post_bias_dtype;
-    norm_sums_kernel<<<dim3((a->dim + 31) / 32, q.sums), 256, 0, st>>>(part, q.blocks, q.sums, a->dim, o);
+    norm_sums_kernel<<<dim3((a->dim + 31) / 32, q.sums), 1024, 0, st>>>(part, q.blocks, q.sums, a->dim, o);
   }
   return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
 }

@@ -287,6 +287,7 @@ def _norm_forward(x, y, w, b, gate, pw, pb, opts, want_stats):
     w, b, pw, pb = (None if t is None else t.contiguous() for t in (w, b, pw, pb))
     g, gst = _gate_rows(gate, kind, d)
     a = _norm_args(T, d, x.dtype, dt, g, kind, gst, scale, norm, post, eps, post_eps, w, b, pw, pb)
+    a.status = _status(dev, _raw_stream(dev))
     a.x, a.x_stride = xr.data_ptr(), xst
     r = x
     if y is not None:
@@ -327,6 +328,7 @@ class _NormFn(torch.autograd.Function):
         wc, bc, pwc, pbc = (None if t is None else t.contiguous() for t in (w, b, pw, pb))
         g, gst = _gate_rows(gate, kind, d)
         a = _norm_args(T, d, x.dtype, dt, g, kind, gst, scale, norm, post, eps, post_eps, wc, bc, pwc, pbc)
+        a.status = _status(dev, _raw_stream(dev))
         a.stats = stats.data_ptr()
         a.x_stride = xst
         if ctx.full:
