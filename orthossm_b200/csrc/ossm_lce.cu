@@ -39,7 +39,7 @@ constexpr int kM = 128, kN = 256, kK = 64;  // a tile, and the depth of one load
 constexpr int kStages = 4;
 constexpr int kThreads = 320;               // 8 warps read tensor memory, one loads, one issues products
 constexpr int kABytes = kM * kK * 2, kBBytes = kN * kK * 2, kStage = kABytes + kBBytes;
-constexpr int kOut = 8 * 32 * 128;          // a [32 rows x 64 columns] box a warp
+constexpr int kOut = 8 * 2 * 32 * 64;       // two [32 rows x 32 columns] boxes a warp
 constexpr size_t kSmem = kStages * (size_t)kStage + kOut + 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowThreads = 256;
@@ -75,6 +75,9 @@ struct Params {
   float* zt;         // [Tpad] the target's logit
   double* sums;      // [kMaxBlocks]
   float* dh32;       // [tiles] sums of dH over the pieces, in the order of tensor memory
+  float* cuts;       // [2 a CTA] sums of tiles that are cut, the same
+  uint32_t* counts;  // [2 a CTA] steps that are done of tiles that are cut, 0 before a piece
+  int ncounts;
   int panels, pan;   // panels of `pan` tiles of columns
   int v0, vp;        // the piece: columns v0 .. v0 + vp
   int first, last;   // the piece is the first, the last
@@ -118,6 +121,7 @@ OSSM_DEV void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int 
                "r"(smem_u32(src)), "r"(c0), "r"(c1)
                : "memory");
 }
+OSSM_DEV void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 OSSM_DEV void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Instruction descriptor: fp32 accumulator, 16-bit operands (0 = fp16, 1 =
@@ -387,33 +391,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 c2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-lse2, -lse2);
           const float2 a2 = make_float2(fa, fa);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < 4; ++h) {
 #pragma unroll
-            for (int i = 32 * h; i < 32 * h + 32; ++i) {
+            for (int i = 16 * h; i < 16 * h + 16; ++i) {
               float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), c2, m2);
               y = mul2(make_float2(ex2(y.x), ex2(y.y)), a2);
               x[2 * i] = y.x, x[2 * i + 1] = y.y;
             }
             if (here) {
 #pragma unroll
-              for (int i = 64 * h; i < 64 * h + 64; ++i) x[i] = i == at ? x[i] - fb : x[i];
+              for (int i = 32 * h; i < 32 * h + 32; ++i) x[i] = i == at ? x[i] - fb : x[i];
             }
             if (cols < 128 || !live) {
 #pragma unroll
-              for (int i = 64 * h; i < 64 * h + 64; ++i) x[i] = live && i < cols ? x[i] : 0.f;
+              for (int i = 32 * h; i < 32 * h + 32; ++i) x[i] = live && i < cols ? x[i] : 0.f;
             }
-            if (lane == 0) bulk_wait_read0();
+            if (lane == 0) bulk_wait_read1();  // the box before the last has left
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float* y = x + 64 * h + 8 * i;
-              *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+            for (int i = 0; i < 4; ++i) {
+              const float* y = x + 32 * h + 8 * i;
+              *reinterpret_cast<uint4*>(box + (h & 1) * 2048 + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
                   make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&mZ, box, c0 + 64 * h, block * kM + (warp & 3) * 32);
+              tma_store_2d(&mZ, box + (h & 1) * 2048, c0 + 32 * h, block * kM + (warp & 3) * 32);
               bulk_commit();
             }
           }
@@ -427,6 +431,79 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- dW = dZ^T H of the piece, dH += dZ W
+// The tiles of both products.  Whole rounds of them, one a CTA, run side by
+// side, so that the CTAs at work share what they read of dZ; the tiles that are
+// left over stand on a line, which is cut evenly over the CTAs.  A tile that is
+// cut leaves sums in the workspace, and the CTA that finishes it last adds them
+// up in order.  (T = 16384, 512 channels, pieces of 16384 columns: 508 tiles on
+// 148 CTAs, 3.43 rounds.)
+struct Tiles {
+  int nt, tw, th, kw, kh;  // tiles a row of tiles, of dW, of dH; their steps
+  int ncta, rw, rh, lw, lh;  // rounds, and what is left
+  i64 line;
+  OSSM_DEV Tiles(const Params& p, int n, int cols, int grid) {
+    const int nn = max(n, 1);
+    nt = (p.d + kN - 1) / kN;
+    tw = p.dw ? (cols + kM - 1) / kM * nt : 0;
+    th = p.dh ? (nn + kM - 1) / kM * nt : 0;
+    kw = (nn + kK - 1) / kK, kh = (cols + kK - 1) / kK;
+    ncta = grid;
+    rw = tw / ncta, lw = tw % ncta;
+    rh = th / ncta, lh = th % ncta;
+    line = (i64)lw * kw + (i64)lh * kh;
+  }
+  // What is left over: tile i of the line starts at...
+  OSSM_DEV i64 start(int i) const { return i < lw ? (i64)i * kw : (i64)lw * kw + (i64)(i - lw) * kh; }
+  OSSM_DEV int steps(int i) const { return i < lw ? kw : kh; }
+  OSSM_DEV int at(i64 pos) const { return pos < (i64)lw * kw ? (int)(pos / kw) : lw + (int)((pos - (i64)lw * kw) / kh); }
+  // Where CTA c's part of the line begins.  A cut within 16 steps of its tile's
+  // edge (an eighth of a short one) moves to the edge.
+  OSSM_DEV i64 cut(int c) const {
+    if (c >= ncta) return line;
+    const i64 pos = line / ncta * c + line % ncta * c / ncta;
+    const int i = at(pos), k = steps(i), near = min(16, k / 8);
+    const i64 s = start(i);
+    return pos - s <= near ? s : s + k - pos <= near ? s + k : pos;
+  }
+};
+struct Item {
+  bool w;       // of dW
+  int m0, n0;   // the tile
+  int k0, k1;   // its steps here
+  bool split;
+  int rest;     // split: the tile's place on the line
+};
+struct Shares {  // of one CTA, in order
+  const Tiles& t;
+  int cta, round;
+  i64 pos, end;
+  OSSM_DEV Shares(const Tiles& tiles, int c) : t(tiles), cta(c), round(0), pos(tiles.cut(c)), end(tiles.cut(c + 1)) {}
+  OSSM_DEV bool next(Item& x) {
+    int u;
+    if (round < t.rw + t.rh) {
+      x.w = round < t.rw;
+      u = (x.w ? round : round - t.rw) * t.ncta + cta;
+      ++round;
+      x.k0 = 0, x.k1 = x.w ? t.kw : t.kh;
+      x.split = false;
+    } else {
+      if (pos >= end) return false;
+      const int i = t.at(pos);
+      const i64 s = t.start(i);
+      x.w = i < t.lw;
+      u = x.w ? t.rw * t.ncta + i : t.rh * t.ncta + i - t.lw;
+      x.k0 = (int)(pos - s);
+      x.k1 = (int)min((i64)t.steps(i), end - s);
+      x.split = x.k1 - x.k0 < t.steps(i);
+      x.rest = i;
+      pos = s + x.k1;
+    }
+    x.m0 = u / t.nt * kM, x.n0 = u % t.nt * kN;
+    return true;
+  }
+};
+constexpr size_t kPart = (size_t)kM * kN;  // floats of a tile's sums
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     lce_prod_kernel(const __grid_constant__ CUtensorMap mZm, const __grid_constant__ CUtensorMap mZk,
@@ -437,37 +514,33 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Shared s;
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   setup(s, warp);
-  const int n = p.head->n, nn = max(n, 1);
-  const int cols = min(p.vp, p.V - p.v0);
-  const int nt = (p.d + kN - 1) / kN;
-  const int tw = p.dw ? (cols + kM - 1) / kM * nt : 0;  // tiles of dW, then those of dH
-  const int th = p.dh ? (nn + kM - 1) / kM * nt : 0;
-  const int kw = (nn + kK - 1) / kK, kh = (cols + kK - 1) / kK;
+  const int n = p.head->n, cols = min(p.vp, p.V - p.v0);
+  const Tiles tiles(p, n, cols, gridDim.x);
+  Shares todo(tiles, blockIdx.x);
+  Item x;
 
   if (warp == 8) {
     if (lane == 0) {
       const CUtensorMap* hm = n == p.T ? &mH : &mHc;
       Loader ld{s, smem, 0};
       bool ok = true;
-      for (int t = blockIdx.x; t < tw + th && ok; t += gridDim.x) {
-        const bool w = t < tw;
-        const int u = w ? t : t - tw, m0 = u / nt * kM, n0 = u % nt * kN;
-        const int boxes = min(4, (p.d - n0 + 63) / 64), steps = w ? kw : kh;
-        for (int k = 0; k < steps; ++k) {
+      while (ok && todo.next(x)) {
+        const int boxes = min(4, (p.d - x.n0 + 63) / 64);
+        for (int k = x.k0; k < x.k1; ++k) {
           uint64_t* bar;
           uint8_t* to = ld.next(kABytes + boxes * kBox, bar);
           if (!to) {
             ok = false;
             break;
           }
-          if (w) {
-            tma_load_2d(to, &mZm, bar, m0, k * kK);
-            tma_load_2d(to + kBox, &mZm, bar, m0 + 64, k * kK);
-            for (int i = 0; i < boxes; ++i) tma_load_2d(to + kABytes + i * kBox, hm, bar, n0 + 64 * i, k * kK);
+          if (x.w) {
+            tma_load_2d(to, &mZm, bar, x.m0, k * kK);
+            tma_load_2d(to + kBox, &mZm, bar, x.m0 + 64, k * kK);
+            for (int i = 0; i < boxes; ++i) tma_load_2d(to + kABytes + i * kBox, hm, bar, x.n0 + 64 * i, k * kK);
           } else {
-            tma_load_2d(to, &mZk, bar, k * kK, m0);
+            tma_load_2d(to, &mZk, bar, k * kK, x.m0);
             for (int i = 0; i < boxes; ++i)
-              tma_load_2d(to + kABytes + i * kBox, &mW, bar, n0 + 64 * i, p.v0 + k * kK);
+              tma_load_2d(to + kABytes + i * kBox, &mW, bar, x.n0 + 64 * i, p.v0 + k * kK);
           }
         }
       }
@@ -478,65 +551,107 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
     Issuer mm{s, smem_u32(smem), 0, 0};
     bool ok = true;
-    for (int t = blockIdx.x; t < tw + th && ok; t += gridDim.x) {
-      const bool w = t < tw;
-      const int u = w ? t : t - tw, n0 = u % nt * kN, N = min(kN, (p.d - n0 + 63) / 64 * 64);
-      ok = mm.tile(w ? kw : kh, idesc(fmt, w, 1, N), w ? 2048 : 32, 2048, leader);
+    while (ok && todo.next(x)) {
+      const int N = min(kN, (p.d - x.n0 + 63) / 64 * 64);
+      ok = mm.tile(x.k1 - x.k0, idesc(fmt, x.w, 1, N), x.w ? 2048 : 32, 2048, leader);
     }
   } else {
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tl = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
     const float unit = p.head->unit;
-    uint32_t tiles = 0;
+    uint32_t done = 0;
     bool dead = false;
-    for (int t = blockIdx.x; t < tw + th; t += gridDim.x, ++tiles) {
-      const bool w = t < tw;
-      const int u = w ? t : t - tw, m0 = u / nt * kM, n0 = u % nt * kN + half * 128;
-      const uint32_t b = tiles & 1;
-      if (!dead) dead = gave_up(&s.acc_full[b], (tiles >> 1) & 1, &s.failed);
+    for (; todo.next(x); ++done) {
+      const uint32_t b = done & 1;
+      if (!dead) dead = gave_up(&s.acc_full[b], (done >> 1) & 1, &s.failed);
       __syncwarp();
       tc_fence_after();
-      const int r = m0 + row;
+      const int r = x.m0 + row, n0 = x.n0 + half * 128;
       T* to = nullptr;
-      if (w) {
+      if (x.w) {
         if (r < cols) to = static_cast<T*>(p.dw) + (i64)(p.v0 + r) * p.d + n0;
       } else if (r < n) {
         to = static_cast<T*>(p.dh) + (i64)__ldg(p.rows + r) * p.d + n0;
       }
-      float4* sum = w ? nullptr : reinterpret_cast<float4*>(p.dh32) + ((i64)u * 2 + half) * 32 * kM + row;
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        if (n0 + 32 * i >= p.d) break;
-        float x[32];
-        tmem_ld32_nowait(tl + b * kN + 32 * i, x);
-        tmem_wait_ld();
-        pin32(x);
-        if (!w && !p.first) {
+      // dH's sums over the earlier pieces of the vocabulary; float4 e of every row side by side
+      const int u = x.m0 / kM * tiles.nt + x.n0 / kN;
+      float4* sum = x.w ? nullptr : reinterpret_cast<float4*>(p.dh32 + u * kPart) + half * 32 * kM + row;
+      auto finish = [&](int i, float (&y)[32]) {  // columns 32 i .. of this half
+        if (!x.w && !p.first) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float4 y = sum[(8 * i + e) * kM];
-            x[4 * e] += y.x, x[4 * e + 1] += y.y, x[4 * e + 2] += y.z, x[4 * e + 3] += y.w;
+            const float4 q = sum[(8 * i + e) * kM];
+            y[4 * e] += q.x, y[4 * e + 1] += q.y, y[4 * e + 2] += q.z, y[4 * e + 3] += q.w;
           }
         }
-        if (!w && !p.last) {
+        if (!x.w && !p.last) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            sum[(8 * i + e) * kM] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+            sum[(8 * i + e) * kM] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
         } else if (to) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if (n0 + 32 * i + 8 * e >= p.d) break;
-            const float* y = x + 8 * e;
+            const float* z = y + 8 * e;
             *reinterpret_cast<uint4*>(to + 32 * i + 8 * e) =
-                make_uint4(pack2<T>(y[0] * unit, y[1] * unit), pack2<T>(y[2] * unit, y[3] * unit),
-                           pack2<T>(y[4] * unit, y[5] * unit), pack2<T>(y[6] * unit, y[7] * unit));
+                make_uint4(pack2<T>(z[0] * unit, z[1] * unit), pack2<T>(z[2] * unit, z[3] * unit),
+                           pack2<T>(z[4] * unit, z[5] * unit), pack2<T>(z[6] * unit, z[7] * unit));
           }
+        }
+      };
+      float4* part = reinterpret_cast<float4*>(p.cuts + (2 * blockIdx.x + (x.k0 == 0)) * kPart) + half * 32 * kM + row;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        if (n0 + 32 * i >= p.d) break;
+        float y[32];
+        tmem_ld32_nowait(tl + b * kN + 32 * i, y);
+        tmem_wait_ld();
+        pin32(y);
+        if (x.split) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            part[(8 * i + e) * kM] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+        } else {
+          finish(i, y);
         }
         __syncwarp();
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+      if (!x.split) continue;
+      __threadfence();
+      named_sync(1, 256);
+      if (threadIdx.x == 0) {
+        const uint32_t have = atomicAdd(p.counts + x.rest, (uint32_t)(x.k1 - x.k0)) + (x.k1 - x.k0);
+        s.last_in = have == (uint32_t)tiles.steps(x.rest);
+        if (s.last_in) p.counts[x.rest] = 0;  // for the next piece
+      }
+      named_sync(1, 256);
+      if (!s.last_in) continue;
+      __threadfence();
+      // the pieces, in order: the CTA in whose part the tile starts, and the ones after it
+      const i64 from = tiles.start(x.rest), upto = from + tiles.steps(x.rest);
+      int c0 = blockIdx.x;
+      while (c0 > 0 && tiles.cut(c0) > from) --c0;
+      while (tiles.cut(c0 + 1) <= from) ++c0;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        if (n0 + 32 * i >= p.d) break;
+        float y[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) y[e] = 0.f;
+        for (int c = c0; c == c0 || tiles.cut(c) < upto; ++c) {
+          if (c > c0 && tiles.cut(c + 1) == tiles.cut(c)) continue;  // no part at all
+          const float4* q = reinterpret_cast<const float4*>(p.cuts + (2 * c + (c == c0)) * kPart) + half * 32 * kM + row;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 v = __ldcg(q + (8 * i + e) * kM);
+            y[4 * e] += v.x, y[4 * e + 1] += v.y, y[4 * e + 2] += v.z, y[4 * e + 3] += v.w;
+          }
+        }
+        finish(i, y);
+      }
     }
   }
   teardown(s, warp, p.status);
@@ -569,13 +684,28 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   i64 before = 0, all = 0;
   float top = 0.f;
-  for (i64 t = threadIdx.x; t < p.T; t += kRowThreads) {
-    const bool has = __ldg(p.targets + t) != p.ignore;
-    all += has;
-    before += has && t < c0;
-    if (BWD && has) {
-      const float f = p.reduction ? 1.f : fabsf(__ldg(p.g + t));
-      top = fmaxf(top, f * fmaxf(1.f, fabsf(1.f + 2.f * p.zl * __ldg(p.lse + t))));
+  for (i64 t0 = threadIdx.x; t0 < p.T; t0 += 8 * kRowThreads) {  // 8 loads on their way
+    bool has[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const i64 t = t0 + i * kRowThreads;
+      has[i] = t < p.T && __ldg(p.targets + t) != p.ignore;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      all += has[i];
+      before += has[i] && t0 + i * kRowThreads < c0;
+    }
+    if (BWD && (p.zl > 0.f || !p.reduction)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const i64 t = t0 + i * kRowThreads;
+        const float f = p.reduction || t >= p.T ? 1.f : fabsf(__ldg(p.g + t));
+        const float l = p.zl > 0.f && t < p.T ? __ldg(p.lse + t) : 0.f;
+        if (has[i]) top = fmaxf(top, f * fmaxf(1.f, fabsf(1.f + 2.f * p.zl * l)));
+      }
+    } else if (BWD) {
+      top = 1.f;
     }
   }
   auto plus = [](i64 a, i64 b) { return a + b; };
@@ -593,6 +723,8 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
     p.head->unit = inv > 0.f ? scale / inv : 0.f;
     p.head->count = 0;
   }
+  if (BWD && blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.ncounts; i += kRowThreads) p.counts[i] = 0;
   const bool gather = all < p.T;
   const int vecs = p.d / 8;
   i64 base = before;
@@ -630,15 +762,27 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
     }
     if (!gather) continue;
     __syncthreads();
-    for (int i = warp; i < (int)min((i64)kRowThreads, c1 - t0); i += kRowThreads / 32) {
-      const int to = places[i];
-      if (to >= 0) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.hidden) + (t0 + i) * p.hst);
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.hc) + (i64)to * p.d);
-        for (int e = lane; e < vecs; e += 32) dst[e] = __ldg(src + e);
-      } else if (BWD && p.dh) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dh) + (t0 + i) * p.d);
-        for (int e = lane; e < vecs; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
+    const int count_here = (int)min((i64)kRowThreads, c1 - t0), pieces = count_here * vecs;
+    for (int e0 = threadIdx.x; e0 < pieces; e0 += 8 * kRowThreads) {
+      uint4 v[8];
+      int row[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = e0 + k * kRowThreads;
+        row[k] = e / vecs;
+        if (e < pieces && places[row[k]] >= 0)
+          v[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.hidden) + (t0 + row[k]) * p.hst) +
+                       (e - row[k] * vecs));
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = e0 + k * kRowThreads, at = e - row[k] * vecs;
+        if (e >= pieces) break;
+        const int to = places[row[k]];
+        if (to >= 0)
+          reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.hc) + (i64)to * p.d)[at] = v[k];
+        else if (BWD && p.dh)
+          reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dh) + (t0 + row[k]) * p.d)[at] = make_uint4(0, 0, 0, 0);
       }
     }
   }
@@ -755,19 +899,22 @@ Plan plan_of(const ossm_lce_args* a, bool bwd) {
     take(2 * T * (size_t)q.vp);  // dz
     const size_t nt = (d + kN - 1) / kN;
     take(a->grad_hidden && q.vp < q.Vpad ? 4 * T * nt * kN : 0);
+    take(2 * q.sms * kPart * 4);
+    take(2 * q.sms * 4);
   }
   q.bytes = at;
   return q;
 }
 
-// [rows, inner] with 128-byte swizzle, box [brows, 64].
-bool encode(CUtensorMap* map, int dtype, const void* base, i64 inner, i64 rows, i64 stride, int brows) {
+// [rows, inner], box [brows, bcols], swizzled over the bytes of a box's row.
+bool encode(CUtensorMap* map, int dtype, const void* base, i64 inner, i64 rows, i64 stride, int brows, int bcols = 64) {
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)brows}, estr[2] = {1, 1};
+  cuuint32_t box[2] = {(cuuint32_t)bcols, (cuuint32_t)brows}, estr[2] = {1, 1};
   return fast::encode_fn()(map, dtype == OSSM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                            2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           bcols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -790,13 +937,16 @@ Params params_of(const ossm_lce_args* a, const Plan& q, char* w, bool bwd) {
     p.fa = reinterpret_cast<float*>(w + q.at[5]);
     p.fb = reinterpret_cast<float*>(w + q.at[6]);
     p.dh32 = reinterpret_cast<float*>(w + q.at[8]);
+    p.cuts = reinterpret_cast<float*>(w + q.at[9]);
+    p.counts = reinterpret_cast<uint32_t*>(w + q.at[10]);
+    p.ncounts = 2 * q.sms;
   }
   p.panels = q.panels, p.pan = q.pan, p.vp = q.vp;
   p.status = a->status;
   return p;
 }
 
-int row_blocks(const Plan& q, i64 T) { return (int)std::min<i64>(q.sms, (T + kRowThreads - 1) / kRowThreads); }
+int row_blocks(const Plan& q, i64 T) { return (int)std::min<i64>(q.sms, (T + 31) / 32); }
 
 template <typename T>
 int forward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
@@ -825,7 +975,7 @@ int backward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kM) ||
       !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kM) ||
       !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kN) ||
-      !encode(&ms, a->dtype, dz, q.vp, q.Tpad, q.vp, 32) || !encode(&mzm, a->dtype, dz, q.vp, q.Tpad, q.vp, 64) ||
+      !encode(&ms, a->dtype, dz, q.vp, q.Tpad, q.vp, 32, 32) || !encode(&mzm, a->dtype, dz, q.vp, q.Tpad, q.vp, 64) ||
       !encode(&mzk, a->dtype, dz, q.vp, q.Tpad, q.vp, kM) ||
       !encode(&hm, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, 64) ||
       !encode(&hcm, a->dtype, p.hc, a->dim, q.Tpad, a->dim, 64) ||
