@@ -35,12 +35,18 @@ using attn::ex2;
 using attn::pack2;
 typedef long long i64;
 
-constexpr int kM = 128, kN = 256, kK = 64;  // a tile, and the depth of one load
-constexpr int kStages = 4;
+// A tile of 256 x 256 is made by the two CTAs of a cluster (cta_group::2): each
+// loads 128 rows of A and 128 of B and holds 128 rows of sums, and one issues the
+// products for both.  A stage is 32 KB and feeds 512 cycles of the tensor core;
+// with a CTA alone on 128 x 256 it was 48 KB, and four stages did not cover the
+// way from HBM (tensor pipe 61 % busy in the products with dz, 1.57 GHz).
+constexpr int kM = 256, kN = 256, kK = 64;  // a tile, and the depth of one load
+constexpr int kHalf = 128;                  // rows of A and of B that a CTA loads
 constexpr int kThreads = 320;               // 8 warps read tensor memory, one loads, one issues products
-constexpr int kABytes = kM * kK * 2, kBBytes = kN * kK * 2, kStage = kABytes + kBBytes;
-constexpr int kOut = 8 * 2 * 32 * 64;       // two [32 rows x 32 columns] boxes a warp
-constexpr size_t kSmem = kStages * (size_t)kStage + kOut + 1024;
+constexpr int kABytes = kHalf * kK * 2, kStage = 2 * kABytes;
+constexpr int kOut = 8 * 2 * 32 * 128;      // gradz: two [32 rows x 64 columns] boxes a warp
+constexpr int kStages = 6, kStagesZ = 5;
+constexpr size_t smem_bytes(int stages, bool out) { return stages * (size_t)kStage + (out ? kOut : 0) + 1024; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowThreads = 256;
 constexpr int kMaxBlocks = 1024;
@@ -88,7 +94,7 @@ struct Params {
 OSSM_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
@@ -108,11 +114,29 @@ OSSM_DEV bool gave_up(uint64_t* bar, uint32_t parity, int* failed) {
   return false;
 }
 
-OSSM_DEV void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+OSSM_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+OSSM_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of a barrier of the pair's first CTA.
+OSSM_DEV uint32_t first_cta(const uint64_t* bar) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+  return r;
+}
+OSSM_DEV void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Into this CTA's shared memory, counted by a barrier of the pair's first CTA.
+OSSM_DEV void tma_load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
 OSSM_DEV void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
@@ -121,7 +145,6 @@ OSSM_DEV void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int 
                "r"(smem_u32(src)), "r"(c0), "r"(c1)
                : "memory");
 }
-OSSM_DEV void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 OSSM_DEV void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Instruction descriptor: fp32 accumulator, 16-bit operands (0 = fp16, 1 =
@@ -141,12 +164,23 @@ OSSM_DEV uint64_t sdesc(uint32_t saddr) {
 OSSM_DEV void mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t id, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(ad), "l"(bd), "r"(id), "r"(acc)
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(ad), "l"(bd), "r"(id), "r"(acc)
       : "memory");
 }
+// Arrives at the barrier of this place in both CTAs once the products are done.
 OSSM_DEV void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+OSSM_DEV void pair_alloc(uint32_t* slot) {  // whole warp, in both CTAs: all columns
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+OSSM_DEV void pair_dealloc(uint32_t taddr) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
 }
 OSSM_DEV bool elect_one() {
   uint32_t r;
@@ -171,71 +205,83 @@ OSSM_DEV void pin32(float* v) {
 }
 
 // ---------------------------------------------------------------- what the tensor-core kernels share
+template <int S>
 struct Shared {
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  uint64_t full[S], empty[S], acc_full[2], acc_empty[2];  // full, acc_empty: those of the first CTA are used
   uint32_t tmem;
   int failed, last_in;
 };
 
 // Barriers, tensor memory: all threads, before the roles part.
-OSSM_DEV void setup(Shared& s, int warp) {
+template <int S>
+OSSM_DEV void setup(Shared<S>& s, int warp) {
   if (threadIdx.x == 0) {
     s.failed = 0;
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < S; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.acc_full[i], 1);
-      mbar_init(&s.acc_empty[i], 8);
+      mbar_init(&s.acc_empty[i], 16);
     }
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc(&s.tmem, 512);
+  if (warp == 9) pair_alloc(&s.tmem);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
 }
-OSSM_DEV void teardown(Shared& s, int warp, uint32_t* status) {
+template <int S>
+OSSM_DEV void teardown(Shared<S>& s, int warp, uint32_t* status) {
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // neither CTA's memory goes before the other is through
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(s.tmem, 512);
+    pair_dealloc(s.tmem);
   }
   if (threadIdx.x == 0 && s.failed && status) atomicExch(status, (uint32_t)OSSM_ETIMEOUT);
 }
 
-// The ring of loaded stages, on the loading side.
+// The ring of loaded stages, on the loading side of either CTA.
+template <int S>
 struct Loader {
-  Shared& s;
+  Shared<S>& s;
   uint8_t* ring;
-  uint32_t i;
-  OSSM_DEV uint8_t* next(uint32_t bytes, uint64_t*& bar) {  // NULL: give up
-    const uint32_t r = i % kStages;
-    if (i >= kStages && gave_up(&s.empty[r], ((i / kStages) & 1) ^ 1, &s.failed)) return nullptr;
-    ++i;
-    bar = &s.full[r];
-    mbar_expect_tx(bar, bytes);
-    return ring + r * kStage;
+  bool first;  // the pair's first CTA expects the bytes of both
+  uint32_t r, turn, n;
+  OSSM_DEV uint8_t* next(uint32_t bytes, uint32_t& bar) {  // NULL: give up
+    if (n >= S && gave_up(&s.empty[r], turn ^ 1, &s.failed)) return nullptr;
+    if (first) mbar_expect_tx(&s.full[r], 2 * bytes);
+    bar = first_cta(&s.full[r]);
+    uint8_t* to = ring + r * kStage;
+    ++n;
+    if (++r == S) r = 0, turn ^= 1;
+    return to;
   }
-  OSSM_DEV void drain() {  // no copy may still be landing when the CTA exits
-    for (uint32_t j = i > kStages ? i - kStages : 0; j < i; ++j) gave_up(&s.full[j % kStages], (j / kStages) & 1, &s.failed);
+  // No copy, and no arrival at this CTA's barriers, may be on its way when the CTAs exit.
+  OSSM_DEV void end(bool ok) {
+    for (uint32_t j = n > S ? n - S : 0; j < n; ++j)
+      if (ok) gave_up(&s.empty[j % S], (j / S) & 1, &s.failed);
+      else if (first) gave_up(&s.full[j % S], (j / S) & 1, &s.failed);
   }
 };
 
-// One tile's products: `steps` stages into the accumulator at column `acc`.
-// a_step, b_step: bytes between the starts of two 16-deep products.
+// One tile's products: `steps` stages into the sums of this turn (the first CTA
+// issues them, a whole warp walks).  a_step, b_step: bytes between the starts of
+// two 16-deep products.
+template <int S>
 struct Issuer {
-  Shared& s;
-  uint32_t ring, i, tiles;
+  Shared<S>& s;
+  uint32_t ring, r, turn, tiles;
   OSSM_DEV bool tile(int steps, uint32_t id, uint32_t a_step, uint32_t b_step, bool leader) {
     const uint32_t b = tiles & 1;
     if (tiles >= 2 && __any_sync(~0u, gave_up(&s.acc_empty[b], ((tiles >> 1) & 1) ^ 1, &s.failed))) return false;
     tc_fence_after();
-    for (int k = 0; k < steps; ++k, ++i) {
-      const uint32_t r = i % kStages;
-      if (__any_sync(~0u, gave_up(&s.full[r], (i / kStages) & 1, &s.failed))) return false;
+    for (int k = 0; k < steps; ++k) {
+      if (__any_sync(~0u, gave_up(&s.full[r], turn, &s.failed))) return false;
       tc_fence_after();
       if (leader) {
         const uint64_t ad = sdesc(ring + r * kStage), bd = sdesc(ring + r * kStage + kABytes);
@@ -245,6 +291,7 @@ struct Issuer {
         mma_commit(&s.empty[r]);
       }
       __syncwarp();
+      if (++r == S) r = 0, turn ^= 1;
     }
     if (leader) mma_commit(&s.acc_full[b]);
     __syncwarp();
@@ -256,8 +303,8 @@ struct Issuer {
 // ---------------------------------------------------------------- logits
 enum { STATS, GRADZ };
 
-// Items of the logits kernels: a block of 128 rows by a panel of columns.  Of
-// 16 blocks of rows all take a panel before the next one, so that the CTAs at
+// Items of the logits kernels: a block of 256 rows by a panel of columns.  Of
+// 8 blocks of rows all take a panel before the next one, so that the CTAs at
 // work read the same columns of W and a few blocks of rows, which L2 keeps.
 struct Walk {
   int blocks, panels, items;
@@ -267,21 +314,23 @@ struct Walk {
     items = blocks * panels;
   }
   OSSM_DEV void at(int it, int& block, int& panel) const {
-    const int g = it / (16 * panels), r = it - g * 16 * panels, rows = min(16, blocks - 16 * g);
+    const int g = it / (8 * panels), r = it - g * 8 * panels, rows = min(8, blocks - 8 * g);
     panel = r / rows;
-    block = 16 * g + r % rows;
+    block = 8 * g + r % rows;
   }
 };
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     lce_logits_kernel(const __grid_constant__ CUtensorMap mH, const __grid_constant__ CUtensorMap mHc,
                       const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mZ,
                       const __grid_constant__ Params p) {
+  constexpr int S = MODE == GRADZ ? kStagesZ : kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ Shared s;
+  __shared__ Shared<S> s;
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   setup(s, warp);
   const int n = p.head->n;
   const Walk walk(p);
@@ -291,46 +340,49 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 8) {
     if (lane == 0) {
       const CUtensorMap* a = n == p.T ? &mH : &mHc;
-      Loader ld{s, smem, 0};
+      Loader<S> ld{s, smem, rank == 0, 0, 0, 0};
       bool ok = true;
-      for (int it = blockIdx.x; it < walk.items && ok; it += gridDim.x) {
+      for (int it = pair; it < walk.items && ok; it += pairs) {
         int block, panel;
         walk.at(it, block, panel);
         for (int nt = panel * p.pan; nt < min(ntiles, (panel + 1) * p.pan) && ok; ++nt)
           for (int k = 0; k < ktiles; ++k) {
-            uint64_t* bar;
+            uint32_t bar;
             uint8_t* to = ld.next(kStage, bar);
             if (!to) {
               ok = false;
               break;
             }
-            tma_load_2d(to, a, bar, k * kK, block * kM);
-            tma_load_2d(to + kABytes, &mW, bar, k * kK, p.v0 + nt * kN);
+            tma_load_2d(to, a, bar, k * kK, block * kM + rank * kHalf);
+            tma_load_2d(to + kABytes, &mW, bar, k * kK, p.v0 + nt * kN + rank * kHalf);
           }
       }
-      if (!ok) ld.drain();
+      ld.end(ok);
     }
   } else if (warp == 9) {
-    const bool leader = elect_one();
-    Issuer mm{s, smem_u32(smem), 0, 0};
-    constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, 0, 0, kN);
-    bool ok = true;
-    for (int it = blockIdx.x; it < walk.items && ok; it += gridDim.x) {
-      int block, panel;
-      walk.at(it, block, panel);
-      for (int nt = panel * p.pan; nt < min(ntiles, (panel + 1) * p.pan) && ok; ++nt)
-        ok = mm.tile(ktiles, id, 32, 32, leader);
+    if (rank == 0) {
+      const bool leader = elect_one();
+      Issuer<S> mm{s, smem_u32(smem), 0, 0, 0};
+      constexpr uint32_t id = idesc(std::is_same<T, __half>::value ? 0 : 1, 0, 0, kN);
+      bool ok = true;
+      for (int it = pair; it < walk.items && ok; it += pairs) {
+        int block, panel;
+        walk.at(it, block, panel);
+        for (int nt = panel * p.pan; nt < min(ntiles, (panel + 1) * p.pan) && ok; ++nt)
+          ok = mm.tile(ktiles, id, 32, 32, leader);
+      }
     }
   } else {
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tl = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
-    uint8_t* box = smem + kStages * kStage + warp * 4096;
+    uint8_t* box = smem + S * kStage + warp * 8192;
+    const uint32_t freed[2] = {first_cta(&s.acc_empty[0]), first_cta(&s.acc_empty[1])};
     uint32_t tiles = 0;
     bool dead = false;
-    for (int it = blockIdx.x; it < walk.items; it += gridDim.x) {
+    for (int it = pair; it < walk.items; it += pairs) {
       int block, panel;
       walk.at(it, block, panel);
-      const int r = block * kM + row;
+      const int r = block * kM + rank * kHalf + row;
       const bool live = r < n;
       const int tcol = live ? __ldg(p.tgt + r) - p.v0 : -1;
       float ms = -INFINITY, l = 0.f;              // STATS
@@ -349,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 4; ++i) pin32(x + 32 * i);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+        if (lane == 0) arrive_cluster(freed[b]);
         const int c0 = nt * kN + half * 128;
         const int cols = min(p.V - p.v0, p.vp) - c0;  // that exist
         const int at = tcol - c0;                     // the target's place
@@ -390,6 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           const float2 c2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-lse2, -lse2);
           const float2 a2 = make_float2(fa, fa);
+          if (lane == 0) bulk_wait_read0();  // the last tile's boxes have left
+          __syncwarp();
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
 #pragma unroll
@@ -406,20 +460,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int i = 32 * h; i < 32 * h + 32; ++i) x[i] = live && i < cols ? x[i] : 0.f;
             }
-            if (lane == 0) bulk_wait_read1();  // the box before the last has left
-            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float* y = x + 32 * h + 8 * i;
-              *reinterpret_cast<uint4*>(box + (h & 1) * 2048 + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+            for (int i = 4 * h; i < 4 * h + 4; ++i) {
+              const float* y = x + 8 * i;
+              *reinterpret_cast<uint4*>(box + (i >> 3) * 4096 + lane * 128 + (((i ^ lane) & 7) << 4)) =
                   make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&mZ, box + (h & 1) * 2048, c0 + 32 * h, block * kM + (warp & 3) * 32);
-              bulk_commit();
-            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            const int to = block * kM + rank * kHalf + (warp & 3) * 32;
+            tma_store_2d(&mZ, box, c0, to);
+            tma_store_2d(&mZ, box + 4096, c0 + 64, to);
+            bulk_commit();
           }
         }
       }
@@ -431,15 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- dW = dZ^T H of the piece, dH += dZ W
-// The tiles of both products.  Whole rounds of them, one a CTA, run side by
-// side, so that the CTAs at work share what they read of dZ; the tiles that are
-// left over stand on a line, which is cut evenly over the CTAs.  A tile that is
-// cut leaves sums in the workspace, and the CTA that finishes it last adds them
-// up in order.  (T = 16384, 512 channels, pieces of 16384 columns: 508 tiles on
-// 148 CTAs, 3.43 rounds.)
+// The tiles of both products.  Whole rounds of them, one a pair of CTAs, run side
+// by side, so that the pairs at work share what they read of dZ; the tiles that
+// are left over stand on a line, which is cut evenly over the pairs.  A tile that
+// is cut leaves sums in the workspace, and the pair that finishes it last adds
+// them up in order.  (T = 16384, 512 channels, pieces of 16384 columns: 254 tiles
+// on 74 pairs, 3.43 rounds.)
 struct Tiles {
   int nt, tw, th, kw, kh;  // tiles a row of tiles, of dW, of dH; their steps
-  int ncta, rw, rh, lw, lh;  // rounds, and what is left
+  int ncta, rw, rh, lw, lh;  // pairs; rounds, and what is left
   i64 line;
   OSSM_DEV Tiles(const Params& p, int n, int cols, int grid) {
     const int nn = max(n, 1);
@@ -456,7 +510,7 @@ struct Tiles {
   OSSM_DEV i64 start(int i) const { return i < lw ? (i64)i * kw : (i64)lw * kw + (i64)(i - lw) * kh; }
   OSSM_DEV int steps(int i) const { return i < lw ? kw : kh; }
   OSSM_DEV int at(i64 pos) const { return pos < (i64)lw * kw ? (int)(pos / kw) : lw + (int)((pos - (i64)lw * kw) / kh); }
-  // Where CTA c's part of the line begins.  A cut within 16 steps of its tile's
+  // Where pair c's part of the line begins.  A cut within 16 steps of its tile's
   // edge (an eighth of a short one) moves to the edge.
   OSSM_DEV i64 cut(int c) const {
     if (c >= ncta) return line;
@@ -473,7 +527,7 @@ struct Item {
   bool split;
   int rest;     // split: the tile's place on the line
 };
-struct Shares {  // of one CTA, in order
+struct Shares {  // of one pair, in order
   const Tiles& t;
   int cta, round;
   i64 pos, end;
@@ -502,63 +556,67 @@ struct Shares {  // of one CTA, in order
     return true;
   }
 };
-constexpr size_t kPart = (size_t)kM * kN;  // floats of a tile's sums
+constexpr size_t kPart = (size_t)kHalf * kN;  // floats of a CTA's half of a tile's sums
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     lce_prod_kernel(const __grid_constant__ CUtensorMap mZm, const __grid_constant__ CUtensorMap mZk,
                     const __grid_constant__ CUtensorMap mH, const __grid_constant__ CUtensorMap mHc,
                     const __grid_constant__ CUtensorMap mW, const __grid_constant__ Params p) {
+  constexpr int S = kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ Shared s;
+  __shared__ Shared<S> s;
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = cluster_rank(), pair = blockIdx.x >> 1;
   setup(s, warp);
   const int n = p.head->n, cols = min(p.vp, p.V - p.v0);
-  const Tiles tiles(p, n, cols, gridDim.x);
-  Shares todo(tiles, blockIdx.x);
+  const Tiles tiles(p, n, cols, gridDim.x >> 1);
+  Shares todo(tiles, pair);
   Item x;
 
   if (warp == 8) {
     if (lane == 0) {
       const CUtensorMap* hm = n == p.T ? &mH : &mHc;
-      Loader ld{s, smem, 0};
+      Loader<S> ld{s, smem, rank == 0, 0, 0, 0};
       bool ok = true;
       while (ok && todo.next(x)) {
-        const int boxes = min(4, (p.d - x.n0 + 63) / 64);
+        const int boxes = p.d - x.n0 > 128 ? 2 : 1;  // a CTA's share of the tile's 256 or 128 columns
+        const int m0 = x.m0 + rank * kHalf, n0 = x.n0 + rank * boxes * 64;
         for (int k = x.k0; k < x.k1; ++k) {
-          uint64_t* bar;
+          uint32_t bar;
           uint8_t* to = ld.next(kABytes + boxes * kBox, bar);
           if (!to) {
             ok = false;
             break;
           }
           if (x.w) {
-            tma_load_2d(to, &mZm, bar, x.m0, k * kK);
-            tma_load_2d(to + kBox, &mZm, bar, x.m0 + 64, k * kK);
-            for (int i = 0; i < boxes; ++i) tma_load_2d(to + kABytes + i * kBox, hm, bar, x.n0 + 64 * i, k * kK);
+            tma_load_2d(to, &mZm, bar, m0, k * kK);
+            tma_load_2d(to + kBox, &mZm, bar, m0 + 64, k * kK);
+            for (int i = 0; i < boxes; ++i) tma_load_2d(to + kABytes + i * kBox, hm, bar, n0 + 64 * i, k * kK);
           } else {
-            tma_load_2d(to, &mZk, bar, k * kK, x.m0);
+            tma_load_2d(to, &mZk, bar, k * kK, m0);
             for (int i = 0; i < boxes; ++i)
-              tma_load_2d(to + kABytes + i * kBox, &mW, bar, x.n0 + 64 * i, p.v0 + k * kK);
+              tma_load_2d(to + kABytes + i * kBox, &mW, bar, n0 + 64 * i, p.v0 + k * kK);
           }
         }
       }
-      if (!ok) ld.drain();
+      ld.end(ok);
     }
   } else if (warp == 9) {
-    const bool leader = elect_one();
-    constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
-    Issuer mm{s, smem_u32(smem), 0, 0};
-    bool ok = true;
-    while (ok && todo.next(x)) {
-      const int N = min(kN, (p.d - x.n0 + 63) / 64 * 64);
-      ok = mm.tile(x.k1 - x.k0, idesc(fmt, x.w, 1, N), x.w ? 2048 : 32, 2048, leader);
+    if (rank == 0) {
+      const bool leader = elect_one();
+      constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
+      Issuer<S> mm{s, smem_u32(smem), 0, 0, 0};
+      bool ok = true;
+      while (ok && todo.next(x))
+        ok = mm.tile(x.k1 - x.k0, idesc(fmt, x.w, 1, p.d - x.n0 > 128 ? 256 : 128), x.w ? 2048 : 32, 2048, leader);
     }
   } else {
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tl = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
     const float unit = p.head->unit;
+    const uint32_t freed[2] = {first_cta(&s.acc_empty[0]), first_cta(&s.acc_empty[1])};
     uint32_t done = 0;
     bool dead = false;
     for (; todo.next(x); ++done) {
@@ -566,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!dead) dead = gave_up(&s.acc_full[b], (done >> 1) & 1, &s.failed);
       __syncwarp();
       tc_fence_after();
-      const int r = x.m0 + row, n0 = x.n0 + half * 128;
+      const int r = x.m0 + rank * kHalf + row, n0 = x.n0 + half * 128;
       T* to = nullptr;
       if (x.w) {
         if (r < cols) to = static_cast<T*>(p.dw) + (i64)(p.v0 + r) * p.d + n0;
@@ -575,19 +633,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // dH's sums over the earlier pieces of the vocabulary; float4 e of every row side by side
       const int u = x.m0 / kM * tiles.nt + x.n0 / kN;
-      float4* sum = x.w ? nullptr : reinterpret_cast<float4*>(p.dh32 + u * kPart) + half * 32 * kM + row;
+      float4* sum = x.w ? nullptr : reinterpret_cast<float4*>(p.dh32 + (2 * u + rank) * kPart) + half * 32 * kHalf + row;
       auto finish = [&](int i, float (&y)[32]) {  // columns 32 i .. of this half
         if (!x.w && !p.first) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float4 q = sum[(8 * i + e) * kM];
+            const float4 q = sum[(8 * i + e) * kHalf];
             y[4 * e] += q.x, y[4 * e + 1] += q.y, y[4 * e + 2] += q.z, y[4 * e + 3] += q.w;
           }
         }
         if (!x.w && !p.last) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            sum[(8 * i + e) * kM] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+            sum[(8 * i + e) * kHalf] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
         } else if (to) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -599,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       };
-      float4* part = reinterpret_cast<float4*>(p.cuts + (2 * blockIdx.x + (x.k0 == 0)) * kPart) + half * 32 * kM + row;
+      float4* part = reinterpret_cast<float4*>(p.cuts + (2 * blockIdx.x + (x.k0 == 0)) * kPart) + half * 32 * kHalf + row;
 #pragma unroll 1
       for (int i = 0; i < 4; ++i) {
         if (n0 + 32 * i >= p.d) break;
@@ -610,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (x.split) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            part[(8 * i + e) * kM] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+            part[(8 * i + e) * kHalf] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
         } else {
           finish(i, y);
         }
@@ -618,21 +676,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+      if (lane == 0) arrive_cluster(freed[b]);
       if (!x.split) continue;
       __threadfence();
       named_sync(1, 256);
       if (threadIdx.x == 0) {
-        const uint32_t have = atomicAdd(p.counts + x.rest, (uint32_t)(x.k1 - x.k0)) + (x.k1 - x.k0);
+        const uint32_t have = atomicAdd(p.counts + 2 * x.rest + rank, (uint32_t)(x.k1 - x.k0)) + (x.k1 - x.k0);
         s.last_in = have == (uint32_t)tiles.steps(x.rest);
-        if (s.last_in) p.counts[x.rest] = 0;  // for the next piece
+        if (s.last_in) p.counts[2 * x.rest + rank] = 0;  // for the next piece
       }
       named_sync(1, 256);
       if (!s.last_in) continue;
       __threadfence();
-      // the pieces, in order: the CTA in whose part the tile starts, and the ones after it
+      // the pieces, in order: the pair in whose part the tile starts, and the ones after it
       const i64 from = tiles.start(x.rest), upto = from + tiles.steps(x.rest);
-      int c0 = blockIdx.x;
+      int c0 = pair;
       while (c0 > 0 && tiles.cut(c0) > from) --c0;
       while (tiles.cut(c0 + 1) <= from) ++c0;
 #pragma unroll 1
@@ -643,10 +701,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 32; ++e) y[e] = 0.f;
         for (int c = c0; c == c0 || tiles.cut(c) < upto; ++c) {
           if (c > c0 && tiles.cut(c + 1) == tiles.cut(c)) continue;  // no part at all
-          const float4* q = reinterpret_cast<const float4*>(p.cuts + (2 * c + (c == c0)) * kPart) + half * 32 * kM + row;
+          const float4* q = reinterpret_cast<const float4*>(p.cuts + (4 * c + 2 * rank + (c == c0)) * kPart) + half * 32 * kHalf + row;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float4 v = __ldcg(q + (8 * i + e) * kM);
+            const float4 v = __ldcg(q + (8 * i + e) * kHalf);
             y[4 * e] += v.x, y[4 * e + 1] += v.y, y[4 * e + 2] += v.z, y[4 * e + 3] += v.w;
           }
         }
@@ -865,17 +923,17 @@ struct Plan {
 // The workspace, and how the vocabulary is cut.
 Plan plan_of(const ossm_lce_args* a, bool bwd) {
   Plan q{};
-  q.sms = device_sms();
+  q.sms = device_sms() & ~1;
   q.Tpad = (int)((a->tokens + 255) / 256 * 256);
   q.Vpad = (a->vocab + kN - 1) / kN * kN;
-  const i64 blocks = (a->tokens + kM - 1) / kM;
+  const i64 blocks = (a->tokens + kM - 1) / kM, pairs = q.sms / 2;
   // Backward: dZ of a piece takes at most 512 MB, but has 4096 columns at
   // least: each piece reads and writes dH's fp32 sums once.
   q.vp = bwd ? (int)std::min<i64>(q.Vpad, std::max<i64>(4096, (1LL << 28) / q.Tpad / kN * kN)) : q.Vpad;
   q.ntiles = q.vp / kN;
   // A row's sums stay in registers over a panel: up to 8 tiles, fewer where
-  // there would not be 6 panels for each CTA to even out.
-  q.pan = bwd ? 1 : (int)std::min<i64>(8, std::max<i64>(1, blocks * q.ntiles / (6 * q.sms)));
+  // there would not be 6 panels for each pair to even out.
+  q.pan = bwd ? 1 : (int)std::min<i64>(8, std::max<i64>(1, blocks * q.ntiles / (6 * pairs)));
   q.panels = (q.ntiles + q.pan - 1) / q.pan;
   size_t at = 0;
   int k = 0;
@@ -906,15 +964,14 @@ Plan plan_of(const ossm_lce_args* a, bool bwd) {
   return q;
 }
 
-// [rows, inner], box [brows, bcols], swizzled over the bytes of a box's row.
-bool encode(CUtensorMap* map, int dtype, const void* base, i64 inner, i64 rows, i64 stride, int brows, int bcols = 64) {
+// [rows, inner] with 128-byte swizzle, box [brows, 64].
+bool encode(CUtensorMap* map, int dtype, const void* base, i64 inner, i64 rows, i64 stride, int brows) {
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
-  cuuint32_t box[2] = {(cuuint32_t)bcols, (cuuint32_t)brows}, estr[2] = {1, 1};
+  cuuint32_t box[2] = {64, (cuuint32_t)brows}, estr[2] = {1, 1};
   return fast::encode_fn()(map, dtype == OSSM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                            2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           bcols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -952,16 +1009,17 @@ template <typename T>
 int forward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   Params p = params_of(a, q, w, false);
   CUtensorMap mh, mc, mw;
-  if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kM) ||
-      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kM) ||
-      !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kN))
+  if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kHalf) ||
+      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kHalf) ||
+      !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kHalf))
     return OSSM_EINVAL;
   lce_rows_kernel<false><<<row_blocks(q, a->tokens), kRowThreads, 0, st>>>(p);
   static std::atomic<uint64_t> done{0};
   auto kern = lce_logits_kernel<T, STATS>;
-  if (allow_smem(kern, (int)kSmem, done) != cudaSuccess) return OSSM_ELAUNCH;
+  constexpr size_t smem = smem_bytes(kStages, false);
+  if (allow_smem(kern, (int)smem, done) != cudaSuccess) return OSSM_ELAUNCH;
   const i64 items = (a->tokens + kM - 1) / kM * q.panels;
-  kern<<<(int)std::min<i64>(q.sms, items), kThreads, kSmem, st>>>(mh, mc, mw, mw, p);
+  kern<<<(int)std::min<i64>(q.sms, 2 * items), kThreads, smem, st>>>(mh, mc, mw, mw, p);
   const int blocks = (int)std::min<i64>(kMaxBlocks, (a->tokens + kRowThreads / 32 - 1) / (kRowThreads / 32));
   lce_finish_kernel<<<blocks, kRowThreads, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
@@ -972,11 +1030,11 @@ int backward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   Params p = params_of(a, q, w, true);
   void* dz = w + q.at[7];
   CUtensorMap mh, mc, mw, ms, mzm, mzk, hm, hcm, wm;
-  if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kM) ||
-      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kM) ||
-      !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kN) ||
-      !encode(&ms, a->dtype, dz, q.vp, q.Tpad, q.vp, 32, 32) || !encode(&mzm, a->dtype, dz, q.vp, q.Tpad, q.vp, 64) ||
-      !encode(&mzk, a->dtype, dz, q.vp, q.Tpad, q.vp, kM) ||
+  if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kHalf) ||
+      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kHalf) ||
+      !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kHalf) ||
+      !encode(&ms, a->dtype, dz, q.vp, q.Tpad, q.vp, 32) || !encode(&mzm, a->dtype, dz, q.vp, q.Tpad, q.vp, 64) ||
+      !encode(&mzk, a->dtype, dz, q.vp, q.Tpad, q.vp, kHalf) ||
       !encode(&hm, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, 64) ||
       !encode(&hcm, a->dtype, p.hc, a->dim, q.Tpad, a->dim, 64) ||
       !encode(&wm, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, 64))
@@ -985,12 +1043,13 @@ int backward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   static std::atomic<uint64_t> done_z{0}, done_p{0};
   auto gradz = lce_logits_kernel<T, GRADZ>;
   auto prod = lce_prod_kernel<T>;
-  if (allow_smem(gradz, (int)kSmem, done_z) != cudaSuccess || allow_smem(prod, (int)kSmem, done_p) != cudaSuccess)
+  constexpr size_t smem_z = smem_bytes(kStagesZ, true), smem_p = smem_bytes(kStages, false);
+  if (allow_smem(gradz, (int)smem_z, done_z) != cudaSuccess || allow_smem(prod, (int)smem_p, done_p) != cudaSuccess)
     return OSSM_ELAUNCH;
   for (int v0 = 0; v0 < a->vocab; v0 += q.vp) {
     p.v0 = v0, p.first = v0 == 0, p.last = v0 + q.vp >= a->vocab;
-    gradz<<<q.sms, kThreads, kSmem, st>>>(mh, mc, mw, ms, p);
-    prod<<<q.sms, kThreads, kSmem, st>>>(mzm, mzk, hm, hcm, wm, p);
+    gradz<<<q.sms, kThreads, smem_z, st>>>(mh, mc, mw, ms, p);
+    prod<<<q.sms, kThreads, smem_p, st>>>(mzm, mzk, hm, hcm, wm, p);
   }
   return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
 }
