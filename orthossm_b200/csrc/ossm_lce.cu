@@ -48,7 +48,7 @@ constexpr int kOut = 8 * 2 * 32 * 128;      // gradz: two [32 rows x 64 columns]
 constexpr int kStages = 6, kStagesZ = 5;
 constexpr size_t smem_bytes(int stages, bool out) { return stages * (size_t)kStage + (out ? kOut : 0) + 1024; }
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 1024;
 constexpr int kMaxBlocks = 1024;
 
 struct Head {      // of the workspace
@@ -76,7 +76,8 @@ struct Params {
   Head* head;
   int *rows, *tgt;   // [n] token and target of each row
   float *lse2, *fa, *fb;  // [n] lse log2(e), factors of the softmax and of the target
-  void* hc;          // [Tpad, d] states of the rows side by side, where tokens were left out
+  void* hc;          // [Tpad, dst] states of the rows side by side, where tokens were left out
+  int dst;           // d up to whole 128 bytes: the copies are read by lines
   float2* part;      // [Tpad, 2 * panels] maximum (base 2) and sum of a row over a panel's half columns
   float* zt;         // [Tpad] the target's logit
   double* sums;      // [kMaxBlocks]
@@ -303,20 +304,22 @@ struct Issuer {
 // ---------------------------------------------------------------- logits
 enum { STATS, GRADZ };
 
-// Items of the logits kernels: a block of 256 rows by a panel of columns.  Of
-// 8 blocks of rows all take a panel before the next one, so that the CTAs at
-// work read the same columns of W and a few blocks of rows, which L2 keeps.
+// Items of the logits kernels: a block of 256 rows by a panel of columns.  The
+// blocks stand in groups whose rows L2 keeps (32 MB); of a group all take a panel
+// before the next one, so that W is read once a group.
 struct Walk {
-  int blocks, panels, items;
+  int blocks, panels, items, group;
   OSSM_DEV Walk(const Params& p) {
     blocks = max(1, (p.head->n + kM - 1) / kM);
     panels = p.panels;
     items = blocks * panels;
+    const int most = max(8, (32 << 20) / (kM * 2 * p.d)), groups = (blocks + most - 1) / most;
+    group = (blocks + groups - 1) / groups;
   }
   OSSM_DEV void at(int it, int& block, int& panel) const {
-    const int g = it / (8 * panels), r = it - g * 8 * panels, rows = min(8, blocks - 8 * g);
+    const int g = it / (group * panels), r = it - g * group * panels, rows = min(group, blocks - group * g);
     panel = r / rows;
-    block = 8 * g + r % rows;
+    block = group * g + r % rows;
   }
 };
 
@@ -716,16 +719,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- rows
-template <typename V, typename F>
-OSSM_DEV V block_reduce(V v, V* warps, F f) {  // of kRowThreads threads, the same in all of them
+template <int THREADS, typename V, typename F>
+OSSM_DEV V block_reduce(V v, V* warps, F f) {  // of a block's threads, the same in all of them
 #pragma unroll
   for (int w = 16; w; w >>= 1) v = f(v, __shfl_xor_sync(~0u, v, w));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = warps[0];
+  v = warps[threadIdx.x % (THREADS / 32)];
 #pragma unroll
-  for (int i = 1; i < kRowThreads / 32; ++i) v = f(v, warps[i]);
+  for (int w = THREADS / 64; w; w >>= 1) v = f(v, __shfl_xor_sync(~0u, v, w));
   return v;
 }
 
@@ -767,12 +770,12 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
     }
   }
   auto plus = [](i64 a, i64 b) { return a + b; };
-  all = block_reduce(all, wi, plus);
-  before = block_reduce(before, wi, plus);
+  all = block_reduce<kRowThreads>(all, wi, plus);
+  before = block_reduce<kRowThreads>(before, wi, plus);
   const int n = (int)all;
   float scale = 1.f;
   if (BWD) {
-    top = block_reduce(top, wf, [](float a, float b) { return fmaxf(a, b); });
+    top = block_reduce<kRowThreads>(top, wf, [](float a, float b) { return fmaxf(a, b); });
     if (p.reduction) scale = __ldg(p.g) / (p.reduction == 1 ? (float)max(n, 1) : 1.f);
   }
   const float inv = top > 0.f ? fminf(kDzScale / top, 0x1p120f) : 0.f;
@@ -838,7 +841,7 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
         if (e >= pieces) break;
         const int to = places[row[k]];
         if (to >= 0)
-          reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.hc) + (i64)to * p.d)[at] = v[k];
+          reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.hc) + (i64)to * p.dst)[at] = v[k];
         else if (BWD && p.dh)
           reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dh) + (t0 + row[k]) * p.d)[at] = make_uint4(0, 0, 0, 0);
       }
@@ -846,36 +849,47 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
   }
   if (gather && blockIdx.x == gridDim.x - 1) {  // the last block of rows is read whole
     const int to = (max(n, 1) + kM - 1) / kM * kM;
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.hc) + (i64)n * p.d);
-    for (i64 e = threadIdx.x; e < (i64)(to - n) * vecs; e += kRowThreads) dst[e] = make_uint4(0, 0, 0, 0);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.hc) + (i64)n * p.dst);
+    for (i64 e = threadIdx.x; e < (i64)(to - n) * (p.dst / 8); e += kRowThreads) dst[e] = make_uint4(0, 0, 0, 0);
   }
 }
 
 // ---------------------------------------------------------------- losses
-// A warp a row joins the partial sums; block sums in float64, added in order by
-// the last block.
-__global__ void __launch_bounds__(kRowThreads) lce_finish_kernel(const __grid_constant__ Params p) {
-  __shared__ double ws[kRowThreads / 32];
+// 2 to 32 lanes a row join the partial sums, by their number; block sums in
+// float64, added in order by the last block.
+constexpr int kFinishThreads = 256;
+__global__ void __launch_bounds__(kFinishThreads) lce_finish_kernel(const __grid_constant__ Params p, const int lanes) {
+  __shared__ double ws[kFinishThreads / 32];
   __shared__ bool last;
-  const int n = p.head->n, lane = threadIdx.x & 31, warps = gridDim.x * (kRowThreads / 32);
+  const int n = p.head->n, mine = threadIdx.x & (lanes - 1), per = kFinishThreads / lanes;
   double sum = 0.0;
-  for (int r = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5); r < n; r += warps) {
-    const float2* q = p.part + (i64)r * 2 * p.panels;
+  for (int r0 = blockIdx.x * per; r0 < n; r0 += gridDim.x * per) {
+    const int r = r0 + threadIdx.x / lanes;
     float m = -INFINITY, l = 0.f;
-    for (int i = lane; i < 2 * p.panels; i += 32) {
-      const float2 v = q[i];
-      const float top = fmaxf(m, v.x), ref = top == -INFINITY ? 0.f : top;
-      l = l * ex2(m - ref) + v.y * ex2(v.x - ref);
-      m = top;
-    }
+    if (r < n) {
+      const float2* q = p.part + (i64)r * 2 * p.panels;
+      for (int i0 = mine; i0 < 2 * p.panels; i0 += 8 * lanes) {
+        float2 v[8];
+        float top = m;
 #pragma unroll
-    for (int w = 16; w; w >>= 1) {
+        for (int k = 0; k < 8; ++k) {
+          v[k] = i0 + k * lanes < 2 * p.panels ? __ldg(q + i0 + k * lanes) : make_float2(-INFINITY, 0.f);
+          top = fmaxf(top, v[k].x);
+        }
+        const float ref = top == -INFINITY ? 0.f : top;
+        l *= ex2(m - ref);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) l = fmaf(v[k].y, ex2(v[k].x - ref), l);
+        m = top;
+      }
+    }
+    for (int w = lanes >> 1; w; w >>= 1) {
       const float m2 = __shfl_xor_sync(~0u, m, w), l2 = __shfl_xor_sync(~0u, l, w);
       const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
       l = l * ex2(m - ref) + l2 * ex2(m2 - ref);
       m = top;
     }
-    if (lane == 0) {
+    if (r < n && mine == 0) {
       const int t = p.rows[r];
       const double lse = ((double)m + log2((double)l)) * 0.6931471805599453;
       double loss = lse - (double)p.zt[r] + (double)p.zl * lse * lse;
@@ -887,7 +901,7 @@ __global__ void __launch_bounds__(kRowThreads) lce_finish_kernel(const __grid_co
   }
   if (!p.reduction) return;
   auto plus = [](double a, double b) { return a + b; };
-  sum = block_reduce(sum, ws, plus);
+  sum = block_reduce<kFinishThreads>(sum, ws, plus);
   if (threadIdx.x == 0) {
     p.sums[blockIdx.x] = sum;
     __threadfence();
@@ -897,8 +911,8 @@ __global__ void __launch_bounds__(kRowThreads) lce_finish_kernel(const __grid_co
   if (!last) return;
   __threadfence();
   double all = 0.0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += kRowThreads) all += __ldcg(p.sums + i);
-  all = block_reduce(all, ws, plus);
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kFinishThreads) all += __ldcg(p.sums + i);
+  all = block_reduce<kFinishThreads>(all, ws, plus);
   if (threadIdx.x == 0) *p.loss = (float)(p.reduction == 1 ? all / max(n, 1) : all);
 }
 
@@ -945,7 +959,7 @@ Plan plan_of(const ossm_lce_args* a, bool bwd) {
   take(sizeof(Head));
   take(4 * T);              // rows
   take(4 * T);              // targets
-  take(2 * T * d);          // states side by side
+  take(2 * T * ((d + 63) / 64 * 64));  // states side by side
   if (!bwd) {
     take(8 * T * 2 * q.panels);
     take(4 * T);
@@ -978,6 +992,7 @@ bool encode(CUtensorMap* map, int dtype, const void* base, i64 inner, i64 rows, 
 Params params_of(const ossm_lce_args* a, const Plan& q, char* w, bool bwd) {
   Params p{};
   p.T = a->tokens, p.Tpad = q.Tpad, p.d = a->dim, p.V = a->vocab;
+  p.dst = (a->dim + 63) / 64 * 64;
   p.hidden = a->hidden, p.hst = a->hidden_stride;
   p.targets = a->targets, p.ignore = a->ignore_index, p.zl = a->z_loss, p.reduction = a->reduction;
   p.loss = a->loss, p.lse = a->lse, p.g = a->grad_loss, p.dh = a->grad_hidden, p.dw = a->grad_weight;
@@ -1003,6 +1018,7 @@ Params params_of(const ossm_lce_args* a, const Plan& q, char* w, bool bwd) {
   return p;
 }
 
+// A block for 32 tokens, up to one an SM.
 int row_blocks(const Plan& q, i64 T) { return (int)std::min<i64>(q.sms, (T + 31) / 32); }
 
 template <typename T>
@@ -1010,7 +1026,7 @@ int forward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   Params p = params_of(a, q, w, false);
   CUtensorMap mh, mc, mw;
   if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kHalf) ||
-      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kHalf) ||
+      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, p.dst, kHalf) ||
       !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kHalf))
     return OSSM_EINVAL;
   lce_rows_kernel<false><<<row_blocks(q, a->tokens), kRowThreads, 0, st>>>(p);
@@ -1020,8 +1036,10 @@ int forward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   if (allow_smem(kern, (int)smem, done) != cudaSuccess) return OSSM_ELAUNCH;
   const i64 items = (a->tokens + kM - 1) / kM * q.panels;
   kern<<<(int)std::min<i64>(q.sms, 2 * items), kThreads, smem, st>>>(mh, mc, mw, mw, p);
-  const int blocks = (int)std::min<i64>(kMaxBlocks, (a->tokens + kRowThreads / 32 - 1) / (kRowThreads / 32));
-  lce_finish_kernel<<<blocks, kRowThreads, 0, st>>>(p);
+  int lanes = 2;
+  while (lanes < 32 && lanes * 8 < 2 * q.panels) lanes *= 2;
+  const int blocks = (int)std::min<i64>(kMaxBlocks, (a->tokens * lanes + kFinishThreads - 1) / kFinishThreads);
+  lce_finish_kernel<<<blocks, kFinishThreads, 0, st>>>(p, lanes);
   return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
 }
 
@@ -1031,12 +1049,12 @@ int backward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   void* dz = w + q.at[7];
   CUtensorMap mh, mc, mw, ms, mzm, mzk, hm, hcm, wm;
   if (!encode(&mh, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, kHalf) ||
-      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, a->dim, kHalf) ||
+      !encode(&mc, a->dtype, p.hc, a->dim, q.Tpad, p.dst, kHalf) ||
       !encode(&mw, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, kHalf) ||
       !encode(&ms, a->dtype, dz, q.vp, q.Tpad, q.vp, 32) || !encode(&mzm, a->dtype, dz, q.vp, q.Tpad, q.vp, 64) ||
       !encode(&mzk, a->dtype, dz, q.vp, q.Tpad, q.vp, kHalf) ||
       !encode(&hm, a->dtype, a->hidden, a->dim, a->tokens, a->hidden_stride, 64) ||
-      !encode(&hcm, a->dtype, p.hc, a->dim, q.Tpad, a->dim, 64) ||
+      !encode(&hcm, a->dtype, p.hc, a->dim, q.Tpad, p.dst, 64) ||
       !encode(&wm, a->dtype, a->weight, a->dim, a->vocab, a->weight_stride, 64))
     return OSSM_EINVAL;
   lce_rows_kernel<true><<<row_blocks(q, a->tokens), kRowThreads, 0, st>>>(p);
