@@ -6,7 +6,7 @@
 // order of a sum is that of the positions), cuts the sorted list into chunks, a
 // warp each, which add their rows up in fp32, and joins the sums of tokens that
 // reach over several chunks in order: the result depends on nothing but the
-// arguments.  Every row of dW is written once, untouched ones with zeros.
+// arguments.  dW is filled with zeros while the first digits are counted.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -42,6 +42,17 @@ template <>
 OSSM_DEV void store8<float>(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <typename T>
+OSSM_DEV void take8(const T* p, float (&v)[8]) {  // of registers
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const float2 a = to_f2<T>(u.x), b = to_f2<T>(u.y), c = to_f2<T>(u.z), d = to_f2<T>(u.w);
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+}
+template <>
+OSSM_DEV void take8<float>(const float* p, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = p[i];
 }
 OSSM_DEV float get1(const float* p) { return __ldg(p); }
 OSSM_DEV float get1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -83,7 +94,7 @@ constexpr int kMaxSortBlocks = 128;
 
 struct Sort {
   i64 T;
-  int V, per;              // keys of a block, a multiple of kKeys
+  int V, per, blocks;      // keys of a block, a multiple of kKeys
   int shift, bits;         // the digit
   const int64_t* ids;      // first pass: the tokens themselves
   const uint32_t *key, *pos;
@@ -96,8 +107,19 @@ OSSM_DEV uint32_t key_of(const Sort& s, i64 i) {
   return id >= 0 && id < s.V ? (uint32_t)id : (uint32_t)s.V;  // what is no row comes last
 }
 
-__global__ void __launch_bounds__(kThreads) embed_hist_kernel(const __grid_constant__ Sort s) {
+// The blocks past s.blocks fill dW with zeros.
+__global__ void __launch_bounds__(kThreads)
+    embed_hist_kernel(const __grid_constant__ Sort s, char* __restrict__ dw, i64 dw_bytes) {
   __shared__ uint32_t h[kMaxBins];
+  if ((int)blockIdx.x >= s.blocks) {
+    char* const from = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(dw) + 15) & ~(uintptr_t)15);
+    const i64 head = min((i64)(from - dw), dw_bytes), whole = (dw_bytes - head) / 16, tail = dw_bytes - head - 16 * whole;
+    const i64 step = (i64)(gridDim.x - s.blocks) * kThreads, i0 = (i64)(blockIdx.x - s.blocks) * kThreads + threadIdx.x;
+    for (i64 i = i0; i < whole; i += step) reinterpret_cast<uint4*>(from)[i] = make_uint4(0, 0, 0, 0);
+    if (i0 < head) dw[i0] = 0;
+    if (i0 < tail) from[16 * whole + i0] = 0;
+    return;
+  }
   const int bins = 1 << s.bits;
   for (int i = threadIdx.x; i < bins; i += kThreads) h[i] = 0;
   __syncthreads();
@@ -118,10 +140,15 @@ __global__ void __launch_bounds__(kThreads) embed_scatter_kernel(const __grid_co
     const int i = i0 + threadIdx.x;
     uint32_t before = 0, all = 0;
     if (i < bins)
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const uint32_t v = __ldg(s.hist + (i64)b * bins + i);
-        all += v;
-        before += b < (int)blockIdx.x ? v : 0;
+      for (int b0 = 0; b0 < s.blocks; b0 += 16) {  // 16 loads on their way
+        uint32_t v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = b0 + k < s.blocks ? __ldg(s.hist + (i64)(b0 + k) * bins + i) : 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          all += v[k];
+          before += b0 + k < (int)blockIdx.x ? v[k] : 0;
+        }
       }
     uint32_t scan = all;
 #pragma unroll
@@ -191,43 +218,45 @@ struct Sum {
   float* part;  // [chunks][2][slices * kSlice]: of the token that began before the chunk, of the one that goes on after it
 };
 constexpr int kSlice = 512;     // channels of a warp: 16 a lane
-constexpr int kZeroRows = 64;   // of a block that looks for untouched rows
-
-OSSM_DEV i64 lower_bound(const uint32_t* key, i64 n, uint32_t v) {
-  i64 lo = 0, hi = n;
-  while (lo < hi) {
-    const i64 mid = (lo + hi) >> 1;
-    if (__ldg(key + mid) < v) lo = mid + 1; else hi = mid;
-  }
-  return lo;
-}
-
 // A lane's 16 channels of a slice: two runs of eight, or every 32nd.
 template <typename T, bool VEC>
 struct Lane {
   int c0, d, lane;
   OSSM_DEV int at(int i) const { return VEC ? c0 + (i >> 3) * 256 + lane * 8 + (i & 7) : c0 + lane + 32 * i; }
-  OSSM_DEV void add(const T* row, float (&v)[16]) const {
+  OSSM_DEV bool has(int i) const { return at(VEC ? i & ~7 : i) < d; }
+  struct alignas(16) Row {  // as it lies in memory
+    T e[16];
+  };
+  OSSM_DEV void load(const T* row, Row& r) const {
     if (VEC) {
+      constexpr int Q = sizeof(T) / 2;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (at(8 * h) < d) {
-          float u[8];
-          load8<T>(row + at(8 * h), u);
+        if (has(8 * h)) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[8 * h + i] += u[i];
+          for (int q = 0; q < Q; ++q)
+            reinterpret_cast<uint4*>(r.e + 8 * h)[q] = __ldcs(reinterpret_cast<const uint4*>(row + at(8 * h)) + q);
         }
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (at(i) < d) v[i] += get1(row + at(i));
+        if (has(i)) r.e[i] = row[at(i)];
+    }
+  }
+  OSSM_DEV void add(const Row& r, float (&v)[16]) const {  // past the row's end: anything, never stored
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float u[8];
+      take8(r.e + 8 * h, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[8 * h + i] += u[i];
     }
   }
   OSSM_DEV void put(T* row, const float (&v)[16], float f) const {
     if (VEC) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (at(8 * h) < d) {
+        if (has(8 * h)) {
           float u[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) u[i] = v[8 * h + i] * f;
@@ -236,31 +265,15 @@ struct Lane {
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (at(i) < d) put1(row + at(i), v[i] * f);
+        if (has(i)) put1(row + at(i), v[i] * f);
     }
   }
 };
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-    embed_sum_kernel(const __grid_constant__ Sum s, const T* __restrict__ g, T* __restrict__ dw, int sum_blocks) {
+    embed_sum_kernel(const __grid_constant__ Sum s, const T* __restrict__ g, T* __restrict__ dw) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if ((int)blockIdx.x >= sum_blocks) {  // untouched rows
-    __shared__ i64 range[2];
-    __shared__ bool used[kZeroRows];
-    const int v0 = (blockIdx.x - sum_blocks) * kZeroRows, v1 = min(s.V, v0 + kZeroRows);
-    if (threadIdx.x < kZeroRows) used[threadIdx.x] = false;
-    if (threadIdx.x < 64 && lane == 0) range[warp] = lower_bound(s.key, s.T, warp ? v1 : v0);
-    __syncthreads();
-    for (i64 i = range[0] + threadIdx.x; i < range[1]; i += kThreads) used[__ldg(s.key + i) - v0] = true;
-    __syncthreads();
-    const float zero[16] = {};
-    for (int u = warp; u < (v1 - v0) * s.slices; u += kWarps) {
-      const int v = u / s.slices;
-      if (!used[v]) Lane<T, VEC>{u % s.slices * kSlice, s.d, lane}.put(dw + (i64)(v0 + v) * s.d, zero, 0.f);
-    }
-    return;
-  }
   const i64 unit = (i64)blockIdx.x * kWarps + warp;
   const int slice = (int)(unit % s.slices);
   const i64 c = unit / s.slices;
@@ -268,10 +281,10 @@ __global__ void __launch_bounds__(kThreads)
   const i64 a = c * s.chunk, b = min(s.T, a + s.chunk);
   const Lane<T, VEC> my{slice * kSlice, s.d, lane};
   float acc[16] = {};
-  const uint32_t first = __ldg(s.key + a);
-  uint32_t now = first;
-  bool begun = a > 0 && __ldg(s.key + a - 1) == first;  // the token at hand began in an earlier chunk
-  const uint32_t after = b < s.T ? __ldg(s.key + b) : ~0u;
+  uint32_t keys = __ldg(s.key + min(a + lane, b - 1)), poss = __ldg(s.pos + min(a + lane, b - 1));
+  const uint32_t before = a > 0 ? __ldg(s.key + a - 1) : ~0u, after = b < s.T ? __ldg(s.key + b) : ~0u;
+  uint32_t now = __shfl_sync(~0u, keys, 0);
+  bool begun = before == now;  // the token at hand began in an earlier chunk
   auto leave = [&](bool goes_on) {  // the token at hand is summed up
     if (now < (uint32_t)s.V) {
       if (begun || goes_on) {
@@ -285,54 +298,118 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
   };
+  // kAhead rows on their way at a time; the positions of the next 32 too
+  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;
   for (i64 i0 = a; i0 < b; i0 += 32) {
-    const i64 i = min(i0 + lane, b - 1);
-    const uint32_t keys = __ldg(s.key + i), poss = __ldg(s.pos + i);
     const int m = (int)min((i64)32, b - i0);
-    for (int j = 0; j < m; ++j) {
-      const uint32_t k = __shfl_sync(~0u, keys, j), t = __shfl_sync(~0u, poss, j);
-      if (k != now) {
-        leave(false);
-        now = k;
-        begun = false;
+    const i64 next = min(i0 + 32 + lane, b - 1);
+    const uint32_t keys_n = __ldg(s.key + next), poss_n = __ldg(s.pos + next);
+    for (int j0 = 0; j0 < m; j0 += kAhead) {
+      typename Lane<T, VEC>::Row row[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const uint32_t k = __shfl_sync(~0u, keys, (j0 + j) & 31), t = __shfl_sync(~0u, poss, (j0 + j) & 31);
+        if (j0 + j < m && k < (uint32_t)s.V) my.load(g + (i64)t * s.gst, row[j]);
       }
-      if (k < (uint32_t)s.V) my.add(g + (i64)t * s.gst, acc);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const uint32_t k = __shfl_sync(~0u, keys, (j0 + j) & 31);
+        if (j0 + j < m) {
+          if (k != now) {
+            leave(false);
+            now = k;
+            begun = false;
+          }
+          if (k < (uint32_t)s.V) my.add(row[j], acc);
+        }
+      }
     }
+    keys = keys_n, poss = poss_n;
   }
   leave(after == now);
 }
 
-// A block a chunk: the token that begins there and goes on, from its pieces in
-// order, a run of them a warp.
+// Adds the pieces of tokens that go on over chunks up, in order.  A block looks
+// through a run of chunks for those where such a token begins; a warp takes a
+// token of up to 8 pieces, the block together one of more, a run of them a warp.
+constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32, kMaxRun = 512;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads)
-    embed_join_kernel(const __grid_constant__ Sum s, T* __restrict__ dw) {
-  __shared__ float sums[kWarps][kSlice];
+__global__ void __launch_bounds__(kJoinThreads)
+    embed_join_kernel(const __grid_constant__ Sum s, T* __restrict__ dw, int run) {
+  __shared__ float sums[kJoinWarps / 2][kSlice];
+  __shared__ int begins[kMaxRun], longs[kMaxRun], nbegins, nlongs;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const i64 c = blockIdx.x / s.slices;
-  const int slice = blockIdx.x % s.slices;
-  const i64 a = c * s.chunk, b = min(s.T, a + s.chunk);
-  if (b >= s.T) return;
-  const uint32_t k = __ldg(s.key + b - 1);
-  if (k >= (uint32_t)s.V || __ldg(s.key + b) != k) return;             // does not go on
-  if (a > 0 && __ldg(s.key + a) == k && __ldg(s.key + a - 1) == k) return;  // began before
-  const i64 end = b + lower_bound(s.key + b, s.T - b, k + 1);           // past its last place
-  const int pieces = (int)((end - 1) / s.chunk - c) + 1, each = (pieces + kWarps - 1) / kWarps;
-  float acc[16] = {};
-#pragma unroll 4
-  for (int q = warp * each; q < min(pieces, (warp + 1) * each); ++q) {
-    const float* from = s.part + (((c + q) * 2 + (q ? 0 : 1)) * s.slices + slice) * kSlice;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] += __ldg(from + i * 32 + lane);
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) sums[warp][i * 32 + lane] = acc[i];
+  const int slice = blockIdx.y;
+  if (threadIdx.x == 0) nbegins = nlongs = 0;
   __syncthreads();
-  if (warp) return;
-  for (int w = 1; w < kWarps; ++w)
+  const i64 c0 = (i64)blockIdx.x * run;
+  for (int i = threadIdx.x; i < run && c0 + i < s.chunks; i += kJoinThreads) {
+    const i64 a = (c0 + i) * s.chunk, b = a + s.chunk;
+    if (b >= s.T) break;
+    const uint32_t k = __ldg(s.key + b - 1), after = __ldg(s.key + b);
+    const uint32_t before = a > 0 ? __ldg(s.key + a - 1) : ~0u;
+    if (k < (uint32_t)s.V && after == k && before != k) begins[atomicAdd(&nbegins, 1)] = i;
+  }
+  __syncthreads();
+  auto pieces_of = [&](i64 c, uint32_t k) {  // a warp: 1, and one for every later chunk that starts with the token
+    int pieces = 1, n = 32;
+    while (n == 32) {
+      const i64 i = (c + pieces + lane) * s.chunk;
+      n = __popc(__ballot_sync(~0u, i < s.T && __ldg(s.key + i) == k));
+      pieces += n;
+    }
+    return pieces;
+  };
+  auto add = [&](i64 c, int from, int upto, float (&acc)[16]) {  // 4 pieces on their way
+    for (int q0 = from; q0 < upto; q0 += 4) {
+      float v[4][16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] += sums[w][i * 32 + lane];
-  Lane<T, VEC>{slice * kSlice, s.d, lane}.put(dw + (i64)k * s.d, acc, s.scale);
+      for (int h = 0; h < 4; ++h) {
+        const int q = min(q0 + h, upto - 1);
+        const float* p = s.part + (((c + q) * 2 + (q ? 0 : 1)) * s.slices + slice) * kSlice;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[h][i] = __ldg(p + i * 32 + lane);
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        if (q0 + h < upto)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[i] += v[h][i];
+    }
+  };
+  auto token = [&](i64 c) { return __ldg(s.key + (c + 1) * s.chunk); };
+  const Lane<T, VEC> my{slice * kSlice, s.d, lane};
+  for (int j = warp; j < nbegins; j += kJoinWarps) {
+    const i64 c = c0 + begins[j];
+    const uint32_t k = token(c);
+    const int pieces = pieces_of(c, k);
+    if (pieces > 8) {
+      if (lane == 0) longs[atomicAdd(&nlongs, 1)] = begins[j];
+      continue;
+    }
+    float acc[16] = {};
+    add(c, 0, pieces, acc);
+    my.put(dw + (i64)k * s.d, acc, s.scale);
+  }
+  __syncthreads();
+  for (int j = 0; j < nlongs; ++j) {
+    const i64 c = c0 + longs[j];
+    const uint32_t k = token(c);
+    const int pieces = pieces_of(c, k), each = (pieces + kJoinWarps - 1) / kJoinWarps;
+    float acc[16] = {};
+    add(c, min(pieces, warp * each), min(pieces, (warp + 1) * each), acc);
+    for (int w = kJoinWarps / 2; w; w >>= 1) {  // halves of the warps
+      __syncthreads();
+      if (warp >= w && warp < 2 * w)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[warp - w][i * 32 + lane] = acc[i];
+      __syncthreads();
+      if (warp < w)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] += sums[warp][i * 32 + lane];
+    }
+    if (warp == 0) my.put(dw + (i64)k * s.d, acc, s.scale);
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -359,8 +436,9 @@ Plan plan_of(const ossm_embed_args* a) {
   q.per = (int)((T + (i64)kKeys * kMaxSortBlocks - 1) / ((i64)kKeys * kMaxSortBlocks)) * kKeys;
   q.blocks = (int)((T + q.per - 1) / q.per);
   q.slices = (a->dim + kSlice - 1) / kSlice;
-  // enough chunks for 32 warps an SM, of 8 to 64 positions
-  q.chunk = (int)std::min<i64>(64, std::max<i64>(8, T * q.slices / (32 * (i64)device_sms())));
+  // a chunk for each of the 16 warps that an SM holds, of 8 positions at least
+  const i64 warps = 16LL * device_sms();
+  q.chunk = (int)std::max<i64>(8, (T * q.slices + warps - 1) / warps);
   q.chunks = (int)((T + q.chunk - 1) / q.chunk);
   size_t at = 0;
   int k = 0;
@@ -391,22 +469,22 @@ int forward(const ossm_embed_args* a, cudaStream_t st) {
 
 template <typename T>
 int backward(const ossm_embed_args* a, const Plan& q, char* w, cudaStream_t st) {
-  if (!a->tokens)
-    return cudaMemsetAsync(a->grad_weight, 0, (size_t)a->vocab * a->dim * sizeof(T), st) == cudaSuccess ? OSSM_OK
-                                                                                                      : OSSM_ELAUNCH;
   uint32_t* buf[4];
   for (int i = 0; i < 4; ++i) buf[i] = reinterpret_cast<uint32_t*>(w + q.at[i]);
   Sort s{};
-  s.T = a->tokens, s.V = a->vocab, s.per = q.per, s.bits = q.bits;
+  s.T = a->tokens, s.V = a->vocab, s.per = q.per, s.blocks = q.blocks, s.bits = q.bits;
   s.hist = reinterpret_cast<uint32_t*>(w + q.at[4]);
-  for (int i = 0; i < q.passes; ++i) {
+  for (int i = 0; i < (a->tokens ? q.passes : 1); ++i) {
     s.shift = i * q.bits;
     s.ids = i ? nullptr : a->ids;
     s.key = buf[2 * (i & 1)], s.pos = buf[2 * (i & 1) + 1];
     s.key_to = buf[2 * (~i & 1)], s.pos_to = buf[2 * (~i & 1) + 1];
-    embed_hist_kernel<<<q.blocks, kThreads, 0, st>>>(s);
-    embed_scatter_kernel<<<q.blocks, kThreads, 0, st>>>(s);
+    const i64 bytes = i ? 0 : (i64)a->vocab * a->dim * (i64)sizeof(T);
+    const int zero = (int)std::min<i64>(4LL * device_sms(), (bytes + 16 * kThreads - 1) / (16 * kThreads));
+    embed_hist_kernel<<<q.blocks + zero, kThreads, 0, st>>>(s, static_cast<char*>(a->grad_weight), bytes);
+    if (a->tokens) embed_scatter_kernel<<<q.blocks, kThreads, 0, st>>>(s);
   }
+  if (!a->tokens) return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
   const T* g = static_cast<const T*>(a->grad_out);
   T* dw = static_cast<T*>(a->grad_weight);
   Sum m{};
@@ -416,11 +494,13 @@ int backward(const ossm_embed_args* a, const Plan& q, char* w, cudaStream_t st) 
   constexpr int kUnit = 16 / sizeof(T);
   const bool vec = a->dim % 8 == 0 && a->grad_out_stride % kUnit == 0 && (uintptr_t)g % 16 == 0 && (uintptr_t)dw % 16 == 0;
   const int sum_blocks = (int)(((i64)q.chunks * q.slices + kWarps - 1) / kWarps);
-  const int zero_blocks = (a->vocab + kZeroRows - 1) / kZeroRows;
   auto sum = vec ? embed_sum_kernel<T, true> : embed_sum_kernel<T, false>;
   auto join = vec ? embed_join_kernel<T, true> : embed_join_kernel<T, false>;
-  sum<<<sum_blocks + zero_blocks, kThreads, 0, st>>>(m, g, dw, sum_blocks);
-  if (q.chunks > 1) join<<<q.chunks * q.slices, kThreads, 0, st>>>(m, dw);
+  sum<<<sum_blocks, kThreads, 0, st>>>(m, g, dw);
+  if (q.chunks > 1) {
+    const int run = (int)std::min<i64>(kMaxRun, std::max<i64>(8, (q.chunks + 2LL * device_sms() - 1) / (2LL * device_sms())));
+    join<<<dim3((q.chunks + run - 1) / run, q.slices), kJoinThreads, 0, st>>>(m, dw, run);
+  }
   return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
 }
 
