@@ -219,14 +219,13 @@ def _declare(lib):
         if size() != C.sizeof(args):
             raise RuntimeError("orthossm_b200: ctypes struct layout does not match the C ABI")
         getattr(lib, f"ossm_{name}_workspace_bytes").restype = C.c_size_t
-        getattr(lib, f"ossm_{name}_workspace_bytes").argtypes = \
-            [C.POINTER(args), C.c_int] if name == "lce" else [C.POINTER(args)]
-    for name, args, ws in (("lce_fwd", LceArgs, True), ("lce_bwd", LceArgs, True), ("embed_fwd", EmbedArgs, False),
-                           ("embed_bwd", EmbedArgs, True), ("residual_norm_fwd", NormArgs, False),
-                           ("residual_norm_bwd", NormArgs, True)):
+        # _vp: a struct by reference, or its packed bytes
+        getattr(lib, f"ossm_{name}_workspace_bytes").argtypes = [_vp, C.c_int] if name == "lce" else [_vp]
+    for name, ws in (("lce_fwd", True), ("lce_bwd", True), ("embed_fwd", False), ("embed_bwd", True),
+                     ("residual_norm_fwd", False), ("residual_norm_bwd", True)):
         f = getattr(lib, "ossm_" + name)
         f.restype = C.c_int
-        f.argtypes = [C.POINTER(args), _vp, C.c_size_t, _vp] if ws else [C.POINTER(args), _vp]
+        f.argtypes = [_vp, _vp, C.c_size_t, _vp] if ws else [_vp, _vp]
     lib.ossm_sizeof_attn_args.restype = C.c_size_t
     lib.ossm_sizeof_sample_args.restype = C.c_size_t
     if lib.ossm_sizeof_attn_args() != C.sizeof(AttnArgs) or lib.ossm_sizeof_sample_args() != C.sizeof(SampleArgs):
