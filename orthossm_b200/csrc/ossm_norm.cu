@@ -210,56 +210,122 @@ struct Rows {
   }
 };
 
-// Sums over the threads of a row, the same in all of them.  Rows of several
+// Arithmetic on a thread's channels, two an instruction.
+OSSM_DEV float2 both(float f) { return make_float2(f, f); }
+template <int M>
+OSSM_DEV float2 pair(const float (&v)[M], int i) { return make_float2(v[2 * i], v[2 * i + 1]); }
+template <int M>
+OSSM_DEV void set(float (&v)[M], int i, float2 f) { v[2 * i] = f.x, v[2 * i + 1] = f.y; }
+template <int M>
+OSSM_DEV void mul(float (&a)[M], const float (&b)[M]) {
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) set(a, i, mul2(pair(a, i), pair(b, i)));
+}
+template <int M>
+OSSM_DEV void mul(float (&a)[M], float f) {
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) set(a, i, mul2(pair(a, i), both(f)));
+}
+template <int M>
+OSSM_DEV void add(float (&a)[M], const float (&b)[M]) {
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) set(a, i, attn::add2(pair(a, i), pair(b, i)));
+}
+template <int M>
+OSSM_DEV void add(float (&a)[M], float f) {
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) set(a, i, attn::add2(pair(a, i), both(f)));
+}
+template <int M>
+OSSM_DEV void fma(float (&d)[M], const float (&a)[M], const float (&b)[M]) {  // d += a b
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) set(d, i, fma2(pair(a, i), pair(b, i), pair(d, i)));
+}
+template <int M>
+OSSM_DEV void fma(float (&d)[M], const float (&a)[M], float f) {  // d += a f
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) set(d, i, fma2(pair(a, i), both(f), pair(d, i)));
+}
+template <int M>
+OSSM_DEV float dot(const float (&a)[M], const float (&b)[M]) {
+  float2 s = both(0.f);
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) s = fma2(pair(a, i), pair(b, i), s);
+  return s.x + s.y;
+}
+template <int M>
+OSSM_DEV float total(const float (&a)[M]) {
+  float2 s = both(0.f);
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) s = attn::add2(s, pair(a, i));
+  return s.x + s.y;
+}
+
+// Sums over the threads of a row, the same in all of them.  Of two sums the
+// lower lanes of a warp take one and the upper ones the other.  Rows of several
 // warps take the two buffers in turn, so that one barrier a sum is enough.
+template <int MAXT>
 struct RowSum {
-  float (*buf)[32][2];
+  float (*buf)[2][32];
   int R, turn;
-  template <int K>
-  OSSM_DEV void operator()(float (&v)[K]) {
+  OSSM_DEV float warp_sum(float v) const {
 #pragma unroll
-    for (int w = 16; w; w >>= 1)
-#pragma unroll
-      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(~0u, v[k], w);
+    for (int w = 16; w; w >>= 1) v += __shfl_xor_sync(~0u, v, w);
+    return v;
+  }
+  OSSM_DEV void operator()(float& v) {
+    v = warp_sum(v);
     if (R == 32) return;
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-      for (int k = 0; k < K; ++k) buf[turn][threadIdx.x >> 5][k] = v[k];
-    __syncthreads();
     const int lane = threadIdx.x & 31;
+    if (lane == 0) buf[turn][0][threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < R / 32 ? buf[turn][0][lane] : 0.f;
+    constexpr int W = MAXT > 256 ? 16 : 4;  // eight warps' sums lie in eight lanes
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = lane < R / 32 ? buf[turn][lane][k] : 0.f;
-    for (int w = R > 256 ? 16 : 4; w; w >>= 1)
-#pragma unroll
-      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(~0u, v[k], w);
-    if (R <= 256)  // eight warps' sums, in the first lanes of each eight
-#pragma unroll
-      for (int k = 0; k < K; ++k) v[k] = __shfl_sync(~0u, v[k], 0);
+    for (int w = W; w; w >>= 1) v += __shfl_xor_sync(~0u, v, w);
+    if (W == 4) v = __shfl_sync(~0u, v, 0);
     turn ^= 1;
+  }
+  OSSM_DEV void operator()(float& a, float& b) {
+    const int lane = threadIdx.x & 31;
+    const bool upper = lane & 16;
+    float v = upper ? b : a;
+    v += __shfl_xor_sync(~0u, upper ? a : b, 16);
+#pragma unroll
+    for (int w = 8; w; w >>= 1) v += __shfl_xor_sync(~0u, v, w);
+    if (R > 32) {
+      if ((lane & 15) == 0) buf[turn][lane >> 4][threadIdx.x >> 5] = v;
+      __syncthreads();
+      if (MAXT > 256) {  // 32 warps' sums, 16 a lane group at a time
+        v = (lane & 15) < R / 32 ? buf[turn][lane >> 4][lane & 15] : 0.f;
+        v += (lane & 15) + 16 < R / 32 ? buf[turn][lane >> 4][(lane & 15) + 16] : 0.f;
+      } else {
+        v = (lane & 15) < R / 32 ? buf[turn][lane >> 4][lane & 15] : 0.f;
+      }
+#pragma unroll
+      for (int w = MAXT > 256 ? 8 : 4; w; w >>= 1) v += __shfl_xor_sync(~0u, v, w);
+      turn ^= 1;
+    }
+    a = __shfl_sync(~0u, v, 0), b = __shfl_sync(~0u, v, 16);
   }
 };
 
 // Mean and inverse deviation of a row; v becomes the normed values.
-template <int N, bool VEC>
+template <int MAXT, int N, bool VEC>
 OSSM_DEV void normalise(const Own<N, VEC>& o, float (&v)[8 * N], int kind, float eps, float inv_d, float& mean, float& inv,
-                        RowSum& sum) {
+                        RowSum<MAXT>& sum) {
   mean = 0.f;
   if (kind == N_LAYER) {
-    float s[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < 8 * N; ++i) s[0] += v[i];
-    sum(s);
-    mean = s[0] * inv_d;
+    mean = total(v);
+    sum(mean);
+    mean *= inv_d;
 #pragma unroll
     for (int i = 0; i < 8 * N; ++i) v[i] = o.has(i) ? v[i] - mean : 0.f;
   }
-  float s[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < 8 * N; ++i) s[0] = fmaf(v[i], v[i], s[0]);
+  float s = dot(v, v);
   sum(s);
-  inv = 1.f / sqrtf(fmaf(s[0], inv_d, eps));
-#pragma unroll
-  for (int i = 0; i < 8 * N; ++i) v[i] *= inv;
+  inv = 1.f / sqrtf(fmaf(s, inv_d, eps));
+  mul(v, inv);
 }
 
 constexpr int kWarpRows = 8;  // rows of a block where a warp takes one
@@ -286,10 +352,10 @@ struct Shares {
 // MAXT: the most threads of a block; a block is one row, or 8 rows of a warp each.
 template <typename TX, typename TY, int N, bool VEC, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 3 : 1) norm_fwd_kernel(const __grid_constant__ Params p) {
-  __shared__ float buf[2][32][2];
+  __shared__ float buf[2][2][32];
   __shared__ uint64_t full[kWarpRows][kMaxStages];
   extern __shared__ __align__(16) char ring[];
-  RowSum sum{buf, p.R, 0};
+  RowSum<MAXT> sum{buf, p.R, 0};
   const int per = blockDim.x / p.R, mine = threadIdx.x / p.R;
   const i64 step = (i64)gridDim.x * per;
   i64 t = (i64)blockIdx.x * per + mine;
@@ -312,37 +378,30 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 3 : 1) norm_fwd_kernel(con
         normalise(o, u, p.post, p.post_eps, p.inv_d, pmean, pinv, sum);
         float a[8 * N];
         load(o, own.pw, 0, p.pw_vec, 1.f, a);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) u[i] *= a[i];
+        mul(u, a);
         if (p.pb.p) {
           load(o, own.pb, 0, p.pb_vec, 0.f, a);
-#pragma unroll
-          for (int i = 0; i < 8 * N; ++i) u[i] += a[i];
+          add(u, a);
         }
       }
       if (p.gate_kind == G_TOKEN) {
         const float g = p.gate.one(t);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) u[i] *= g;
+        mul(u, g);
       } else if (p.gate_kind) {
         float a[8 * N];
         load(o, own.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, a);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) u[i] *= a[i];
+        mul(u, a);
       }
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) v[i] = fmaf(p.scale, u[i], v[i]);
+      fma(v, u, p.scale);
       store<TX>(o, static_cast<TX*>(p.r) + t * p.d, v);
     }
     normalise(o, v, p.norm, p.eps, p.inv_d, mean, inv, sum);
     rows.taken(t);
     load(o, own.w, 0, p.w_vec, 1.f, u);
-#pragma unroll
-    for (int i = 0; i < 8 * N; ++i) v[i] *= u[i];
+    mul(v, u);
     if (p.b.p) {
       load(o, own.b, 0, p.b_vec, 0.f, u);
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) v[i] += u[i];
+      add(v, u);
     }
     store<TY>(o, static_cast<TY*>(p.h) + t * p.d, v);
     if (p.stats && o.t == 0) {
@@ -365,10 +424,10 @@ template <typename TX, typename TY, int N, bool VEC, int SUMS, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2 : 1)
     norm_bwd_kernel(const __grid_constant__ Params p) {
   constexpr bool FULL = SUMS == (int)kSums;
-  __shared__ float buf[2][32][2];
+  __shared__ float buf[2][2][32];
   __shared__ uint64_t full[kWarpRows][kMaxStages];
   extern __shared__ __align__(16) char ring[];
-  RowSum row_sum{buf, p.R, 0};
+  RowSum<MAXT> row_sum{buf, p.R, 0};
   const int per = blockDim.x / p.R, mine = threadIdx.x / p.R;
   const i64 step = (i64)gridDim.x * per;
   const Own<N, VEC> o{p.R, (int)(threadIdx.x % p.R), p.d};
@@ -419,53 +478,48 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2
     if constexpr (FULL) {
       // n becomes y normed (or y); a: the block's output after that; v: r again
       if (p.post) {
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) n[i] = (n[i] - pmean) * pinv;
+        if (p.post == N_LAYER) add(n, -pmean);
+        mul(n, pinv);
       }
       float c[8 * N];
       load(o, own.pw, 0, p.pw_vec, 1.f, a);
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) a[i] *= n[i];
+      mul(a, n);
       if (p.pb.p) {
         load(o, own.pb, 0, p.pb_vec, 0.f, c);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) a[i] += c[i];
+        add(a, c);
       }
       if (p.gate_kind == G_TOKEN) gt = p.gate.one(t);
       if (p.gate_kind == G_CHANNEL || p.gate_kind == G_FULL) {
         load(o, own.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, c);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) v[i] = fmaf(p.scale, c[i] * a[i], v[i]);
+        mul(c, a);
+        fma(v, c, p.scale);
       } else {
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) v[i] = fmaf(p.scale, gt * a[i], v[i]);
+        fma(v, a, p.scale * gt);
       }
     }
-#pragma unroll
-    for (int i = 0; i < 8 * N; ++i) v[i] = (v[i] - mean) * inv;
+    if (p.norm == N_LAYER) add(v, -mean);
+    mul(v, inv);
     if (p.dh) {
-      float s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) {
-        sum[S_W][i] = fmaf(e[i], v[i], sum[S_W][i]);
-        if (SUMS > 1) sum[SUMS > 1 ? S_B : 0][i] += e[i];
-      }
+      fma(sum[S_W], e, v);
+      if (SUMS > 1) add(sum[SUMS > 1 ? S_B : 0], e);
       if (own.w.p) {
         float f[8 * N];
         load(o, own.w, 0, p.w_vec, 1.f, f);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) e[i] *= f[i];
+        mul(e, f);
       }
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) {
-        s[0] = fmaf(e[i], v[i], s[0]);
-        s[1] += e[i];
+      float m0 = dot(e, v), m1 = 0.f;
+      if (p.norm == N_LAYER) {
+        m1 = total(e);
+        row_sum(m0, m1);
+        m1 *= p.inv_d;
+      } else {
+        row_sum(m0);
       }
-      row_sum(s);
       rows.taken(t);
-      const float m0 = s[0] * p.inv_d, m1 = p.norm == N_LAYER ? s[1] * p.inv_d : 0.f;
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) g[i] = fmaf(inv, e[i] - m1 - v[i] * m0, g[i]);
+      m0 *= p.inv_d;
+      fma(e, v, -m0);
+      if (p.norm == N_LAYER) add(e, -m1);
+      fma(g, e, inv);
     } else {
       rows.meet();
       rows.taken(t);
@@ -473,30 +527,24 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2
     if (p.dx) store<TX>(o, static_cast<TX*>(p.dx) + t * p.d, g);
     if constexpr (!FULL) {
       if (p.dy) {
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) g[i] *= p.scale;
+        mul(g, p.scale);
         store<TY>(o, static_cast<TY*>(p.dy) + t * p.d, g);
       }
     } else {
-      float s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 8 * N; ++i) {
-        g[i] *= p.scale;
-        a[i] *= g[i];  // the gate's gradient
-        s[0] += a[i];
-        sum[S_GATE][i] += a[i];
-      }
+      mul(g, p.scale);
+      mul(a, g);  // the gate's gradient
+      add(sum[S_GATE], a);
       if (p.gate_kind == G_TOKEN) {
         if (p.dgate) {
+          float s = total(a);
           row_sum(s);
           if (o.t == 0) {
-            if (p.dgate_dtype == OSSM_F32) put1(static_cast<float*>(p.dgate) + t, s[0]);
-            else if (p.dgate_dtype == OSSM_BF16) put1(static_cast<__nv_bfloat16*>(p.dgate) + t, s[0]);
-            else put1(static_cast<__half*>(p.dgate) + t, s[0]);
+            if (p.dgate_dtype == OSSM_F32) put1(static_cast<float*>(p.dgate) + t, s);
+            else if (p.dgate_dtype == OSSM_BF16) put1(static_cast<__nv_bfloat16*>(p.dgate) + t, s);
+            else put1(static_cast<__half*>(p.dgate) + t, s);
           }
         }
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) g[i] *= gt;
+        mul(g, gt);
       } else if (p.gate_kind) {
         if (p.gate_kind == G_FULL && p.dgate) {
           if (p.dgate_dtype == OSSM_F32) store<float>(o, static_cast<float*>(p.dgate) + t * p.d, a);
@@ -504,27 +552,25 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2
           else store<__half>(o, static_cast<__half*>(p.dgate) + t * p.d, a);
         }
         load(o, own.gate, p.gate_kind == G_FULL ? t * p.gst : 0, p.gate_vec, 1.f, a);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) g[i] *= a[i];
+        mul(g, a);
       }
       if (p.post) {
-        s[0] = s[1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) {
-          sum[S_PW][i] = fmaf(g[i], n[i], sum[S_PW][i]);
-          sum[S_PB][i] += g[i];
-        }
+        fma(sum[S_PW], g, n);
+        add(sum[S_PB], g);
         load(o, own.pw, 0, p.pw_vec, 1.f, a);
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) {
-          g[i] *= a[i];
-          s[0] = fmaf(g[i], n[i], s[0]);
-          s[1] += g[i];
+        mul(g, a);
+        float m0 = dot(g, n), m1 = 0.f;
+        if (p.post == N_LAYER) {
+          m1 = total(g);
+          row_sum(m0, m1);
+          m1 *= p.inv_d;
+        } else {
+          row_sum(m0);
         }
-        row_sum(s);
-        const float m0 = s[0] * p.inv_d, m1 = p.post == N_LAYER ? s[1] * p.inv_d : 0.f;
-#pragma unroll
-        for (int i = 0; i < 8 * N; ++i) g[i] = pinv * (g[i] - m1 - n[i] * m0);
+        m0 *= p.inv_d;
+        fma(g, n, -m0);
+        if (p.post == N_LAYER) add(g, -m1);
+        mul(g, pinv);
       }
       if (p.dy) store<TY>(o, static_cast<TY*>(p.dy) + t * p.d, g);
     }
