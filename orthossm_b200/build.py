@@ -11,6 +11,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -44,13 +46,20 @@ def build(verbose: bool = False, force: bool = False) -> str:
     if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(d) for d in deps):
         return out
     cuda_lib = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "lib64")
-    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-cudart", "shared", f"-I{INCLUDE}", f"-I{CSRC}", "-Xlinker", f"-rpath,{cuda_lib}",
-           "-o", out + ".tmp", *srcs]
+    cc = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", f"-I{INCLUDE}", f"-I{CSRC}"]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+        cc.insert(1, "-Xptxas=-v")
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in srcs]
+        # the largest first: a file a process
+        order = sorted(zip(srcs, objs), key=lambda so: -os.path.getsize(so[0]))
+        cmds = [[*cc, "-split-compile", "0", "-c", "-o", o, s] for s, o in order]
+        cmds_link = [nvcc(), *ARCH, "-shared", "-cudart", "shared", "-Xlinker", f"-rpath,{cuda_lib}", "-o", out + ".tmp",
+                     *objs]
+        if verbose:
+            print("\n".join(" ".join(c) for c in [*cmds, cmds_link]), flush=True)
+        list(pool.map(lambda c: subprocess.run(c, check=True), cmds))
+        subprocess.run(cmds_link, check=True)
     os.replace(out + ".tmp", out)
     return out
 
