@@ -541,7 +541,7 @@ enum ossm_norm_kind { OSSM_NORM_NONE = 0, OSSM_NORM_RMS = 1, OSSM_NORM_LAYER = 2
 enum ossm_gate_kind { OSSM_GATE_NONE = 0, OSSM_GATE_CHANNEL = 1, OSSM_GATE_TOKEN = 2, OSSM_GATE_FULL = 3 };
 typedef struct {
   int64_t tokens;                    /* below 2^31 */
-  int32_t dim;                       /* at most 16384 */
+  int32_t dim;                       /* at most 8192 */
   int32_t stream_dtype, dtype;       /* of x, r and of y, h: the same, or fp32 and a 16-bit type */
   const void* x;                     /* [tokens, dim], unit channel stride */
   int64_t x_stride;                  /* row strides in elements */

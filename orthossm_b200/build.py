@@ -22,7 +22,8 @@ LIBDIR = os.path.join(PKG, "_lib")
 LIBNAME = "liborthossm_b200.so"
 SOURCES = ["ossm_attn.cu", "ossm_attn_prompt.cu", "ossm_attn_token.cu", "ossm_capi.cu", "ossm_embed.cu",
            "ossm_forward.cu", "ossm_forward_3p.cu", "ossm_forward_grp.cu", "ossm_host.cu", "ossm_lce.cu",
-           "ossm_lion.cu", "ossm_noalloc.cu", "ossm_norm.cu", "ossm_reverse.cu", "ossm_sample.cu", "ossm_ttt.cu"]
+           "ossm_lion.cu", "ossm_noalloc.cu", "ossm_norm.cu", "ossm_norm_bf16.cu", "ossm_norm_f16.cu", "ossm_norm_f32.cu",
+           "ossm_norm_f32_bf16.cu", "ossm_norm_f32_f16.cu", "ossm_reverse.cu", "ossm_sample.cu", "ossm_ttt.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -51,9 +52,9 @@ def build(verbose: bool = False, force: bool = False) -> str:
         cc.insert(1, "-Xptxas=-v")
     with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(os.cpu_count() or 1) as pool:
         objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in srcs]
-        # the largest first: a file a process
-        order = sorted(zip(srcs, objs), key=lambda so: -os.path.getsize(so[0]))
-        cmds = [[*cc, "-split-compile", "0", "-c", "-o", o, s] for s, o in order]
+        # a file a process (nvcc's own -split-compile made kernels up to half slower), the longest ones first
+        order = sorted(zip(srcs, objs), key=lambda so: ("_norm_" not in so[0], -os.path.getsize(so[0])))
+        cmds = [[*cc, "-c", "-o", o, s] for s, o in order]
         cmds_link = [nvcc(), *ARCH, "-shared", "-cudart", "shared", "-Xlinker", f"-rpath,{cuda_lib}", "-o", out + ".tmp",
                      *objs]
         if verbose:

@@ -44,9 +44,10 @@ constexpr int kM = 256, kN = 256, kK = 64;  // a tile, and the depth of one load
 constexpr int kHalf = 128;                  // rows of A and of B that a CTA loads
 constexpr int kThreads = 320;               // 8 warps read tensor memory, one loads, one issues products
 constexpr int kABytes = kHalf * kK * 2, kStage = 2 * kABytes;
-constexpr int kOut = 8 * 2 * 32 * 128;      // gradz: two [32 rows x 64 columns] boxes a warp
+constexpr int kOutZ = 8 * 2 * 32 * 128;     // gradz: two [32 rows x 64 columns] boxes a warp
+constexpr int kOutP = 8 * 32 * 64;          // the products: a [32 rows x 32 columns] box a warp
 constexpr int kStages = 6, kStagesZ = 5;
-constexpr size_t smem_bytes(int stages, bool out) { return stages * (size_t)kStage + (out ? kOut : 0) + 1024; }
+constexpr size_t smem_bytes(int stages, int out) { return stages * (size_t)kStage + out + 1024; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowThreads = 1024;
 constexpr int kMaxBlocks = 1024;
@@ -83,8 +84,6 @@ struct Params {
   double* sums;      // [kMaxBlocks]
   float* dh32;       // [tiles] sums of dH over the pieces, in the order of tensor memory
   float* cuts;       // [2 a CTA] sums of tiles that are cut, the same
-  uint32_t* counts;  // [2 a CTA] steps that are done of tiles that are cut, 0 before a piece
-  int ncounts;
   int panels, pan;   // panels of `pan` tiles of columns
   int v0, vp;        // the piece: columns v0 .. v0 + vp
   int first, last;   // the piece is the first, the last
@@ -210,7 +209,7 @@ template <int S>
 struct Shared {
   uint64_t full[S], empty[S], acc_full[2], acc_empty[2];  // full, acc_empty: those of the first CTA are used
   uint32_t tmem;
-  int failed, last_in;
+  int failed;
 };
 
 // Barriers, tensor memory: all threads, before the roles part.
@@ -491,8 +490,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // The tiles of both products.  Whole rounds of them, one a pair of CTAs, run side
 // by side, so that the pairs at work share what they read of dZ; the tiles that
 // are left over stand on a line, which is cut evenly over the pairs.  A tile that
-// is cut leaves sums in the workspace, and the pair that finishes it last adds
-// them up in order.  (T = 16384, 512 channels, pieces of 16384 columns: 254 tiles
+// is cut leaves sums in the workspace, which a kernel after this one adds up in
+// order.  (The pair that finished last did that first: with 64 tokens and 50000
+// columns, where two tiles of dH are cut into 37, it took 290 of 323 us.)  (T = 16384, 512 channels, pieces of 16384 columns: 254 tiles
 // on 74 pairs, 3.43 rounds.)
 struct Tiles {
   int nt, tw, th, kw, kh;  // tiles a row of tiles, of dW, of dH; their steps
@@ -561,6 +561,38 @@ struct Shares {  // of one pair, in order
 };
 constexpr size_t kPart = (size_t)kHalf * kN;  // floats of a CTA's half of a tile's sums
 
+// What becomes of a row's sums of a tile, 8 columns at a time.
+template <typename T>
+struct Finish {
+  const Params& p;
+  T* to;            // where the row's columns of this half go, or NULL
+  float4* sum;      // dH's sums over the pieces of the vocabulary; float4 e of every row side by side
+  int left;         // columns of this half that exist
+  float unit;
+  OSSM_DEV Finish(const Params& q, bool w, int tile, int rank, int row, int half, int r, int n, int cols, int n0)
+      : p(q), to(nullptr), sum(nullptr), left(q.d - n0), unit(q.head->unit) {
+    if (w) {
+      if (r < cols) to = static_cast<T*>(p.dw) + (i64)(p.v0 + r) * p.d + n0;
+    } else {
+      if (r < n) to = static_cast<T*>(p.dh) + (i64)__ldg(p.rows + r) * p.d + n0;
+      sum = reinterpret_cast<float4*>(p.dh32 + (2 * tile + rank) * kPart) + half * 32 * kHalf + row;
+    }
+  }
+  OSSM_DEV bool out() const { return !sum || p.last; }  // they are outputs
+  OSSM_DEV uint4 value(int e, const float* y) const {    // columns 8 e .. 8 e + 7, as outputs
+    float4 a = make_float4(y[0], y[1], y[2], y[3]), b = make_float4(y[4], y[5], y[6], y[7]);
+    if (8 * e >= left) return make_uint4(0, 0, 0, 0);
+    if (sum && !p.first) {
+      const float4 u = sum[2 * e * kHalf], v = sum[(2 * e + 1) * kHalf];
+      a.x += u.x, a.y += u.y, a.z += u.z, a.w += u.w;
+      b.x += v.x, b.y += v.y, b.z += v.z, b.w += v.w;
+    }
+    if (!out()) sum[2 * e * kHalf] = a, sum[(2 * e + 1) * kHalf] = b;
+    return make_uint4(pack2<T>(a.x * unit, a.y * unit), pack2<T>(a.z * unit, a.w * unit),
+                      pack2<T>(b.x * unit, b.y * unit), pack2<T>(b.z * unit, b.w * unit));
+  }
+};
+
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     lce_prod_kernel(const __grid_constant__ CUtensorMap mZm, const __grid_constant__ CUtensorMap mZk,
@@ -618,8 +650,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else {
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tl = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
-    const float unit = p.head->unit;
     const uint32_t freed[2] = {first_cta(&s.acc_empty[0]), first_cta(&s.acc_empty[1])};
+    uint8_t* const box = smem + S * kStage + warp * 2048;  // 32 rows x 32 columns
     uint32_t done = 0;
     bool dead = false;
     for (; todo.next(x); ++done) {
@@ -628,38 +660,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
       tc_fence_after();
       const int r = x.m0 + rank * kHalf + row, n0 = x.n0 + half * 128;
-      T* to = nullptr;
-      if (x.w) {
-        if (r < cols) to = static_cast<T*>(p.dw) + (i64)(p.v0 + r) * p.d + n0;
-      } else if (r < n) {
-        to = static_cast<T*>(p.dh) + (i64)__ldg(p.rows + r) * p.d + n0;
-      }
-      // dH's sums over the earlier pieces of the vocabulary; float4 e of every row side by side
-      const int u = x.m0 / kM * tiles.nt + x.n0 / kN;
-      float4* sum = x.w ? nullptr : reinterpret_cast<float4*>(p.dh32 + (2 * u + rank) * kPart) + half * 32 * kHalf + row;
-      auto finish = [&](int i, float (&y)[32]) {  // columns 32 i .. of this half
-        if (!x.w && !p.first) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 q = sum[(8 * i + e) * kHalf];
-            y[4 * e] += q.x, y[4 * e + 1] += q.y, y[4 * e + 2] += q.z, y[4 * e + 3] += q.w;
-          }
-        }
-        if (!x.w && !p.last) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            sum[(8 * i + e) * kHalf] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
-        } else if (to) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (n0 + 32 * i + 8 * e >= p.d) break;
-            const float* z = y + 8 * e;
-            *reinterpret_cast<uint4*>(to + 32 * i + 8 * e) =
-                make_uint4(pack2<T>(z[0] * unit, z[1] * unit), pack2<T>(z[2] * unit, z[3] * unit),
-                           pack2<T>(z[4] * unit, z[5] * unit), pack2<T>(z[6] * unit, z[7] * unit));
-          }
-        }
-      };
+      const Finish<T> fin(p, x.w, x.m0 / kM * tiles.nt + x.n0 / kN, rank, row, half, r, n, cols, n0);
       float4* part = reinterpret_cast<float4*>(p.cuts + (2 * blockIdx.x + (x.k0 == 0)) * kPart) + half * 32 * kHalf + row;
 #pragma unroll 1
       for (int i = 0; i < 4; ++i) {
@@ -673,49 +674,82 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 8; ++e)
             part[(8 * i + e) * kHalf] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
         } else {
-          finish(i, y);
+          // outputs by way of shared memory, so that a store has whole sectors (16 bytes of 32 rows each
+          // kept the tiles of a short product, 64 tokens and 50000 columns, at 0.6 TB/s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint4 v = fin.value(4 * i + e, y + 8 * e);
+            *reinterpret_cast<uint4*>(box + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = v;
+          }
+          __syncwarp();
+          if (fin.out()) {
+            const int c = lane & 3;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int q = 8 * k + (lane >> 2);
+              T* const at = reinterpret_cast<T*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(fin.to), q));
+              const uint4 v = *reinterpret_cast<const uint4*>(box + q * 64 + ((c ^ ((q >> 1) & 3)) << 4));
+              if (at && 32 * i + 8 * c < fin.left) *reinterpret_cast<uint4*>(at + 32 * i + 8 * c) = v;
+            }
+          }
         }
         __syncwarp();
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(freed[b]);
-      if (!x.split) continue;
-      __threadfence();
-      named_sync(1, 256);
-      if (threadIdx.x == 0) {
-        const uint32_t have = atomicAdd(p.counts + 2 * x.rest + rank, (uint32_t)(x.k1 - x.k0)) + (x.k1 - x.k0);
-        s.last_in = have == (uint32_t)tiles.steps(x.rest);
-        if (s.last_in) p.counts[2 * x.rest + rank] = 0;  // for the next piece
-      }
-      named_sync(1, 256);
-      if (!s.last_in) continue;
-      __threadfence();
-      // the pieces, in order: the pair in whose part the tile starts, and the ones after it
-      const i64 from = tiles.start(x.rest), upto = from + tiles.steps(x.rest);
-      int c0 = pair;
-      while (c0 > 0 && tiles.cut(c0) > from) --c0;
-      while (tiles.cut(c0 + 1) <= from) ++c0;
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        if (n0 + 32 * i >= p.d) break;
-        float y[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) y[e] = 0.f;
-        for (int c = c0; c == c0 || tiles.cut(c) < upto; ++c) {
-          if (c > c0 && tiles.cut(c + 1) == tiles.cut(c)) continue;  // no part at all
-          const float4* q = reinterpret_cast<const float4*>(p.cuts + (4 * c + 2 * rank + (c == c0)) * kPart) + half * 32 * kHalf + row;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 v = __ldcg(q + (8 * i + e) * kHalf);
-            y[4 * e] += v.x, y[4 * e + 1] += v.y, y[4 * e + 2] += v.z, y[4 * e + 3] += v.w;
-          }
-        }
-        finish(i, y);
-      }
     }
   }
   teardown(s, warp, p.status);
+}
+
+// The tiles that were cut: blocks (.., c) take the one that pair c + 1's part
+// begins in, if no earlier part begins there; a block adds up 32 columns of 128
+// rows of it, a thread 8 columns of a row, 8 pieces on their way.
+constexpr int kJoinThreads = 4 * kHalf, kMaxPairs = 128;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) lce_join_kernel(const __grid_constant__ Params p, int pairs) {
+  const int n = p.head->n, cols = min(p.vp, p.V - p.v0);
+  const Tiles t(p, n, cols, pairs);
+  const int rank = blockIdx.x & 1, half = blockIdx.x >> 1 & 1, row = threadIdx.x % kHalf;
+  const int e = 4 * (blockIdx.x >> 2) + threadIdx.x / kHalf;
+  __shared__ i64 cuts[kMaxPairs + 1];
+  for (int c = threadIdx.x; c <= pairs; c += kJoinThreads) cuts[c] = t.cut(c);
+  __syncthreads();
+  const i64 begin = cuts[blockIdx.y + 1];
+  if (begin >= t.line) return;
+  const int i = t.at(begin);
+  const i64 from = t.start(i), upto = from + t.steps(i);
+  if (begin == from || cuts[blockIdx.y] > from) return;  // no cut, or not its first
+  const bool w = i < t.lw;
+  const int u = w ? t.rw * t.ncta + i : t.rh * t.ncta + i - t.lw;
+  const int m0 = u / t.nt * kM, n0 = u % t.nt * kN + half * 128;
+  if (n0 + 8 * e >= p.d) return;
+  // from the pair in whose part the tile starts to the one where it ends
+  const int c0 = blockIdx.y;
+  int c1 = c0 + 1;
+  while (cuts[c1] < upto) ++c1;
+  float y[8] = {};
+  const float4* q = reinterpret_cast<const float4*>(p.cuts) + (half * 32 + 2 * e) * kHalf + row;
+  for (int c = c0; c < c1; c += 8) {
+    float4 a[8], b[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool in = c + k < c1 && (c + k == c0 || cuts[c + k + 1] > cuts[c + k]);  // has a part at all
+      const float4* v = q + (4 * (i64)(c + k) + 2 * rank + (c + k == c0)) * (kPart / 4);
+      a[k] = in ? __ldg(v) : make_float4(0.f, 0.f, 0.f, 0.f);
+      b[k] = in ? __ldg(v + kHalf) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      y[0] += a[k].x, y[1] += a[k].y, y[2] += a[k].z, y[3] += a[k].w;
+      y[4] += b[k].x, y[5] += b[k].y, y[6] += b[k].z, y[7] += b[k].w;
+    }
+  }
+  const int r = m0 + rank * kHalf + row;
+  const Finish<T> fin(p, w, m0 / kM * t.nt + u % t.nt, rank, row, half, r, n, cols, n0);
+  const uint4 v = fin.value(e, y);
+  if (fin.out() && fin.to) *reinterpret_cast<uint4*>(fin.to + 8 * e) = v;
 }
 
 // ---------------------------------------------------------------- rows
@@ -784,8 +818,6 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
     p.head->unit = inv > 0.f ? scale / inv : 0.f;
     p.head->count = 0;
   }
-  if (BWD && blockIdx.x == 0)
-    for (int i = threadIdx.x; i < p.ncounts; i += kRowThreads) p.counts[i] = 0;
   const bool gather = all < p.T;
   const int vecs = p.d / 8;
   i64 base = before;
@@ -937,7 +969,7 @@ struct Plan {
 // The workspace, and how the vocabulary is cut.
 Plan plan_of(const ossm_lce_args* a, bool bwd) {
   Plan q{};
-  q.sms = device_sms() & ~1;
+  q.sms = std::min(device_sms(), 2 * kMaxPairs) & ~1;
   q.Tpad = (int)((a->tokens + 255) / 256 * 256);
   q.Vpad = (a->vocab + kN - 1) / kN * kN;
   const i64 blocks = (a->tokens + kM - 1) / kM, pairs = q.sms / 2;
@@ -972,7 +1004,6 @@ Plan plan_of(const ossm_lce_args* a, bool bwd) {
     const size_t nt = (d + kN - 1) / kN;
     take(a->grad_hidden && q.vp < q.Vpad ? 4 * T * nt * kN : 0);
     take(2 * q.sms * kPart * 4);
-    take(2 * q.sms * 4);
   }
   q.bytes = at;
   return q;
@@ -1010,8 +1041,6 @@ Params params_of(const ossm_lce_args* a, const Plan& q, char* w, bool bwd) {
     p.fb = reinterpret_cast<float*>(w + q.at[6]);
     p.dh32 = reinterpret_cast<float*>(w + q.at[8]);
     p.cuts = reinterpret_cast<float*>(w + q.at[9]);
-    p.counts = reinterpret_cast<uint32_t*>(w + q.at[10]);
-    p.ncounts = 2 * q.sms;
   }
   p.panels = q.panels, p.pan = q.pan, p.vp = q.vp;
   p.status = a->status;
@@ -1032,7 +1061,7 @@ int forward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   lce_rows_kernel<false><<<row_blocks(q, a->tokens), kRowThreads, 0, st>>>(p);
   static std::atomic<uint64_t> done{0};
   auto kern = lce_logits_kernel<T, STATS>;
-  constexpr size_t smem = smem_bytes(kStages, false);
+  constexpr size_t smem = smem_bytes(kStages, 0);
   if (allow_smem(kern, (int)smem, done) != cudaSuccess) return OSSM_ELAUNCH;
   const i64 items = (a->tokens + kM - 1) / kM * q.panels;
   kern<<<(int)std::min<i64>(q.sms, 2 * items), kThreads, smem, st>>>(mh, mc, mw, mw, p);
@@ -1061,13 +1090,14 @@ int backward(const ossm_lce_args* a, const Plan& q, char* w, cudaStream_t st) {
   static std::atomic<uint64_t> done_z{0}, done_p{0};
   auto gradz = lce_logits_kernel<T, GRADZ>;
   auto prod = lce_prod_kernel<T>;
-  constexpr size_t smem_z = smem_bytes(kStagesZ, true), smem_p = smem_bytes(kStages, false);
+  constexpr size_t smem_z = smem_bytes(kStagesZ, kOutZ), smem_p = smem_bytes(kStages, kOutP);
   if (allow_smem(gradz, (int)smem_z, done_z) != cudaSuccess || allow_smem(prod, (int)smem_p, done_p) != cudaSuccess)
     return OSSM_ELAUNCH;
   for (int v0 = 0; v0 < a->vocab; v0 += q.vp) {
     p.v0 = v0, p.first = v0 == 0, p.last = v0 + q.vp >= a->vocab;
     gradz<<<q.sms, kThreads, smem_z, st>>>(mh, mc, mw, ms, p);
     prod<<<q.sms, kThreads, smem_p, st>>>(mzm, mzk, hm, hcm, wm, p);
+    lce_join_kernel<T><<<dim3(16, q.sms / 2 - 1), kJoinThreads, 0, st>>>(p, q.sms / 2);
   }
   return cudaGetLastError() == cudaSuccess ? OSSM_OK : OSSM_ELAUNCH;
 }

@@ -431,8 +431,8 @@ def _refuse_norm(x, y, weight, bias, norm, eps, gate, scale, post_norm, post_wei
         raise ValueError("residual_norm: " + why)
 
     _need_cuda(x, y, weight, bias, gate, post_weight, post_bias)
-    if x.dim() < 1 or x.dtype not in _DT or not 1 <= x.shape[-1] <= 16384 or x.numel() // x.shape[-1] >= 1 << 31:
-        refuse(f"x [..., d] in fp32, bf16 or fp16 with d from 1 to 16384 and below 2^31 rows expected, got "
+    if x.dim() < 1 or x.dtype not in _DT or not 1 <= x.shape[-1] <= 8192 or x.numel() // x.shape[-1] >= 1 << 31:
+        refuse(f"x [..., d] in fp32, bf16 or fp16 with d from 1 to 8192 and below 2^31 rows expected, got "
                f"{tuple(x.shape)} {x.dtype}")
     d = x.shape[-1]
     if dt not in _DT or (dt != x.dtype and x.dtype != torch.float32) or (y is not None and y.dtype != dt):
@@ -470,7 +470,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Opt
     Returns ``(r, h)``: the residual stream and the next block's input.
 
     x: [..., d], the stream (CUDA); y: the block's output, of its shape, or None
-    (then r is x).  d at most 16384.  Both of one dtype (fp32, bf16, fp16), or
+    (then r is x).  d at most 8192.  Both of one dtype (fp32, bf16, fp16), or
     an fp32 stream beside a 16-bit y.  r has x's dtype and h y's (without y:
     ``out_dtype``, by default x's).
     norm, post_norm: "rms" (v * weight / sqrt(mean(v^2) + eps), plus a bias if
@@ -488,7 +488,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Opt
     code, post = _NORMS.get(norm), 0 if post_norm is None else _NORMS.get(post_norm)
     post_eps = eps if post_eps is None else post_eps
     kind = L.OSSM_GATE_NONE
-    ok = (dev >= 0 and xdt in _DT and dt in _DT and (dt is xdt or xdt is torch.float32) and 1 <= d <= 16384
+    ok = (dev >= 0 and xdt in _DT and dt in _DT and (dt is xdt or xdt is torch.float32) and 1 <= d <= 8192
           and x.numel() < d << 31 and code and post is not None
           and 0.0 <= eps < math.inf and 0.0 <= post_eps < math.inf and math.isfinite(scale))
     if ok:

@@ -380,7 +380,7 @@ def test_norm_plain(shape, xdt, ydt):
 
 
 @pytest.mark.parametrize("xdt,ydt", [(BF, BF), (FP, HF), (FP, FP)])
-@pytest.mark.parametrize("shape", [(1, 3), (2, 300, 64), (50, 384), (20, 520), (17, 1111), (5, 6000), (2, 16384)])
+@pytest.mark.parametrize("shape", [(1, 3), (2, 300, 64), (50, 384), (20, 520), (17, 1111), (5, 6000), (3, 8191), (2, 8192)])
 @pytest.mark.parametrize("gate,post", [(g, p) for g in (None, "channel", "token", "full")
                                        for p in (None, "rms", "layer") if g or p])
 def test_norm_gated(shape, gate, post, xdt, ydt):
@@ -486,7 +486,7 @@ def test_norm_refusals():
                 lambda: f(x, x, post_norm="batch"), lambda: f(x, gate=w), lambda: f(x, post_norm="rms"),
                 lambda: f(x, x, post_weight=w), lambda: f(x, x, gate=w[:5]), lambda: f(x, x, gate=torch.ones(4, device="cuda")),
                 lambda: f(x, eps=-1.0), lambda: f(x, x, scale=float("nan")),
-                lambda: f(torch.zeros(2, 16385, device="cuda")), lambda: f(x.bfloat16(), out_dtype=FP)):
+                lambda: f(torch.zeros(2, 8193, device="cuda")), lambda: f(x.bfloat16(), out_dtype=FP)):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(RuntimeError):
