@@ -54,7 +54,7 @@ OSSM_DEV void take8<float>(const float* p, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = p[i];
 }
-OSSM_DEV float get1(const float* p) { return __ldg(p); }
+OSSM_DEV float get1(const float* p) { return *p; }
 OSSM_DEV float get1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 OSSM_DEV float get1(const __half* p) { return __half2float(*p); }
 OSSM_DEV void put1(float* p, float v) { *p = v; }
@@ -67,22 +67,36 @@ constexpr int kThreads = 256;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     embed_fwd_kernel(const int64_t* ids, i64 tokens, int d, int V, const T* w, i64 wst, float scale, T* out) {
-  const int per = VEC ? d / 8 : d;  // pieces of a row
+  if (!VEC) {  // rows that are not whole 16-byte pieces: a warp a token, 8 loads on their way
+    const int lane = threadIdx.x & 31;
+    for (i64 t = (i64)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); t < tokens; t += (i64)gridDim.x * (kThreads / 32)) {
+      const i64 id = __ldg(ids + t);
+      const bool known = id >= 0 && id < V;
+      const T* const from = w + (known ? id * wst : 0);
+      T* const to = out + t * d;
+      for (int e0 = lane; e0 < d; e0 += 256) {
+        T v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (e0 + 32 * k < d) v[k] = from[e0 + 32 * k];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (e0 + 32 * k < d) put1(to + e0 + 32 * k, known ? get1(&v[k]) * scale : 0.f);
+      }
+    }
+    return;
+  }
+  const int per = d / 8;  // pieces of a row
   const i64 all = tokens * per, step = (i64)gridDim.x * kThreads;
   for (i64 i = (i64)blockIdx.x * kThreads + threadIdx.x; i < all; i += step) {
     const i64 t = i / per;
     const int e = (int)(i - t * per);
     const i64 id = __ldg(ids + t);
-    const bool known = id >= 0 && id < V;
-    if (VEC) {
-      float v[8] = {};
-      if (known) load8<T>(w + id * wst + 8 * e, v);
+    float v[8] = {};
+    if (id >= 0 && id < V) load8<T>(w + id * wst + 8 * e, v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= scale;
-      store8<T>(out + t * d + 8 * e, v);
-    } else {
-      put1(out + t * d + e, known ? get1(w + id * wst + e) * scale : 0.f);
-    }
+    for (int k = 0; k < 8; ++k) v[k] *= scale;
+    store8<T>(out + t * d + 8 * e, v);
   }
 }
 
@@ -211,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) embed_scatter_kernel(const __grid_co
 // ---------------------------------------------------------------- sums
 struct Sum {
   i64 T;
-  int V, d, chunk, chunks, slices;
+  int V, d, chunk, chunks, slices, width;  // width: channels of a slice
   const uint32_t *key, *pos;  // sorted
   i64 gst;
   float scale;
@@ -221,7 +235,7 @@ constexpr int kSlice = 512;     // channels of a warp: 16 a lane
 // A lane's 16 channels of a slice: two runs of eight, or every 32nd.
 template <typename T, bool VEC>
 struct Lane {
-  int c0, d, lane;
+  int c0, d, lane;  // of channels c0 .. d
   OSSM_DEV int at(int i) const { return VEC ? c0 + (i >> 3) * 256 + lane * 8 + (i & 7) : c0 + lane + 32 * i; }
   OSSM_DEV bool has(int i) const { return at(VEC ? i & ~7 : i) < d; }
   struct alignas(16) Row {  // as it lies in memory
@@ -279,7 +293,7 @@ __global__ void __launch_bounds__(kThreads)
   const i64 c = unit / s.slices;
   if (c >= s.chunks) return;
   const i64 a = c * s.chunk, b = min(s.T, a + s.chunk);
-  const Lane<T, VEC> my{slice * kSlice, s.d, lane};
+  const Lane<T, VEC> my{slice * s.width, min(s.d, (slice + 1) * s.width), lane};
   float acc[16] = {};
   uint32_t keys = __ldg(s.key + min(a + lane, b - 1)), poss = __ldg(s.pos + min(a + lane, b - 1));
   const uint32_t before = a > 0 ? __ldg(s.key + a - 1) : ~0u, after = b < s.T ? __ldg(s.key + b) : ~0u;
@@ -299,7 +313,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
   };
   // kAhead rows on their way at a time; the positions of the next 32 too
-  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;
+  constexpr int kAhead = sizeof(T) == 4 || !VEC ? 4 : 8;
   for (i64 i0 = a; i0 < b; i0 += 32) {
     const int m = (int)min((i64)32, b - i0);
     const i64 next = min(i0 + 32 + lane, b - 1);
@@ -378,7 +392,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     }
   };
   auto token = [&](i64 c) { return __ldg(s.key + (c + 1) * s.chunk); };
-  const Lane<T, VEC> my{slice * kSlice, s.d, lane};
+  const Lane<T, VEC> my{slice * s.width, min(s.d, (slice + 1) * s.width), lane};
   for (int j = warp; j < nbegins; j += kJoinWarps) {
     const i64 c = c0 + begins[j];
     const uint32_t k = token(c);
@@ -460,7 +474,7 @@ int forward(const ossm_embed_args* a, cudaStream_t st) {
   T* out = static_cast<T*>(a->out);
   constexpr int kUnit = 16 / sizeof(T);
   const bool vec = a->dim % 8 == 0 && a->weight_stride % kUnit == 0 && (uintptr_t)w % 16 == 0 && (uintptr_t)out % 16 == 0;
-  const i64 all = a->tokens * (vec ? a->dim / 8 : a->dim);
+  const i64 all = vec ? a->tokens * (a->dim / 8) : 32 * a->tokens;
   const int grid = (int)std::min<i64>((all + kThreads - 1) / kThreads, 16LL * device_sms());
   auto kern = vec ? embed_fwd_kernel<T, true> : embed_fwd_kernel<T, false>;
   kern<<<grid, kThreads, 0, st>>>(a->ids, a->tokens, a->dim, a->vocab, w, a->weight_stride, a->scale, out);
@@ -488,6 +502,7 @@ int backward(const ossm_embed_args* a, const Plan& q, char* w, cudaStream_t st) 
   const T* g = static_cast<const T*>(a->grad_out);
   T* dw = static_cast<T*>(a->grad_weight);
   Sum m{};
+  m.width = ((a->dim + q.slices - 1) / q.slices + 7) / 8 * 8;
   m.T = a->tokens, m.V = a->vocab, m.d = a->dim, m.chunk = q.chunk, m.chunks = q.chunks, m.slices = q.slices;
   m.key = s.key_to, m.pos = s.pos_to, m.gst = a->grad_out_stride, m.scale = a->scale;
   m.part = reinterpret_cast<float*>(w + q.at[5]);
