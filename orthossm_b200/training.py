@@ -169,7 +169,7 @@ class _LceFn(torch.autograd.Function):
         return dh, dw, None, None
 
 
-def _refuse_loss(hidden, weight, targets, z_loss, reduction):
+def _refuse_loss(hidden, weight, targets, ignore_index, z_loss, reduction):
     """Raises for the first argument of linear_cross_entropy that does not fit."""
     _need_cuda(hidden, weight, targets)
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
@@ -192,6 +192,8 @@ def _refuse_loss(hidden, weight, targets, z_loss, reduction):
         raise ValueError("linear_cross_entropy: hidden, weight and targets must be on one device")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if not -1 << 63 <= ignore_index < 1 << 63:
+        raise ValueError(f"linear_cross_entropy: ignore_index must fit 64 bits, got {ignore_index}")
     raise ValueError(f"linear_cross_entropy: z_loss must be finite and not negative, got {z_loss}")
 
 
@@ -210,21 +212,23 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     reduction: "mean" over the tokens that have a target (0 if none has),
     "sum", or "none": the losses [...], 0 where there is no target.
     Returns fp32.  Differentiable in ``hidden`` and ``weight``; the gradients
-    have their types.  Memory beside inputs and gradients: a piece of the
-    logits' gradient of at most 512 MB (or 4096 of the V columns, if more) in
-    the inputs' type and, if that is not all columns, fp32 sums of hidden's
-    size; with ignored tokens a copy of the others' states."""
+    have their types.  Memory beside inputs and gradients: forward 16
+    bytes a token for each panel of columns (2048, fewer for few tokens); backward a piece of the logits' gradient of
+    at most 512 MB (or 4096 of the V columns, if more) in the inputs' type, 40
+    MB of sums and, if the piece is not all columns, fp32 sums of hidden's
+    size; in both room for a copy of hidden, used if tokens are ignored."""
     dev, dt, shape = hidden.get_device(), hidden.dtype, targets.shape
     code = _REDUCTIONS.get(reduction)
     ok = (dev >= 0 and (dt is torch.bfloat16 or dt is torch.float16) and weight.dtype is dt and weight.dim() == 2
           and hidden.dim() == len(shape) + 1 and code is not None and 0.0 <= z_loss < math.inf
+          and -1 << 63 <= ignore_index < 1 << 63
           and weight.get_device() == dev and targets.get_device() == dev and targets.dtype in _INTS)
     if ok:
         V, d = weight.shape
         ok = hidden.shape == (*shape, d) and d % 8 == 0 and 8 <= d <= 1 << 16 and 1 <= V <= 1 << 27 \
             and targets.numel() <= 1 << 27
     if not ok:
-        _refuse_loss(hidden, weight, targets, z_loss, reduction)
+        _refuse_loss(hidden, weight, targets, ignore_index, z_loss, reduction)
     if forward_ad._current_level >= 0:
         _no_tangents("linear_cross_entropy", hidden, weight)
     if targets.dtype is not torch.int64:

@@ -214,7 +214,8 @@ def test_loss_refusals():
     for bad in (lambda: f(h.float(), w.float(), t), lambda: f(h, w.half(), t), lambda: f(h[:, :32], w, t),
                 lambda: f(h[:, :60].contiguous(), w[:, :60].contiguous(), t), lambda: f(h, w, t[:5]),
                 lambda: f(h, w, t.float()), lambda: f(h, w, t, reduction="max"), lambda: f(h, w, t, z_loss=-1.0),
-                lambda: f(h, w, t, z_loss=float("nan")), lambda: f(h, w[:0], t)):
+                lambda: f(h, w, t, z_loss=float("nan")), lambda: f(h, w[:0], t),
+                lambda: f(h, w, t, ignore_index=1 << 63)):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(RuntimeError):
