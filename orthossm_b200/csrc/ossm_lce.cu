@@ -505,6 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // order.  (The pair that finished last did that first: with 64 tokens and 50000
 // columns, where two tiles of dH are cut into 37, it took 290 of 323 us.)  (T = 16384, 512 channels, pieces of 16384 columns: 254 tiles
 // on 74 pairs, 3.43 rounds.)
+constexpr int kEnd = 10;  // a tile's end (its sums read, converted, stored) takes as long as so many steps of the next
 struct Tiles {
   int nt, tw, th, kw, kh;  // tiles a row of tiles, of dW, of dH; their steps
   int ncta, rw, rh, lw, lh;  // pairs; rounds, and what is left
@@ -518,12 +519,19 @@ struct Tiles {
     ncta = grid;
     rw = tw / ncta, lw = tw % ncta;
     rh = th / ncta, lh = th % ncta;
-    line = (i64)lw * kw + (i64)lh * kh;
+    line = (i64)lw * max(kw, kEnd) + (i64)lh * max(kh, kEnd);
   }
-  // What is left over: tile i of the line starts at...
-  OSSM_DEV i64 start(int i) const { return i < lw ? (i64)i * kw : (i64)lw * kw + (i64)(i - lw) * kh; }
+  // What is left over: tile i of the line starts at...  It is as long as its
+  // steps, or kEnd if they are fewer.  (Without that, 22 tiles of one step went to
+  // one pair beside others' 21 steps of a long one: 64 tokens, 113 us and not 44.)
+  OSSM_DEV i64 start(int i) const {
+    return i < lw ? (i64)i * max(kw, kEnd) : (i64)lw * max(kw, kEnd) + (i64)(i - lw) * max(kh, kEnd);
+  }
   OSSM_DEV int steps(int i) const { return i < lw ? kw : kh; }
-  OSSM_DEV int at(i64 pos) const { return pos < (i64)lw * kw ? (int)(pos / kw) : lw + (int)((pos - (i64)lw * kw) / kh); }
+  OSSM_DEV int at(i64 pos) const {
+    const i64 w = (i64)lw * max(kw, kEnd);
+    return pos < w ? (int)(pos / max(kw, kEnd)) : lw + (int)((pos - w) / max(kh, kEnd));
+  }
   // Where pair c's part of the line begins.  A cut within 16 steps of its tile's
   // edge (an eighth of a short one) moves to the edge.
   OSSM_DEV i64 cut(int c) const {
@@ -531,7 +539,7 @@ struct Tiles {
     const i64 pos = line / ncta * c + line % ncta * c / ncta;
     const int i = at(pos), k = steps(i), near = min(16, k / 8);
     const i64 s = start(i);
-    return pos - s <= near ? s : s + k - pos <= near ? s + k : pos;
+    return pos - s <= near ? s : pos - s >= k - near ? s + max(k, kEnd) : pos;
   }
 };
 struct Item {
@@ -564,7 +572,7 @@ struct Shares {  // of one pair, in order
       x.k1 = (int)min((i64)t.steps(i), end - s);
       x.split = x.k1 - x.k0 < t.steps(i);
       x.rest = i;
-      pos = s + x.k1;
+      pos = x.k1 == t.steps(i) ? s + max(x.k1, kEnd) : end;
     }
     x.m0 = u / t.nt * kM, x.n0 = u % t.nt * kN;
     return true;
@@ -716,10 +724,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // The tiles that were cut: blocks (.., c) take the one that pair c + 1's part
 // begins in, if no earlier part begins there; a block adds up 32 columns of 128
-// rows of it, a thread 8 columns of a row, 8 pieces on their way.
+// rows of it, a thread 8 columns of a row, 4 pieces on their way.
 constexpr int kJoinThreads = 4 * kHalf, kMaxPairs = 128;
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) lce_join_kernel(const __grid_constant__ Params p, int pairs) {
+__global__ void __launch_bounds__(kJoinThreads, 2) lce_join_kernel(const __grid_constant__ Params p, int pairs) {
   const int n = p.head->n, cols = min(p.vp, p.V - p.v0);
   const Tiles t(p, n, cols, pairs);
   const int rank = blockIdx.x & 1, half = blockIdx.x >> 1 & 1, row = threadIdx.x % kHalf;
@@ -735,30 +743,30 @@ __global__ void __launch_bounds__(kJoinThreads) lce_join_kernel(const __grid_con
   const bool w = i < t.lw;
   const int u = w ? t.rw * t.ncta + i : t.rh * t.ncta + i - t.lw;
   const int m0 = u / t.nt * kM, n0 = u % t.nt * kN + half * 128;
-  if (n0 + 8 * e >= p.d) return;
   // from the pair in whose part the tile starts to the one where it ends
   const int c0 = blockIdx.y;
   int c1 = c0 + 1;
   while (cuts[c1] < upto) ++c1;
+  const int r = m0 + rank * kHalf + row;
+  const Finish<T> fin(p, w, m0 / kM * t.nt + u % t.nt, rank, row, half, r, n, cols, n0);
+  if (n0 + 8 * e >= p.d) return;
   float y[8] = {};
   const float4* q = reinterpret_cast<const float4*>(p.cuts) + (half * 32 + 2 * e) * kHalf + row;
-  for (int c = c0; c < c1; c += 8) {
-    float4 a[8], b[8];
+  for (int c = c0; c < c1; c += 4) {
+    float4 a[4], b[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 4; ++k) {
       const bool in = c + k < c1 && (c + k == c0 || cuts[c + k + 1] > cuts[c + k]);  // has a part at all
       const float4* v = q + (4 * (i64)(c + k) + 2 * rank + (c + k == c0)) * (kPart / 4);
       a[k] = in ? __ldg(v) : make_float4(0.f, 0.f, 0.f, 0.f);
       b[k] = in ? __ldg(v + kHalf) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 4; ++k) {
       y[0] += a[k].x, y[1] += a[k].y, y[2] += a[k].z, y[3] += a[k].w;
       y[4] += b[k].x, y[5] += b[k].y, y[6] += b[k].z, y[7] += b[k].w;
     }
   }
-  const int r = m0 + rank * kHalf + row;
-  const Finish<T> fin(p, w, m0 / kM * t.nt + u % t.nt, rank, row, half, r, n, cols, n0);
   const uint4 v = fin.value(e, y);
   if (fin.out() && fin.to) *reinterpret_cast<uint4*>(fin.to + 8 * e) = v;
 }

@@ -46,7 +46,7 @@ def check_lce(h, w, t, reduction="mean", z_loss=0.0, seed=1, scale=1.0, **kw):
     (129, 72, 1001, 0.3, "mean", 0.0), (128, 128, 256, 0.0, "none", 1e-3), (300, 512, 777, 0.9, "none", 0.0),
     (257, 320, 4097, 0.02, "sum", 1e-4), (5, 1000, 257, 0.4, "mean", 1e-1), (640, 2048, 513, 0.5, "mean", 0.0),
     (4000, 264, 9999, 0.1, "mean", 0.0), (127, 8, 50001, 1.0, "mean", 0.0), (1000, 16, 300, 1.0, "none", 0.0),
-    (2500, 256, 40000, 0.0, "none", 0.0)])
+    (2500, 256, 40000, 0.0, "none", 0.0), (64, 512, 50000, 0.1, "mean", 0.0)])
 def test_loss(T, d, V, ignored, reduction, z_loss, dt):
     check_lce(*lce_inputs(T, d, V, dt, ignored), reduction=reduction, z_loss=z_loss)
 
