@@ -105,7 +105,7 @@ struct Params {
 OSSM_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
@@ -139,8 +139,10 @@ OSSM_DEV uint32_t first_cta(const uint64_t* bar) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
   return r;
 }
+// Orders nothing in memory: what is handed over is tensor memory that has been
+// read (a release at cluster scope stalled the readers' warps).
 OSSM_DEV void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // Into this CTA's shared memory, counted by a barrier of the pair's first CTA.
 OSSM_DEV void tma_load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
