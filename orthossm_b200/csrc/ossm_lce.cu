@@ -9,7 +9,8 @@
 // (logits tile by tile on the tensor core, a running maximum and sum a row),
 // finish (joins the sums, the losses and their sum).  Backward: rows, then for
 // each piece of the vocabulary gradz (the logits again, dz rounded to the
-// inputs' type into the workspace) and prod (dW of the piece, dH).
+// inputs' type into the workspace), prod (dW of the piece, dH) and join (the
+// tiles that several CTAs made parts of).
 //
 // Tokens without a target have no part in any product: their states are not
 // read, so NaN there harms nothing, and they cost nothing.
@@ -19,9 +20,10 @@
 //
 // What bounds it: the tensor pipe, 8 T d V operations where keeping the logits
 // would take 6, and in long runs the power cap.  Measured in bursts, 16384
-// tokens, 512 channels, 32000 columns, bf16: stats 326 us (1615 TFLOP/s), gradz
-// 478 (its dz, a gigabyte, costs 100 of them), the products 799 and their joins
-// 66; 8192, 2048, 131072: 2854, 3112, 7018 and 134 us (1540, 1413, 1253 TFLOP/s).
+// tokens, 512 channels, 32000 columns, bf16: stats 316 to 324 us (1625 to 1665
+// TFLOP/s, the pipe 97 % busy), gradz 444 to 454 (its dz, a gigabyte, costs 100 of
+// them), the products 786 to 821 and their joins 42 to 44; 8192, 2048, 131072: 2872, 3076, 6843 and 87 us (1531,
+// 1430, 1286 TFLOP/s).
 // Tried: pieces of 32 to 256 MB (3 to 60 % slower), A's tile resident (2 % in a
 // timing probe at 512 channels), one CTA a tile (6 to 17 % slower in the products).
 #include <cuda.h>

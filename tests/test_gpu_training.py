@@ -208,6 +208,44 @@ def test_loss_captured_and_on_other_streams():
     assert O.workspace_status() == 0
 
 
+def test_calls_at_once():
+    """The three operators on two streams at the same time, eagerly and as two
+    graphs: each call has its own workspace."""
+    sets = [(lce_inputs(700, 264, 9000, BF, 0.2, seed), torch.randint(0, 900, (5000,), device="cuda", generator=gen(seed)),
+             torch.randn(5000, 264, device="cuda", generator=gen(seed)).to(BF)) for seed in (1, 2)]
+
+    def step(inputs):
+        (h, w, t), ids, g = inputs
+        loss = O.linear_cross_entropy(h, w, t, z_loss=1e-3)
+        out = O.embed_tokens(ids, w)
+        r, n = O.residual_norm(out, g, norm="layer", post_norm="rms")
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)), *torch.autograd.grad((r, n), w, (g, g)))
+
+    want = [step(s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append([step(s) for _ in range(3)])
+        torch.cuda.synchronize()
+        for a, many in zip(want, got):
+            assert all(torch.equal(x, y) for b in many for x, y in zip(a, b))
+    graphs, held = [torch.cuda.CUDAGraph() for _ in sets], []
+    for gr, s in zip(graphs, sets):
+        with torch.cuda.graph(gr):
+            held.append(step(s))
+    for _ in range(3):
+        for st, gr in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, held):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert O.workspace_status() == 0
+
+
 def test_loss_refusals():
     h, w, t = lce_inputs(10, 64, 100, BF, 0.0)
     f = O.linear_cross_entropy
