@@ -42,7 +42,8 @@ bool valid(const ossm_norm_args* a, bool bwd) {
     return true;
   }
   if (!a->stats) return false;
-  if (full ? (!a->x || a->x_stride < a->dim || !a->y || a->y_stride < a->dim) : (!a->r || a->x_stride < a->dim)) return false;
+  if (a->x_stride < a->dim || (full && !a->y)) return false;
+  if (a->y ? (!a->x || a->y_stride < a->dim) : !a->r) return false;
   if ((a->grad_r && a->grad_r_stride < a->dim) || (a->grad_h && a->grad_h_stride < a->dim)) return false;
   return a->grad_r || a->grad_h;
 }

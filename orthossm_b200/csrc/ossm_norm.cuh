@@ -7,10 +7,13 @@
 // gradients of what all rows share are added up in registers, a block's rows in
 // order, and the blocks' sums in order by a second kernel.
 //
-// h is of the fp32 r, not of the rounded one that is returned.  Backward reads
-// r as it was rounded where n is y itself (no norm or gate of the block's
-// output): one tensor less to read; its rounding moves the normed values by
-// half a step of the stream's type, as much as rounding a gradient does.
+// h is of the fp32 r, not of the rounded one that is returned.  Where n is y itself
+// (no norm or gate of the block's output), RMSNorm's backward reads r as it was
+// rounded: one tensor less to read; its rounding moves each normed value by half a
+// step of the stream's type, as much as rounding a gradient does.  LayerNorm's, of
+// a 16-bit stream, adds x and y again: a row whose values lie close together would
+// lose what is left after its mean to that rounding (60364 rows of 3 channels, bf16:
+// dx off by 0.19 of its norm, 1.6e-3 this way).
 //
 // What bounds it: HBM where there are few sums (131072 x 512 bf16, RMSNorm: 89 us
 // forward, 100 backward, 6.0 and 5.4 TB/s); with a norm and a gate of y the
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 3 : 1) norm_fwd_kernel(con
 enum { S_W, S_B, S_GATE, S_PW, S_PB, kSums };  // sums over the rows
 
 // SUMS: how many of the sums are kept: the weight's, the bias's too, or all,
-// where the block's output has a norm or a gate, so that y is read.
+// where the block's output has a norm or a gate.
 template <typename TX, typename TY, int N, bool VEC, int SUMS, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2 : 1)
     norm_bwd_kernel(const __grid_constant__ Params p) {
@@ -441,12 +444,12 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2
     for (int i = 0; i < 8 * N; ++i) sum[k][i] = 0.f;
   i64 t = (i64)blockIdx.x * per + mine;
   constexpr int SX = sizeof(TX), SY = sizeof(TY);
-  // r (or x), its gradient, the gradient of h, y
+  // x (or r alone), the gradient of r, of h, y
   const int at1 = p.d * SX, at2 = at1 + (p.dr ? p.d * SX : 0), at3 = at2 + (p.dh ? p.d * SY : 0);
-  Rows<VEC> rows{{{static_cast<const char*>(FULL ? p.x : p.r), p.xst * SX, p.d * SX, 0},
+  Rows<VEC> rows{{{static_cast<const char*>(p.y ? p.x : p.r), p.xst * SX, p.d * SX, 0},
                   {static_cast<const char*>(p.dr), p.drst * SX, p.d * SX, at1},
                   {static_cast<const char*>(p.dh), p.dhst * SY, p.d * SY, at2},
-                  {static_cast<const char*>(FULL ? p.y : nullptr), p.yst * SY, p.d * SY, at3}},
+                  {static_cast<const char*>(p.y), p.yst * SY, p.d * SY, at3}},
                  ring + mine * p.stages * p.stage_bytes, full[mine], p.stages, p.stage_bytes, p.R, o.t, step, p.T,
                  p.status, 0, 0};
   rows.begin(t);
@@ -476,7 +479,13 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2
       for (int i = 0; i < 8 * N; ++i) g[i] = 0.f;
     }
     if (p.dh) rows.template get<TY>(o, 2, t, e);
-    if constexpr (FULL) rows.template get<TY>(o, 3, t, n);
+    if constexpr (FULL) {
+      rows.template get<TY>(o, 3, t, n);
+    } else if (p.y) {
+      float u[8 * N];
+      rows.template get<TY>(o, 3, t, u);
+      fma(v, u, p.scale);
+    }
     float gt = 1.f;
     if constexpr (FULL) {
       // n becomes y normed (or y); a: the block's output after that; v: r again
@@ -670,7 +679,7 @@ inline Params params_of(const ossm_norm_args* a, const Plan& q, bool bwd) {
   };
   rows(a->x, a->x_stride, sx);
   rows(a->y, a->y_stride, sy);
-  rows(a->r, bwd && q.sums < (int)kSums ? a->x_stride : a->dim, sx);
+  rows(a->r, bwd ? a->x_stride : a->dim, sx);
   if (bwd) {
     rows(a->grad_r, a->grad_r_stride, sx);
     rows(a->grad_h, a->grad_h_stride, sy);
@@ -741,7 +750,7 @@ int forward(const ossm_norm_args* a, cudaStream_t st) {
 template <typename TX, typename TY, int SUMS>
 bool launch_bwd(const Plan& q, Params& p, cudaStream_t st) {
   const size_t smem = ring_of(p, q, true, p.d * (int)(sizeof(TX) + (p.dr ? sizeof(TX) : 0) + (p.dh ? sizeof(TY) : 0) +
-                                                      (SUMS == (int)kSums ? sizeof(TY) : 0)));
+                                                      (p.y ? sizeof(TY) : 0)));
   const int which = variant(p, q);
   static constexpr void (*kerns[])(Params) = {
       norm_bwd_kernel<TX, TY, 1, true, SUMS, 256>,  norm_bwd_kernel<TX, TY, 2, true, SUMS, 256>,

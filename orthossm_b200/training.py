@@ -380,7 +380,9 @@ class _NormFn(torch.autograd.Function):
         r, h, stats = _norm_forward((x, y, w, b, gate, pw, pb), opts, True)
         ctx.full = bool(opts[1]) or gate is not None
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*((x, y) if ctx.full else (r, None)), w, b, gate, pw, pb, stats)
+        # r stands for x and y; but less its mean a rounded one may have lost what is normed
+        ctx.sum = ctx.full or (y is not None and opts[0] == L.OSSM_NORM_LAYER and x.dtype is not torch.float32)
+        ctx.save_for_backward(*((x, y) if ctx.sum else (r, None)), w, b, gate, pw, pb, stats)
         ctx.opts = opts
         ctx.has_y = y is not None
         return r, h
@@ -413,7 +415,7 @@ class _NormFn(torch.autograd.Function):
             with _On(dev):
                 stream = _raw_stream(dev)
                 at = xr.data_ptr()
-                a = _NORM.pack(*head, at if full else 0, xst, _at(yr), yst, *mid, 0 if full else at, 0, stats.data_ptr(),
+                a = _NORM.pack(*head, at if ctx.sum else 0, xst, _at(yr), yst, *mid, 0 if ctx.sum else at, 0, stats.data_ptr(),
                                _at(gr), grst, _at(ghr), ghst, _at(dx), _at(dy), _at(dgate), _at(dw), _at(db), _at(dpw),
                                _at(dpb), _status(dev, stream))
                 _run("residual_norm backward", lib.ossm_residual_norm_bwd, a, stream, lib.ossm_norm_workspace_bytes(a),

@@ -427,6 +427,18 @@ def test_norm_gated(shape, gate, post, xdt, ydt):
     check_norm(norm_inputs(shape, xdt, ydt, norm, post, gate, wdt=FP if shape[-1] == 384 else None), norm, post, 0.5)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_norm_rows_of_close_values(dt):
+    """Rows whose spread is below a step of the stream's type: backward norms the sum, not what was returned of it."""
+    ts = norm_inputs((400, 3), dt, dt, "layer", None, None)
+    check_norm(ts, "layer", scale=0.5)
+    ts = norm_inputs((50, 512), dt, dt, "layer", None, None)
+    with torch.no_grad():
+        ts["x"].fill_(100.0)
+        ts["y"].mul_(0.05)
+    check_norm(ts, "layer")
+
+
 def test_norm_many_rows():
     """Sums over more rows than blocks, in fixed order."""
     a = check_norm(norm_inputs((70001, 64), BF, BF, "rms", None, None), "rms")

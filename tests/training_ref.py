@@ -115,9 +115,11 @@ def norm_ref(ts, opts, dr, dh):
         wa = abs(one(v["weight"])) if v["weight"] is None else v["weight"].abs()
         bounds["h"] = (h, 1.01 * u(dt) * h.abs() + 4 * fp * (qm * wa + abs(zero(v["bias"]) if v["bias"] is None
                                                                             else v["bias"].abs())))
-        # backward; without norm or gate of y it starts from the rounded r (or x itself)
+        # backward; without norm or gate of y it starts from the rounded r (or x itself),
+        # but LayerNorm's of a 16-bit stream from x and y
         dhd = dh.double()
-        rounded = y is not None and not post and v["gate"] is None
+        rounded = y is not None and not post and v["gate"] is None and (
+            norm == "rms" or ts["x"].dtype == torch.float32)
         eq = 4 * fp * qm + (1.01 * ux * r.abs() * inv * (1 + q.abs()) if rounded else 0.0)  # of q
         e = dhd * (wa if v["weight"] is None else v["weight"])
         m0 = (e * q).mean(-1, keepdim=True)
