@@ -261,7 +261,7 @@ class OrthoSSMLM(nn.Module):
             raise ValueError(f"loss runs in bf16: cast the model first (parameters are {p.dtype})")
         B, S = input_ids.shape
         if targets is None:
-            targets = torch.full_like(input_ids, ignore_index)
+            targets = torch.full_like(input_ids, ignore_index, dtype=torch.int64)  # uint8 ids do not hold -100
             targets[:, :-1] = input_ids[:, 1:]
             targets.masked_fill_(targets == -1, ignore_index)
         if states is None:
