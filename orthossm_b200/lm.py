@@ -255,7 +255,9 @@ class OrthoSSMLM(nn.Module):
         ``targets`` (default: the next token, none after the last), without the
         logits; arguments and reductions as ``linear_cross_entropy`` has them.
         Differentiable as ``forward`` is (the decay gates are constants).  A
-        position that holds -1 is padding: its embedding is zero."""
+        position that holds -1 is padding: its embedding is zero, and by default
+        neither it nor the position before it has a target.  The states that
+        ``return_state`` adds count padded positions, and decay over them."""
         p = self.embedding.weight
         if p.dtype != torch.bfloat16:
             raise ValueError(f"loss runs in bf16: cast the model first (parameters are {p.dtype})")
@@ -263,7 +265,7 @@ class OrthoSSMLM(nn.Module):
         if targets is None:
             targets = torch.full_like(input_ids, ignore_index, dtype=torch.int64)  # uint8 ids do not hold -100
             targets[:, :-1] = input_ids[:, 1:]
-            targets.masked_fill_(targets == -1, ignore_index)
+            targets.masked_fill_((targets == -1) | (input_ids == -1), ignore_index)
         if states is None:
             states = self.fresh_states(B, input_ids.device)
         norms = [layer.norm_in for layer in self.layers] + [self.final_norm]

@@ -1,5 +1,5 @@
 """The targets that OrthoSSMLM.loss makes of its input: the next token of each
-position, whatever integer type the ids have."""
+position, whatever integer type the ids have, none around padding."""
 import pytest
 import torch
 
@@ -34,6 +34,34 @@ def test_any_integer_type(monkeypatch, dtype, ignore):
     ids = torch.tensor([[3, 100, 7, 120], [0, 1, 2, 3]], dtype=dtype)
     t = made(monkeypatch, ids, ignore_index=ignore)
     assert t.long().tolist() == [[100, 7, 120, ignore], [1, 2, 3, ignore]]
+
+
+def test_padding_anywhere(monkeypatch):
+    """Padding (-1) before, between or after tokens has no target, and is none: what follows it begins a text."""
+    ids = torch.tensor([[-1, -1, 4, 5, 6], [7, -1, -1, 8, 9], [1, 2, 3, -1, -1]])
+    assert made(monkeypatch, ids, ignore_index=-7).tolist() == [[-7, -7, 5, 6, -7], [-7, -7, -7, 9, -7],
+                                                                [2, 3, -7, -7, -7]]
+
+
+@pytest.mark.gpu
+def test_loss_of_left_padding_and_gaps():
+    """No loss where a position or the one after it is padding, and the mean is over the others."""
+    torch.manual_seed(0)
+    model = lm.OrthoSSMLM(lm.OrthoLMConfig(vocab_size=300, n_layers=1, window=64)).to("cuda", torch.bfloat16)
+    ids = torch.randint(0, 300, (2, 150), device="cuda")
+    ids[0, :40] = -1
+    ids[1, 60:70] = -1
+    st = model.fresh_states(2, "cuda", generator_seed=1)
+    with torch.no_grad():
+        each = model.loss(ids, states=st, reduction="none")
+        mean = model.loss(ids, states=st)
+    has = torch.zeros_like(ids, dtype=torch.bool)
+    has[0, 40:-1] = True
+    has[1, :59] = True
+    has[1, 70:-1] = True
+    assert torch.equal(each != 0, has) and each.isfinite().all()
+    # a mean and a sum of 247 fp32 losses, each rounded to 2^-24
+    assert abs(float(mean) - float(each.double().sum() / has.sum())) <= 2.0 ** -23 * float(mean)
 
 
 @pytest.mark.gpu
