@@ -533,8 +533,8 @@ int ossm_embed_bwd(const ossm_embed_args* a, void* workspace, size_t workspace_b
  * Statistics and sums are fp32, in an order that depends on the arguments
  * alone.  Backward from grad_r and grad_h (either may be NULL: zeros).  It
  * reads x and y; or, with y == NULL, r alone (with x_stride): x itself where
- * there was no y, or, with no gate and no post_norm, what forward returned.  Of
- * a 16-bit r that is right for RMSNorm; LayerNorm wants x and y there.
+ * there was no y, or, with no gate and no post_norm, the fp32 r that forward
+ * returned.  (A 16-bit r has been rounded: give x and y there.)
  * The reference composes nn.RMSNorm, a product and a sum
  * (sdpc_engine.py:420-426).
  * ------------------------------------------------------------------------ */

@@ -7,16 +7,16 @@
 // gradients of what all rows share are added up in registers, a block's rows in
 // order, and the blocks' sums in order by a second kernel.
 //
-// h is of the fp32 r, not of the rounded one that is returned.  Where n is y itself
-// (no norm or gate of the block's output), RMSNorm's backward reads r as it was
-// rounded: one tensor less to read; its rounding moves each normed value by half a
-// step of the stream's type, as much as rounding a gradient does.  LayerNorm's, of
-// a 16-bit stream, adds x and y again: a row whose values lie close together would
-// lose what is left after its mean to that rounding (60364 rows of 3 channels, bf16:
-// dx off by 0.19 of its norm, 1.6e-3 this way).
+// h is of the fp32 r, not of the rounded one that is returned, and so are the
+// gradients: backward adds x and y again, unless r is fp32 itself.  Normed values
+// of a rounded r are off by half a step each, and the gradients are differences
+// of them: dx = inv (e - v mean(e v) - mean(e)) takes off what is parallel to v, and
+// LayerNorm's v is less its mean.  (RMSNorm of 512 channels with e about parallel
+// to v, dx from the rounded r: off by 1.1 times its norm, 1.6e-3 from x and y.
+// LayerNorm, 60364 rows of 3 channels, bf16: 0.19 and 1.6e-3.)
 //
 // What bounds it: HBM where there are few sums (131072 x 512 bf16, RMSNorm: 89 us
-// forward, 100 backward, 6.0 and 5.4 TB/s); with a norm and a gate of y the
+// forward, 111 backward, 6.0 TB/s each); with a norm and a gate of y the
 // instructions of a row and the way between its two sums (16384 x 2048, fp32
 // stream: 80 and 173 us, 5.0 and 3.5 TB/s).
 #pragma once

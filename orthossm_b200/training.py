@@ -380,8 +380,8 @@ class _NormFn(torch.autograd.Function):
         r, h, stats = _norm_forward((x, y, w, b, gate, pw, pb), opts, True)
         ctx.full = bool(opts[1]) or gate is not None
         ctx.set_materialize_grads(False)
-        # r stands for x and y; but less its mean a rounded one may have lost what is normed
-        ctx.sum = ctx.full or (y is not None and opts[0] == L.OSSM_NORM_LAYER and x.dtype is not torch.float32)
+        # an fp32 r stands for x and y; a rounded one may have lost what the gradients are a difference of
+        ctx.sum = ctx.full or (y is not None and x.dtype is not torch.float32)
         ctx.save_for_backward(*((x, y) if ctx.sum else (r, None)), w, b, gate, pw, pb, stats)
         ctx.opts = opts
         ctx.has_y = y is not None
