@@ -173,6 +173,9 @@ struct Params {
 // (A row ahead in registers kept 48 KB an SM on its way and cost 24 to 48 of
 // them: 131072 x 512 bf16, backward: 119 us.)
 constexpr int kMaxStages = 8;
+#ifndef OSSM_NORM_POLLS
+#define OSSM_NORM_POLLS (1u << 22)  // of a wait for a row; a test compiles the kernels with none
+#endif
 struct Tensor {
   const char* p;  // NULL: not there
   i64 stride;     // in bytes
@@ -205,8 +208,19 @@ struct Rows {
   OSSM_DEV void meet() const {
     if (R == 32) __syncwarp(); else __syncthreads();
   }
-  OSSM_DEV void wait() const {
-    if (VEC && !sm100::mbar_wait(full + slot, turn) && status) atomicExch(status, (uint32_t)OSSM_ETIMEOUT);
+  // For the row at hand.  A thread whose wait runs out goes on without waiting;
+  // the one that issues copies issues no more, and stays until those on their
+  // way have landed: none may be when the ring is used again or the block ends.
+  OSSM_DEV void wait(i64 row) {
+    if (!VEC || turn > 1 || sm100::mbar_wait(full + slot, turn, OSSM_NORM_POLLS)) return;
+    if (status) atomicExch(status, (uint32_t)OSSM_ETIMEOUT);
+    if (lane == 0) {
+      for (int i = 0; i < stages && row + i * step < T; ++i) {
+        const bool next = (int)slot + i >= stages;
+        sm100::mbar_wait(full + slot + i - (next ? stages : 0), turn ^ (next ? 1 : 0));
+      }
+    }
+    T = 0, turn |= 2;
   }
   // Tensor i's row `row`, the row at hand.
   template <typename E, int N>
@@ -375,7 +389,7 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 3 : 1) norm_fwd_kernel(con
   const Shares own(p, ring, per);
   for (; t < p.T; t += step) {
     float v[8 * N], u[8 * N];
-    rows.wait();
+    rows.wait(t);
     rows.template get<TX>(o, 0, t, v);
     if (p.y) rows.template get<TY>(o, 1, t, u);
     float mean, inv, pmean = 0.f, pinv = 1.f;
@@ -470,7 +484,7 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 && (N == 1 || SUMS <= 2) ? 2
     float v[8 * N], g[8 * N], e[8 * N], n[FULL ? 8 * N : 1], a[FULL ? 8 * N : 1];
     const float inv = inv_a, mean = mean_a, pinv = pinv_a, pmean = pmean_a;
     stats(t + step);
-    rows.wait();
+    rows.wait(t);
     rows.template get<TX>(o, 0, t, v);
     if (p.dr) {
       rows.template get<TX>(o, 1, t, g);

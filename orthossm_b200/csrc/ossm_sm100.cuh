@@ -24,9 +24,9 @@ OSSM_DEV void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
                : "memory");
 }
 // Bounded parity wait; returns false when it gave up (the caller records an error).
-OSSM_DEV bool mbar_wait(uint64_t* bar, uint32_t parity) {
+OSSM_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t polls = 1u << 22) {
   const uint32_t a = smem_u32(bar);
-  for (uint32_t it = 0; it < (1u << 22); ++it) {
+  for (uint32_t it = 0; it < polls; ++it) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
