@@ -820,7 +820,8 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
         const i64 t = t0 + i * kRowThreads;
         const float f = p.reduction || t >= p.T ? 1.f : fabsf(__ldg(p.g + t));
         const float l = p.zl > 0.f && t < p.T ? __ldg(p.lse + t) : 0.f;
-        if (has[i]) top = fmaxf(top, f * fmaxf(1.f, fabsf(1.f + 2.f * p.zl * l)));
+        const float factor = f * fmaxf(1.f, fabsf(1.f + 2.f * p.zl * l));
+        if (has[i] && isfinite(factor)) top = fmaxf(top, factor);  // others spoil their own row alone
       }
     } else if (BWD) {
       top = 1.f;
