@@ -490,6 +490,8 @@ typedef struct {
   void* grad_hidden;                 /* [tokens, dim] contiguous, 16-byte aligned, or NULL */
   void* grad_weight;                 /* [vocab, dim] contiguous, 16-byte aligned, or NULL */
   uint32_t* status;                  /* a device word that a wait that ran out sets to OSSM_ETIMEOUT, or NULL */
+  float* lse_rest;                   /* [tokens] or NULL: what lse's rounding left, written and read as lse is; without it
+                                        the probabilities of backward are off by up to lse 2^-24, relative */
 } ossm_lce_args;
 
 /* Bytes of device workspace (0 for invalid arguments), 256-byte aligned, with

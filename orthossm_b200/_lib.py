@@ -131,7 +131,7 @@ class LceArgs(C.Structure):
         ("tokens", _i64), ("dim", _i32), ("vocab", _i32), ("dtype", _i32), ("hidden", _vp), ("hidden_stride", _i64),
         ("weight", _vp), ("weight_stride", _i64), ("targets", _vp), ("ignore_index", _i64), ("z_loss", _f32),
         ("reduction", _i32), ("loss", _vp), ("lse", _vp), ("grad_loss", _vp), ("grad_hidden", _vp),
-        ("grad_weight", _vp), ("status", _vp),
+        ("grad_weight", _vp), ("status", _vp), ("lse_rest", _vp),
     ]
 
 

@@ -84,7 +84,7 @@ struct Params {
   i64 ignore;
   float zl;
   int reduction;
-  float *loss, *lse;
+  float *loss, *lse, *rest;
   const float* g;
   void *dh, *dw;
   Head* head;
@@ -869,12 +869,17 @@ __global__ void __launch_bounds__(kRowThreads) lce_rows_kernel(const __grid_cons
         const float lse = __ldg(p.lse + t), g = p.reduction ? 1.f : __ldg(p.g + t);
         // a target outside the vocabulary: NaN, as its loss
         const float f = known ? g * inv : NAN;
-        p.lse2[place] = lse * kLog2e;
-        p.fa[place] = f * (1.f + 2.f * p.zl * lse);
+        // the exponent takes lse in fp32, its factor what that leaves: a sure token's
+        // gradient is the difference of a probability and 1
+        const double l2 = ((double)lse + (p.rest ? (double)__ldg(p.rest + t) : 0.0)) * 1.4426950408889634;
+        const float hi = (float)l2, left = (float)((double)hi - l2);
+        p.lse2[place] = hi;
+        p.fa[place] = f * (1.f + 2.f * p.zl * lse) * (fabsf(left) < 1.f ? fmaf(left, 0.6931472f, 1.f) : 1.f);
         p.fb[place] = f;
       }
     } else if (!BWD && t < c1) {
       p.lse[t] = 0.f;
+      if (p.rest) p.rest[t] = 0.f;
       if (!p.reduction) p.loss[t] = 0.f;
     }
     if (!gather) continue;
@@ -947,10 +952,12 @@ __global__ void __launch_bounds__(kFinishThreads) lce_finish_kernel(const __grid
     }
     if (r < n && mine == 0) {
       const int t = p.rows[r];
-      const double lse = ((double)m + log2((double)l)) * 0.6931471805599453;
-      double loss = lse - (double)p.zt[r] + (double)p.zl * lse * lse;
+      const double lse2 = (double)m + log2((double)l), lse = lse2 * 0.6931471805599453;
+      // less the target's logit in the same units: log2(e) is kLog2e in both
+      double loss = (lse2 - (double)p.zt[r] * (double)kLog2e) * 0.6931471805599453 + (double)p.zl * lse * lse;
       if (p.tgt[r] < 0) loss = NAN;
       p.lse[t] = (float)lse;
+      if (p.rest) p.rest[t] = isfinite(lse) ? (float)(lse - (double)(float)lse) : 0.f;
       if (!p.reduction) p.loss[t] = (float)loss;
       sum += loss;
     }
@@ -1050,7 +1057,7 @@ Params params_of(const ossm_lce_args* a, const Plan& q, char* w, bool bwd) {
   p.dst = (a->dim + 63) / 64 * 64;
   p.hidden = a->hidden, p.hst = a->hidden_stride;
   p.targets = a->targets, p.ignore = a->ignore_index, p.zl = a->z_loss, p.reduction = a->reduction;
-  p.loss = a->loss, p.lse = a->lse, p.g = a->grad_loss, p.dh = a->grad_hidden, p.dw = a->grad_weight;
+  p.loss = a->loss, p.lse = a->lse, p.rest = a->lse_rest, p.g = a->grad_loss, p.dh = a->grad_hidden, p.dw = a->grad_weight;
   p.head = reinterpret_cast<Head*>(w + q.at[0]);
   p.rows = reinterpret_cast<int*>(w + q.at[1]);
   p.tgt = reinterpret_cast<int*>(w + q.at[2]);

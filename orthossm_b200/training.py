@@ -30,7 +30,7 @@ _REDUCTIONS = {"none": L.OSSM_LOSS_NONE, "mean": L.OSSM_LOSS_MEAN, "sum": L.OSSM
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a Stream object (2 us)
 _current_device = torch._C._cuda_getDevice
 # The argument structs of the C ABI as bytes, with its alignment: packed in a third of a ctypes struct's time.
-_LCE = struct.Struct("@qiiiPqPqPqfiPPPPPP")
+_LCE = struct.Struct("@qiiiPqPqPqfiPPPPPPP")
 _EMBED = struct.Struct("@qiiiPPqfPPqP")
 _NORM = struct.Struct("@qiiiPqPqPiiqfiiffPPPPiiiiPPPPqPqPPPPPPPP")
 for _s, _c in ((_LCE, L.LceArgs), (_EMBED, L.EmbedArgs), (_NORM, L.NormArgs)):
@@ -110,7 +110,7 @@ def _rows(t, d, align=False):
 # ----------------------------------------------------------------------------
 
 def _lce_call(hidden, weight, targets, opts, loss, lse, dev, bwd, grads=(0, 0, 0)):
-    """Forward (loss, lse: None or where to) or backward (grads: of the loss, where to); returns the first lse."""
+    """Forward (loss, lse: None or [2, T], its value and what rounding left) or backward (grads: of the loss, where to)."""
     ignore, z_loss, reduction = opts
     V, d = weight.shape
     h, hst = _rows(hidden, d, align=True)
@@ -121,7 +121,8 @@ def _lce_call(hidden, weight, targets, opts, loss, lse, dev, bwd, grads=(0, 0, 0
     with _On(dev):
         lib, stream = L.lib(), _raw_stream(dev)
         values = [T, d, V, _DT[weight.dtype], h.data_ptr(), hst, w.data_ptr(), wst, targets.data_ptr(), ignore, z_loss,
-                  reduction, _at(loss), 1 if lse is None else lse.data_ptr(), *grads, _status(dev, stream)]
+                  reduction, _at(loss), 1 if lse is None else lse.data_ptr(), *grads, _status(dev, stream),
+                  0 if lse is None else lse.data_ptr() + 4 * T]
         nbytes = lib.ossm_lce_workspace_bytes(_LCE.pack(*values), bwd)
         if nbytes == 0:
             L.check(L.OSSM_EINVAL, "linear_cross_entropy (argument check)")
@@ -141,7 +142,7 @@ def _lce_forward(hidden, weight, targets, opts, keep_lse=False):
         loss = torch.zeros(targets.shape if opts[2] == 0 else (), device=hidden.device)
         return loss, torch.empty(0, device=hidden.device)
     loss = torch.empty(targets.shape if opts[2] == 0 else (), device=hidden.device)
-    lse = torch.empty(T, device=hidden.device) if keep_lse else None
+    lse = torch.empty(2, T, device=hidden.device) if keep_lse else None
     _lce_call(hidden, weight, targets, opts, loss, lse, dev, 0)
     return loss, lse
 

@@ -1,9 +1,11 @@
-"""linear_cross_entropy where few tests reach: rows of very different weights."""
+"""linear_cross_entropy where few tests reach: rows of very different weights,
+sure tokens."""
 import pytest
 import torch
 
 import orthossm_b200 as O
 from tests.test_gpu_training import BF, HF, gen, lce_inputs
+from tests.training_ref import assert_within, u
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +26,59 @@ def test_a_weight_that_is_not_finite(bad, dt):
     rest = torch.arange(300, device="cuda") != k
     assert float(want[rest].float().norm()) > 0 and torch.equal(dh[rest], want[rest])
     assert not dh[k].isfinite().any() and not dw.isfinite().any()
+
+
+def sure_inputs(T, V, dt, gap, shift):
+    """Tokens whose target's logit lies about ``gap`` above log of the others' sum,
+    all logits near ``shift``: the first channel shifts, the others tell targets apart."""
+    d = 64
+    g = gen(4)
+    w = torch.randn(V, d, device="cuda", generator=g) / 8
+    w[:, 0] = 1.0
+    w = w.to(dt)
+    t = torch.randperm(V, device="cuda", generator=g)[:T]
+    rest = w.double().clone()
+    rest[:, 0] = 0
+    h = torch.zeros(T, d, device="cuda", dtype=torch.float64)
+    for _ in range(60):  # along the target's row until it is as far above the others
+        h[:, 0] = 0
+        z = h @ rest.t()
+        zt = z.gather(1, t[:, None])[:, 0]
+        z.scatter_(1, t[:, None], -torch.inf)
+        h += (gap - (zt - z.logsumexp(1)))[:, None].clamp(-2, 2) * 0.7 * rest[t] / rest[t].square().sum(1, keepdim=True)
+    h[:, 0] = shift
+    return h.to(dt).requires_grad_(), w.requires_grad_(), t
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("gap", [5.0, 9.0])
+@pytest.mark.parametrize("shift", [0.0, 20.0, 100.0])
+def test_sure_tokens(shift, gap, dt):
+    """A token of probability 1 - q has gradients of the size of q.  dW of the
+    targets' rows is -g q h: q's own error is at most exp's of the logits' fp32
+    sums (64 + 8 terms within 2^-23 of their magnitudes, of the target and of the
+    others), and beside it, relative to 1 and not to q, the softmax's fp32 sum
+    and 2^x: 42 additions of 2^-24 that the largest term sees (the 32 of its run,
+    and those of the runs, halves and tiles of 1000 columns) and twice 2^-22."""
+    V, T = 1000, 200
+    h, w, t = sure_inputs(T, V, dt, gap, shift)
+    loss = O.linear_cross_entropy(h, w, t, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    H, W = h.detach().double(), w.detach().double()
+    z = H @ W.t()
+    p = z.softmax(1)
+    q = 1 - p.gather(1, t[:, None])[:, 0]
+    assert q.median() < 2 * torch.tensor(-gap).exp()
+    ez = 72 * 2.0 ** -23 * (H.abs() @ W.abs().t()).amax(1)
+    eq = q * 2 * ez * 1.01 + 42 * 2.0 ** -24 + 2 * 2.0 ** -22
+    dz = p.clone()
+    dz.scatter_add_(1, t[:, None], torch.full_like(q, -1.0)[:, None])
+    want = -q[:, None] * H + (dz.scatter(1, t[:, None], 0.0).t() @ H)[t]  # other tokens' small part too
+    mag = q[:, None] * H.abs() + (dz.scatter(1, t[:, None], 0.0).t() @ H.abs())[t]
+    bound = eq[:, None] * H.abs() + 2.02 * u(dt) * mag + 2e-3 * (mag - q[:, None] * H.abs()) + T * 2.0 ** -23 * mag
+    if dt is HF:  # probabilities below 2^-28 of the largest factor, outputs below the normal numbers
+        bound = bound + 2.0 ** -39 * H.abs().sum(0) + 2.0 ** -25
+    assert_within(dw[t], want, bound, "dweight")
+    with torch.no_grad():  # the loss, -log(1 - q), of that size too
+        each = O.linear_cross_entropy(h, w, t, reduction="none")
+    assert_within(each, -torch.log1p(-q), 1.1 * eq + q * 2.0 ** -24, "loss")
