@@ -515,7 +515,7 @@ typedef struct {
   const int64_t* ids;                /* [tokens] on the device */
   const void* weight;                /* [vocab, dim], unit channel stride */
   int64_t weight_stride;
-  float scale;
+  float scale;                       /* finite */
   void* out;                         /* [tokens, dim] contiguous */
   const void* grad_out;              /* backward: [tokens, dim], unit channel stride */
   int64_t grad_out_stride;

@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "ossm_attn.cuh"
 
@@ -435,7 +436,7 @@ bool valid(const ossm_embed_args* a, bool bwd) {
   if (!a || a->tokens < 0 || a->tokens > (1LL << 31) - 1 || a->dim < 1 || a->dim > (1 << 16)) return false;
   if (a->vocab < 1 || a->vocab >= (1 << 27)) return false;
   if (a->dtype != OSSM_F32 && a->dtype != OSSM_BF16 && a->dtype != OSSM_F16) return false;
-  if (a->tokens && !a->ids) return false;
+  if ((a->tokens && !a->ids) || !std::isfinite(a->scale)) return false;
   if (bwd) return a->grad_weight && (a->tokens == 0 || (a->grad_out && a->grad_out_stride >= a->dim));
   return a->weight && a->weight_stride >= a->dim && (a->tokens == 0 || a->out);
 }

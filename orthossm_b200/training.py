@@ -11,7 +11,6 @@ gradients and forward-mode derivatives are refused.
 """
 from __future__ import annotations
 
-import math
 import struct
 from typing import Optional, Tuple
 
@@ -23,6 +22,7 @@ from . import _lib as L
 from .sdpc_kernel import _WS_TRAIN, _captured_workspace, _is_capturing, _need_cuda, _workspace
 
 _DT = {torch.float32: L.OSSM_F32, torch.bfloat16: L.OSSM_BF16, torch.float16: L.OSSM_F16}
+_F32_MAX = torch.finfo(torch.float32).max  # the kernels take scalars in fp32
 _INTS = (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8)
 _NORMS = {"rms": L.OSSM_NORM_RMS, "layer": L.OSSM_NORM_LAYER}
 _REDUCTIONS = {"none": L.OSSM_LOSS_NONE, "mean": L.OSSM_LOSS_MEAN, "sum": L.OSSM_LOSS_SUM}
@@ -195,7 +195,7 @@ def _refuse_loss(hidden, weight, targets, ignore_index, z_loss, reduction):
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if not -1 << 63 <= ignore_index < 1 << 63:
         raise ValueError(f"linear_cross_entropy: ignore_index must fit 64 bits, got {ignore_index}")
-    raise ValueError(f"linear_cross_entropy: z_loss must be finite and not negative, got {z_loss}")
+    raise ValueError(f"linear_cross_entropy: z_loss must be finite in fp32 and not negative, got {z_loss}")
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
@@ -221,7 +221,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     dev, dt, shape = hidden.get_device(), hidden.dtype, targets.shape
     code = _REDUCTIONS.get(reduction)
     ok = (dev >= 0 and (dt is torch.bfloat16 or dt is torch.float16) and weight.dtype is dt and weight.dim() == 2
-          and hidden.dim() == len(shape) + 1 and code is not None and 0.0 <= z_loss < math.inf
+          and hidden.dim() == len(shape) + 1 and code is not None and 0.0 <= z_loss <= _F32_MAX
           and -1 << 63 <= ignore_index < 1 << 63
           and weight.get_device() == dev and targets.get_device() == dev and targets.dtype in _INTS)
     if ok:
@@ -298,7 +298,7 @@ def _refuse_embed(ids, weight, scale):
         raise ValueError(f"embed_tokens: below 2^31 integer ids expected, got {ids.numel()} {ids.dtype}")
     if ids.get_device() != weight.get_device():
         raise ValueError("embed_tokens: ids and weight must be on one device")
-    raise ValueError(f"embed_tokens: scale must be finite, got {scale}")
+    raise ValueError(f"embed_tokens: scale must be finite in fp32, got {scale}")
 
 
 def embed_tokens(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
@@ -312,7 +312,7 @@ def embed_tokens(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0)
     fixed pieces) and rounded once; rows without a position get zeros."""
     dev = weight.get_device()
     ok = (dev >= 0 and ids.get_device() == dev and weight.dim() == 2 and weight.dtype in _DT and ids.dtype in _INTS
-          and ids.numel() < 1 << 31 and math.isfinite(scale))
+          and ids.numel() < 1 << 31 and -_F32_MAX <= scale <= _F32_MAX)
     if ok:
         V, d = weight.shape
         ok = 1 <= V < 1 << 27 and 1 <= d <= 1 << 16
@@ -461,7 +461,7 @@ def _refuse_norm(x, y, weight, bias, norm, eps, gate, scale, post_norm, post_wei
                f"{tuple(gate.shape)} {gate.dtype}")
     if any(t is not None and t.get_device() != x.get_device() for t in (y, weight, bias, gate, post_weight, post_bias)):
         refuse("all tensors must be on one device")
-    refuse(f"eps {eps} and post_eps {post_eps} must be finite and not negative, scale {scale} finite")
+    refuse(f"eps {eps} and post_eps {post_eps} must be finite in fp32 and not negative, scale {scale} finite in fp32")
 
 
 def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
@@ -497,7 +497,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Opt
     kind = L.OSSM_GATE_NONE
     ok = (dev >= 0 and xdt in _DT and dt in _DT and (dt is xdt or xdt is torch.float32) and 1 <= d <= 8192
           and x.numel() < d << 31 and code and post is not None
-          and 0.0 <= eps < math.inf and 0.0 <= post_eps < math.inf and math.isfinite(scale))
+          and 0.0 <= eps <= _F32_MAX and 0.0 <= post_eps <= _F32_MAX and -_F32_MAX <= scale <= _F32_MAX)
     if ok:
         if y is not None:
             ok = y.shape == shape and y.dtype is dt and y.get_device() == dev
