@@ -46,6 +46,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
     deps.append(os.path.join(INCLUDE, "orthossm_b200.h"))
     if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(d) for d in deps):
         return out
+    stamps = {d: os.stat(d).st_mtime_ns for d in deps}
     cuda_lib = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "lib64")
     cc = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", f"-I{INCLUDE}", f"-I{CSRC}"]
     if verbose:
@@ -61,6 +62,11 @@ def build(verbose: bool = False, force: bool = False) -> str:
             print("\n".join(" ".join(c) for c in [*cmds, cmds_link]), flush=True)
         list(pool.map(lambda c: subprocess.run(c, check=True), cmds))
         subprocess.run(cmds_link, check=True)
+    # files compiled before and after an edit of a header do not agree on its structs
+    changed = [os.path.basename(d) for d, t in stamps.items() if not os.path.exists(d) or os.stat(d).st_mtime_ns != t]
+    if changed:
+        os.unlink(out + ".tmp")
+        raise RuntimeError(f"{', '.join(changed)} changed while the library was compiled: build again")
     os.replace(out + ".tmp", out)
     return out
 
