@@ -1,11 +1,12 @@
 """linear_cross_entropy where few tests reach: rows of very different weights,
-sure tokens."""
+sure tokens, several groups of rows, several pieces, very wide states, and
+differences."""
 import pytest
 import torch
 
 import orthossm_b200 as O
-from tests.test_gpu_training import BF, HF, gen, lce_inputs
-from tests.training_ref import assert_within, u
+from tests.test_gpu_training import BF, HF, check_lce, gen, lce_inputs
+from tests.training_ref import assert_within, lce_ref, u
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +83,75 @@ def test_sure_tokens(shift, gap, dt):
     with torch.no_grad():  # the loss, -log(1 - q), of that size too
         each = O.linear_cross_entropy(h, w, t, reduction="none")
     assert_within(each, -torch.log1p(-q), 1.1 * eq + q * 2.0 ** -24, "loss")
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_weights_over_decades(dt):
+    """Per-token weights from 4096 down to 2^-12: dz is in units of the largest
+    weight of the call, so a row of a share rho of it keeps probabilities down to
+    2^-28 / rho in fp16.  Each element within lce_ref's bound, which counts that."""
+    T, d, V = 260, 128, 4000
+    h, w, t = lce_inputs(T, d, V, dt, 0.1)
+    loss = O.linear_cross_entropy(h, w, t, reduction="none")
+    up = 4096.0 * 2.0 ** (-24 * torch.arange(T, device="cuda") / (T - 1))
+    got = torch.autograd.grad(loss, (h, w), up)
+    want, bound = lce_ref(h, w, t, up, reduction="none")
+    for a, b, c, what in zip(got, want[1:], bound[1:], ("dhidden", "dweight")):
+        assert_within(a, b, c, what)
+    # in norm: a row's softmax part loses at most 2^-25 2^-14 of the largest weight an element, as noise over the columns
+    on = t != -100
+    off = (got[0].double() - want[1]).norm(dim=1)[on]
+    tiny = 2.0 ** -25 if dt is HF else 0.0  # half of the output's smallest step
+    allowed = (2.02 * u(dt) * want[1].norm(dim=1) + tiny * d ** 0.5)[on]
+    allowed = allowed + (4096.0 * 2.0 ** -39 * w.detach().double().norm() if dt is HF else 0.0) + 1e-4 * up[on]
+    assert (off <= allowed).all()
+
+
+@pytest.mark.parametrize("T,d,V,ignored", [(8400, 2048, 700, 0.0), (8900, 2048, 300, 0.05), (33500, 512, 600, 0.0)])
+def test_several_groups_of_row_blocks(T, d, V, ignored):
+    """More than 32 MB of states: the blocks of rows stand in two groups, the last one smaller."""
+    check_lce(*lce_inputs(T, d, V, BF, ignored), z_loss=1e-4)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_several_pieces_and_no_token_ignored(reduction):
+    """40000 tokens take pieces of 6656 columns: two, the second a ragged one; the states are read where they lie."""
+    check_lce(*lce_inputs(40000, 24, 7003, HF, 0.0), reduction=reduction)
+
+
+@pytest.mark.parametrize("T,d,V", [(130, 16392, 300), (5, 65536, 257)])
+def test_very_wide_states(T, d, V):
+    check_lce(*lce_inputs(T, d, V, BF, 0.1))
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("of", ["hidden", "weight"])
+def test_differences(of, dt):
+    """The slope along a direction from the loss alone, in float64: central
+    differences at two steps (their difference bounds what the finer one is off
+    by), along the gradient's own signs, along its positive part, and at random.
+    The allowance is the gradient's rounding bound along the direction; it has to
+    be a small part of the slope, so a gradient that is 0 or twice as large fails."""
+    h, w, t = lce_inputs(64, 64, 500, dt, 0.2)
+    loss = O.linear_cross_entropy(h, w, t, reduction="sum", z_loss=1e-3)
+    grad = torch.autograd.grad(loss, (h, w))[of == "weight"].double()
+    on = t != -100
+    H, W = h.detach().double(), w.detach().double()
+
+    def f(v):
+        z = (v if of == "hidden" else H)[on] @ (W if of == "hidden" else v).t()
+        lse = z.logsumexp(1)
+        return (lse - z.gather(1, t[on][:, None])[:, 0] + 1e-3 * lse ** 2).sum()
+
+    at = H if of == "hidden" else W
+    _, bound = lce_ref(h, w, t, torch.ones((), device="cuda"), z_loss=1e-3, reduction="sum")
+    bound = bound[1 + (of == "weight")]
+    exact = torch.autograd.grad(f(at.requires_grad_()), at)[0]
+    at = at.detach()
+    noise = torch.randn(at.shape, device="cuda", dtype=torch.float64, generator=gen(3))
+    for e in (exact.sign(), exact.clamp(min=0), noise + 2 * exact.abs().mean() ** -1 * exact):
+        e = e / e.norm()
+        d1, d2 = ((f(at + s * e) - f(at - s * e)) / (2 * s) for s in (2.0 ** -6, 2.0 ** -7))
+        allowed = (bound * e.abs()).sum() + 2 * (d1 - d2).abs()
+        assert allowed < 0.1 * d2.abs()
+        assert ((grad * e).sum() - d2).abs() <= allowed
