@@ -466,8 +466,9 @@ int ossm_sample_tokens(const ossm_sample_args* a, ossm_stream_t stream);
  *   dz_tv = g_t ((1 + 2 z_loss lse_t) exp(z_tv - lse_t) - [v = target])
  *   grad_hidden = dz weight,  grad_weight = dz^T hidden
  * with the logits computed again, a piece of the vocabulary at a time; dz is
- * rounded to the inputs' type, as the tensor core takes it.  Sums are fp32 or
- * wider and their order depends on the arguments alone.
+ * rounded to the inputs' type, as the tensor core takes it, in units of the
+ * largest factor of all tokens.  Sums are fp32 (the products' on the tensor core,
+ * which cuts) or wider and their order depends on the arguments alone.
  * No counterpart in the reference, whose training script takes
  * F.cross_entropy of whole logits (model.py:23-187 returns them).
  * ------------------------------------------------------------------------ */

@@ -15,15 +15,18 @@
 // Tokens without a target have no part in any product: their states are not
 // read, so NaN there harms nothing, and they cost nothing.
 //
-// dz is rounded to the inputs' 16 bits, as the tensor core takes it: outputs are
-// 1.1 to 1.2 times as far from float64 as fp32 products leave them.
+// dz is rounded to the inputs' 16 bits, as the tensor core takes it: gradients are
+// 1.1 to 1.5 times as far from float64 as fp32 products leave them (up to 2.7 and
+// 7.6 times, dH and dW, for single tokens, where its largest entry is everything).
+// The logits' sums are the tensor core's, which cut where fp32 rounds: a loss is off
+// by 2e-7 of its value at 512 channels, 6e-7 (one token: 1e-5) at 2000.
 //
 // What bounds it: the tensor pipe, 8 T d V operations where keeping the logits
 // would take 6, and in long runs the power cap.  Measured in bursts, 16384
 // tokens, 512 channels, 32000 columns, bf16: stats 316 to 324 us (1625 to 1665
-// TFLOP/s, the pipe 97 % busy), gradz 444 to 454 (its dz, a gigabyte, costs 100 of
-// them), the products 786 to 821 and their joins 42 to 44; 8192, 2048, 131072: 2872, 3076, 6843 and 87 us (1531,
-// 1430, 1286 TFLOP/s).
+// TFLOP/s, the pipe 97 % busy), gradz 439 to 454 (its dz, a gigabyte, costs 100 of
+// them), the products 786 to 821 and their joins 42 to 44; 8192, 2048, 131072: 2872 to 2910, 3076 to 3160, 6843 to
+// 6949 and 87 to 92 us (1511 to 1531, 1392 to 1430, 1266 to 1286 TFLOP/s).
 // Tried: pieces of 32 to 256 MB (3 to 60 % slower), A's tile resident (2 % in a
 // timing probe at 512 channels), one CTA a tile (6 to 17 % slower in the products).
 #include <cuda.h>
@@ -70,9 +73,11 @@ struct Head {      // of the workspace
   float unit;      // backward: what dz in the workspace is in units of
   uint32_t count;  // finished blocks
 };
-// dz is written in units that bring the largest factor of a row to kDzScale:
-// probabilities down to 2^-28 stay out of fp16's subnormals, whatever the loss
-// was multiplied by.  (bf16 has the exponents, but one rule does.)
+// dz is written in units that bring the largest factor of all rows to kDzScale:
+// its row's probabilities down to 2^-28 stay out of fp16's subnormals, whatever the
+// loss was multiplied by, and those down to 2^-28 / rho of a row with a share rho
+// of that factor.  One unit, as dW sums over rows.  (bf16 has the exponents, but
+// one rule does.)
 constexpr float kDzScale = 16384.f;
 
 struct Params {

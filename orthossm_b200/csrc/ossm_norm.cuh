@@ -12,13 +12,13 @@
 // of a rounded r are off by half a step each, and the gradients are differences
 // of them: dx = inv (e - v mean(e v) - mean(e)) takes off what is parallel to v, and
 // LayerNorm's v is less its mean.  (RMSNorm of 512 channels with e about parallel
-// to v, dx from the rounded r: off by 1.1 times its norm, 1.6e-3 from x and y.
+// to v, dx from the rounded r: off by 1.1 times its norm, bf16 1.7e-3 from x and y.
 // LayerNorm, 60364 rows of 3 channels, bf16: 0.19 and 1.6e-3.)
 //
 // What bounds it: HBM where there are few sums (131072 x 512 bf16, RMSNorm: 89 us
 // forward, 111 backward, 6.0 TB/s each); with a norm and a gate of y the
-// instructions of a row and the way between its two sums (16384 x 2048, fp32
-// stream: 80 and 173 us, 5.0 and 3.5 TB/s).
+// latency of a row, whose two sums wait for each other with two rows an SM (16384 x
+// 2048, fp32 stream: 80 and 175 us, 5.0 and 3.5 TB/s).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -660,8 +660,8 @@ constexpr int kRingBytes = 208 << 10;
 // Threads of a row: a warp up to 512 channels (8 rows a block), beyond that a
 // block with 16 channels a thread; backward, which keeps up to five sums a
 // channel in registers, 8 channels up to 2048 (with all five from 256 on).  (16384 x 2048, fp32 stream, two
-// norms and a gate: 103 us forward with 8 channels a thread, 86 us with 16;
-// 197 and 219 us backward.)
+// norms and a gate, side by side before two channels an instruction: 103 us forward
+// with 8 channels a thread, 86 with 16; 197 and 219 us backward.)
 inline Plan plan_of(const ossm_norm_args* a, bool bwd) {
   Plan q{};
   const int runs = (a->dim + 7) / 8;
