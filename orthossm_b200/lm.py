@@ -263,9 +263,10 @@ class OrthoSSMLM(nn.Module):
             raise ValueError(f"loss runs in bf16: cast the model first (parameters are {p.dtype})")
         B, S = input_ids.shape
         if targets is None:
-            targets = torch.full_like(input_ids, ignore_index, dtype=torch.int64)  # uint8 ids do not hold -100
-            targets[:, :-1] = input_ids[:, 1:]
-            targets.masked_fill_((targets == -1) | (input_ids == -1), ignore_index)
+            ids = input_ids.long()  # uint8 does not hold -100, and takes 255 for -1
+            targets = torch.full_like(ids, ignore_index)
+            targets[:, :-1] = ids[:, 1:]
+            targets.masked_fill_((targets == -1) | (ids == -1), ignore_index)
         if states is None:
             states = self.fresh_states(B, input_ids.device)
         norms = [layer.norm_in for layer in self.layers] + [self.final_norm]

@@ -492,7 +492,8 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Opt
     gate: None, [d] (a value per channel), [..., 1] (per token), or y's shape.
 
     Differentiable in all tensors.  Arithmetic, statistics and sums are fp32; h
-    is the norm of r before its rounding."""
+    is the norm of r before its rounding.  Backward keeps x and y (r alone where
+    it is fp32 and y has neither norm nor gate)."""
     dev, xdt = x.get_device(), x.dtype
     shape = x.shape
     d = shape[-1] if shape else 0

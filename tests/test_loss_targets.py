@@ -36,6 +36,12 @@ def test_any_integer_type(monkeypatch, dtype, ignore):
     assert t.long().tolist() == [[100, 7, 120, ignore], [1, 2, 3, ignore]]
 
 
+def test_the_last_byte_is_a_token(monkeypatch):
+    """255 of a byte vocabulary is no padding, although uint8 compares it equal to -1."""
+    ids = torch.tensor([[255, 7, 255, 255, 0]], dtype=torch.uint8)
+    assert made(monkeypatch, ids).tolist() == [[7, 255, 255, 0, -100]]
+
+
 def test_padding_anywhere(monkeypatch):
     """Padding (-1) before, between or after tokens has no target, and is none: what follows it begins a text."""
     ids = torch.tensor([[-1, -1, 4, 5, 6], [7, -1, -1, 8, 9], [1, 2, 3, -1, -1]])
@@ -71,6 +77,7 @@ def test_loss_of_small_id_types(dtype):
     torch.manual_seed(0)
     model = lm.OrthoSSMLM(lm.OrthoLMConfig(vocab_size=256, n_layers=1, window=64)).to("cuda", torch.bfloat16)
     ids = torch.randint(0, 256, (2, 130), device="cuda")
+    ids[0, ::9], ids[1, -1] = 255, 255
     st = model.fresh_states(2, "cuda", generator_seed=1)
     out = []
     for i in (ids, ids.to(dtype)):
